@@ -21,9 +21,11 @@ from .ring import (  # noqa: F401
     stripe_bytes,
     BLOCK_Q4_0_BYTES,
 )
+from .pages import KVPages  # noqa: F401
 
 __all__ = [
     "KVRing",
+    "KVPages",
     "RingError",
     "Session",
     "launch_decode_attention",

@@ -59,6 +59,20 @@ SIGNATURES = {
     "bmo_attn_session_sync": (i32, [P]),
     "bmo_attn_session_capture_begin": (i32, [P]),
     "bmo_attn_session_capture_end": (i32, [P]),
+    "bmo_kv_pages_create": (P, [i32, i32, i32, i32, i32]),
+    "bmo_kv_pages_free": (None, [P]),
+    "bmo_kv_pages_bytes": (i64, [P]),
+    "bmo_kv_pages_last_error": (ctypes.c_char_p, [P]),
+    "bmo_kv_pages_list_init": (i32, [P, P, P]),
+    "bmo_kv_pages_plan": (i32, [P, P, i32, P, P, P, i32, P, i32, P, P, P, P, P]),
+    "bmo_kv_pages_append": (i32, [P, i32, i32, P, i32, P, P, i64, P]),
+    "bmo_kv_pages_gather": (i32, [P, i32, i32, P, i32, P, P, i64, P]),
+    "bmo_kv_pages_workspace_bytes": (i64, [P, i32]),
+    "bmo_kv_pages_decode": (i32, [P, i32, i32, P, P, i32, i32, i32, P, i64, P, f32, i32, i32, P, i64, P]),
+    "bmo_kv_pages_append_decode": (i32, [P, i32, i32, P, P, i32, i32, i32, P, i64, P, P, i64, P, f32, i32, i32, P,
+                                         i64, P]),
+    "bmo_kv_pages_attend": (i32, [P, i32, i32, P, P, P, i32, i32, i32, i32, P, i64, P, f32, i32, i32, i32, i32, P,
+                                  i64, P]),
 }
 
 

@@ -445,6 +445,135 @@ BMO_ATTN_API int bmo_launch_gemv_q4_0_q8_1(const void *W_dev, const float *x_dev
                                            float *y_dev, int rows, int cols,
                                            void *q8_scratch, void *stream);
 
+/* ---- paged cache ------------------------------------------------------------- */
+/*
+ * For requests whose lengths differ and grow (the ring gives every session
+ * n_ctx slots): a pool of pages of page_size slots, a block table that names
+ * each request's pages, and the same Q4_0 blocks.  No counterpart in the
+ * reference, whose handle has one session.
+ *
+ * Position p of entry b is in slot table[b][p / page_size] * page_size +
+ * p % page_size of every layer.  Tables, lengths and the list of free pages
+ * are the caller's DEVICE int arrays, so that a captured step runs on with
+ * what earlier ones left in them: table [n_batch][max_pages], lens [n_batch].
+ * A page id out of range is not followed: its positions are masked and an
+ * append to it is dropped.  The length of an entry counts at most
+ * max_pages * page_size positions (at most 2^30), a negative one as 0.
+ * q, k, v and out are rows [heads][head_dim] of `type`, out dense, the others
+ * `stride` elements apart from token to token (0: dense; a packed QKV row has
+ * a longer one), 16-byte aligned.  Calls that write slots must be ordered with
+ * the calls that read them, as for the ring.  K and V must be finite and, for
+ * attend, lie in fp16 range; what masked positions hold never shows.
+ */
+typedef struct bmo_kv_pages bmo_kv_pages_t;
+
+/* Element types of rows. */
+#define BMO_ATTN_F32 0
+#define BMO_ATTN_F16 1
+#define BMO_ATTN_BF16 2
+#define BMO_ATTN_Q4_0 3 /* append and gather: ggml blocks [n_tok][n_kv_heads][head_dim / 32] of 18 bytes */
+
+/* Allocates and zeroes a pool on the current HIP device.  head_dim 64 or 128;
+ * page_size a power of two from 2048 / head_dim to 1024.  NULL on failure
+ * (bmo_kv_pages_last_error(NULL) has the calling thread's reason). */
+BMO_ATTN_API bmo_kv_pages_t *bmo_kv_pages_create(int n_layers, int n_pages, int page_size,
+                                                 int n_kv_heads, int head_dim);
+/* NULL-safe. */
+BMO_ATTN_API void bmo_kv_pages_free(bmo_kv_pages_t *pages);
+BMO_ATTN_API int64_t bmo_kv_pages_bytes(const bmo_kv_pages_t *pages);
+BMO_ATTN_API const char *bmo_kv_pages_last_error(const bmo_kv_pages_t *pages);
+
+/* Makes free_list [n_pages + 2] (device) hold every page: word 0 is the number
+ * of free pages, word 1 belongs to the library, ids follow, the last of them
+ * given out first (page 0 is first of a fresh list). */
+BMO_ATTN_API int bmo_kv_pages_list_init(bmo_kv_pages_t *pages, int *free_list, void *stream);
+
+/* Block tables and slot maps from what the requests ask for.  Entry b gets
+ * n_new[b] more positions; a negative n_new[b] takes that many back (a
+ * rejected draft; -lens[b] or less ends the request, length 0), and pages that
+ * are no longer needed return to the list.  A growth is granted when the pages
+ * that it and the entries before it need are free; the first that is not, and
+ * whoever needs a page after it, is left as it was.  A growth that a later
+ * call takes back leaves the list as it found it.
+ *   tok_start [n_batch + 1]: running sum of the positive n_new (of refused
+ *             entries too, whose rows the caller has)
+ *   tok_slot, tok_pos, tok_entry [max_tok]: of the t-th new token, entry after
+ *             entry: its slot and position (-1 for a refused entry) and entry
+ *   status [n_batch]: 0 done, 1 no free pages, 2 out of range (a negative
+ *             length, longer than the table, or tokens past max_tok)
+ * These five may be NULL.  Table columns past an entry's length, and tokens
+ * past the last, are left as they were.  A page belongs to one entry.  Calls
+ * on one list must be ordered.  Asynchronous, allocates nothing, one launch. */
+BMO_ATTN_API int bmo_kv_pages_plan(bmo_kv_pages_t *pages, int *free_list, int n_batch,
+                                   const int *n_new, int *lens, int *table, int max_pages,
+                                   int *tok_start, int max_tok, int *tok_slot, int *tok_pos,
+                                   int *tok_entry, int *status, void *stream);
+
+/* Quantizes row t of k and v [n_tok][n_kv_heads][head_dim] into slot slots[t]
+ * of one layer, bit-exactly as bmo_kv_ring_append; type BMO_ATTN_Q4_0 copies
+ * blocks as they are.  Rows with a slot out of range are skipped.  The slots
+ * of one call must be distinct. */
+BMO_ATTN_API int bmo_kv_pages_append(bmo_kv_pages_t *pages, int layer, int n_tok,
+                                     const int *slots, int type, const void *k, const void *v,
+                                     int64_t stride, void *stream);
+
+/* The reverse: the values (or blocks) of slots slots[t] into row t of k and v;
+ * zeros for a slot out of range. */
+BMO_ATTN_API int bmo_kv_pages_gather(bmo_kv_pages_t *pages, int layer, int n_tok,
+                                     const int *slots, int type, void *k, void *v,
+                                     int64_t stride, void *stream);
+
+/* Bytes of workspace with which decode and attend may cut long entries in
+ * runs, for calls with n_heads query heads; 0 for a bad argument.  The
+ * workspace holds nothing between calls; calls that may overlap need one
+ * each.  Without one (NULL) nothing is cut. */
+BMO_ATTN_API int64_t bmo_kv_pages_workspace_bytes(const bmo_kv_pages_t *pages, int n_heads);
+
+/* Attention of one row per entry: q and out [n_batch][n_heads][head_dim] of
+ * type F32, F16 or BF16; entry b's row attends to its last min(lens[b],
+ * window) positions (window 0: all), query head h to kv head
+ * h / (n_heads / n_kv_heads).  scale <= 0: 1/sqrt(head_dim).  An entry
+ * without positions gets zeros.  max_len: no entry is longer (0: not known);
+ * it only chooses how the call is cut.  fp32 results are as close as fp32
+ * arithmetic; the result does not depend on the other entries' rows, but how
+ * the entries' lengths together cut an entry decides its rounding. */
+BMO_ATTN_API int bmo_kv_pages_decode(bmo_kv_pages_t *pages, int layer, int n_batch,
+                                     const int *lens, const int *table, int max_pages,
+                                     int n_heads, int type, const void *q, int64_t q_stride,
+                                     void *out, float scale, int window, int max_len,
+                                     void *workspace, int64_t workspace_bytes, void *stream);
+
+/* The same with the append of the newest position: k_new and v_new
+ * [n_batch][n_kv_heads][head_dim] are quantized into position lens[b] - 1 and
+ * attended to with their quantized values.  Entries must not share the page of
+ * that position. */
+BMO_ATTN_API int bmo_kv_pages_append_decode(bmo_kv_pages_t *pages, int layer, int n_batch,
+                                            const int *lens, const int *table, int max_pages,
+                                            int n_heads, int type, const void *q,
+                                            int64_t q_stride, const void *k_new,
+                                            const void *v_new, int64_t kv_stride, void *out,
+                                            float scale, int window, int max_len,
+                                            void *workspace, int64_t workspace_bytes,
+                                            void *stream);
+
+/* Attention of ragged rows: entry b has rows q_start[b] .. q_start[b + 1] - 1
+ * of q and out [n_rows][n_heads][head_dim] (type F16 or BF16; q_start
+ * [n_batch + 1] on the device, a running sum; rows past its last are left as
+ * they were).  causal: an entry's rows are its last positions, row i of n at
+ * position lens[b] - n + i, and see the positions up to their own (a chunk of
+ * a prompt, appended before the call); otherwise every row sees all lens[b]
+ * positions (an encoder's states, of another length).  window: as in decode,
+ * counted back from the row's last position.  Rows that see nothing are
+ * zeros.  max_rows: no entry has more rows (0: not known; rows past it may be
+ * left as they were), max_len as in decode.  Scores and sums in fp32, K, V and
+ * weights in fp16 on the matrix cores. */
+BMO_ATTN_API int bmo_kv_pages_attend(bmo_kv_pages_t *pages, int layer, int n_batch,
+                                     const int *q_start, const int *lens, const int *table,
+                                     int max_pages, int n_rows, int n_heads, int type,
+                                     const void *q, int64_t q_stride, void *out, float scale,
+                                     int causal, int window, int max_rows, int max_len,
+                                     void *workspace, int64_t workspace_bytes, void *stream);
+
 /* ---- node-level drop-in ------------------------------------------------------ */
 
 /* Same signature and semantics as the reference's launch_decode_attention

@@ -1,0 +1,219 @@
+"""Ragged rows over their entries' pages, causal chunks and cross attention,
+against 64 bits (bounds in _pages.py)."""
+import numpy as np
+import pytest
+
+from _pages import attention, check, i32, kv_rows, pool, rel, slot_of, to_type
+from bmo_jetson_amd import KVPages, RingError
+
+pytestmark = pytest.mark.gpu
+
+
+def _run(gpu, rows, lens, page, heads, kv, dim, type_="bfloat16", causal=True, window=0, seed=0, max_rows=None, tail=3,
+         table_edit=None, cache_edit=None, workspace=True, scale=0.0, gap=1, tol=True):
+    pages, cache, table = pool(gpu, lens, page, kv, dim, seed + 40)
+    if cache_edit:
+        cache_edit(pages, cache, table)
+    if table_edit is not None:
+        table = table_edit(table)
+    total = sum(rows)
+    packed, x = to_type(gpu, np.random.default_rng(seed).standard_normal((total + tail, heads + gap, dim)), type_)
+    q = packed[:, :heads]
+    out = gpu.full((total + tail, heads, dim), 7.0, dtype=q.dtype, device="cuda")
+    start = np.concatenate(([0], np.cumsum(rows)))
+    work = None
+    if workspace:
+        work = gpu.full((pages.workspace_bytes(heads) // 4,), float("nan"), device="cuda")
+    pages.attend(0, i32(gpu, start), i32(gpu, lens), i32(gpu, table), q, out, causal=causal, window=window, scale=scale,
+                 max_rows=max(rows) if max_rows is None else max_rows, workspace=work, stream=gpu.cuda.current_stream())
+    got = out.double().cpu().numpy()
+    assert (got[total:] == 7.0).all()  # rows behind the last
+    refs, bounds = np.zeros((total, heads, dim)), np.zeros((total, heads, dim))
+    for b, (n, L) in enumerate(zip(rows, lens)):
+        L = min(L, table.shape[1] * page)
+        last = [L - n + i if causal else L - 1 for i in range(n)]
+        a, e = attention(cache, table[b], page, L, x[start[b]:start[b + 1], :heads], last, window, "attend", type_,
+                         scale or None)
+        refs[start[b]:start[b + 1]], bounds[start[b]:start[b + 1]] = a, e
+    if tol:
+        check(got[:total], refs, bounds, f"rows {rows} lens {lens} heads {heads}/{kv}x{dim} page {page} causal {causal}")
+        # on the whole: the output's rounding, and 16-bit operands
+        assert rel(got[:total], refs) < {"bfloat16": 2.0**-8, "float16": 2.0**-9}[type_]
+    pages.close()
+    return got[:total], refs
+
+
+@pytest.mark.parametrize("dim,page", [(128, 16), (128, 128), (64, 32), (64, 64)])
+@pytest.mark.parametrize("heads,kv", [(1, 1), (4, 2), (6, 2), (16, 1), (5, 5)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_rows_lengths_and_head_layouts(gpu, dim, page, heads, kv, causal):
+    _run(gpu, [1, 0, 5, 33, 130, 17, 64], [1, 50, 70, 33, 200, 16, 257], page, heads, kv, dim, causal=causal)
+
+
+@pytest.mark.parametrize("type_", ["bfloat16", "float16"])
+@pytest.mark.parametrize("rows", [[1], [2, 8], [31, 32, 33], [127, 128, 129], [300]])
+@pytest.mark.parametrize("causal", [True, False])
+def test_types_and_tiles(gpu, type_, rows, causal):
+    _run(gpu, rows, [n + 90 * i for i, n in enumerate(rows)], 64, 4, 2, 128, type_, causal=causal)
+
+
+@pytest.mark.parametrize("window", [1, 30, 64, 65, 200])
+@pytest.mark.parametrize("causal", [True, False])
+def test_windows(gpu, window, causal):
+    _run(gpu, [100, 3, 150], [100, 300, 400], 32, 4, 2, 64, window=window, causal=causal)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_rows_that_see_nothing(gpu, causal):
+    # more rows than positions, and no positions at all
+    got, _ = _run(gpu, [40, 9, 4], [10, 0, 50], 32, 2, 2, 64, causal=causal)
+    assert not got[40:49].any()
+    if causal:
+        assert not got[:30].any() and got[30:40].any()
+
+
+def test_few_rows_of_long_entries(gpu):
+    for causal in (True, False):
+        for heads, kv in ((2, 2), (8, 1), (16, 1)):
+            _run(gpu, [1, 3, 2], [4000, 20, 2500], 64, heads, kv, 128, causal=causal, type_="float16")
+            _run(gpu, [1, 3, 2], [4000, 20, 2500], 64, heads, kv, 128, causal=causal, workspace=False)
+
+
+def test_many_entries(gpu):
+    r = np.random.default_rng(3)
+    rows = [int(x) for x in r.integers(0, 40, 150)]
+    _run(gpu, rows, [n + int(x) for n, x in zip(rows, r.integers(0, 60, 150))], 32, 2, 1, 64, max_rows=0)
+    _run(gpu, rows, [n + int(x) for n, x in zip(rows, r.integers(0, 60, 150))], 32, 2, 1, 64)
+
+
+def test_scale(gpu):
+    _run(gpu, [20], [90], 64, 2, 2, 64, scale=0.05)
+
+
+def _spoil(gpu, pages, slots, kv, dim):
+    x = np.full((len(slots), kv, dim), np.nan, dtype=np.float32)
+    x[::2] = np.inf
+    pages.append(0, i32(gpu, slots), gpu.from_numpy(x).cuda(), gpu.from_numpy(x).cuda(),
+                 stream=gpu.cuda.current_stream())
+
+
+@pytest.mark.parametrize("rows", [[2, 1], [60, 200]])
+@pytest.mark.parametrize("window", [0, 70])
+def test_what_masked_positions_hold_does_not_show(gpu, rows, window):
+    lens, page, kv, dim = [rows[0] + 100, rows[1]], 64, 2, 128
+
+    def edit(pages, cache, table):
+        used = set()
+        for b, (n, L) in enumerate(zip(rows, lens)):
+            lo = max(0, L - n + 1 - window) if window else 0
+            used |= {slot_of(table, b, p, page) for p in range(lo, L)}
+        _spoil(gpu, pages, np.array(sorted(set(range(len(cache.k))) - used)), kv, dim)
+    _run(gpu, rows, lens, page, 4, kv, dim, window=window, cache_edit=edit)
+
+
+@pytest.mark.parametrize("rows,at", [(150, 90), (3, 98)])
+def test_a_value_that_is_not_finite_reaches_only_rows_that_see_it(gpu, rows, at):
+    """V block 1 of position `at` is infinite: rows before it are as they are
+    without it, later ones are not finite in that block alone."""
+    page, kv, dim, heads = 32, 1, 128, 2
+    L = max(rows, 100)
+    pages, cache, table = pool(gpu, [L], page, kv, dim, 60)
+    q = gpu.randn(rows, heads, dim, device="cuda").bfloat16()
+    start, lens, t = i32(gpu, [0, rows]), i32(gpu, [L]), i32(gpu, table)
+    want, out = gpu.zeros_like(q), gpu.zeros_like(q)
+    pages.attend(0, start, lens, t, q, want)
+    slot = i32(gpu, [slot_of(table, 0, at, page)])
+    k, v = (gpu.zeros(1, kv, dim // 32, 18, dtype=gpu.uint8, device="cuda") for _ in range(2))
+    pages.gather(0, slot, k, v)
+    v[0, 0, 1, :2] = gpu.tensor([0, 0x7C], dtype=gpu.uint8)
+    pages.append(0, slot, k, v)
+    pages.attend(0, start, lens, t, q, out)
+    gpu.cuda.synchronize()
+    sees = L - rows + np.arange(rows) >= at
+    assert 0 < sees.sum() < rows
+    sees = gpu.from_numpy(sees).cuda()
+    assert gpu.equal(out[~sees], want[~sees])
+    assert not bool(out[sees][:, :, 32:64].isfinite().any())
+    rest = [c for c in range(dim) if not 32 <= c < 64]
+    assert gpu.equal(out[sees][:, :, rest], want[sees][:, :, rest])
+    pages.close()
+
+
+@pytest.mark.parametrize("rows", [[2, 1, 2], [70, 33, 40]])
+def test_bad_page_ids_are_masked(gpu, rows):
+    def edit(table):
+        t = table.copy()
+        t[0, 1], t[1, 0], t[2, :] = -1, 10**8, -2**31
+        return t
+    got, _ = _run(gpu, rows, [200, 60, 90], 64, 4, 2, 128, table_edit=edit, causal=False)
+    assert not got[rows[0]:].any()
+
+
+def test_nan_in_one_query_stays_in_its_row(gpu):
+    pages, cache, table = pool(gpu, [100], 64, 2, 128, 5)
+    q = gpu.randn(50, 4, 128, device="cuda").half()
+    out, want = gpu.zeros_like(q), gpu.zeros_like(q)
+    args = (0, i32(gpu, [0, 50]), i32(gpu, [100]), i32(gpu, table))
+    pages.attend(*args, q, want)
+    q[7, 2, 3] = float("nan")
+    pages.attend(*args, q, out)
+    bad = gpu.zeros(50, 4, dtype=gpu.bool, device="cuda")
+    bad[7, 2] = True
+    assert bool(out[bad].isnan().all()) and gpu.equal(out[~bad], want[~bad])
+    pages.close()
+
+
+def test_starts_that_are_no_running_sum(gpu):
+    """Entries whose rows are not within q are skipped."""
+    pages, cache, table = pool(gpu, [50, 50, 50], 64, 2, 64, 8)
+    q = gpu.randn(20, 2, 64, device="cuda").half()
+    for start in ([0, 30, 5, 10], [-4, 5, 10, 20], [2**31 - 1, 0, 2**31 - 1, -2**31]):
+        out = gpu.full_like(q, 7.0)
+        pages.attend(0, i32(gpu, start), i32(gpu, [50] * 3), i32(gpu, table), q, out, causal=False)
+        gpu.cuda.synchronize()
+        if start[0] == 0:
+            assert bool((out[:5] == 7.0).all()) and bool((out[10:] == 7.0).all())
+    pages.close()
+
+
+def test_replayed_from_a_graph(gpu):
+    for rows, heads in (([40, 200], 4), ([1, 2], 4)):
+        lens = [900, 250]
+        pages, cache, table = pool(gpu, lens, 64, 2, 128, 9)
+        q = gpu.randn(sum(rows), heads, 128, device="cuda").half()
+        start, ln, t = i32(gpu, [0, rows[0], sum(rows)]), i32(gpu, lens), i32(gpu, table)
+        work, work2 = (gpu.zeros(pages.workspace_bytes(heads), dtype=gpu.uint8, device="cuda") for _ in range(2))
+        out, eager = gpu.zeros_like(q), gpu.zeros_like(q)
+        graph, side = gpu.cuda.CUDAGraph(), gpu.cuda.Stream()
+        side.wait_stream(gpu.cuda.current_stream())
+        with gpu.cuda.stream(side), gpu.cuda.graph(graph, stream=side):
+            pages.attend(0, start, ln, t, q, out, max_rows=max(rows), workspace=work, stream=gpu.cuda.current_stream())
+        gpu.cuda.current_stream().wait_stream(side)
+        for _ in range(4):
+            q.mul_(1.05)
+            graph.replay()
+            pages.attend(0, start, ln, t, q, eager, max_rows=max(rows), workspace=work2, stream=gpu.cuda.current_stream())
+            gpu.cuda.synchronize()
+            assert gpu.equal(out, eager) and bool(out.any())
+        pages.close()
+
+
+def test_refusals(gpu):
+    pages = KVPages(1, 4, 32, 2, 64)
+    lens, table, start = i32(gpu, [3, 4]), i32(gpu, [[0, 1], [2, 3]]), i32(gpu, [0, 1, 2])
+    q = gpu.zeros(2, 4, 64, device="cuda").half()
+    with pytest.raises(RingError, match="fp16 or bf16"):
+        pages.attend(0, start, lens, table, q.float(), q.float())
+    with pytest.raises(RingError, match="layer"):
+        pages.attend(-1, start, lens, table, q, q.clone())
+    for kw in ({"window": -1}, {"max_len": -1}, {"max_rows": -1}, {"scale": float("nan")}):
+        if "scale" in kw:
+            pages.attend(0, start, lens, table, q, q.clone(), **kw)  # not positive: the default
+            continue
+        with pytest.raises(RingError):
+            pages.attend(0, start, lens, table, q, q.clone(), **kw)
+    with pytest.raises(ValueError):
+        pages.attend(0, start[:2], lens, table, q, q.clone())
+    pages.attend(0, start, lens, table, q[:0], q[:0].clone())  # nothing to do
+    gpu.cuda.synchronize()
+    pages.close()
