@@ -105,7 +105,7 @@ struct Place {
         const int tb = t * NB + w.blk;
         uint8_t *grp = p.base + p.g.group_offset(w.slot, w.h);
         codes = w.which == 0 ? grp + key * 16 + tb * 4 : grp + kVCodeOff + (key >> 2) * 256 + tb * 4 + (key & 3);
-        scale = reinterpret_cast<uint16_t *>(grp + (w.which == 0 ? kPageScaleK : kPageScaleV)) + tb * 16 + key;
+        scale = reinterpret_cast<uint16_t *>(grp + page_scale_offset(tb, key, w.which));
     }
 };
 

@@ -173,6 +173,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, 2) void pages_attend_kernel(Atte
         int flag;
     };
     Load ld[LG];
+    const Patterns pat;
     const int last_group = max((len - 1) / G, 0);
     const int key16 = lane & 15, oct = lane >> 4;
     auto fetch = [&](int stage) {
@@ -188,11 +189,13 @@ __global__ __launch_bounds__(64 * kAttendWaves, 2) void pages_attend_kernel(Atte
             ld[i].flag = ok ? 0 : 1;
             ld[i].k = *reinterpret_cast<const uint4 *>(at + lane * 16);
             ld[i].v = *reinterpret_cast<const uint4 *>(at + kVCodeOff + lane * 16);
-            const uint16_t *ks = reinterpret_cast<const uint16_t *>(at + kPageScaleK) + key16;
-            ld[i].ks = make_uint4(ks[0], ks[16], ks[32], ks[48]);
+            uint32_t ks[4];
 #pragma unroll
-            for (int tb = 0; tb < 4; ++tb)
-                ld[i].vs[tb] = *reinterpret_cast<const uint2 *>(at + kPageScaleV + tb * 32 + oct * 8);
+            for (int tb = 0; tb < 4; ++tb) {
+                ks[tb] = *reinterpret_cast<const uint16_t *>(at + page_scale_offset(tb, key16, 0));
+                ld[i].vs[tb] = *reinterpret_cast<const uint2 *>(at + page_scale_offset(tb, 4 * oct, 1));
+            }
+            ld[i].ks = make_uint4(ks[0], ks[1], ks[2], ks[3]);
         }
     };
     auto fill = [&](int buf) {
@@ -229,19 +232,15 @@ __global__ __launch_bounds__(64 * kAttendWaves, 2) void pages_attend_kernel(Atte
                 const int t = tb / NB, blk = tb % NB;
                 // K: row of the key, octet `oct` of the block
                 const _Float16 d = __builtin_bit_cast(_Float16, (uint16_t) kd[tb]);
-                const pg_half8 kx = k_octet(kw[tb]) * pg_half8{d, d, d, d, d, d, d, d};
+                const pg_half8 kx = k_octet(kw[tb], pat) * pg_half8{d, d, d, d, d, d, d, d};
                 const int key = gi * G + t * 16 + key16;
                 *reinterpret_cast<pg_half8 *>(&s_k[buf][key * KROW + (blk * 4 + oct) * 8]) = kx;
                 // V: rows key16 and key16 + 16 of the block (elements), quad of keys
                 const uint32_t w = vw[tb], y = w >> 8;
-                const pg_half2 lo16 = {(_Float16) -1032.0f, (_Float16) -1032.0f};
-                const pg_half2 hi16 = {(_Float16) -72.0f, (_Float16) -72.0f};
                 const pg_half2 da = __builtin_bit_cast(pg_half2, (ld[i].vs[tb].x & 0xFFFFu) | (ld[i].vs[tb].y << 16));
                 const pg_half2 db = __builtin_bit_cast(pg_half2, (ld[i].vs[tb].x >> 16) | (ld[i].vs[tb].y & 0xFFFF0000u));
-                const pg_half2 e0 = (__builtin_bit_cast(pg_half2, (w & 0x000F000Fu) | 0x64006400u) + lo16) * da;
-                const pg_half2 e1 = (__builtin_bit_cast(pg_half2, (y & 0x000F000Fu) | 0x64006400u) + lo16) * db;
-                const pg_half2 h0 = (__builtin_bit_cast(pg_half2, (w & 0x00F000F0u) | 0x54005400u) + hi16) * da;
-                const pg_half2 h1 = (__builtin_bit_cast(pg_half2, (y & 0x00F000F0u) | 0x54005400u) + hi16) * db;
+                const pg_half2 e0 = codes_lo(w, pat) * da, e1 = codes_lo(y, pat) * db;
+                const pg_half2 h0 = codes_hi(w, pat) * da, h1 = codes_hi(y, pat) * db;
                 const int quad = (gi * G + t * 16) / 4 + oct;  // of the stage
                 const int place = (quad & ~3) + 2 * (quad & 1) + ((quad >> 1) & 1);
                 _Float16 *row = &s_v[buf][(blk * kQK + key16) * VROW + place * 4];
@@ -347,11 +346,12 @@ __global__ __launch_bounds__(64 * kAttendWaves, 2) void pages_attend_kernel(Atte
                     }
                     const uint8_t *at = p.base + (int64_t) id * g.page_bytes +
                                         (((int64_t) kvh << g.group_shift) + (grp & ((1 << g.group_shift) - 1))) * kGroupBytes;
-                    const uint16_t *vs = reinterpret_cast<const uint16_t *>(at + kPageScaleV);
                     for (int k = 0; k < G; ++k) {
                         const int pos = grp * G + k;
                         for (int blk = 0; blk < NB; ++blk)
-                            if (!finite16(vs[((k >> 4) * NB + blk) * 16 + (k & 15)]) && pos >= lo && pos < hi)
+                            if (!finite16(*reinterpret_cast<const uint16_t *>(
+                                    at + page_scale_offset((k >> 4) * NB + blk, k & 15, 1))) &&
+                                pos >= lo && pos < hi)
                                 poison |= 1 << blk;
                     }
                 }

@@ -6,23 +6,26 @@
 //
 // One wave step takes 32 positions of one kv head: 16 bytes of K codes and of
 // V codes a lane and tile of 16 (pages_layout.hpp), straight from HBM to the
-// operands of v_mfma_f32_16x16x32.  The 16 columns of the products hold
+// operands of the matrix instructions.  The 16 columns of the products hold
 //   (head r, block b): heads of the kv head's group, up to 16 / NB of them,
 //                      each column with the query of its own block only; or
 //   head r:            up to 16 heads, when the group has more than 16 / NB.
 // In the first form a lane has one block's products, so the block scales cost
 // one multiply a score and one a weight instead of NB each.
 //
-// K side: q (times scale * log2 e) enters as two fp16 parts hi + lo of
-// q * 2^e, e chosen per row, exact to 2^-22 of the row's largest element; the
-// codes minus 8 are exact in fp16, products are summed in fp32 per block and
-// multiplied by the block's scale in fp32.  V side: p * d (weight times V
-// scale) enters as two bf16 parts, exact to 2^-17 of itself whatever its
-// range, against the plain codes 0..15, exact in bf16; 8 times the parts' sum,
-// from the same matrix instruction with a constant operand, is taken off every
-// eight steps, so that this debt does not grow.  An fp32 call is therefore as
-// close as fp32 sums (about 1e-6); 16-bit calls use the same kernel, whose
-// time the bytes decide.
+// K side, first form: q becomes a whole number of 22 bits (fp32; 15 bits for
+// 16-bit rows) times a power of two per row, in signed base-256 digits, and
+// the codes 0..15 enter v_mfma_i32_16x16x64_i8 as the bytes that a mask
+// leaves; the digits' sums and the -8 of every code join exactly in 32 bits.
+// Second form: q as two fp16 parts (16-bit rows: one, exactly), the codes
+// minus 8 exact in fp16.  Either way a query is within 2^-22 (2^-15) of its
+// row's largest element, and a block's product meets its scale in fp32.
+//
+// V side: weight times V scale, brought to fp16's range by a power of two per
+// column (from the largest scale so far), enters as two truncated fp16 parts,
+// exact to 2^-21 (16-bit rows: one part, rounded), against the codes minus 8,
+// exact in fp16, sums in fp32.  An fp32 call is as close as fp32 sums; the
+// 16-bit parts stay below the outputs' own rounding.
 //
 // Softmax is online with a running maximum per column, raised only when a
 // score passes it by 8 (log2 units), so that the exchange between the four
@@ -30,36 +33,42 @@
 // 0 by select, whatever their slots hold.
 //
 // Work: an item is a run of steps of one (entry, kv head, head set), walked
-// by the NW waves of a workgroup in turn and joined in LDS.  When the entries
-// are few or long, an entry's steps are cut in ceil(n / c) even runs, with c
-// from all entries' steps and the workgroups wanted (every workgroup sums the
-// lengths itself), their results kept as (max, sum, row) in the workspace and
-// joined by a second kernel in the order of the runs.
+// by the NW waves of a workgroup in turn and joined in LDS.  The host knows
+// how long an entry can be, not how long each is: where that is long for the
+// units there are, an entry of n steps has ceil(n / c) even runs, up to a
+// number of them for which the grid has workgroups (those of shorter entries
+// end at once); results of entries that have several are kept as (max, sum,
+// row) in the workspace and joined by a second kernel in the order of the runs.
+#include <algorithm>
+
 #include "pages_device.hpp"
 
 namespace bmo {
 
 namespace {
 
-constexpr int kStep = 32;        // positions a wave step
-constexpr int kDecodeWaves = 4;  // waves a workgroup
-constexpr int kSettle = 8;       // steps between taking off 8 * sum p d
-// Workgroups a split launch is cut for, and the fewest steps a run has.
-constexpr int kWantWorkgroups = 512;
-constexpr int kMinRun = 8;
+constexpr int kStep = 32;  // positions a wave step
+constexpr int kWaves = 4;  // of a workgroup, where it is not one
+// How a launch is cut, see launch_pages_decode: waves of a launch that fills
+// the card once (few units) and the fewest steps of a run for each of them,
+// and the same for launches of several rounds.
+constexpr int kFillWaves = 1024, kFillSteps = 4;
+constexpr int kSplitWaves = 4096, kSplitSteps = 16;
+constexpr int kMaxRuns = 128;  // of an entry
 
 struct DecodeArgs {
     PagesDecodeParams p;
-    int group;    // query heads a kv head
-    int n_hs;     // head sets a kv head
-    int units;    // n_kv * n_hs
-    int split;    // 0: every entry is one run
+    int group;     // query heads a kv head
+    int n_hs;      // head sets a kv head
+    int units;     // n_kv * n_hs
+    int max_runs;  // of an entry; 1: nothing is cut
+    int run;       // steps up to which an entry is one run
     int append;
 };
 
 // Steps of an entry: its visible positions are [lo, len).
 struct Span {
-    int len, lo, step0, n;
+    int len, lo, step0, n, runs;
 };
 __device__ __forceinline__ Span span_of(const DecodeArgs &a, int len) {
     Span s;
@@ -67,98 +76,71 @@ __device__ __forceinline__ Span span_of(const DecodeArgs &a, int len) {
     s.len = (int) min((int64_t) max(len, 0), room);
     s.lo = a.p.window > 0 && s.len > a.p.window ? s.len - a.p.window : 0;
     s.step0 = s.lo / kStep;
-    s.n = (int) (((int64_t) s.len + kStep - 1) / kStep) - s.step0;
+    s.n = (s.len + kStep - 1) / kStep - s.step0;  // (room is at most 2^30)
+    s.runs = a.max_runs == 1 ? 1 : min(max((s.n + a.run - 1) / a.run, 1), a.max_runs);
     return s;
 }
-__device__ __forceinline__ int runs_of(int n, int c) { return n <= c ? 1 : (n + c - 1) / c; }
 
-
-// The longest run of steps, from the steps of all entries.
-__device__ __forceinline__ int run_length(const DecodeArgs &a, int lane) {
-    int64_t total = 0;
-    for (int b0 = 0; b0 < a.p.n_batch; b0 += 64) {
-        const int b = b0 + lane;
-        const int n = b < a.p.n_batch ? span_of(a, a.p.lens[b]).n : 0;
-        // (64 entries of at most 2^25 steps)
-        total += (uint32_t) __shfl(wave_prefix(n, lane), 63);
-    }
-    const int64_t c = (total * a.units + kWantWorkgroups - 1) / kWantWorkgroups;
-    return (int) min(max(c, (int64_t) kMinRun), (int64_t) INT32_MAX);
-}
-
-// Item `item` of a split launch: its entry, run, and the index of its entry's
-// first partial result.  False past the last item.
-struct Item {
-    int b, run, runs, unit, part0;
-};
-__device__ __forceinline__ bool find_item(const DecodeArgs &a, int item, int c, int lane, Item &it) {
-    const int row = item / a.units;  // (entry, run)
-    it.unit = item - row * a.units;
-    int rows = 0, parts = 0;
-    for (int b0 = 0; b0 < a.p.n_batch; b0 += 64) {
-        const int b = b0 + lane;
-        const int runs = b < a.p.n_batch ? runs_of(span_of(a, a.p.lens[b]).n, c) : 0;
-        const int upto = wave_prefix(runs, lane) + rows;
-        const int parts_upto = wave_prefix(runs > 1 ? runs : 0, lane) + parts;
-        const uint64_t past = __ballot(upto > row);
-        if (past) {
-            const int l = __ffsll((unsigned long long) past) - 1;
-            it.b = b0 + l;
-            it.runs = __shfl(runs, l);
-            it.run = row - (__shfl(upto, l) - it.runs);
-            it.part0 = __shfl(parts_upto, l) - (it.runs > 1 ? it.runs : 0);
-            return true;
-        }
-        rows = __shfl(upto, 63);
-        parts = __shfl(parts_upto, 63);
-    }
-    return false;
-}
-
-// Floats of a partial result of HC heads.
+// Floats of a partial result of HC heads: their rows, and maximum and sum of
+// every block (whose weights have a scale of their own).
 template <int D>
-__host__ __device__ constexpr int part_floats(int hc) { return hc * (D + 2); }
+__host__ __device__ constexpr int part_floats(int hc) { return hc * (D + 2 * (D / kQK)); }
 
 }  // namespace
 
-// SPREAD: the columns are (head, block); otherwise heads.
-template <int D, bool SPREAD>
-__global__ __launch_bounds__(64 * kDecodeWaves) void pages_decode_kernel(DecodeArgs a) {
-    constexpr int NW = kDecodeWaves;
+// SPREAD: the columns are (head, block); otherwise heads.  F32: the rows are
+// fp32, and the query and the weights take a part more.
+template <int D, bool SPREAD, int NW, bool F32>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD || D == 64 ? 3 : 2))) void pages_decode_kernel(DecodeArgs a) {
     constexpr int NB = D / kQK;
     constexpr int TG = kStep * D / 2048;    // groups a step
     constexpr int T = 2 / TG;               // tiles of 16 a group
     constexpr int CB = SPREAD ? NB : 1;     // columns a head
     constexpr int HC = 16 / CB;             // heads a head set
     constexpr int PB = NB / CB;             // blocks a column
+    constexpr int QP = F32 ? 2 : 1;         // fp16 parts of the query
+    constexpr int QD = F32 ? 3 : 2;         // or base-256 digits
+    constexpr int QBITS = F32 ? 21 : 14;    // |Q| <= 2^QBITS
+    constexpr int WP = F32 ? 2 : 1;         // parts of a weight
+    constexpr int BUF = 2;  // steps resident in registers
     const PagesDecodeParams &p = a.p;
     const PagesGeom &g = p.g;
 
-    __shared__ float s_out[NW][HC][D];
-    __shared__ float s_m[NW][HC], s_l[NW][HC];
+    __shared__ __align__(16) float s_out[NW][HC][D];
+    __shared__ float s_m[NW][HC][NB], s_l[NW][HC][NB];
 
+    // (16-bit kernels: known not to be fp32)
+    const int type = F32 ? (int) kTypeF32 : p.type == kTypeF16 ? (int) kTypeF16 : (int) kTypeBF16;
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
+    const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
     const int col = lane & 15, oct = lane >> 4;
     const int r = col / CB, cb = col % CB;
 
-    Item it{};
-    if (a.split) {
-        const int c = run_length(a, lane);
-        if (!find_item(a, (int) blockIdx.x, c, lane, it)) return;
-    } else {
-        it.b = (int) blockIdx.x / a.units;
-        it.unit = (int) blockIdx.x - it.b * a.units;
-        it.runs = 1;
-    }
-    const int b = __builtin_amdgcn_readfirstlane(it.b);
-    const int kvh = it.unit / a.n_hs, hs = it.unit - kvh * a.n_hs;
+    // items: run by run, entry by entry, unit by unit
+    const int row = (int) blockIdx.x / a.units;
+    const int unit = (int) blockIdx.x - row * a.units;
+    const int run = row / p.n_batch, b = row - run * p.n_batch;
+    const int kvh = unit / a.n_hs, hs = unit - kvh * a.n_hs;
     const int heads = min(HC, a.group - hs * HC);  // heads of this set
     const int head0 = kvh * a.group + hs * HC;
-    const Span sp = span_of(a, p.lens[b]);
-    const int s_begin = sp.step0 + (int) ((int64_t) sp.n * it.run / it.runs);
-    const int s_end = sp.step0 + (int) ((int64_t) sp.n * (it.run + 1) / it.runs);
+    const Span sp = span_of(a, uniform_int(p.lens, b));
+    if (run >= sp.runs) return;
+    const int s_begin = sp.step0 + (int) ((int64_t) sp.n * run / sp.runs);
+    const int s_end = sp.step0 + (int) ((int64_t) sp.n * (run + 1) / sp.runs);
     const int *table = p.table + (int64_t) b * p.max_pages;
+
+    // The query's elements of the column's blocks (requested ahead of the
+    // steps, so that waiting for them does not wait for those).
+    pg_float4 qx[PB][2];
+    {
+        const int64_t src = (int64_t) b * p.q_stride + (int64_t) (head0 + (r < heads ? r : 0)) * D;
+#pragma unroll
+        for (int i = 0; i < PB; ++i) {
+            const int blk = SPREAD ? cb : i;
+            qx[i][0] = load4(p.q, src + blk * kQK + 4 * oct, type);
+            qx[i][1] = load4(p.q, src + blk * kQK + 4 * oct + 16, type);
+        }
+    }
 
     // The new token's row goes to its slot before the wave that will read it
     // starts on its steps (of several head sets each writes the same bytes).
@@ -170,8 +152,8 @@ __global__ __launch_bounds__(64 * kDecodeWaves) void pages_decode_kernel(DecodeA
         float x[NE];
 #pragma unroll
         for (int t = 0; t < HE; ++t) {
-            x[t] = load1(row, src + t, p.type);
-            x[HE + t] = load1(row, src + 16 + t, p.type);
+            x[t] = load1(row, src + t, type);
+            x[HE + t] = load1(row, src + 16 + t, type);
         }
         uint16_t d16;
         const uint32_t dw = quantize_block_q4_0_lanes<BL>(x, gi, d16);
@@ -192,30 +174,73 @@ __global__ __launch_bounds__(64 * kDecodeWaves) void pages_decode_kernel(DecodeA
                     grp[kVCodeOff + ((key >> 2) * 16 + i) * 16 + tb * 4 + (key & 3)] = (uint8_t) (dw >> (8 * (i & 3)));
                 }
             }
-            if (gi == 0)
-                reinterpret_cast<uint16_t *>(grp + (nb < NB ? kPageScaleK : kPageScaleV))[tb * 16 + key] = d16;
+            if (gi == 0) *reinterpret_cast<uint16_t *>(grp + page_scale_offset(tb, key, nb < NB ? 0 : 1)) = d16;
         }
         __threadfence_block();
     }
 
-    // The query: hi and lo halves of the column's row, of every block (zero
-    // outside the column's own when columns are blocks).
-    pg_half8 qh[NB], ql[NB];
+    // Page ids come through the scalar cache, a step ahead of the loads that
+    // need them; groups past the entry's last are taken as the last (masked).
+    struct Ids {
+        int id[TG];
+    };
+    struct Tile {
+        uint4 k[TG], v[TG];
+        uint4 sc[2][PB];  // K's and V's scales of the lane's four keys of a tile
+        int ok;  // bit i: group i's page is there
+    };
+    const int last_group = max((sp.len - 1) / (2048 / D), 0);
+    auto ids_of = [&](int step, Ids &t) {
+#pragma unroll
+        for (int i = 0; i < TG; ++i)
+            t.id[i] = uniform_int(table, min(step * TG + i, last_group) >> g.group_shift);
+    };
+    auto load = [&](int step, const Ids &ids, Tile &t) {
+        t.ok = 0;
+#pragma unroll
+        for (int i = 0; i < TG; ++i) {
+            const int grp = min(step * TG + i, last_group);
+            const bool ok = (unsigned) ids.id[i] < (unsigned) g.n_pages;
+            t.ok |= ok ? 1 << i : 0;
+            const uint8_t *at = p.base + (int64_t) (ok ? ids.id[i] : 0) * g.page_bytes +
+                                (((int64_t) kvh << g.group_shift) + (grp & ((1 << g.group_shift) - 1))) * kGroupBytes;
+            t.k[i] = stream16(at + lane * 16);
+            t.v[i] = stream16(at + kVCodeOff + lane * 16);
+#pragma unroll
+            for (int u = 0; u < T; ++u)
+#pragma unroll
+                for (int j = 0; j < PB; ++j)
+                    t.sc[i * T + u][j] =
+                        stream16(at + page_scale_offset(u * NB + (SPREAD ? cb : j), 4 * oct, 0));
+        }
+    };
+    const int first = s_begin + wave, last = max(s_end - 1, s_begin);
+    // (unconditional, so that the counts of loads in flight are known: an
+    // entry without positions reads some page and uses nothing of it)
+    Tile buf[BUF];
+    Ids ids[BUF];
+#pragma unroll
+    for (int j = 0; j < BUF; ++j) ids_of(min(first + j * NW, last), ids[j]);
+#pragma unroll
+    for (int j = 0; j < BUF - 1; ++j) load(min(first + j * NW, last), ids[j], buf[j]);
+    __builtin_amdgcn_sched_barrier(0);
+
+    // The query, of every block (zero outside the column's own when columns are
+    // blocks); what the products make of it is multiplied by sq.
+    typedef int int4_t __attribute__((ext_vector_type(4)));
+    pg_half8 qp[SPREAD ? 1 : QP][SPREAD ? 1 : NB];
+    int4_t qd[SPREAD ? QD : 1][NB / 2];  // digits of blocks 2 i, 2 i + 1
+    int q8 = 0;                          // -8 times the sum of the row's Q in the column's block
     float sq;
     {
-        const int64_t src = (int64_t) b * p.q_stride + (int64_t) (head0 + (r < heads ? r : 0)) * D;
         float amax = 0.0f, bad = 0.0f;
         float x[PB][8];
 #pragma unroll
         for (int i = 0; i < PB; ++i) {
-            const int blk = SPREAD ? cb : i;
-            const pg_float4 lo = load4(p.q, src + blk * kQK + 4 * oct, p.type);
-            const pg_float4 hi = load4(p.q, src + blk * kQK + 4 * oct + 16, p.type);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int e = octet_elem(0, j);  // 0..3, 16..19
-                x[i][j] = (e < 16 ? lo[e & 3] : hi[e & 3]) * p.qscale;
-                if (r >= heads) x[i][j] = 0.0f;
+                const int e = SPREAD ? (j & 3) + (j & 4) * 4 : octet_elem(0, j);  // 0..3, 16..19
+                x[i][j] = r >= heads ? 0.0f : e < 16 ? qx[i][0][e & 3] : qx[i][1][e & 3];
                 amax = fmaxf(amax, __builtin_fabsf(x[i][j]));
                 bad += x[i][j] * 0.0f;  // NaN if it is not finite
             }
@@ -232,188 +257,268 @@ __global__ __launch_bounds__(64 * kDecodeWaves) void pages_decode_kernel(DecodeA
         amax = fmaxf(amax, __shfl_xor(amax, 32));
         bad += __shfl_xor(bad, 16);
         bad += __shfl_xor(bad, 32);
-        const int ex = __builtin_amdgcn_frexp_expf(amax);
-        sq = bad == 0.0f ? __builtin_amdgcn_ldexpf(1.0f, ex - 15) : __builtin_nanf("");
+        // (rows below 2^-90 count as zeros: their scores do)
+        const int ex = max(__builtin_amdgcn_frexp_expf(amax), -90);
+        constexpr int shift = SPREAD ? QBITS : 15;
+        // (never 0: masked scores are -inf times it)
+        sq = bad == 0.0f ? fmaxf(__builtin_amdgcn_ldexpf(p.qscale, ex - shift), 1e-37f) : __builtin_nanf("");
+        if constexpr (SPREAD) {
+            uint32_t dig[QD][2];
 #pragma unroll
-        for (int blk = 0; blk < NB; ++blk) {
-            const bool mine = !SPREAD || blk == cb;
+            for (int k = 0; k < QD; ++k) dig[k][0] = dig[k][1] = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float y = __builtin_amdgcn_ldexpf(x[SPREAD ? 0 : blk][j], 15 - ex);
-                const _Float16 h = (_Float16) y;
-                qh[blk][j] = mine ? h : (_Float16) 0.0f;
-                ql[blk][j] = mine ? (_Float16) (y - (float) h) : (_Float16) 0.0f;
+                int Q = (int) __builtin_rintf(__builtin_amdgcn_ldexpf(x[0][j], shift - ex));
+                q8 -= 8 * Q;
+#pragma unroll
+                for (int k = 0; k < QD; ++k) {
+                    const int low = k + 1 < QD ? (int) (int8_t) Q : Q;
+                    dig[k][j >> 2] |= (uint32_t) (low & 0xFF) << (8 * (j & 3));
+                    Q = (Q - low) >> 8;
+                }
             }
+            q8 += __shfl_xor(q8, 16);
+            q8 += __shfl_xor(q8, 32);
+#pragma unroll
+            for (int k = 0; k < QD; ++k)
+#pragma unroll
+                for (int i = 0; i < NB / 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) qd[k][i][e] = cb == 2 * i + (e >> 1) ? (int) dig[k][e & 1] : 0;
+        } else {
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float y = __builtin_amdgcn_ldexpf(x[SPREAD ? 0 : blk][j], shift - ex);
+#pragma unroll
+                    for (int i = 0; i < QP; ++i) {
+                        const _Float16 h = (_Float16) y;
+                        qp[i][blk][j] = h;
+                        y -= (float) h;
+                    }
+                }
         }
     }
 
-    struct Tile {
-        uint4 k[TG], v[TG];
-        uint2 ks[2][PB], vs[2][PB];
-        bool ok[TG];
-    };
-    // Page ids, 64 at a time in the lanes.
-    int ids = 0, ids0 = -1;
-    auto page_of = [&](int col_) {
-        if ((col_ & ~63) != ids0) {
-            ids0 = col_ & ~63;
-            ids = ids0 + lane < p.max_pages ? table[ids0 + lane] : -1;
-        }
-        return __builtin_amdgcn_readlane(ids, col_ & 63);
-    };
-    const int last_group = max((sp.len - 1) / (2048 / D), 0);
-    auto load = [&](int step, Tile &t) {
-#pragma unroll
-        for (int i = 0; i < TG; ++i) {
-            const int grp = min(step * TG + i, last_group);
-            const int id = page_of(grp >> g.group_shift);
-            t.ok[i] = (unsigned) id < (unsigned) g.n_pages;
-            const uint8_t *at = p.base + (int64_t) (t.ok[i] ? id : 0) * g.page_bytes +
-                                (((int64_t) kvh << g.group_shift) + (grp & ((1 << g.group_shift) - 1))) * kGroupBytes;
-            t.k[i] = *reinterpret_cast<const uint4 *>(at + lane * 16);
-            t.v[i] = *reinterpret_cast<const uint4 *>(at + kVCodeOff + lane * 16);
-#pragma unroll
-            for (int u = 0; u < T; ++u)
-#pragma unroll
-                for (int j = 0; j < PB; ++j) {
-                    const int tb = u * NB + (SPREAD ? cb : j);
-                    t.ks[i * T + u][j] = *reinterpret_cast<const uint2 *>(at + kPageScaleK + tb * 32 + oct * 8);
-                    t.vs[i * T + u][j] = *reinterpret_cast<const uint2 *>(at + kPageScaleV + tb * 32 + oct * 8);
-                }
-        }
-    };
-
-    float m = kPagesFloor, mt = kPagesFloor, l = 0.0f;
-    pg_float4 acc[NB][2], owed[PB];
+    // A column's running maximum m (log2 units), the raw score past which it
+    // is raised, and per block the power of two 2^kd that its scales are
+    // brought up by (mm = m - kd) and the scale past which that changes.  l
+    // is the sum of this lane's weights times 2^kd of block 0.
+    float m = kPagesFloor, mt = -INFINITY, l = 0.0f;
+    float mm[PB], kd[PB];
+    uint32_t dt[PB];  // fp16 bits of the largest scale that kd allows for
+    pg_float4 acc[NB][2];
     const pg_float4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int4_t izero = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < NB; ++i) acc[i][0] = acc[i][1] = zero;
 #pragma unroll
-    for (int i = 0; i < PB; ++i) owed[i] = zero;
-    pg_bf16x8 eight;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) eight[j] = (__bf16) 8.0f;
-
-    auto settle = [&]() {
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            acc[i][0] -= owed[SPREAD ? 0 : i];
-            acc[i][1] -= owed[SPREAD ? 0 : i];
-        }
-#pragma unroll
-        for (int i = 0; i < PB; ++i) owed[i] = zero;
-    };
+    for (int i = 0; i < PB; ++i) {
+        mm[i] = kPagesFloor;
+        kd[i] = 0.0f;
+        dt[i] = 0;
+    }
+    const Patterns pat;
+    float minus_one = -1.0f;  // not known to be: a mixed fma takes it
+    asm volatile("" : "+v"(minus_one));
 
     auto word = [](const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; };
-    auto scale_of = [](const uint2 &v, int i) {
-        const uint32_t w = i < 2 ? v.x : v.y;
-        const pg_half2 h = __builtin_bit_cast(pg_half2, w);
-        return (float) (i & 1 ? h.y : h.x);
+    // x times the scale of key i of a tile, x as it is where y is 0 (one mixed
+    // fma, which takes the scale as fp16)
+    auto times_scale = [&](float x, const uint4 &v, int which, int i, float y) {
+        const pg_half2 h = __builtin_bit_cast(pg_half2, word(v, 2 * which + (i >> 1)));
+        return __builtin_fmaf(x, (float) (i & 1 ? h.y : h.x), y);
     };
 
-    auto compute = [&](int step, const Tile &t) {
-        float s[8];
+    auto compute = [&](int step, Tile &t) {
+        float s[8];  // scores, to be multiplied by sq
+        if constexpr (SPREAD) {
+            int4_t d[2][QD];
+            const int4_t start = {q8, q8, q8, q8};
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            pg_float4 d = zero;
+            for (int i = 0; i < NB / 2; ++i) {
+                int4_t kc[2];
 #pragma unroll
-            for (int blk = 0; blk < NB; ++blk) {
-                const pg_half8 kc = k_octet(word(t.k[u / T], (u % T) * NB + blk));
-                if constexpr (!SPREAD) d = zero;
-                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, qh[blk], d, 0, 0, 0);
-                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, ql[blk], d, 0, 0, 0);
-                if constexpr (!SPREAD) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) part[i] = __builtin_fmaf(d[i], scale_of(t.ks[u][blk], i), part[i]);
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t w0 = word(t.k[u / T], (u % T) * NB + 2 * i);
+                    const uint32_t w1 = word(t.k[u / T], (u % T) * NB + 2 * i + 1);
+                    kc[u] = int4_t{(int) (w0 & 0x0F0F0F0Fu), (int) ((w0 >> 4) & 0x0F0F0F0Fu), (int) (w1 & 0x0F0F0F0Fu),
+                                   (int) ((w1 >> 4) & 0x0F0F0F0Fu)};
                 }
+#pragma unroll
+                for (int k = 0; k < QD; ++k)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        d[u][k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                            kc[u], qd[k][i], i > 0 ? d[u][k] : k == 0 ? start : izero, 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float x = part[i];
-                if constexpr (SPREAD) {
-                    x = d[i] * scale_of(t.ks[u][0], i);
-                    x += pg_dpp<0xB1>(x);
-                    if constexpr (NB == 4) x += pg_dpp<0x4E>(x);
+            for (int i = 0; i < 8; ++i) {
+                const int u = i >> 2, e = i & 3;
+                int sum = d[u][QD - 1][e];
+#pragma unroll
+                for (int k = QD - 2; k >= 0; --k) sum = (sum << 8) + d[u][k][e];
+                float x = times_scale((float) sum, t.sc[u][0], 0, e, 0.0f);
+                x += pg_dpp<0xB1>(x);
+                if constexpr (NB == 4) x += pg_dpp<0x4E>(x);
+                s[i] = x;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] = 0.0f;
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk) {
+                pg_float4 d[2] = {zero, zero};
+                pg_half8 kc[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) kc[u] = k_octet(word(t.k[u / T], (u % T) * NB + blk), pat);
+#pragma unroll
+                for (int i = 0; i < QP; ++i)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        d[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[u], qp[SPREAD ? 0 : i][SPREAD ? 0 : blk], d[u], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    s[i] = times_scale(d[i >> 2][i & 3], t.sc[i >> 2][SPREAD ? 0 : blk], 0, i & 3, s[i]);
+            }
+        }
+        if (!(step * kStep >= sp.lo && step * kStep + kStep <= sp.len && t.ok == (1 << TG) - 1)) {
+            // some position is not visible: score -inf, V scale 0
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int u = i >> 2;
+                const int pos = step * kStep + u * 16 + 4 * oct + (i & 3);
+                const bool ok = pos >= sp.lo && pos < sp.len && ((t.ok >> (u / T)) & 1);
+                s[i] = ok ? s[i] : -INFINITY;
+                const uint32_t keep = ok ? 0xFFFFFFFFu : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+#pragma unroll
+                for (int j = 0; j < PB; ++j) {
+                    if ((i & 3) < 2)
+                        t.sc[u][j].z &= keep;
+                    else
+                        t.sc[u][j].w &= keep;
                 }
-                const int pos = step * kStep + u * 16 + 4 * oct + i;
-                const bool ok = pos >= sp.lo && pos < sp.len && t.ok[u / T];
-                s[4 * u + i] = ok ? x * sq : -INFINITY;
             }
         }
         float mx = s[0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i]);
-        if (__any(mx > mt)) {
+        bool raise = mx > mt;
+        uint32_t dx[PB];  // the largest scale's fp16 bits
+#pragma unroll
+        for (int j = 0; j < PB; ++j) {
+            typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+            auto mag = [](uint32_t x) { return __builtin_bit_cast(ushort2_t, x & 0x7FFF7FFFu); };
+            const ushort2_t top = __builtin_elementwise_max(
+                __builtin_elementwise_max(mag(t.sc[0][j].z), mag(t.sc[0][j].w)),
+                __builtin_elementwise_max(mag(t.sc[1][j].z), mag(t.sc[1][j].w)));
+            dx[j] = max((uint32_t) top.x, (uint32_t) top.y);
+            raise = raise || dx[j] > dt[j];
+        }
+        if (__any(raise)) {
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float m_new = fmaxf(m, mx);
-            const float alpha = __builtin_amdgcn_exp2f(m - m_new);
-            m = m_new;
-            mt = m_new + kPagesLazy;
-            l *= alpha;
+            // (a maximum that is not past its limit stays, so that lanes of
+            // one column agree whichever of them asked)
+            const float m_new = mx > mt ? fmaxf(m, mx * sq) : m;
+            float alpha[PB];
+#pragma unroll
+            for (int j = 0; j < PB; ++j) {
+                dx[j] = max(dx[j], (uint32_t) __shfl_xor((int) dx[j], 16));
+                dx[j] = max(dx[j], (uint32_t) __shfl_xor((int) dx[j], 32));
+                // weights are below 2^8 and scales below 2^(ex + 1), so that
+                // their product times 2^kd stays below 2^15
+                if (dx[j] > dt[j] || dt[j] == 0) {
+                    const float d = f16_bits_to_f32(dx[j]);
+                    const int ex = d == 0.0f ? -24 : __builtin_amdgcn_frexp_expf(d);
+                    kd[j] = (float) (6 - ex);
+                    // 2^(ex + 1), or infinity: then nothing is past it but NaN
+                    dt[j] = f32_to_f16_bits(__builtin_amdgcn_ldexpf(1.0f, ex + 1));
+                }
+                alpha[j] = __builtin_amdgcn_exp2f(mm[j] - (m_new - kd[j]));
+                mm[j] = m_new - kd[j];
+            }
+            if (mx > mt) {
+                m = m_new;
+                mt = (m_new + kPagesLazy) / sq;
+            }
+            l *= alpha[0];
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
-                acc[i][0] *= alpha;
-                acc[i][1] *= alpha;
+                acc[i][0] *= alpha[SPREAD ? 0 : i];
+                acc[i][1] *= alpha[SPREAD ? 0 : i];
             }
-#pragma unroll
-            for (int i = 0; i < PB; ++i) owed[i] *= alpha;
         }
+        // weights times 2^kd of block 0; the other blocks' come by a factor
         float w[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            w[i] = __builtin_amdgcn_exp2f(s[i] - m);
+            w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sq, -mm[0]));
             l += w[i];
         }
 #pragma unroll
         for (int j = 0; j < PB; ++j) {
-            pg_bf16x8 ph, pl;
+            const float f = j == 0 ? 1.0f : __builtin_amdgcn_exp2f(mm[0] - mm[j]);
+            // keys 0, 2, 1, 3 of each tile's quad, as the masks leave the codes
+            pg_half8 wp[WP];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float d = scale_of(t.vs[i >> 2][j], i & 3);
-                const float x = s[i] == -INFINITY ? 0.0f : w[i] * d;
-                const __bf16 h = (__bf16) x;
-                ph[i] = h;
-                pl[i] = (__bf16) (x - (float) h);
+            for (int i = 0; i < 8; i += 2) {
+                const int a0 = (i & 4) + ((i & 2) >> 1), a1 = a0 + 2;
+                float x = w[a0], y = w[a1];
+                if (j > 0) {
+                    x *= f;
+                    y *= f;
+                }
+                x = times_scale(x, t.sc[a0 >> 2][j], 1, a0 & 3, 0.0f);
+                y = times_scale(y, t.sc[a1 >> 2][j], 1, a1 & 3, 0.0f);
+                if constexpr (WP == 1) {
+                    wp[0][i] = (_Float16) x;
+                    wp[0][i + 1] = (_Float16) y;
+                } else {
+                    const pg_half2 h = __builtin_bit_cast(pg_half2, __builtin_amdgcn_cvt_pkrtz(x, y));
+                    const pg_half2 g2 = __builtin_bit_cast(
+                        pg_half2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float) h.x, minus_one, x),
+                                                             __builtin_fmaf((float) h.y, minus_one, y)));
+                    wp[0][i] = h.x;
+                    wp[0][i + 1] = h.y;
+                    wp[WP - 1][i] = g2.x;
+                    wp[WP - 1][i + 1] = g2.y;
+                }
             }
-            owed[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight, ph, owed[j], 0, 0, 0);
-            owed[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight, pl, owed[j], 0, 0, 0);
 #pragma unroll
             for (int blk = 0; blk < NB; ++blk) {
                 if (!SPREAD && blk != j) continue;
-                const uint32_t x0 = word(t.v[0], blk);
-                const uint32_t x1 = word(t.v[1 / T], (1 % T) * NB + blk);
-                const pg_bf16x8 vl = v_octet(x0, x1), vh = v_octet(x0 >> 4, x1 >> 4);
-                acc[blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vl, ph, acc[blk][0], 0, 0, 0);
-                acc[blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vl, pl, acc[blk][0], 0, 0, 0);
-                acc[blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh, ph, acc[blk][1], 0, 0, 0);
-                acc[blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh, pl, acc[blk][1], 0, 0, 0);
+                const uint32_t x0 = word(t.v[0], blk), y0 = x0 >> 8;
+                const uint32_t x1 = word(t.v[1 / T], (1 % T) * NB + blk), y1 = x1 >> 8;
+                const pg_half2 a = codes_lo(x0, pat), b2 = codes_lo(y0, pat), c = codes_lo(x1, pat), d2 = codes_lo(y1, pat);
+                const pg_half8 vl = {a.x, a.y, b2.x, b2.y, c.x, c.y, d2.x, d2.y};
+                const pg_half2 e = codes_hi(x0, pat), f2 = codes_hi(y0, pat), h = codes_hi(x1, pat), i2 = codes_hi(y1, pat);
+                const pg_half8 vh = {e.x, e.y, f2.x, f2.y, h.x, h.y, i2.x, i2.y};
+#pragma unroll
+                for (int k = 0; k < WP; ++k) {
+                    acc[blk][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, wp[k], acc[blk][0], 0, 0, 0);
+                    acc[blk][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, wp[k], acc[blk][1], 0, 0, 0);
+                }
             }
         }
     };
 
-    // Steps s_begin + wave, + NW, ...; the next step's loads are in flight
-    // while one is computed.
-    int step = s_begin + wave;
-    if (step < s_end) {
-        Tile t0, t1;
-        load(step, t0);
-        int settle_in = kSettle;
-        for (;;) {
-            load(min(step + NW, s_end - 1), t1);
-            compute(step, t0);
-            if ((step += NW) >= s_end) break;
-            load(min(step + NW, s_end - 1), t0);
-            compute(step, t1);
-            if ((step += NW) >= s_end) break;
-            if ((settle_in -= 2) <= 0) {
-                settle();
-                settle_in = kSettle;
-            }
+    // Steps first, first + NW, ...: at the top of a pass buf[u] holds the u-th
+    // next step, u < BUF - 1, and ids[BUF - 1] the pages of the one after.
+    const int n_steps = (s_end - first + NW - 1) / NW;
+    int i = 0;
+    for (; i + BUF <= n_steps; i += BUF) {
+#pragma unroll
+        for (int u = 0; u < BUF; ++u) {
+            load(min(first + (i + u + BUF - 1) * NW, last), ids[BUF - 1], buf[(u + BUF - 1) % BUF]);
+            ids_of(min(first + (i + u + BUF) * NW, last), ids[BUF - 1]);
+            compute(first + (i + u) * NW, buf[u]);
         }
     }
-    settle();
+#pragma unroll
+    for (int u = 0; u < BUF - 1; ++u)
+        if (i + u < n_steps) compute(first + (i + u) * NW, buf[u]);
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
 
@@ -427,70 +532,91 @@ __global__ __launch_bounds__(64 * kDecodeWaves) void pages_decode_kernel(DecodeA
                 *reinterpret_cast<pg_float4 *>(&s_out[wave][r][blk * kQK + half * 16 + 4 * oct]) = acc[blk][half];
         }
     }
-    if (oct == 0 && cb == 0) {
-        s_m[wave][r] = m;
-        s_l[wave][r] = l;
+    if (oct == 0) {
+#pragma unroll
+        for (int j = 0; j < PB; ++j) {
+            s_m[wave][r][SPREAD ? cb : j] = mm[j];
+            s_l[wave][r][SPREAD ? cb : j] = j == 0 ? l : l * __builtin_amdgcn_exp2f(mm[0] - mm[j]);
+        }
     }
     __syncthreads();
-    const int part = it.part0 + it.run;
     for (int i = threadIdx.x; i < heads * D; i += 64 * NW) {
-        const int rr = i / D, e = i % D;
-        float M = s_m[0][rr];
+        const int rr = i / D, e = i % D, blk = e / kQK;
+        float M = s_m[0][rr][blk];
 #pragma unroll
-        for (int w = 1; w < NW; ++w) M = fmaxf(M, s_m[w][rr]);
+        for (int w = 1; w < NW; ++w) M = fmaxf(M, s_m[w][rr][blk]);
         float L = 0.0f, o = 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-            const float f = __builtin_amdgcn_exp2f(s_m[w][rr] - M);
-            L = __builtin_fmaf(f, s_l[w][rr], L);
+            const float f = __builtin_amdgcn_exp2f(s_m[w][rr][blk] - M);
+            L = __builtin_fmaf(f, s_l[w][rr][blk], L);
             o = __builtin_fmaf(f, s_out[w][rr][e], o);
         }
-        if (it.runs == 1) {
+        if (sp.runs == 1) {
             const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-            store1(p.out, ((int64_t) b * p.n_heads + head0 + rr) * D + e, o * inv, p.type);
+            store1(p.out, ((int64_t) b * p.n_heads + head0 + rr) * D + e, o * inv, type);
         } else {
-            float *dst = p.work + ((int64_t) part * a.units + it.unit) * part_floats<D>(HC);
+            float *dst = p.work + (int64_t) blockIdx.x * part_floats<D>(HC);
             dst[rr * D + e] = o;
-            if (e == 0) {
-                dst[HC * D + rr] = M;
-                dst[HC * D + HC + rr] = L;
+            if (e % kQK == 0) {
+                dst[HC * D + rr * NB + blk] = M;
+                dst[HC * (D + NB) + rr * NB + blk] = L;
             }
         }
     }
 }
 
-// Joins the runs of the entries that were cut, in order: a workgroup of D
-// threads takes one (entry, query head).
+// Joins the runs of the entries that were cut: a workgroup takes one (entry,
+// query head), its waves every fourth run.
 template <int D, bool SPREAD>
-__global__ __launch_bounds__(D) void pages_join_kernel(DecodeArgs a) {
+__global__ __launch_bounds__(256) void pages_join_kernel(DecodeArgs a) {
     constexpr int HC = SPREAD ? 16 / (D / kQK) : 16;
+    constexpr int NB = D / kQK, E = D / 64, NW = 4;
     const PagesDecodeParams &p = a.p;
-    const int lane = threadIdx.x & 63;
+    __shared__ float s_w[kMaxRuns][NB];
+    __shared__ float s_o[NW][D];
     const int b = (int) blockIdx.x / p.n_heads, h = (int) blockIdx.x - b * p.n_heads;
-    const int c = run_length(a, lane);
-    const int runs = runs_of(span_of(a, p.lens[b]).n, c);
+    const int runs = span_of(a, uniform_int(p.lens, b)).runs;
     if (runs == 1) return;
-    int part0 = 0;
-    for (int b0 = 0; b0 < b; b0 += 64) {
-        const int i = b0 + lane;
-        const int n = i < b ? runs_of(span_of(a, p.lens[i]).n, c) : 0;
-        part0 += __shfl(wave_prefix(n > 1 ? n : 0, lane), 63);
-    }
     const int kvh = h / a.group, in_group = h - kvh * a.group;
     const int hs = in_group / HC, rr = in_group - hs * HC;
-    const int64_t stride = (int64_t) a.units * part_floats<D>(HC);
-    const float *src = p.work + ((int64_t) part0 * a.units + kvh * a.n_hs + hs) * part_floats<D>(HC);
-    float M = kPagesFloor;
-    for (int i = 0; i < runs; ++i) M = fmaxf(M, src[i * stride + HC * D + rr]);
-    float L = 0.0f, o = 0.0f;
-    for (int i = 0; i < runs; ++i) {
-        const float *q = src + i * stride;
-        const float f = __builtin_amdgcn_exp2f(q[HC * D + rr] - M);
-        L = __builtin_fmaf(f, q[HC * D + HC + rr], L);
-        o = __builtin_fmaf(f, q[rr * D + threadIdx.x], o);
+    const int64_t stride = (int64_t) p.n_batch * a.units * part_floats<D>(HC);
+    const float *src = p.work + ((int64_t) b * a.units + kvh * a.n_hs + hs) * part_floats<D>(HC);
+    const int lane = threadIdx.x & 63, wave = (int) threadIdx.x >> 6;
+    // lane e has elements e, e + 64 of the head, of blocks e / 32, + 2
+    float o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.0f;
+    // block `wave`: every run's share of the whole, a run a lane
+    if (wave < NB) {
+        const float *q = src + HC * D + rr * NB + wave;
+        float M = kPagesFloor, L = 0.0f;
+        for (int i = lane; i < runs; i += 64) M = fmaxf(M, q[i * stride]);
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
+        for (int i = lane; i < runs; i += 64) {
+            const float f = __builtin_amdgcn_exp2f(q[i * stride] - M);
+            s_w[i][wave] = f;
+            L = __builtin_fmaf(f, q[i * stride + HC * NB], L);
+        }
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) L += __shfl_xor(L, d);
+        const float inv = L > 0.0f ? 1.0f / L : L * 0.0f;  // (NaN stays)
+        for (int i = lane; i < runs; i += 64) s_w[i][wave] *= inv;
     }
-    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-    store1(p.out, ((int64_t) b * p.n_heads + h) * D + threadIdx.x, o * inv, p.type);
+    __syncthreads();
+#pragma unroll 8
+    for (int i = wave; i < runs; i += NW)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            o[e] = __builtin_fmaf(s_w[i][2 * e + lane / kQK], src[i * stride + rr * D + e * 64 + lane], o[e]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) s_o[wave][e * 64 + lane] = o[e];
+    __syncthreads();
+    if (threadIdx.x < D) {
+        const int e = threadIdx.x;
+        store1(p.out, ((int64_t) b * p.n_heads + h) * D + e, (s_o[0][e] + s_o[1][e]) + (s_o[2][e] + s_o[3][e]), p.type);
+    }
 }
 
 namespace {
@@ -499,28 +625,44 @@ namespace {
 bool spread(const PagesGeom &g, int group) { return group <= 16 / (g.dim / kQK); }
 int set_heads(const PagesGeom &g, int group) { return spread(g, group) ? 16 / (g.dim / kQK) : 16; }
 
+template <int D, bool SPREAD, int NW>
+const void *kernel_of(int type) {
+    return type == kTypeF32 ? reinterpret_cast<const void *>(pages_decode_kernel<D, SPREAD, NW, true>)
+                            : reinterpret_cast<const void *>(pages_decode_kernel<D, SPREAD, NW, false>);
+}
+
 template <int D, bool SPREAD>
-hipError_t launch_of(const DecodeArgs &arg, int64_t items, hipStream_t stream) {
+hipError_t launch_of(const DecodeArgs &arg, int nw, int64_t items, hipStream_t stream) {
     DecodeArgs a = arg;
     void *args[] = {&a};
-    hipError_t e = hipLaunchKernel(reinterpret_cast<const void *>(pages_decode_kernel<D, SPREAD>),
-                                   dim3((unsigned) items), dim3(64 * kDecodeWaves), args, 0, stream);
-    if (e == hipSuccess && a.split)
+    const void *kernel = nw == 1 ? kernel_of<D, SPREAD, 1>(a.p.type) : kernel_of<D, SPREAD, kWaves>(a.p.type);
+    hipError_t e = hipLaunchKernel(kernel, dim3((unsigned) items), dim3(64 * nw), args, 0, stream);
+    if (e == hipSuccess && a.max_runs > 1)
         e = hipLaunchKernel(reinterpret_cast<const void *>(pages_join_kernel<D, SPREAD>),
-                            dim3((unsigned) (a.p.n_batch * a.p.n_heads)), dim3(D), args, 0, stream);
+                            dim3((unsigned) (a.p.n_batch * a.p.n_heads)), dim3(256), args, 0, stream);
     return e;
 }
 
 }  // namespace
 
-// Entries that are cut have n > c steps in ceil(n / c) < 2 n / c runs, and
-// c >= units * sum n / kWantWorkgroups, so a launch has fewer than
-// 2 * kWantWorkgroups partial results.
+// Head sets of 16 heads have four times as long results as the others, and the
+// launch a quarter of the units: a quarter of the workgroups may be cut off.
+static int split_workgroups(const PagesGeom &g, int group) { return kSplitWaves / kWaves / (spread(g, group) ? 1 : 4); }
+
 int64_t pages_work_bytes(const PagesGeom &g, int n_heads) {
-    const int hc = set_heads(g, n_heads / g.n_kv);
-    return (int64_t) 2 * kWantWorkgroups * hc * (g.dim + 2) * 4;
+    const int group = n_heads / g.n_kv, hc = set_heads(g, group);
+    return (int64_t) split_workgroups(g, group) * hc * (g.dim + 2 * (g.dim / kQK)) * 4;
 }
 
+// Shape of a launch, from its units and the steps that its longest entry can
+// have.  us a launch in a graph, dim 128, fp32, 32 heads:
+//   one wave a unit or four:  2048 units x 16 steps 27.9 / 31.2, 8192 x 7
+//     48 / 68, 1024 x 16 18.2 / 18.7; 2048 x 32 53.9 / 54.9, x 63 100 / 97,
+//     of 3 to 63 steps 77 / 60 (a long unit's one wave is the last to end).
+//   runs of at least 4 steps a wave, of 16, or nothing cut:  32 units x 94
+//     steps 11.2 / 21.6 / 21.6, x 250 14.5 / 16.8 / 49, 8 x 1000 17.7 / 18.7 /
+//     184; 256 x 32 13.7 / 10.7 / 10.7, 512 x 32 21.5 / 16.3 / 16.2; 96 units
+//     of 62 to 1000 steps 56 / 54 / 183.
 hipError_t launch_pages_decode(const PagesDecodeParams &p, hipStream_t stream) {
     DecodeArgs a{};
     a.p = p;
@@ -529,15 +671,26 @@ hipError_t launch_pages_decode(const PagesDecodeParams &p, hipStream_t stream) {
     a.n_hs = (a.group + hc - 1) / hc;
     a.units = p.g.n_kv * a.n_hs;
     a.append = p.k_new != nullptr;
+    a.max_runs = 1;
+    const int64_t units = (int64_t) p.n_batch * a.units;
     int64_t longest = (int64_t) p.max_pages << p.g.page_shift;
     if (p.max_len > 0 && p.max_len < longest) longest = p.max_len;
     if (p.window > 0 && p.window + kStep < longest) longest = p.window + kStep;
     const int64_t steps = (longest + kStep - 1) / kStep;
-    a.split = steps > kMinRun && p.work && p.work_bytes >= pages_work_bytes(p.g, p.n_heads);
-    const int64_t items = (int64_t) p.n_batch * a.units + (a.split ? 2 * kWantWorkgroups : 0);
+    const int nw = units >= 1024 && steps <= 24 ? 1 : kWaves;
+    if (nw == kWaves && p.work && p.work_bytes >= pages_work_bytes(p.g, p.n_heads)) {
+        const int64_t fill = std::min<int64_t>(kFillWaves / kWaves / units, steps / (kFillSteps * kWaves));
+        const int64_t split = std::min<int64_t>(split_workgroups(p.g, a.group) / units, steps / (kSplitSteps * kWaves));
+        const int64_t runs = std::min<int64_t>(std::max(fill, split), kMaxRuns);
+        if (runs > 1) {
+            a.max_runs = (int) runs;
+            a.run = (int) ((steps + runs - 1) / runs);
+        }
+    }
+    const int64_t items = units * a.max_runs;
     if (p.g.dim == 128)
-        return spread(p.g, a.group) ? launch_of<128, true>(a, items, stream) : launch_of<128, false>(a, items, stream);
-    return spread(p.g, a.group) ? launch_of<64, true>(a, items, stream) : launch_of<64, false>(a, items, stream);
+        return spread(p.g, a.group) ? launch_of<128, true>(a, nw, items, stream) : launch_of<128, false>(a, nw, items, stream);
+    return spread(p.g, a.group) ? launch_of<64, true>(a, nw, items, stream) : launch_of<64, false>(a, nw, items, stream);
 }
 
 }  // namespace bmo

@@ -25,33 +25,47 @@ __host__ __device__ constexpr int octet_elem(int c, int r) {
     return 4 * c + (r & 4 ? 16 : 0) + (r & 1 ? 2 : 0) + ((r >> 1) & 1);
 }
 
-// The codes of dword w (bytes 4c..4c+3 of a block) minus 8 as 8 fp16 values,
-// exactly, in octet_elem order.  A low nibble n under the fp16 pattern 0x6400
-// reads 1024 + n; a high nibble in place (16 n) under 0x5400 reads 64 + n.
-__device__ __forceinline__ pg_half8 k_octet(uint32_t w) {
-    const pg_half2 lo = {(_Float16) -1032.0f, (_Float16) -1032.0f};
-    const pg_half2 hi = {(_Float16) -72.0f, (_Float16) -72.0f};
+// Patterns under which a 4-bit code reads as fp16: a low nibble n under 0x6400
+// is 1024 + n, a nibble in place (16 n) under 0x5400 is 64 + n.  Kept in vector
+// registers, so that and-or is one instruction (it takes one scalar operand).
+struct Patterns {
+    uint32_t lo = 0x64006400u, hi = 0x54005400u;
+    __device__ __forceinline__ Patterns() { asm volatile("" : "+v"(lo), "+v"(hi)); }
+};
+// Codes minus 8, exactly, of the low (high) nibbles of bytes 0 and 2 of x.
+__device__ __forceinline__ pg_half2 codes_lo(uint32_t x, const Patterns &c) {
+    const pg_half2 off = {(_Float16) -1032.0f, (_Float16) -1032.0f};
+    return __builtin_bit_cast(pg_half2, (x & 0x000F000Fu) | c.lo) + off;
+}
+__device__ __forceinline__ pg_half2 codes_hi(uint32_t x, const Patterns &c) {
+    const pg_half2 off = {(_Float16) -72.0f, (_Float16) -72.0f};
+    return __builtin_bit_cast(pg_half2, (x & 0x00F000F0u) | c.hi) + off;
+}
+
+// The codes of dword w (bytes 4c..4c+3 of a block) minus 8 as 8 fp16 values
+// in octet_elem order.
+__device__ __forceinline__ pg_half8 k_octet(uint32_t w, const Patterns &p) {
     const uint32_t y = w >> 8;
-    const pg_half2 a = __builtin_bit_cast(pg_half2, (w & 0x000F000Fu) | 0x64006400u) + lo;
-    const pg_half2 b = __builtin_bit_cast(pg_half2, (y & 0x000F000Fu) | 0x64006400u) + lo;
-    const pg_half2 c = __builtin_bit_cast(pg_half2, (w & 0x00F000F0u) | 0x54005400u) + hi;
-    const pg_half2 d = __builtin_bit_cast(pg_half2, (y & 0x00F000F0u) | 0x54005400u) + hi;
+    const pg_half2 a = codes_lo(w, p), b = codes_lo(y, p), c = codes_hi(w, p), d = codes_hi(y, p);
     return pg_half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
-// Four 4-bit codes, one a byte, as bf16: the byte n (0..15) read as fp8 e4m3
-// is n * 2^-9 (its subnormals run on into the first exponent), which the
-// conversion scales back to n exactly.
-__device__ __forceinline__ void v_quad(uint32_t nibbles, pg_bf16x2 &a, pg_bf16x2 &b) {
-    a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(nibbles, 512.0f, false);
-    b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(nibbles, 512.0f, true);
+template <bool B>
+struct Flag {
+    static constexpr bool value = B;
+};
+
+// p[i] at a wave-uniform index through the scalar cache, for arrays that no
+// kernel writes while the reading one runs (lengths, tables).
+__device__ __forceinline__ int uniform_int(const int *p, int i) {
+    return ((const __attribute__((address_space(4))) int *) p)[i];
 }
-// Eight keys' codes of one V column: nibbles of two tiles' dwords.
-__device__ __forceinline__ pg_bf16x8 v_octet(uint32_t x0, uint32_t x1) {
-    pg_bf16x2 a, b, c, d;
-    v_quad(x0 & 0x0F0F0F0Fu, a, b);
-    v_quad(x1 & 0x0F0F0F0Fu, c, d);
-    return pg_bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+
+// 16 bytes that a launch reads once.
+__device__ __forceinline__ uint4 stream16(const uint8_t *p) {
+    typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
+    return make_uint4(v.x, v.y, v.z, v.w);
 }
 
 template <int CTRL>
@@ -73,16 +87,19 @@ __device__ __forceinline__ int wave_prefix(int v, int lane) {
 __device__ __forceinline__ pg_float4 load4(const void *p, int64_t i, int type) {
     if (type == kTypeF32) return *reinterpret_cast<const pg_float4 *>(static_cast<const float *>(p) + i);
     const uint2 u = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + i);
-    if (type == kTypeF16)
-        return pg_float4{f16_bits_to_f32(u.x & 0xFFFFu), f16_bits_to_f32(u.x >> 16), f16_bits_to_f32(u.y & 0xFFFFu),
-                         f16_bits_to_f32(u.y >> 16)};
-    return pg_float4{__builtin_bit_cast(float, u.x << 16), __builtin_bit_cast(float, u.x & 0xFFFF0000u),
-                     __builtin_bit_cast(float, u.y << 16), __builtin_bit_cast(float, u.y & 0xFFFF0000u)};
+    const bool f16 = type == kTypeF16;  // (both conversions, so that no branch waits for the load)
+    pg_float4 v;
+    v[0] = f16 ? f16_bits_to_f32(u.x & 0xFFFFu) : __builtin_bit_cast(float, u.x << 16);
+    v[1] = f16 ? f16_bits_to_f32(u.x >> 16) : __builtin_bit_cast(float, u.x & 0xFFFF0000u);
+    v[2] = f16 ? f16_bits_to_f32(u.y & 0xFFFFu) : __builtin_bit_cast(float, u.y << 16);
+    v[3] = f16 ? f16_bits_to_f32(u.y >> 16) : __builtin_bit_cast(float, u.y & 0xFFFF0000u);
+    return v;
 }
 __device__ __forceinline__ float load1(const void *p, int64_t i, int type) {
     if (type == kTypeF32) return static_cast<const float *>(p)[i];
     const uint32_t u = static_cast<const uint16_t *>(p)[i];
-    return type == kTypeF16 ? f16_bits_to_f32(u) : __builtin_bit_cast(float, u << 16);
+    const float h = f16_bits_to_f32(u), b = __builtin_bit_cast(float, u << 16);
+    return type == kTypeF16 ? h : b;
 }
 // One value of TYPE, rounded to nearest even.
 __device__ __forceinline__ void store1(void *p, int64_t i, float x, int type) {

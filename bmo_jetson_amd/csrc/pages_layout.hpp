@@ -11,8 +11,9 @@
 //                 4c .. 4c+3 of ggml's block b of key t * 16 + key;
 //   [1024, 2048)  V codes: byte j of dword ((c * 16 + i) * 4 + t * NB + b) is
 //                 byte i of block b of key t * 16 + 4 c + j;
-//   [2048, 2176)  K scales, fp16, at (t * NB + b) * 16 + key;
-//   [2176, 2304)  V scales, the same.
+//   [2048, 2304)  scales, fp16: 16 bytes at ((t * NB + b) * 4 + c) * 16 are
+//                 those of block b of keys t * 16 + 4 c + 0 .. 3, K's four
+//                 and then V's four.
 //
 // So the 16 bytes at lane * 16 of either code region are what lane c * 16 + i
 // of v_mfma_f32_16x16x32 takes of the group: K rows with 8 elements of each
@@ -29,8 +30,11 @@
 
 namespace bmo {
 
-constexpr int kPageScaleK = 2048;
-constexpr int kPageScaleV = 2176;
+// Byte offset in a group of the scale of block tb = t * NB + b of key `key`
+// of its tile, of K (which 0) or V (which 1).
+__host__ __device__ constexpr int page_scale_offset(int tb, int key, int which) {
+    return kScaleOff + (tb * 4 + (key >> 2)) * 16 + which * 8 + (key & 3) * 2;
+}
 
 struct PagesGeom {
     int n_layers;

@@ -535,8 +535,8 @@ BMO_ATTN_API int64_t bmo_kv_pages_workspace_bytes(const bmo_kv_pages_t *pages, i
  * h / (n_heads / n_kv_heads).  scale <= 0: 1/sqrt(head_dim).  An entry
  * without positions gets zeros.  max_len: no entry is longer (0: not known);
  * it only chooses how the call is cut.  fp32 results are as close as fp32
- * arithmetic; the result does not depend on the other entries' rows, but how
- * the entries' lengths together cut an entry decides its rounding. */
+ * arithmetic.  An entry's result depends on no other entry's; its rounding
+ * depends on how it is cut (n_batch, max_len, the table's width). */
 BMO_ATTN_API int bmo_kv_pages_decode(bmo_kv_pages_t *pages, int layer, int n_batch,
                                      const int *lens, const int *table, int max_pages,
                                      int n_heads, int type, const void *q, int64_t q_stride,

@@ -2,12 +2,13 @@
 
 Bounds (per output, from the kernels' arithmetic):
 
-decode   a weight enters as two bf16 parts (2^-17 of itself), codes 0..15 are
-         exact, sums are fp32 (a few dozen roundings of 2^-24 of at most
-         15 sum p|d|): 2^-16 * 16 sum p|d| in all; a score is off by at most
-         2^-21 max|q| sum|k| (the query's two fp16 parts of 2^-22 of the row's
-         largest, and its scaling) in log2 units, which moves a weight and the
-         sum by ln 2 of that each.
+decode   fp32: a weight enters as two truncated fp16 parts (2^-21 of itself),
+         codes are exact, sums are fp32 (some hundred roundings of 2^-24 of at
+         most 8 sum p|d|): 2^-16 * 16 sum p|d| covers both; a score is off by at
+         most 2^-21 max|q| sum|k| (half a step of the query's 22 bits, the step
+         being at most 2^-20 of the row's largest) in log2 units, which moves a
+         weight and the sum by ln 2 of that each.  16 bits: a weight rounds to
+         fp16, 2^-11 of sum p|v|, and the query has 15 bits, 2^-14 there.
 attend   V and the weights round to fp16 (2^-11 each; a weight below 2^-14 is
          off by 2^-25 of the largest instead), K too, which moves a score by
          2^-11 sum|q k|, a weight and the sum by ln 2 of that each.
@@ -77,8 +78,9 @@ def attention(cache, table_row, page, length, q, last, window, kind, type_, scal
             o = p @ v
             out[i, h] = o
             if kind == "decode":
-                off = 2.0**-21 * np.abs(q[i, h]).max() * np.abs(k).sum(axis=1).max() * scale / LN2
-                b = (2.0**-16 + 2 * LN2 * off) * 16 * (p @ d)
+                full = type_ == "float32"
+                off = 2.0**(-21 if full else -14) * np.abs(q[i, h]).max() * np.abs(k).sum(axis=1).max() * scale / LN2
+                b = 2.0**-16 * 16 * (p @ d) + (2 * LN2 * off + (0 if full else 2.0**-11)) * (p @ np.abs(v))
             else:
                 off = 2.0**-11 * (np.abs(k) @ np.abs(q[i, h])).max() * scale / LN2
                 b = (2 * 2.0**-11 + 2 * LN2 * off) * (p @ np.abs(v)) + 2.0**-25 * np.abs(v).sum(axis=0)

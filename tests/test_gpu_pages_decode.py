@@ -214,9 +214,9 @@ def test_two_graphs_with_their_own_workspaces(gpu):
         gpu.cuda.current_stream().wait_stream(side)
         eager = gpu.zeros_like(q)
         call(eager, _work(gpu, pages, heads))
-        calls.append((graph, out, eager, q, call, pages))
+        calls.append((graph, out, eager, q, call, pages, work))  # (a graph keeps no tensor alive)
     for step in range(5):
-        for graph, out, eager, q, call, pages in calls:
+        for graph, out, eager, q, call, pages, _ in calls:
             q.mul_(1.1)
             call(eager, None if step == 3 else _work(gpu, pages, q.shape[1]))
             graph.replay()
@@ -226,7 +226,7 @@ def test_two_graphs_with_their_own_workspaces(gpu):
             else:
                 assert gpu.equal(out, eager)
     for c in calls:
-        c[-1].close()
+        c[5].close()
 
 
 def test_refusals(gpu):
