@@ -73,8 +73,15 @@ struct PagesDecodeParams {
     int max_len;   // no entry is longer (0: not known); what is longer is still read
     float *work;   // partial results, nullable
     int64_t work_bytes;
+    // several rows an entry (launch_pages_few_rows), see PagesAttendParams
+    const int *q_start;
+    int n_rows;
+    int causal;
+    int max_rows;
 };
 hipError_t launch_pages_decode(const PagesDecodeParams &p, hipStream_t stream);
+// Ragged rows, no more than max_rows an entry, in 16 bits, by the same kernel.
+hipError_t launch_pages_few_rows(const PagesDecodeParams &p, hipStream_t stream);
 // Bytes of partial results that a split launch of n_heads query heads needs.
 int64_t pages_work_bytes(const PagesGeom &g, int n_heads);
 

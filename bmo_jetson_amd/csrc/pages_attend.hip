@@ -9,22 +9,34 @@
 // A workgroup of four waves takes 128 rows of one (entry, kv head), 32 a wave.
 // A row is a (token, query head of the kv head's group), heads fastest, so
 // that grouped queries fill a tile from few tokens.  Positions pass in stages
-// of 64: each wave loads its groups of the next stage while the present one is
-// multiplied, then dequantizes them into the other of two LDS buffers, K as
+// of 64: the waves load the groups of the next stage while the present one is
+// multiplied, then dequantize them into the other of two LDS buffers, K as
 // [key][element] and V as [element][key] (pages_layout.hpp gives four keys of
 // a V column to a lane, so nothing is transposed); one barrier a stage.
 // S^T = K Q^T with v_mfma_f32_32x32x16_f16 leaves 8 + 8 keys of one row in a
 // lane, which is the operand of the next product, O^T = V^T P^T, once V's
-// keys stand in the same order: the weights never leave the registers.
+// keys stand in the same order: the weights never leave the registers.  Both
+// products read their LDS operands eight matrix instructions ahead.
 // Row padding: K rows 16 bytes and V rows 16 bytes longer than their data, so
 // that 16 lanes reading 16 bytes each from consecutive rows meet every LDS
 // bank once.
+//
+// Measured, 32 query heads on 8 of 128: eight chunks of 200 to 1024 rows over
+// 300 to 4000 positions 321 us, 763 TFLOP/s; of 1024 rows over 4096 positions
+// each about 840 (a large library product reaches 1173).  Bound by issue:
+// of a SIMD's cycles 52% are VALU (exponentials, dequantizing, masks) and 37%
+// matrix instructions, two waves a SIMD.  Eight waves a workgroup (half the
+// dequantizing a row) win 4% with full tiles of one length and lose 10% with
+// ragged ones; stages of 32 with three waves a SIMD are 16% slower, scores one
+// stage ahead of the weights 5%.
 //
 // Precision: K and V enter as (code - 8) * d rounded to fp16, the weights as
 // fp16, sums in fp32; q enters scaled by its row's own power of two, exactly.
 // That is below the rounding of the 16-bit outputs (2e-4 against 2e-3 for
 // bf16).  K and V must lie in fp16's range; a V block whose scale is not
 // finite makes the rows that see it NaN in that block and leaves the others.
+#include <algorithm>
+
 #include "kernels.hpp"
 #include "pages_device.hpp"
 
@@ -46,7 +58,7 @@ struct AttendArgs {
     FastDiv div_group;
 };
 
-// The entry and first row of tile `tile`; false past the last.
+// The entry and first row of tile `tile` of `size` rows; false past the last.
 struct RowTile {
     int b, row0, rows;  // row0 and rows count (token, head) pairs
 };
@@ -54,23 +66,35 @@ __device__ __forceinline__ int entry_rows(const AttendArgs &a, int b) {
     const int s = a.p.q_start[b], e = a.p.q_start[b + 1];
     return s < 0 || e < s || e > a.p.n_rows ? 0 : e - s;
 }
-__device__ __forceinline__ bool find_tile(const AttendArgs &a, int tile, int lane, RowTile &t) {
+// Tiles of up to 64 entries come longest entry first, and an entry's from its
+// last rows on: the workgroups that run longest start first.
+__device__ __forceinline__ bool find_tile(const AttendArgs &a, int tile, int size, int lane, RowTile &t) {
     int before = 0;
     for (int b0 = 0; b0 < a.p.n_batch; b0 += 64) {
-        const int b = b0 + lane;
-        const int rows = b < a.p.n_batch ? entry_rows(a, b) * a.group : 0;
-        const int tiles = (rows + kTileRows - 1) / kTileRows;
+        int b = b0 + lane;
+        int rows = b < a.p.n_batch ? entry_rows(a, b) * a.group : 0;
+        if (a.p.n_batch <= 64) {
+            const int key = rows > 0 ? max(a.p.lens[b], 0) : -1;
+            int rank = 0;
+            for (int j = 0; j < 64; ++j) {
+                const int other = __builtin_amdgcn_readlane(key, j);
+                rank += other > key || (other == key && j < lane) ? 1 : 0;
+            }
+            b = __builtin_amdgcn_ds_permute(rank * 4, b);
+            rows = __builtin_amdgcn_ds_permute(rank * 4, rows);
+        }
+        const int tiles = (rows + size - 1) / size;
         const int upto = wave_prefix(tiles, lane) + before;
         const uint64_t past = __ballot(upto > tile);
         if (past) {
             const int l = __ffsll((unsigned long long) past) - 1;
-            t.b = b0 + l;
-            t.rows = __shfl(rows, l);
-            t.row0 = (tile - (__shfl(upto, l) - __shfl(tiles, l))) * kTileRows;
+            t.b = __builtin_amdgcn_readlane(b, l);
+            t.rows = __builtin_amdgcn_readlane(rows, l);
+            t.row0 = (__builtin_amdgcn_readlane(upto, l) - 1 - tile) * size;
             // (always so, unless q_start is no running sum)
-            return (unsigned) t.row0 < (unsigned) t.rows;
+            return t.b < a.p.n_batch && (unsigned) t.row0 < (unsigned) t.rows;
         }
-        before = __shfl(upto, 63);
+        before = __builtin_amdgcn_readlane(upto, 63);
     }
     return false;
 }
@@ -80,20 +104,22 @@ __device__ __forceinline__ bool finite16(uint32_t h) { return (h & 0x7C00u) != 0
 }  // namespace
 
 template <int D>
-__global__ __launch_bounds__(64 * kAttendWaves, 2) void pages_attend_kernel(AttendArgs a) {
+__global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_eu(2))) void pages_attend_kernel(AttendArgs a) {
     constexpr int NW = kAttendWaves;
     constexpr int NB = D / kQK;
-    constexpr int G = 2048 / D;           // keys a group
-    constexpr int NG = kStage / G;        // groups a stage
-    constexpr int KROW = D + 8;           // halves of a K row
-    constexpr int VROW = kStage + 8;      // halves of a V row
-    constexpr int KK = D / 16;            // products of 16 elements a key
+    constexpr int G = 2048 / D;            // keys a group
+    constexpr int NG = kStage / G;         // groups a stage
+    constexpr int KROW = D + 8;            // halves of a K row
+    constexpr int VROW = kStage + 8;       // halves of a V row
+    constexpr int KK = D / 16;             // products of 16 elements a key
+    constexpr int WPG = NW / NG;           // waves that fill a group
+    static_assert(WPG == 1 || WPG == 2, "every wave fills, all groups are filled");
     const PagesAttendParams &p = a.p;
     const PagesGeom &g = p.g;
 
     __shared__ __align__(16) _Float16 s_k[2][kStage * KROW];
     __shared__ __align__(16) _Float16 s_v[2][D * VROW];
-    __shared__ int s_flag[2][NG];  // nonzero: a bad page, or a V scale that is not finite
+    __shared__ int s_flag[2][NW];  // nonzero: a bad page, or a V scale that is not finite
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
@@ -102,12 +128,12 @@ __global__ __launch_bounds__(64 * kAttendWaves, 2) void pages_attend_kernel(Atte
     const int tile = (int) blockIdx.x / g.n_kv;
     const int kvh = (int) blockIdx.x - tile * g.n_kv;
     RowTile rt;
-    if (!find_tile(a, tile, lane, rt)) return;
-    const int b = __builtin_amdgcn_readfirstlane(rt.b);
+    if (!find_tile(a, tile, kTileRows, lane, rt)) return;
+    const int b = rt.b;
     const int start = p.q_start[b];
     const int n_tok = entry_rows(a, b);
     const int64_t room = (int64_t) p.max_pages << g.page_shift;
-    const int len = (int) min((int64_t) max(p.lens[b], 0), room);
+    const int len = (int) min((int64_t) max(uniform_int(p.lens, b), 0), room);
     const int *table = p.table + (int64_t) b * p.max_pages;
 
     // This lane's row, and the positions [lo, hi) it sees.
@@ -133,6 +159,100 @@ __global__ __launch_bounds__(64 * kAttendWaves, 2) void pages_attend_kernel(Atte
     const int w_hi_min = max(last_of(w_tok0) + 1, 0), w_hi_max = max(last_of(w_tok1) + 1, 0);
     const int w_lo_min = low_of(w_tok0), w_lo_max = low_of(w_tok1);
 
+    // ---- filling: WPG waves take a group of a stage, alone K and V, two one each ----
+    constexpr int TB = 4;  // (tile, block) pairs of a group
+    const int my_group = wave / WPG;
+    const bool do_k = WPG == 1 || wave % WPG == 0;
+    const bool do_v = WPG == 1 || !do_k;
+    const int key16 = lane & 15, oct = lane >> 4;
+    const Patterns pat;
+    uint32_t kw[TB], vw[TB], kd[TB];
+    uint2 vd[TB];
+    int flag = 0;
+    const int last_group = max((len - 1) / G, 0);
+    auto id_of = [&](int stage) { return uniform_int(table, min(stage * NG + my_group, last_group) >> g.group_shift); };
+    auto fetch = [&](int stage, int id) {
+        const int grp = min(stage * NG + my_group, last_group);
+        const bool ok = (unsigned) id < (unsigned) g.n_pages;
+        const uint8_t *at = p.base + (int64_t) (ok ? id : 0) * g.page_bytes +
+                            (((int64_t) kvh << g.group_shift) + (grp & ((1 << g.group_shift) - 1))) * kGroupBytes;
+        flag = ok ? 0 : 1;
+        auto codes = [&](const uint8_t *c, uint32_t (&w)[TB]) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(c + lane * 16);
+            w[0] = x.x;
+            w[1] = x.y;
+            w[2] = x.z;
+            w[3] = x.w;
+        };
+        if (do_k) {
+            codes(at, kw);
+#pragma unroll
+            for (int i = 0; i < TB; ++i)
+                kd[i] = *reinterpret_cast<const uint16_t *>(at + page_scale_offset(i, key16, 0));
+        }
+        if (do_v) {
+            codes(at + kVCodeOff, vw);
+#pragma unroll
+            for (int i = 0; i < TB; ++i)
+                vd[i] = *reinterpret_cast<const uint2 *>(at + page_scale_offset(i, 4 * oct, 1));
+        }
+    };
+    auto fill = [&](int buf) {
+        if (do_k) {
+#pragma unroll
+            for (int i = 0; i < TB; ++i) {
+                // row of the key, octet `oct` of the block
+                const int t = i / NB, blk = i % NB;
+                const _Float16 d = __builtin_bit_cast(_Float16, (uint16_t) kd[i]);
+                const pg_half8 x = k_octet(kw[i], pat) * pg_half8{d, d, d, d, d, d, d, d};
+                const int key = my_group * G + t * 16 + key16;
+                *reinterpret_cast<pg_half8 *>(&s_k[buf][key * KROW + (blk * 4 + oct) * 8]) = x;
+            }
+        }
+        if (do_v) {
+            pg_half2 check = {(_Float16) 0.0f, (_Float16) 0.0f};
+#pragma unroll
+            for (int i = 0; i < TB; ++i) {
+                const pg_half2 z = {(_Float16) 0.0f, (_Float16) 0.0f};
+                check = __builtin_elementwise_fma(__builtin_bit_cast(pg_half2, vd[i].x), z, check);
+                check = __builtin_elementwise_fma(__builtin_bit_cast(pg_half2, vd[i].y), z, check);
+            }
+            const bool odd = !(check.x == (_Float16) 0.0f && check.y == (_Float16) 0.0f);
+            if (__any(odd)) {  // rare: such blocks are taken as zeros here and marked
+                flag = 1;
+#pragma unroll
+                for (int i = 0; i < TB; ++i) {
+                    uint32_t w[2] = {vd[i].x, vd[i].y};
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        if (!finite16(w[j])) w[j] &= 0xFFFF0000u;
+                        if (!finite16(w[j] >> 16)) w[j] &= 0x0000FFFFu;
+                    }
+                    vd[i] = make_uint2(w[0], w[1]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < TB; ++i) {
+                // rows key16 and key16 + 16 of the block (elements), a quad of keys
+                const int t = i / NB, blk = i % NB;
+                const uint32_t w = vw[i], y = w >> 8;
+                const pg_half2 da = __builtin_bit_cast(pg_half2, (vd[i].x & 0xFFFFu) | (vd[i].y << 16));
+                const pg_half2 db = __builtin_bit_cast(pg_half2, (vd[i].x >> 16) | (vd[i].y & 0xFFFF0000u));
+                const pg_half2 e0 = codes_lo(w, pat) * da, e1 = codes_lo(y, pat) * db;
+                const pg_half2 h0 = codes_hi(w, pat) * da, h1 = codes_hi(y, pat) * db;
+                const int quad = (my_group * G + t * 16) / 4 + oct;  // of the stage
+                const int place = (quad & ~3) + 2 * (quad & 1) + ((quad >> 1) & 1);
+                _Float16 *row = &s_v[buf][(blk * kQK + key16) * VROW + place * 4];
+                *reinterpret_cast<pg_half4 *>(row) = pg_half4{e0.x, e0.y, e1.x, e1.y};  // keys 0, 2, 1, 3
+                *reinterpret_cast<pg_half4 *>(row + 16 * VROW) = pg_half4{h0.x, h0.y, h1.x, h1.y};
+            }
+        }
+        if (lane == 0) s_flag[buf][wave] = flag;
+    };
+    const bool any_stage = stage0 < n_stage;
+    int id_next = id_of(stage0 + 1);
+    if (any_stage) fetch(stage0, id_of(stage0));
+
     // The row's query as fp16, times its own power of two.
     pg_half8 q[KK];
     float f;  // what the row's scores are multiplied by
@@ -153,8 +273,9 @@ __global__ __launch_bounds__(64 * kAttendWaves, 2) void pages_attend_kernel(Atte
         }
         amax = fmaxf(amax, __shfl_xor(amax, 32));
         bad += __shfl_xor(bad, 32);
-        const int ex = __builtin_amdgcn_frexp_expf(amax) - 15;
-        f = bad == 0.0f ? __builtin_amdgcn_ldexpf(p.qscale, ex) : __builtin_nanf("");
+        const int ex = max(__builtin_amdgcn_frexp_expf(amax), -90) - 15;
+        // (never 0: masked scores are -inf times it)
+        f = bad == 0.0f ? fmaxf(__builtin_amdgcn_ldexpf(p.qscale, ex), 1e-37f) : __builtin_nanf("");
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
@@ -164,94 +285,9 @@ __global__ __launch_bounds__(64 * kAttendWaves, 2) void pages_attend_kernel(Atte
             }
     }
 
-    // ---- filling: wave w takes group w, w + 4 .. of a stage ----
-    constexpr int LG = (NG + NW - 1) / NW;  // groups a wave loads
-    struct Load {
-        uint4 k, v;
-        uint4 ks;       // the key's block scales: [t][b] halves (low half of each dword)
-        uint2 vs[4];    // four keys' scales of each (t, b)
-        int flag;
-    };
-    Load ld[LG];
-    const Patterns pat;
-    const int last_group = max((len - 1) / G, 0);
-    const int key16 = lane & 15, oct = lane >> 4;
-    auto fetch = [&](int stage) {
-#pragma unroll
-        for (int i = 0; i < LG; ++i) {
-            const int gi = wave + i * NW;
-            if (NG % NW != 0 && gi >= NG) break;
-            const int grp = min(stage * NG + gi, last_group);
-            const int id = table[grp >> g.group_shift];
-            const bool ok = (unsigned) id < (unsigned) g.n_pages;
-            const uint8_t *at = p.base + (int64_t) (ok ? id : 0) * g.page_bytes +
-                                (((int64_t) kvh << g.group_shift) + (grp & ((1 << g.group_shift) - 1))) * kGroupBytes;
-            ld[i].flag = ok ? 0 : 1;
-            ld[i].k = *reinterpret_cast<const uint4 *>(at + lane * 16);
-            ld[i].v = *reinterpret_cast<const uint4 *>(at + kVCodeOff + lane * 16);
-            uint32_t ks[4];
-#pragma unroll
-            for (int tb = 0; tb < 4; ++tb) {
-                ks[tb] = *reinterpret_cast<const uint16_t *>(at + page_scale_offset(tb, key16, 0));
-                ld[i].vs[tb] = *reinterpret_cast<const uint2 *>(at + page_scale_offset(tb, 4 * oct, 1));
-            }
-            ld[i].ks = make_uint4(ks[0], ks[1], ks[2], ks[3]);
-        }
-    };
-    auto fill = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < LG; ++i) {
-            const int gi = wave + i * NW;
-            if (NG % NW != 0 && gi >= NG) break;
-            const uint32_t kw[4] = {ld[i].k.x, ld[i].k.y, ld[i].k.z, ld[i].k.w};
-            const uint32_t vw[4] = {ld[i].v.x, ld[i].v.y, ld[i].v.z, ld[i].v.w};
-            const uint32_t kd[4] = {ld[i].ks.x, ld[i].ks.y, ld[i].ks.z, ld[i].ks.w};
-            pg_half2 check = {(_Float16) 0.0f, (_Float16) 0.0f};
-#pragma unroll
-            for (int tb = 0; tb < 4; ++tb) {
-                const pg_half2 z = {(_Float16) 0.0f, (_Float16) 0.0f};
-                check = __builtin_elementwise_fma(__builtin_bit_cast(pg_half2, ld[i].vs[tb].x), z, check);
-                check = __builtin_elementwise_fma(__builtin_bit_cast(pg_half2, ld[i].vs[tb].y), z, check);
-            }
-            const bool odd = !(check.x == (_Float16) 0.0f && check.y == (_Float16) 0.0f);
-            if (__any(odd)) {  // rare: such blocks are taken as zeros here and marked
-                ld[i].flag = 1;
-#pragma unroll
-                for (int tb = 0; tb < 4; ++tb) {
-                    uint32_t w[2] = {ld[i].vs[tb].x, ld[i].vs[tb].y};
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        if (!finite16(w[j])) w[j] &= 0xFFFF0000u;
-                        if (!finite16(w[j] >> 16)) w[j] &= 0x0000FFFFu;
-                    }
-                    ld[i].vs[tb] = make_uint2(w[0], w[1]);
-                }
-            }
-#pragma unroll
-            for (int tb = 0; tb < 4; ++tb) {
-                const int t = tb / NB, blk = tb % NB;
-                // K: row of the key, octet `oct` of the block
-                const _Float16 d = __builtin_bit_cast(_Float16, (uint16_t) kd[tb]);
-                const pg_half8 kx = k_octet(kw[tb], pat) * pg_half8{d, d, d, d, d, d, d, d};
-                const int key = gi * G + t * 16 + key16;
-                *reinterpret_cast<pg_half8 *>(&s_k[buf][key * KROW + (blk * 4 + oct) * 8]) = kx;
-                // V: rows key16 and key16 + 16 of the block (elements), quad of keys
-                const uint32_t w = vw[tb], y = w >> 8;
-                const pg_half2 da = __builtin_bit_cast(pg_half2, (ld[i].vs[tb].x & 0xFFFFu) | (ld[i].vs[tb].y << 16));
-                const pg_half2 db = __builtin_bit_cast(pg_half2, (ld[i].vs[tb].x >> 16) | (ld[i].vs[tb].y & 0xFFFF0000u));
-                const pg_half2 e0 = codes_lo(w, pat) * da, e1 = codes_lo(y, pat) * db;
-                const pg_half2 h0 = codes_hi(w, pat) * da, h1 = codes_hi(y, pat) * db;
-                const int quad = (gi * G + t * 16) / 4 + oct;  // of the stage
-                const int place = (quad & ~3) + 2 * (quad & 1) + ((quad >> 1) & 1);
-                _Float16 *row = &s_v[buf][(blk * kQK + key16) * VROW + place * 4];
-                *reinterpret_cast<pg_half4 *>(row) = pg_half4{e0.x, e0.y, e1.x, e1.y};  // keys 0, 2, 1, 3
-                *reinterpret_cast<pg_half4 *>(row + 16 * VROW) = pg_half4{h0.x, h0.y, h1.x, h1.y};
-            }
-            if (lane == 0) s_flag[buf][gi] = ld[i].flag;
-        }
-    };
-
-    float m = kPagesFloor, mt = kPagesFloor, l = 0.0f;
+    // Running maximum (log2 units), the raw score past which it is raised, sum
+    // of this lane's weights, and the outputs' transposed sums.
+    float m = kPagesFloor, mt = -INFINITY, l = 0.0f;
     int poison = 0;  // blocks whose V is not finite at a position the row sees
     pg_float16 acc[NB];
 #pragma unroll
@@ -259,78 +295,105 @@ __global__ __launch_bounds__(64 * kAttendWaves, 2) void pages_attend_kernel(Atte
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
 
-    // One tile of 32 keys at LDS row `at`, positions base ...  EDGE: some row
-    // of the wave does not see some key.
-    auto tile_of = [&](int buf, int at, int base, bool edge, uint32_t bad_groups) {
-        pg_float16 s;
+    // The stage in buffer buf, positions base ..
+    auto multiply = [&](int buf, int base, bool edge, uint32_t bad_groups) {
+        constexpr int NU = kStage / 32;
+        pg_float16 s[NU];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s[j] = 0.0f;
+        for (int u = 0; u < NU; ++u)
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-            const pg_half8 kx = *reinterpret_cast<const pg_half8 *>(&s_k[buf][(at + n) * KROW + (kk * 2 + half) * 8]);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kx, q[kk], s, 0, 0, 0);
+            for (int j = 0; j < 16; ++j) s[u][j] = 0.0f;
+        {
+            constexpr int N = KK * NU, AHEAD = 8;
+            auto kx = [&](int i) {
+                return *reinterpret_cast<const pg_half8 *>(&s_k[buf][((i % NU) * 32 + n) * KROW + ((i / NU) * 2 + half) * 8]);
+            };
+            pg_half8 ring[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) ring[i] = kx(i);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                s[i % NU] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[i % AHEAD], q[i / NU], s[i % NU], 0, 0, 0);
+                if (i + AHEAD < N) ring[i % AHEAD] = kx(i + AHEAD);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                if (i + AHEAD < N) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
         }
-        // register j holds key 8 (j / 4) + 4 half + j % 4
+        // register j of tile u holds key 32 u + 8 (j / 4) + 4 half + j % 4
         if (edge) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int off = 8 * (j >> 2) + 4 * half + (j & 3);
-                const int pos = base + off;
-                const bool ok = pos >= lo && pos < hi && !((bad_groups >> ((at + off) / G)) & 1u);
-                s[j] = ok ? s[j] * f : -INFINITY;
-            }
-        } else {
+            for (int u = 0; u < NU; ++u)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) s[j] *= f;
+                for (int j = 0; j < 16; ++j) {
+                    const int off = u * 32 + 8 * (j >> 2) + 4 * half + (j & 3);
+                    const int pos = base + off;
+                    const bool ok = pos >= lo && pos < hi && !((bad_groups >> (off / G)) & 1u);
+                    s[u][j] = ok ? s[u][j] : -INFINITY;
+                }
         }
-        float mx = s[0];
+        float mx = s[0][0];
 #pragma unroll
-        for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[j]);
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[u][j]);
         if (__any(mx > mt)) {
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float m_new = fmaxf(m, mx);
+            const float m_new = mx > mt ? fmaxf(m, mx * f) : m;
             const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+            if (mx > mt) mt = (m_new + kPagesLazy) / f;
             m = m_new;
-            mt = m_new + kPagesLazy;
             l *= alpha;
 #pragma unroll
             for (int i = 0; i < NB; ++i)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) acc[i][j] *= alpha;
         }
+        constexpr int N = NB * 2 * NU, AHEAD = NB == 4 ? 8 : 4;
+        auto vx = [&](int i) {  // 2 NU runs of 16 keys, NB blocks of elements each
+            return *reinterpret_cast<const pg_half8 *>(&s_v[buf][((i % NB) * kQK + n) * VROW + (i / NB) * 16 + half * 8]);
+        };
+        pg_half8 ring[AHEAD], w[2 * NU];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            s[j] = __builtin_amdgcn_exp2f(s[j] - m);
-            l += s[j];
+        for (int i = 0; i < AHEAD; ++i) ring[i] = vx(i);
+        const pg_half2 one = {(_Float16) 1.0f, (_Float16) 1.0f};
+#pragma unroll
+        for (int r = 0; r < 2 * NU; ++r) {
+            // keys 0, 2, 1, 3 of each quad, as V's rows hold them; their sum is
+            // taken from the rounded weights, as the products are
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const int u = r / 2, k = 8 * (r & 1) + (j & 4) + ((j >> 1) & 1);
+                const pg_half2 h = {(_Float16) __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][k], f, -m)),
+                                    (_Float16) __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][k + 2], f, -m))};
+                w[r][j] = h.x;
+                w[r][j + 1] = h.y;
+                l = __builtin_amdgcn_fdot2(h, one, l, false);
+            }
         }
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            pg_half8 w;  // keys 0, 2, 1, 3 of each quad, as V's rows hold them
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int k = 8 * ks + (j & 4) + (j & 1 ? 2 : 0) + ((j >> 1) & 1);
-                w[j] = (_Float16) s[k];
-            }
-#pragma unroll
-            for (int blk = 0; blk < NB; ++blk) {
-                const pg_half8 vx = *reinterpret_cast<const pg_half8 *>(
-                    &s_v[buf][(blk * kQK + n) * VROW + at + (ks * 2 + half) * 8]);
-                acc[blk] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vx, w, acc[blk], 0, 0, 0);
-            }
+        for (int i = 0; i < N; ++i) {
+            acc[i % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[i % AHEAD], w[i / NB], acc[i % NB], 0, 0, 0);
+            if (i + AHEAD < N) ring[i % AHEAD] = vx(i + AHEAD);
         }
     };
 
-    if (stage0 < n_stage) {
-        fetch(stage0);
+    if (any_stage) {
         fill(0);
         __syncthreads();
         for (int st = stage0; st < n_stage; ++st) {
             const int buf = (st - stage0) & 1;
             const bool more = st + 1 < n_stage;
-            if (more) fetch(st + 1);
+            if (more) {
+                fetch(st + 1, id_next);
+                id_next = id_of(st + 2);
+            }
             uint32_t flags = 0;
 #pragma unroll
-            for (int i = 0; i < NG; ++i) flags |= s_flag[buf][i] ? 1u << i : 0u;
+            for (int i = 0; i < NW; ++i) flags |= s_flag[buf][i] ? 1u << (i / WPG) : 0u;
             flags = __builtin_amdgcn_readfirstlane(flags);
             uint32_t bad_groups = 0;
             if (flags) {
@@ -356,20 +419,16 @@ __global__ __launch_bounds__(64 * kAttendWaves, 2) void pages_attend_kernel(Atte
                     }
                 }
             }
-#pragma unroll
-            for (int u = 0; u < kStage / 32; ++u) {
-                const int base = st * kStage + u * 32;
-                if (!w_any || base >= w_hi_max || base + 32 <= w_lo_min) continue;
-                const bool edge = !w_full || base + 32 > w_hi_min || base < w_lo_max || bad_groups;
-                tile_of(buf, u * 32, base, edge, bad_groups);
-            }
+            const int base = st * kStage;
+            if (w_any && base < w_hi_max && base + kStage > w_lo_min)
+                multiply(buf, base, !w_full || base + kStage > w_hi_min || base < w_lo_max || bad_groups, bad_groups);
             if (more) fill(buf ^ 1);
             __syncthreads();
         }
     }
     l += __shfl_xor(l, 32);
     if (!row_ok) return;
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l > 0.0f ? 1.0f / l : l * 0.0f;  // (NaN stays)
     uint16_t *out = static_cast<uint16_t *>(p.out) + ((int64_t) (start + tok) * p.n_heads + head) * D;
 #pragma unroll
     for (int blk = 0; blk < NB; ++blk) {
@@ -392,22 +451,64 @@ __global__ __launch_bounds__(64 * kAttendWaves, 2) void pages_attend_kernel(Atte
     }
 }
 
+// Calls with few rows are taken a column a row (pages_decode.hip), 16 columns a
+// workgroup and an entry's positions shared among workgroups.  A tile's
+// workgroup goes over its entry alone, 34 ns a position (23 with every wave
+// full), 95 ps of the whole chip's time; a set of 16 columns takes 30 ps.  So
+// sets win until they fill the chip as tiles do not (1024 of them), and past
+// that where a tile is no more than two sets.  us in a graph, tiles / sets:
+//   32 kv heads of 128, one entry of 4000: 1 row 148 / 12, 16 rows 147 / 19,
+//     64 rows 109 / 33; 64 entries of 1000: 4 rows 193 / 49, 16 rows 195 / 85,
+//     24 rows 195 / 163, 48 rows 197 / 240.
+//   8 kv heads of 128, 32 heads, 16 entries of 8000: 4 rows 283 / 47, 16 rows
+//     (512 sets) 204 / 123, 24 (768) 208 / 186, 32 (1024) 213 / 238.
+//   16 kv heads of 64, 64 entries of 1000: 16 rows 73 / 25, 32 rows 52 / 42.
+static bool few_rows(const PagesAttendParams &p, int max_rows) {
+    const int64_t rows = (int64_t) max_rows * (p.n_heads / p.g.n_kv);
+    const int64_t units = (int64_t) p.n_batch * p.g.n_kv;
+    const int64_t sets = (rows + 15) / 16 * units, tiles = (rows + kTileRows - 1) / kTileRows * units;
+    return sets < 1024 || sets <= 2 * tiles;
+}
+
 hipError_t launch_pages_attend(const PagesAttendParams &p, hipStream_t stream) {
+    // (an entry has no more rows than the call, where max_rows is not known)
+    const int max_rows = p.max_rows > 0 ? std::min(p.max_rows, p.n_rows) : p.n_rows;
+    if (few_rows(p, max_rows)) {
+        PagesDecodeParams d{};
+        d.base = const_cast<uint8_t *>(p.base);
+        d.g = p.g;
+        d.n_batch = p.n_batch;
+        d.n_heads = p.n_heads;
+        d.lens = p.lens;
+        d.table = p.table;
+        d.max_pages = p.max_pages;
+        d.window = p.window;
+        d.type = p.type;
+        d.q = p.q;
+        d.q_stride = p.q_stride;
+        d.out = p.out;
+        d.qscale = p.qscale;
+        d.max_len = p.max_len;
+        d.work = p.work;
+        d.work_bytes = p.work_bytes;
+        d.q_start = p.q_start;
+        d.n_rows = p.n_rows;
+        d.causal = p.causal;
+        d.max_rows = max_rows;
+        return launch_pages_few_rows(d, stream);
+    }
     AttendArgs a{};
     a.p = p;
     a.group = p.n_heads / p.g.n_kv;
     a.div_group = make_fastdiv((uint32_t) a.group);
     // tiles: no more than the rows' and one more an entry, nor than every
     // entry's at its most rows
-    int64_t tiles = ((int64_t) p.n_rows * a.group) / kTileRows + p.n_batch;
-    if (p.max_rows > 0) {
-        const int64_t most = (int64_t) p.n_batch * (((int64_t) p.max_rows * a.group + kTileRows - 1) / kTileRows);
-        tiles = tiles < most ? tiles : most;
-    }
+    const int64_t tiles = std::min(((int64_t) p.n_rows * a.group) / kTileRows + p.n_batch,
+                                   p.n_batch * (((int64_t) max_rows * a.group + kTileRows - 1) / kTileRows));
     void *args[] = {&a};
-    const void *kernel = p.g.dim == 128 ? reinterpret_cast<const void *>(pages_attend_kernel<128>)
-                                        : reinterpret_cast<const void *>(pages_attend_kernel<64>);
-    return hipLaunchKernel(kernel, dim3((unsigned) (tiles * p.g.n_kv)), dim3(64 * kAttendWaves), args, 0, stream);
+    return hipLaunchKernel(p.g.dim == 128 ? reinterpret_cast<const void *>(pages_attend_kernel<128>)
+                                          : reinterpret_cast<const void *>(pages_attend_kernel<64>),
+                           dim3((unsigned) (tiles * p.g.n_kv)), dim3(64 * kAttendWaves), args, 0, stream);
 }
 
 }  // namespace bmo

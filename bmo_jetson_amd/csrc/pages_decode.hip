@@ -13,17 +13,17 @@
 // In the first form a lane has one block's products, so the block scales cost
 // one multiply a score and one a weight instead of NB each.
 //
-// K side, first form: q becomes a whole number of 22 bits (fp32; 15 bits for
+// K side, first form: q becomes a whole number of 23 bits (fp32; 15 bits for
 // 16-bit rows) times a power of two per row, in signed base-256 digits, and
 // the codes 0..15 enter v_mfma_i32_16x16x64_i8 as the bytes that a mask
 // leaves; the digits' sums and the -8 of every code join exactly in 32 bits.
 // Second form: q as two fp16 parts (16-bit rows: one, exactly), the codes
-// minus 8 exact in fp16.  Either way a query is within 2^-22 (2^-15) of its
+// minus 8 exact in fp16.  Either way a query is within 2^-22 (2^-14) of its
 // row's largest element, and a block's product meets its scale in fp32.
 //
 // V side: weight times V scale, brought to fp16's range by a power of two per
-// column (from the largest scale so far), enters as two truncated fp16 parts,
-// exact to 2^-21 (16-bit rows: one part, rounded), against the codes minus 8,
+// column (from the largest scale so far), enters as two fp16 parts, exact to
+// 2^-22 (16-bit rows: one part), against the codes minus 8,
 // exact in fp16, sums in fp32.  An fp32 call is as close as fp32 sums; the
 // 16-bit parts stay below the outputs' own rounding.
 //
@@ -41,6 +41,7 @@
 // row) in the workspace and joined by a second kernel in the order of the runs.
 #include <algorithm>
 
+#include "kernels.hpp"
 #include "pages_device.hpp"
 
 namespace bmo {
@@ -58,27 +59,77 @@ constexpr int kMaxRuns = 128;  // of an entry
 
 struct DecodeArgs {
     PagesDecodeParams p;
-    int group;     // query heads a kv head
-    int n_hs;      // head sets a kv head
-    int units;     // n_kv * n_hs
-    int max_runs;  // of an entry; 1: nothing is cut
-    int run;       // steps up to which an entry is one run
+    int group;          // query heads a kv head
+    int n_hs;           // head sets a kv head (of several rows: sets of 16 or fewer rows)
+    int units;          // n_kv * n_hs
+    int max_runs;       // of an entry; 1: nothing is cut
+    int run;            // steps up to which an entry is one run
     int append;
+    FastDiv div_group;  // several rows
 };
 
-// Steps of an entry: its visible positions are [lo, len).
-struct Span {
-    int len, lo, step0, n, runs;
+// One head set of an entry and kv head: its columns are the kv head's query
+// heads from row0 on, or, of several rows, (token, head) pairs, heads fastest.
+// Its columns see positions of [lo, len); all of them those of [lo_max, hi_min).
+struct Unit {
+    int kvh, row0, cols;
+    int start, n_tok, entry_len;  // several rows
+    int lo, len, lo_max, hi_min;
+    int step0, n, runs;  // steps and runs
 };
-__device__ __forceinline__ Span span_of(const DecodeArgs &a, int len) {
-    Span s;
+// Positions that the token of a multi-row entry sees end before hi_of, and
+// begin with lo_of that.
+__device__ __forceinline__ int hi_of(const DecodeArgs &a, const Unit &u, int tok) {
+    return a.p.causal ? max(u.entry_len - u.n_tok + tok + 1, 0) : u.entry_len;
+}
+__device__ __forceinline__ int lo_of(const DecodeArgs &a, int hi) {
+    return a.p.window > 0 && hi > a.p.window ? hi - a.p.window : 0;
+}
+template <bool MULTI, int HC>
+__device__ __forceinline__ Unit unit_of(const DecodeArgs &a, int b, int unit) {
+    Unit u{};
     const int64_t room = (int64_t) a.p.max_pages << a.p.g.page_shift;
-    s.len = (int) min((int64_t) max(len, 0), room);
-    s.lo = a.p.window > 0 && s.len > a.p.window ? s.len - a.p.window : 0;
-    s.step0 = s.lo / kStep;
-    s.n = (s.len + kStep - 1) / kStep - s.step0;  // (room is at most 2^30)
-    s.runs = a.max_runs == 1 ? 1 : min(max((s.n + a.run - 1) / a.run, 1), a.max_runs);
-    return s;
+    u.kvh = unit / a.n_hs;
+    u.row0 = (unit - u.kvh * a.n_hs) * HC;
+    u.entry_len = (int) min((int64_t) max(uniform_int(a.p.lens, b), 0), room);
+    if constexpr (MULTI) {
+        u.start = uniform_int(a.p.q_start, b);
+        const int end = uniform_int(a.p.q_start, b + 1);
+        u.n_tok = u.start < 0 || end < u.start || end > a.p.n_rows ? 0 : end - u.start;
+        u.cols = min(HC, u.n_tok * a.group - u.row0);
+        if (u.cols <= 0) return u;
+        u.hi_min = hi_of(a, u, (int) a.div_group.div((uint32_t) u.row0));
+        u.len = hi_of(a, u, (int) a.div_group.div((uint32_t) (u.row0 + u.cols - 1)));
+    } else {
+        u.cols = min(HC, a.group - u.row0);
+        u.hi_min = u.len = u.entry_len;
+    }
+    u.lo = lo_of(a, u.hi_min);
+    u.lo_max = lo_of(a, u.len);
+    u.step0 = u.lo / kStep;
+    u.n = (u.len + kStep - 1) / kStep - u.step0;  // (room is at most 2^30)
+    u.runs = a.max_runs == 1 ? 1 : min(max((u.n + a.run - 1) / a.run, 1), a.max_runs);
+    return u;
+}
+// Column r of a unit: where its query and its output row are, and what it sees.
+struct Column {
+    int64_t q, out;
+    int lo, hi;
+};
+template <bool MULTI, int D>
+__device__ __forceinline__ Column column_of(const DecodeArgs &a, const Unit &u, int b, int r) {
+    int row = b, head = u.kvh * a.group + u.row0 + r;
+    Column c{0, 0, u.lo, u.len};
+    if constexpr (MULTI) {
+        const int tok = (int) a.div_group.div((uint32_t) (u.row0 + r));
+        row = u.start + tok;
+        head -= tok * a.group;
+        c.hi = hi_of(a, u, tok);
+        c.lo = lo_of(a, c.hi);
+    }
+    c.q = (int64_t) row * a.p.q_stride + (int64_t) head * D;
+    c.out = ((int64_t) row * a.p.n_heads + head) * D;
+    return c;
 }
 
 // Floats of a partial result of HC heads: their rows, and maximum and sum of
@@ -89,8 +140,9 @@ __host__ __device__ constexpr int part_floats(int hc) { return hc * (D + 2 * (D 
 }  // namespace
 
 // SPREAD: the columns are (head, block); otherwise heads.  F32: the rows are
-// fp32, and the query and the weights take a part more.
-template <int D, bool SPREAD, int NW, bool F32>
+// fp32, and the query and the weights take a part more.  MULTI: an entry has
+// several rows (attend's calls with few of them).
+template <int D, bool SPREAD, int NW, bool F32, bool MULTI>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD || D == 64 ? 3 : 2))) void pages_decode_kernel(DecodeArgs a) {
     constexpr int NB = D / kQK;
     constexpr int TG = kStep * D / 2048;    // groups a step
@@ -100,7 +152,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
     constexpr int PB = NB / CB;             // blocks a column
     constexpr int QP = F32 ? 2 : 1;         // fp16 parts of the query
     constexpr int QD = F32 ? 3 : 2;         // or base-256 digits
-    constexpr int QBITS = F32 ? 21 : 14;    // |Q| <= 2^QBITS
+    constexpr int QBITS = F32 ? 22 : 14;    // |Q| <= 2^QBITS
     constexpr int WP = F32 ? 2 : 1;         // parts of a weight
     constexpr int BUF = 2;  // steps resident in registers
     const PagesDecodeParams &p = a.p;
@@ -120,31 +172,29 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
     const int row = (int) blockIdx.x / a.units;
     const int unit = (int) blockIdx.x - row * a.units;
     const int run = row / p.n_batch, b = row - run * p.n_batch;
-    const int kvh = unit / a.n_hs, hs = unit - kvh * a.n_hs;
-    const int heads = min(HC, a.group - hs * HC);  // heads of this set
-    const int head0 = kvh * a.group + hs * HC;
-    const Span sp = span_of(a, uniform_int(p.lens, b));
-    if (run >= sp.runs) return;
-    const int s_begin = sp.step0 + (int) ((int64_t) sp.n * run / sp.runs);
-    const int s_end = sp.step0 + (int) ((int64_t) sp.n * (run + 1) / sp.runs);
+    const Unit un = unit_of<MULTI, HC>(a, b, unit);
+    if (un.cols <= 0 || run >= un.runs) return;
+    const int kvh = un.kvh;
+    const Column col_r = column_of<MULTI, D>(a, un, b, r < un.cols ? r : 0);
+    const int s_begin = un.step0 + (int) ((int64_t) un.n * run / un.runs);
+    const int s_end = un.step0 + (int) ((int64_t) un.n * (run + 1) / un.runs);
     const int *table = p.table + (int64_t) b * p.max_pages;
 
     // The query's elements of the column's blocks (requested ahead of the
     // steps, so that waiting for them does not wait for those).
     pg_float4 qx[PB][2];
     {
-        const int64_t src = (int64_t) b * p.q_stride + (int64_t) (head0 + (r < heads ? r : 0)) * D;
 #pragma unroll
         for (int i = 0; i < PB; ++i) {
             const int blk = SPREAD ? cb : i;
-            qx[i][0] = load4(p.q, src + blk * kQK + 4 * oct, type);
-            qx[i][1] = load4(p.q, src + blk * kQK + 4 * oct + 16, type);
+            qx[i][0] = load4(p.q, col_r.q + blk * kQK + 4 * oct, type);
+            qx[i][1] = load4(p.q, col_r.q + blk * kQK + 4 * oct + 16, type);
         }
     }
 
     // The new token's row goes to its slot before the wave that will read it
     // starts on its steps (of several head sets each writes the same bytes).
-    if (a.append && sp.len > 0 && s_end == sp.step0 + sp.n && wave == (s_end - 1 - s_begin) % NW) {
+    if (!MULTI && a.append && un.len > 0 && s_end == un.step0 + un.n && wave == (s_end - 1 - s_begin) % NW) {
         constexpr int BL = 32 / NB, NE = NB, HE = NE / 2, LPD = 4 / HE;
         const int nb = lane / BL, gi = lane % BL;
         const int64_t src = (int64_t) b * p.kv_stride + kvh * D + (nb % NB) * kQK + gi * HE;
@@ -157,7 +207,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
         }
         uint16_t d16;
         const uint32_t dw = quantize_block_q4_0_lanes<BL>(x, gi, d16);
-        const int pos = sp.len - 1;
+        const int pos = un.len - 1;
         const int id = table[pos >> g.page_shift];
         if ((unsigned) id < (unsigned) g.n_pages) {
             const int slot = (id << g.page_shift) | (pos & (g.page - 1));
@@ -189,7 +239,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
         uint4 sc[2][PB];  // K's and V's scales of the lane's four keys of a tile
         int ok;  // bit i: group i's page is there
     };
-    const int last_group = max((sp.len - 1) / (2048 / D), 0);
+    const int last_group = max((un.len - 1) / (2048 / D), 0);
     auto ids_of = [&](int step, Ids &t) {
 #pragma unroll
         for (int i = 0; i < TG; ++i)
@@ -240,7 +290,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int e = SPREAD ? (j & 3) + (j & 4) * 4 : octet_elem(0, j);  // 0..3, 16..19
-                x[i][j] = r >= heads ? 0.0f : e < 16 ? qx[i][0][e & 3] : qx[i][1][e & 3];
+                x[i][j] = r >= un.cols ? 0.0f : e < 16 ? qx[i][0][e & 3] : qx[i][1][e & 3];
                 amax = fmaxf(amax, __builtin_fabsf(x[i][j]));
                 bad += x[i][j] * 0.0f;  // NaN if it is not finite
             }
@@ -356,10 +406,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int u = i >> 2, e = i & 3;
-                int sum = d[u][QD - 1][e];
+                // sum (c - 8) Q, below 2^31 (the way there may wrap)
+                uint32_t sum = (uint32_t) d[u][QD - 1][e];
 #pragma unroll
-                for (int k = QD - 2; k >= 0; --k) sum = (sum << 8) + d[u][k][e];
-                float x = times_scale((float) sum, t.sc[u][0], 0, e, 0.0f);
+                for (int k = QD - 2; k >= 0; --k) sum = (sum << 8) + (uint32_t) d[u][k][e];
+                float x = times_scale((float) (int) sum, t.sc[u][0], 0, e, 0.0f);
                 x += pg_dpp<0xB1>(x);
                 if constexpr (NB == 4) x += pg_dpp<0x4E>(x);
                 s[i] = x;
@@ -383,13 +434,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
                     s[i] = times_scale(d[i >> 2][i & 3], t.sc[i >> 2][SPREAD ? 0 : blk], 0, i & 3, s[i]);
             }
         }
-        if (!(step * kStep >= sp.lo && step * kStep + kStep <= sp.len && t.ok == (1 << TG) - 1)) {
+        if (!(step * kStep >= un.lo_max && step * kStep + kStep <= un.hi_min && t.ok == (1 << TG) - 1)) {
             // some position is not visible: score -inf, V scale 0
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int u = i >> 2;
                 const int pos = step * kStep + u * 16 + 4 * oct + (i & 3);
-                const bool ok = pos >= sp.lo && pos < sp.len && ((t.ok >> (u / T)) & 1);
+                const bool ok = pos >= col_r.lo && pos < col_r.hi && ((t.ok >> (u / T)) & 1);
                 s[i] = ok ? s[i] : -INFINITY;
                 const uint32_t keep = ok ? 0xFFFFFFFFu : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
 #pragma unroll
@@ -472,18 +523,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
                 }
                 x = times_scale(x, t.sc[a0 >> 2][j], 1, a0 & 3, 0.0f);
                 y = times_scale(y, t.sc[a1 >> 2][j], 1, a1 & 3, 0.0f);
-                if constexpr (WP == 1) {
-                    wp[0][i] = (_Float16) x;
-                    wp[0][i + 1] = (_Float16) y;
-                } else {
-                    const pg_half2 h = __builtin_bit_cast(pg_half2, __builtin_amdgcn_cvt_pkrtz(x, y));
-                    const pg_half2 g2 = __builtin_bit_cast(
-                        pg_half2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float) h.x, minus_one, x),
-                                                             __builtin_fmaf((float) h.y, minus_one, y)));
-                    wp[0][i] = h.x;
-                    wp[0][i + 1] = h.y;
-                    wp[WP - 1][i] = g2.x;
-                    wp[WP - 1][i + 1] = g2.y;
+                const pg_half2 h = {(_Float16) x, (_Float16) y};
+                wp[0][i] = h.x;
+                wp[0][i + 1] = h.y;
+                if constexpr (WP == 2) {
+                    wp[1][i] = (_Float16) __builtin_fmaf((float) h.x, minus_one, x);
+                    wp[1][i + 1] = (_Float16) __builtin_fmaf((float) h.y, minus_one, y);
                 }
             }
 #pragma unroll
@@ -540,7 +585,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < heads * D; i += 64 * NW) {
+    for (int i = threadIdx.x; i < un.cols * D; i += 64 * NW) {
         const int rr = i / D, e = i % D, blk = e / kQK;
         float M = s_m[0][rr][blk];
 #pragma unroll
@@ -552,9 +597,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
             L = __builtin_fmaf(f, s_l[w][rr][blk], L);
             o = __builtin_fmaf(f, s_out[w][rr][e], o);
         }
-        if (sp.runs == 1) {
+        if (un.runs == 1) {
             const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-            store1(p.out, ((int64_t) b * p.n_heads + head0 + rr) * D + e, o * inv, type);
+            store1(p.out, column_of<MULTI, D>(a, un, b, rr).out + e, o * inv, type);
         } else {
             float *dst = p.work + (int64_t) blockIdx.x * part_floats<D>(HC);
             dst[rr * D + e] = o;
@@ -566,22 +611,22 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
     }
 }
 
-// Joins the runs of the entries that were cut: a workgroup takes one (entry,
-// query head), its waves every fourth run.
-template <int D, bool SPREAD>
+// Joins the runs of the entries that were cut: a workgroup takes one column,
+// its waves every fourth run.
+template <int D, bool SPREAD, bool MULTI>
 __global__ __launch_bounds__(256) void pages_join_kernel(DecodeArgs a) {
     constexpr int HC = SPREAD ? 16 / (D / kQK) : 16;
     constexpr int NB = D / kQK, E = D / 64, NW = 4;
     const PagesDecodeParams &p = a.p;
     __shared__ float s_w[kMaxRuns][NB];
     __shared__ float s_o[NW][D];
-    const int b = (int) blockIdx.x / p.n_heads, h = (int) blockIdx.x - b * p.n_heads;
-    const int runs = span_of(a, uniform_int(p.lens, b)).runs;
-    if (runs == 1) return;
-    const int kvh = h / a.group, in_group = h - kvh * a.group;
-    const int hs = in_group / HC, rr = in_group - hs * HC;
+    const int row = (int) blockIdx.x / HC, rr = (int) blockIdx.x - row * HC;
+    const int b = row / a.units, unit = row - b * a.units;
+    const Unit un = unit_of<MULTI, HC>(a, b, unit);
+    if (rr >= un.cols || un.runs == 1) return;
+    const int runs = un.runs;
     const int64_t stride = (int64_t) p.n_batch * a.units * part_floats<D>(HC);
-    const float *src = p.work + ((int64_t) b * a.units + kvh * a.n_hs + hs) * part_floats<D>(HC);
+    const float *src = p.work + ((int64_t) b * a.units + unit) * part_floats<D>(HC);
     const int lane = threadIdx.x & 63, wave = (int) threadIdx.x >> 6;
     // lane e has elements e, e + 64 of the head, of blocks e / 32, + 2
     float o[E];
@@ -615,43 +660,40 @@ __global__ __launch_bounds__(256) void pages_join_kernel(DecodeArgs a) {
     __syncthreads();
     if (threadIdx.x < D) {
         const int e = threadIdx.x;
-        store1(p.out, ((int64_t) b * p.n_heads + h) * D + e, (s_o[0][e] + s_o[1][e]) + (s_o[2][e] + s_o[3][e]), p.type);
+        store1(p.out, column_of<MULTI, D>(a, un, b, rr).out + e, (s_o[0][e] + s_o[1][e]) + (s_o[2][e] + s_o[3][e]), p.type);
     }
 }
 
 namespace {
 
-// Heads of a head set: columns are (head, block) while a group fits that way.
-bool spread(const PagesGeom &g, int group) { return group <= 16 / (g.dim / kQK); }
-int set_heads(const PagesGeom &g, int group) { return spread(g, group) ? 16 / (g.dim / kQK) : 16; }
-
-template <int D, bool SPREAD, int NW>
-const void *kernel_of(int type) {
-    return type == kTypeF32 ? reinterpret_cast<const void *>(pages_decode_kernel<D, SPREAD, NW, true>)
-                            : reinterpret_cast<const void *>(pages_decode_kernel<D, SPREAD, NW, false>);
+// Columns are (head, block) while there are that few heads (or rows and heads).
+bool spread(const PagesGeom &g, int heads) { return heads <= 16 / (g.dim / kQK); }
+int set_heads(const PagesGeom &g, int heads) { return spread(g, heads) ? 16 / (g.dim / kQK) : 16; }
+int64_t part_bytes(const PagesGeom &g, int heads) {
+    return (int64_t) set_heads(g, heads) * (g.dim + 2 * (g.dim / kQK)) * 4;
 }
 
-template <int D, bool SPREAD>
-hipError_t launch_of(const DecodeArgs &arg, int nw, int64_t items, hipStream_t stream) {
+template <int D, bool SPREAD, bool MULTI>
+const void *kernel_of(int nw, int type) {
+#define BMO_DECODE(NW_, F32_) reinterpret_cast<const void *>(pages_decode_kernel<D, SPREAD, NW_, F32_, MULTI>)
+    if constexpr (!MULTI)
+        if (type == kTypeF32) return nw == 1 ? BMO_DECODE(1, true) : BMO_DECODE(kWaves, true);
+    return nw == 1 ? BMO_DECODE(1, false) : BMO_DECODE(kWaves, false);
+#undef BMO_DECODE
+}
+
+template <int D, bool SPREAD, bool MULTI>
+hipError_t launch_of(const DecodeArgs &arg, int nw, hipStream_t stream) {
+    constexpr int HC = SPREAD ? 16 / (D / kQK) : 16;
     DecodeArgs a = arg;
     void *args[] = {&a};
-    const void *kernel = nw == 1 ? kernel_of<D, SPREAD, 1>(a.p.type) : kernel_of<D, SPREAD, kWaves>(a.p.type);
-    hipError_t e = hipLaunchKernel(kernel, dim3((unsigned) items), dim3(64 * nw), args, 0, stream);
+    const int64_t units = (int64_t) a.p.n_batch * a.units;
+    hipError_t e = hipLaunchKernel(kernel_of<D, SPREAD, MULTI>(nw, a.p.type), dim3((unsigned) (units * a.max_runs)),
+                                   dim3(64 * nw), args, 0, stream);
     if (e == hipSuccess && a.max_runs > 1)
-        e = hipLaunchKernel(reinterpret_cast<const void *>(pages_join_kernel<D, SPREAD>),
-                            dim3((unsigned) (a.p.n_batch * a.p.n_heads)), dim3(256), args, 0, stream);
+        e = hipLaunchKernel(reinterpret_cast<const void *>(pages_join_kernel<D, SPREAD, MULTI>),
+                            dim3((unsigned) (units * HC)), dim3(256), args, 0, stream);
     return e;
-}
-
-}  // namespace
-
-// Head sets of 16 heads have four times as long results as the others, and the
-// launch a quarter of the units: a quarter of the workgroups may be cut off.
-static int split_workgroups(const PagesGeom &g, int group) { return kSplitWaves / kWaves / (spread(g, group) ? 1 : 4); }
-
-int64_t pages_work_bytes(const PagesGeom &g, int n_heads) {
-    const int group = n_heads / g.n_kv, hc = set_heads(g, group);
-    return (int64_t) split_workgroups(g, group) * hc * (g.dim + 2 * (g.dim / kQK)) * 4;
 }
 
 // Shape of a launch, from its units and the steps that its longest entry can
@@ -663,34 +705,54 @@ int64_t pages_work_bytes(const PagesGeom &g, int n_heads) {
 //     steps 11.2 / 21.6 / 21.6, x 250 14.5 / 16.8 / 49, 8 x 1000 17.7 / 18.7 /
 //     184; 256 x 32 13.7 / 10.7 / 10.7, 512 x 32 21.5 / 16.3 / 16.2; 96 units
 //     of 62 to 1000 steps 56 / 54 / 183.
-hipError_t launch_pages_decode(const PagesDecodeParams &p, hipStream_t stream) {
+template <bool MULTI>
+hipError_t launch_units(const PagesDecodeParams &p, int heads, hipStream_t stream) {
     DecodeArgs a{};
     a.p = p;
     a.group = p.n_heads / p.g.n_kv;
-    const int hc = set_heads(p.g, a.group);
-    a.n_hs = (a.group + hc - 1) / hc;
+    a.div_group = make_fastdiv((uint32_t) a.group);
+    const int hc = set_heads(p.g, heads);
+    a.n_hs = (heads + hc - 1) / hc;
     a.units = p.g.n_kv * a.n_hs;
     a.append = p.k_new != nullptr;
     a.max_runs = 1;
     const int64_t units = (int64_t) p.n_batch * a.units;
     int64_t longest = (int64_t) p.max_pages << p.g.page_shift;
     if (p.max_len > 0 && p.max_len < longest) longest = p.max_len;
-    if (p.window > 0 && p.window + kStep < longest) longest = p.window + kStep;
+    const int64_t seen = (int64_t) p.window + (MULTI ? p.max_rows : 0) + kStep;
+    if (p.window > 0 && seen < longest) longest = seen;
     const int64_t steps = (longest + kStep - 1) / kStep;
     const int nw = units >= 1024 && steps <= 24 ? 1 : kWaves;
-    if (nw == kWaves && p.work && p.work_bytes >= pages_work_bytes(p.g, p.n_heads)) {
+    if (nw == kWaves && p.work) {
+        const int64_t room = p.work_bytes / part_bytes(p.g, heads) / units;  // runs that it holds
         const int64_t fill = std::min<int64_t>(kFillWaves / kWaves / units, steps / (kFillSteps * kWaves));
-        const int64_t split = std::min<int64_t>(split_workgroups(p.g, a.group) / units, steps / (kSplitSteps * kWaves));
-        const int64_t runs = std::min<int64_t>(std::max(fill, split), kMaxRuns);
+        const int64_t split = std::min<int64_t>(kSplitWaves / kWaves / units, steps / (kSplitSteps * kWaves));
+        const int64_t runs = std::min({std::max(fill, split), room, (int64_t) kMaxRuns});
         if (runs > 1) {
             a.max_runs = (int) runs;
             a.run = (int) ((steps + runs - 1) / runs);
         }
     }
-    const int64_t items = units * a.max_runs;
     if (p.g.dim == 128)
-        return spread(p.g, a.group) ? launch_of<128, true>(a, nw, items, stream) : launch_of<128, false>(a, nw, items, stream);
-    return spread(p.g, a.group) ? launch_of<64, true>(a, nw, items, stream) : launch_of<64, false>(a, nw, items, stream);
+        return hc == 16 ? launch_of<128, false, MULTI>(a, nw, stream) : launch_of<128, true, MULTI>(a, nw, stream);
+    return hc == 16 ? launch_of<64, false, MULTI>(a, nw, stream) : launch_of<64, true, MULTI>(a, nw, stream);
+}
+
+}  // namespace
+
+// Every workgroup that a split launch of one-row entries can have; sets of 16
+// heads have four times as long results and a quarter of the units.
+int64_t pages_work_bytes(const PagesGeom &g, int n_heads) {
+    const int group = n_heads / g.n_kv;
+    return kSplitWaves / kWaves / (spread(g, group) ? 1 : 4) * part_bytes(g, group);
+}
+
+hipError_t launch_pages_decode(const PagesDecodeParams &p, hipStream_t stream) {
+    return launch_units<false>(p, p.n_heads / p.g.n_kv, stream);
+}
+
+hipError_t launch_pages_few_rows(const PagesDecodeParams &p, hipStream_t stream) {
+    return launch_units<true>(p, p.max_rows * (p.n_heads / p.g.n_kv), stream);
 }
 
 }  // namespace bmo

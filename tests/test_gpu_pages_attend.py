@@ -217,3 +217,31 @@ def test_refusals(gpu):
     pages.attend(0, start, lens, table, q[:0], q[:0].clone())  # nothing to do
     gpu.cuda.synchronize()
     pages.close()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv", [(2, 2), (6, 2), (16, 1)])
+@pytest.mark.parametrize("window", [0, 45])
+@pytest.mark.parametrize("causal", [True, False])
+def test_few_rows_in_sets_of_columns(gpu, dim, heads, kv, window, causal):
+    """Entries whose rows share sets of 4, 8 or 16 columns, full and not, and
+    ends and windows that differ from row to row."""
+    for type_ in ("float16", "bfloat16"):
+        _run(gpu, [7, 1, 0, 17, 4], [300, 1, 5, 17, 0], 64, heads, kv, dim, type_, causal=causal, window=window)
+
+
+def test_few_and_many_rows_agree(gpu):
+    """An entry's rows alone, by sets of columns, and among so many that the
+    call is taken by tiles."""
+    pages, cache, table = pool(gpu, [700] * 70, 64, 4, 128, 9)
+    q = gpu.randn(70 * 48, 4, 128, device="cuda").half()
+    lens, t = i32(gpu, [700] * 70), i32(gpu, table)
+    a, b = gpu.zeros_like(q), gpu.zeros_like(q)
+    stream = gpu.cuda.current_stream()
+    pages.attend(0, i32(gpu, np.arange(71) * 48), lens, t, q, a, max_rows=48, stream=stream)
+    for i in (0, 33, 69):
+        rows = slice(48 * i, 48 * i + 48)
+        pages.attend(0, i32(gpu, [0, 48]), lens[:1], t[i:i + 1], q[rows], b[rows], max_rows=48, stream=stream)
+        # both are within a rounding (2^-11) and the operands' (2^-10) of the exact ones
+        assert rel(b[rows].double().cpu().numpy(), a[rows].double().cpu().numpy()) < 2.0**-9
+    pages.close()
