@@ -50,7 +50,7 @@ struct PagesGeom {
     __host__ __device__ int n_slots() const { return n_pages << page_shift; }
     // Offset, from the layer's start, of the group of slot s in head h.
     __host__ __device__ int64_t group_offset(int slot, int h) const {
-        const int in_page = (slot & (page - 1)) / keys_per_group(dim);
+        const int in_page = (slot & (page - 1)) >> (page_shift - group_shift);  // a group: page_size / 2^group_shift
         return (int64_t) (slot >> page_shift) * page_bytes + (((int64_t) h << group_shift) + in_page) * kGroupBytes;
     }
 };

@@ -138,15 +138,15 @@ __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
     return (uint32_t) __builtin_amdgcn_mov_dpp((int) v, CTRL, 0xF, 0xF, true);
 }
 
-// Reductions over an aligned group of BL = 8 or 16 lanes of one 16-lane row:
-// lane ^ 1 and lane ^ 2 (quad_perm), then the mirrored quad of the half-row
-// (row_half_mirror) and, for 16, the mirrored half-row (row_mirror).  Every
-// lane of the group must be active.
+// Reductions over an aligned group of BL = 4, 8 or 16 lanes of one 16-lane row:
+// lane ^ 1 and lane ^ 2 (quad_perm), then, for 8 and 16, the mirrored quad of
+// the half-row (row_half_mirror) and, for 16, the mirrored half-row
+// (row_mirror).  Every lane of the group must be active.
 template <int BL>
 __device__ __forceinline__ uint32_t group_max_u32(uint32_t v) {
     v = max(v, dpp_u32<0xB1>(v));
     v = max(v, dpp_u32<0x4E>(v));
-    v = max(v, dpp_u32<0x141>(v));
+    if constexpr (BL >= 8) v = max(v, dpp_u32<0x141>(v));
     if constexpr (BL == 16) v = max(v, dpp_u32<0x140>(v));
     return v;
 }
@@ -154,12 +154,12 @@ template <int BL>
 __device__ __forceinline__ uint32_t group_min_u32(uint32_t v) {
     v = min(v, dpp_u32<0xB1>(v));
     v = min(v, dpp_u32<0x4E>(v));
-    v = min(v, dpp_u32<0x141>(v));
+    if constexpr (BL >= 8) v = min(v, dpp_u32<0x141>(v));
     if constexpr (BL == 16) v = min(v, dpp_u32<0x140>(v));
     return v;
 }
 
-// Lane-parallel quantization of one block spread over BL = 8 or 16
+// Lane-parallel quantization of one block spread over BL = 4, 8 or 16
 // consecutive lanes (the group starts at a multiple of BL): lane i of the
 // group holds E = 32 / BL elements, x[t] = element i*E/2 + t and
 // x[E/2 + t] = element i*E/2 + t + 16 (t < E/2), so its codes fill E/2 whole
@@ -212,7 +212,7 @@ __device__ __forceinline__ uint32_t quantize_block_q4_0_lanes(const float (&x)[3
         w |= byte << (8 * ((i * HE + t) & 3));
     }
     // the 4 / HE lanes of one dword are adjacent
-    w |= dpp_u32<0xB1>(w);
+    if constexpr (HE <= 2) w |= dpp_u32<0xB1>(w);
     if constexpr (HE == 1) w |= dpp_u32<0x4E>(w);
     return w;
 }

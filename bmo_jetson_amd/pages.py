@@ -9,22 +9,34 @@ from .ring import RingError, _ptr, _stream
 _TYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "uint8": 3}
 
 
+_NAMES: dict = {}  # dtype objects' names (formatting one costs as much as a call)
+
+
+def _dtype(x) -> str:
+    """The name of a tensor's element type."""
+    d = getattr(x, "dtype", None)
+    name = _NAMES.get(d)
+    if name is None:
+        name = _NAMES[d] = str(d).rsplit(".", 1)[-1]
+    return name
+
+
 def _type(x) -> int:
     """The element type (BMO_ATTN_F32 ..) of a tensor."""
-    name = str(getattr(x, "dtype", None)).rsplit(".", 1)[-1]
-    if name not in _TYPES:
-        raise TypeError(f"expected a float32, float16, bfloat16 or uint8 tensor, got {name}")
-    return _TYPES[name]
+    code = _TYPES.get(_NAMES.get(x.dtype) or _dtype(x))
+    if code is None:
+        raise TypeError(f"expected a float32, float16, bfloat16 or uint8 tensor, got {_dtype(x)}")
+    return code
 
 
 def _ints(x, what: str, n: int | None = None) -> int | None:
     """Address of a dense int32 tensor (of n elements), or None."""
     if x is None:
         return None
-    if str(x.dtype).rsplit(".", 1)[-1] != "int32" or not x.is_contiguous() or (n is not None and x.numel() != n):
+    if (_NAMES.get(x.dtype) or _dtype(x)) != "int32" or not x.is_contiguous() or (n is not None and x.numel() != n):
         size = "" if n is None else f" of {n} elements"
         raise ValueError(f"{what} must be a contiguous int32 tensor{size}")
-    return _ptr(x)
+    return x.data_ptr()
 
 
 class KVPages:
@@ -92,30 +104,32 @@ class KVPages:
     # -- rows -------------------------------------------------------------------
     def _rows(self, x, heads: int | None, what: str):
         """(address, stride, type, heads, tokens) of rows [tokens][heads][head_dim]."""
-        if x.dim() != 3 or x.shape[2] != self.head_dim or (heads is not None and x.shape[1] != heads):
-            raise ValueError(f"{what} must be [tokens][{heads or 'heads'}][{self.head_dim}], got {tuple(x.shape)}")
-        n, h, d = x.shape
-        if n and ((x.stride(2) != 1) or (h > 1 and x.stride(1) != d)):
+        shape = x.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
+            raise ValueError(f"{what} must be [tokens][{heads or 'heads'}][{self.head_dim}], got {tuple(shape)}")
+        n, h, d = shape
+        stride = x.stride()
+        if n and (stride[2] != 1 or (h > 1 and stride[1] != d)):
             raise ValueError(f"{what}: a token's heads must be contiguous")
-        return _ptr(x), int(x.stride(0)) if n > 1 else 0, _type(x), int(h), int(n)
+        return x.data_ptr(), stride[0] if n > 1 else 0, _type(x), h, n
 
     def _out(self, x, n: int, heads: int, type_: int):
-        if tuple(x.shape) != (n, heads, self.head_dim) or not x.is_contiguous() or _type(x) != type_:
+        if x.shape != (n, heads, self.head_dim) or not x.is_contiguous() or _type(x) != type_:
             raise ValueError(f"out must be a contiguous [{n}][{heads}][{self.head_dim}] tensor of q's type")
-        return _ptr(x)
+        return x.data_ptr()
 
     @staticmethod
     def _table(lens, table):
-        n = int(lens.numel())
-        if table.dim() != 2 or table.shape[0] != n:
+        n, shape = lens.numel(), table.shape
+        if len(shape) != 2 or shape[0] != n:
             raise ValueError("table must be [n_batch][max_pages]")
-        return n, _ints(lens, "lens"), _ints(table, "table"), int(table.shape[1])
+        return n, _ints(lens, "lens"), _ints(table, "table"), shape[1]
 
     @staticmethod
     def _work(workspace):
         if workspace is None:
             return None, 0
-        return _ptr(workspace), int(workspace.numel() * workspace.element_size())
+        return _ptr(workspace), workspace.numel() * workspace.element_size()
 
     # -- plan -------------------------------------------------------------------
     def list_init(self, free, stream=None) -> None:
@@ -130,7 +144,7 @@ class KVPages:
         [max_tok] tell the new tokens' places, tok_start [n_batch + 1] where an
         entry's tokens begin, status [n_batch] 0 where it was done."""
         n, lens_p, table_p, width = self._table(lens, table)
-        sizes = {int(x.numel()) for x in (slots, positions, entries) if x is not None}
+        sizes = {x.numel() for x in (slots, positions, entries) if x is not None}
         if len(sizes) > 1:
             raise ValueError("slots, positions and entries must have the same size")
         self._check("bmo_kv_pages_plan", lib().bmo_kv_pages_plan(
@@ -140,7 +154,7 @@ class KVPages:
 
     # -- rows in and out ----------------------------------------------------------
     def _slots(self, fn: str, call, layer: int, slots, k, v, stream) -> None:
-        n = int(slots.numel())
+        n = slots.numel()
         if _type(k) == 3:  # ggml blocks
             shape = (n, self.n_kv_heads, self.head_dim // 32, 18)
             if tuple(k.shape) != shape or tuple(v.shape) != shape or not (k.is_contiguous() and v.is_contiguous()):
