@@ -62,6 +62,7 @@ SIGNATURES = {
     "bmo_kv_pages_create": (P, [i32, i32, i32, i32, i32]),
     "bmo_kv_pages_free": (None, [P]),
     "bmo_kv_pages_bytes": (i64, [P]),
+    "bmo_kv_pages_device": (i32, [P]),
     "bmo_kv_pages_last_error": (ctypes.c_char_p, [P]),
     "bmo_kv_pages_list_init": (i32, [P, P, P]),
     "bmo_kv_pages_plan": (i32, [P, P, i32, P, P, P, i32, P, i32, P, P, P, P, P]),

@@ -124,7 +124,8 @@ int slots_call(bmo_kv_pages_t *h, const char *fn, bool append, int layer, int n_
             stride = given;
             if (const char *why = row_fault(v, stride, (int64_t) g.n_kv * g.dim, type)) return c.arg(why);
         }
-        if ((int64_t) n_tok * g.n_kv * (g.dim / 32) > INT_MAX) return c.arg("n_tok too large (2^31 blocks)");
+        // (four lanes a block: the grid's threads stay below 2^32)
+        if ((int64_t) n_tok * g.n_kv * (g.dim / 32) > (1 << 29)) return c.arg("n_tok too large (2^29 blocks)");
         if (n_tok == 0) return c.done(hipSuccess);
         c.enter();
         bmo::SlotsParams p{};
@@ -151,7 +152,8 @@ int decode_call(bmo_kv_pages_t *h, const char *fn, bool append, int layer, int n
         if (int rc = check_table(c, n_batch, max_pages)) return rc;
         if (int rc = check_heads(c, n_heads)) return rc;
         const bmo::PagesGeom &g = c.h->g;
-        if ((int64_t) n_batch * n_heads > (1 << 24)) return c.arg("n_batch * n_heads must be at most 2^24");
+        // (a workgroup of 256 a head at most: the grid's threads stay below 2^32)
+        if ((int64_t) n_batch * n_heads > (1 << 23)) return c.arg("n_batch * n_heads must be at most 2^23");
         if (type < bmo::kTypeF32 || type > bmo::kTypeBF16) return c.arg("rows must be fp32, fp16 or bf16");
         if (const char *why = row_fault(q, q_stride, (int64_t) n_heads * g.dim, type)) return c.arg(why);
         if (append) {
@@ -250,6 +252,8 @@ void bmo_kv_pages_free(bmo_kv_pages_t *h) {
 
 int64_t bmo_kv_pages_bytes(const bmo_kv_pages_t *h) { return h ? h->g.layer_bytes * h->g.n_layers : 0; }
 
+int bmo_kv_pages_device(const bmo_kv_pages_t *h) { return h ? h->device : -1; }
+
 const char *bmo_kv_pages_last_error(const bmo_kv_pages_t *h) {
     if (!h) return t_create_error.empty() ? nullptr : t_create_error.c_str();
     thread_local std::string t_copy;
@@ -340,8 +344,8 @@ int bmo_kv_pages_attend(bmo_kv_pages_t *h, int layer, int n_batch, const int *q_
         if (type != bmo::kTypeF16 && type != bmo::kTypeBF16) return c.arg("rows must be fp16 or bf16");
         if (n_rows < 0 || (int64_t) n_rows * n_heads > (1 << 30))
             return c.arg("n_rows must not be negative, n_rows * n_heads at most 2^30");
-        if (n_batch > (1 << 20) || (int64_t) n_batch * g.n_kv > (1 << 24))
-            return c.arg("n_batch * n_kv_heads must be at most 2^24");
+        // (tiles: 2^23 of rows and one an entry and kv head, 256 threads each)
+        if ((int64_t) n_batch * g.n_kv > (1 << 22)) return c.arg("n_batch * n_kv_heads must be at most 2^22");
         if (const char *why = row_fault(q, q_stride, (int64_t) n_heads * g.dim, type)) return c.arg(why);
         if (!aligned(out, 16) || !aligned(workspace, 16)) return c.arg("out and workspace must be aligned to 16 bytes");
         if (window < 0 || max_rows < 0 || max_len < 0 || workspace_bytes < 0)

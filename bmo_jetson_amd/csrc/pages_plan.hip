@@ -23,6 +23,8 @@
 // prompts 7.1 us in a graph (one workgroup per 1024 tokens; per 4096 8.7 us,
 // waves of a quarter as many threads 13 us).  Four returned pages a thread at
 // a time cost a token's step 0.5 us more than they save.
+#include <algorithm>
+
 #include "pages.hpp"
 
 namespace bmo {
@@ -268,7 +270,9 @@ __global__ __launch_bounds__(256) void list_init_kernel(int *list, int n_pages) 
 hipError_t launch_plan(const PlanParams &p, hipStream_t stream) {
     PlanParams arg = p;
     void *args[] = {&arg};
-    const int wgs = p.max_tok <= kPlanShare ? 1 : (int) ((p.max_tok + (int64_t) kPlanShare - 1) / kPlanShare);
+    // without arrays max_tok tells nothing: a token each is what such calls ask for
+    const int64_t tokens = p.tok_slot || p.tok_pos || p.tok_entry ? p.max_tok : std::min(p.max_tok, p.n_batch);
+    const int64_t wgs = std::max<int64_t>((tokens + kPlanShare - 1) / kPlanShare, 1);
     return hipLaunchKernel(reinterpret_cast<const void *>(plan_kernel), dim3((unsigned) (wgs < 128 ? wgs : 128)),
                            dim3(kPlanThreads), args, 0, stream);
 }

@@ -4,7 +4,7 @@ single tokens (``decode``) and ragged rows (``attend``) over them."""
 from __future__ import annotations
 
 from ._lib import lib
-from .ring import RingError, _ptr, _stream
+from .ring import RingError, _stream
 
 _TYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "uint8": 3}
 
@@ -29,16 +29,6 @@ def _type(x) -> int:
     return code
 
 
-def _ints(x, what: str, n: int | None = None) -> int | None:
-    """Address of a dense int32 tensor (of n elements), or None."""
-    if x is None:
-        return None
-    if (_NAMES.get(x.dtype) or _dtype(x)) != "int32" or not x.is_contiguous() or (n is not None and x.numel() != n):
-        size = "" if n is None else f" of {n} elements"
-        raise ValueError(f"{what} must be a contiguous int32 tensor{size}")
-    return x.data_ptr()
-
-
 class KVPages:
     """A device-resident pool of n_pages pages of page_size slots, for n_layers
     layers of n_kv_heads heads.
@@ -60,6 +50,7 @@ class KVPages:
             raise RuntimeError(f"bmo_kv_pages_create failed: {err.decode() if err else 'unknown'}")
         self._h = h
         self._free = L.bmo_kv_pages_free  # (__del__ needs no module globals)
+        self._device = L.bmo_kv_pages_device(h)
         self.n_layers = n_layers
         self.n_pages = n_pages
         self.page_size = page_size
@@ -101,7 +92,22 @@ class KVPages:
         if rc != 0:
             raise RingError(fn, rc, self.last_error())
 
-    # -- rows -------------------------------------------------------------------
+    # -- arguments --------------------------------------------------------------
+    def _at(self, x, what: str) -> int:
+        """Address of a tensor of the pool's device."""
+        if x.get_device() != self._device:
+            raise ValueError(f"{what} must be on the pool's device ({self._device}), not on {x.device}")
+        return x.data_ptr()
+
+    def _ints(self, x, what: str, n: int | None = None) -> int | None:
+        """Address of a dense int32 tensor (of n elements), or None."""
+        if x is None:
+            return None
+        if (_NAMES.get(x.dtype) or _dtype(x)) != "int32" or not x.is_contiguous() or (n is not None and x.numel() != n):
+            size = "" if n is None else f" of {n} elements"
+            raise ValueError(f"{what} must be a contiguous int32 tensor{size}")
+        return self._at(x, what)
+
     def _rows(self, x, heads: int | None, what: str):
         """(address, stride, type, heads, tokens) of rows [tokens][heads][head_dim]."""
         shape = x.shape
@@ -111,46 +117,50 @@ class KVPages:
         stride = x.stride()
         if n and (stride[2] != 1 or (h > 1 and stride[1] != d)):
             raise ValueError(f"{what}: a token's heads must be contiguous")
-        return x.data_ptr(), stride[0] if n > 1 else 0, _type(x), h, n
+        if n > 1 and stride[0] < h * d:
+            raise ValueError(f"{what}: rows must not overlap (an expanded tensor)")
+        return self._at(x, what), stride[0] if n > 1 else 0, _type(x), h, n
 
     def _out(self, x, n: int, heads: int, type_: int):
         if x.shape != (n, heads, self.head_dim) or not x.is_contiguous() or _type(x) != type_:
             raise ValueError(f"out must be a contiguous [{n}][{heads}][{self.head_dim}] tensor of q's type")
-        return x.data_ptr()
+        return self._at(x, "out")
 
-    @staticmethod
-    def _table(lens, table):
+    def _table(self, lens, table):
         n, shape = lens.numel(), table.shape
         if len(shape) != 2 or shape[0] != n:
             raise ValueError("table must be [n_batch][max_pages]")
-        return n, _ints(lens, "lens"), _ints(table, "table"), shape[1]
+        return n, self._ints(lens, "lens"), self._ints(table, "table"), shape[1]
 
-    @staticmethod
-    def _work(workspace):
+    def _work(self, workspace):
         if workspace is None:
             return None, 0
-        return _ptr(workspace), workspace.numel() * workspace.element_size()
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+        return self._at(workspace, "workspace"), workspace.numel() * workspace.element_size()
 
     # -- plan -------------------------------------------------------------------
     def list_init(self, free, stream=None) -> None:
         """Makes free (int32 [n_pages + 2]) hold every page."""
         self._check("bmo_kv_pages_list_init", lib().bmo_kv_pages_list_init(
-            self._h, _ints(free, "free", self.n_pages + 2), _stream(stream)))
+            self._h, self._ints(free, "free", self.n_pages + 2), _stream(stream)))
 
     def plan(self, free, n_new, lens, table, tok_start=None, slots=None, positions=None, entries=None, status=None,
              stream=None) -> None:
         """n_new[b] more (or, negative, fewer) positions for every entry: lens,
         table and free become the new state; slots, positions and entries
-        [max_tok] tell the new tokens' places, tok_start [n_batch + 1] where an
-        entry's tokens begin, status [n_batch] 0 where it was done."""
+        [max_tok] tell the new tokens' places (append_decode needs none of them),
+        tok_start [n_batch + 1] where an entry's tokens begin, status [n_batch] 0
+        where it was done, 1 without pages, 2 out of range (or past max_tok)."""
         n, lens_p, table_p, width = self._table(lens, table)
-        sizes = {x.numel() for x in (slots, positions, entries) if x is not None}
+        sizes = {x.numel() for x in (slots, positions, entries) if x is not None} or {2**31 - 1}
         if len(sizes) > 1:
             raise ValueError("slots, positions and entries must have the same size")
         self._check("bmo_kv_pages_plan", lib().bmo_kv_pages_plan(
-            self._h, _ints(free, "free", self.n_pages + 2), n, _ints(n_new, "n_new", n), lens_p, table_p, width,
-            _ints(tok_start, "tok_start", n + 1), sizes.pop() if sizes else 0, _ints(slots, "slots"),
-            _ints(positions, "positions"), _ints(entries, "entries"), _ints(status, "status", n), _stream(stream)))
+            self._h, self._ints(free, "free", self.n_pages + 2), n, self._ints(n_new, "n_new", n), lens_p, table_p, width,
+            self._ints(tok_start, "tok_start", n + 1), sizes.pop(), self._ints(slots, "slots"),
+            self._ints(positions, "positions"), self._ints(entries, "entries"), self._ints(status, "status", n),
+            _stream(stream)))
 
     # -- rows in and out ----------------------------------------------------------
     def _slots(self, fn: str, call, layer: int, slots, k, v, stream) -> None:
@@ -159,7 +169,7 @@ class KVPages:
             shape = (n, self.n_kv_heads, self.head_dim // 32, 18)
             if tuple(k.shape) != shape or tuple(v.shape) != shape or not (k.is_contiguous() and v.is_contiguous()):
                 raise ValueError(f"blocks must be contiguous uint8 {shape}")
-            kp, vp, stride, type_, vtype = _ptr(k), _ptr(v), 0, 3, _type(v)
+            kp, vp, stride, type_, vtype = self._at(k, "k"), self._at(v, "v"), 0, 3, _type(v)
         else:
             kp, stride, type_, _, nk = self._rows(k, self.n_kv_heads, "k")
             vp, vstride, vtype, _, nv = self._rows(v, self.n_kv_heads, "v")
@@ -167,7 +177,7 @@ class KVPages:
                 raise ValueError("k and v must have one row a slot and the same stride")
         if vtype != type_:
             raise ValueError("k and v must have the same type")
-        self._check(fn, call(self._h, int(layer), n, _ints(slots, "slots"), type_, kp, vp, stride, _stream(stream)))
+        self._check(fn, call(self._h, int(layer), n, self._ints(slots, "slots"), type_, kp, vp, stride, _stream(stream)))
 
     def append(self, layer: int, slots, k, v, stream=None) -> None:
         """Quantizes rows k, v [n_tok][n_kv_heads][head_dim] (or copies uint8
@@ -219,6 +229,6 @@ class KVPages:
         n, lens_p, table_p, width = self._table(lens, table)
         qp, stride, type_, heads, rows = self._rows(q, None, "q")
         self._check("bmo_kv_pages_attend", lib().bmo_kv_pages_attend(
-            self._h, int(layer), n, _ints(q_start, "q_start", n + 1), lens_p, table_p, width, rows, heads, type_, qp,
+            self._h, int(layer), n, self._ints(q_start, "q_start", n + 1), lens_p, table_p, width, rows, heads, type_, qp,
             stride, self._out(out, rows, heads, type_), float(scale), int(bool(causal)), int(window), int(max_rows),
             int(max_len), *self._work(workspace), _stream(stream)))

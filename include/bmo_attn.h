@@ -481,6 +481,8 @@ BMO_ATTN_API bmo_kv_pages_t *bmo_kv_pages_create(int n_layers, int n_pages, int 
 /* NULL-safe. */
 BMO_ATTN_API void bmo_kv_pages_free(bmo_kv_pages_t *pages);
 BMO_ATTN_API int64_t bmo_kv_pages_bytes(const bmo_kv_pages_t *pages);
+/* The device that the pages are on (the one current at create); -1 for NULL. */
+BMO_ATTN_API int bmo_kv_pages_device(const bmo_kv_pages_t *pages);
 BMO_ATTN_API const char *bmo_kv_pages_last_error(const bmo_kv_pages_t *pages);
 
 /* Makes free_list [n_pages + 2] (device) hold every page: word 0 is the number
@@ -501,8 +503,9 @@ BMO_ATTN_API int bmo_kv_pages_list_init(bmo_kv_pages_t *pages, int *free_list, v
  *             entry: its slot and position (-1 for a refused entry) and entry
  *   status [n_batch]: 0 done, 1 no free pages, 2 out of range (a negative
  *             length, longer than the table, or tokens past max_tok)
- * These five may be NULL.  Table columns past an entry's length, and tokens
- * past the last, are left as they were.  A page belongs to one entry.  Calls
+ * These five may be NULL (max_tok bounds the tokens all the same).  Table
+ * columns past an entry's length, and tokens past the last, are left as they
+ * were.  A page belongs to one entry.  Calls
  * on one list must be ordered.  Asynchronous, allocates nothing, one launch. */
 BMO_ATTN_API int bmo_kv_pages_plan(bmo_kv_pages_t *pages, int *free_list, int n_batch,
                                    const int *n_new, int *lens, int *table, int max_pages,

@@ -2,11 +2,11 @@
 
 Bounds (per output, from the kernels' arithmetic):
 
-decode   fp32: a weight enters as two truncated fp16 parts (2^-21 of itself),
-         codes are exact, sums are fp32 (some hundred roundings of 2^-24 of at
+decode   fp32: a weight enters as two fp16 parts (2^-21 of itself, were the
+         parts truncated; they are rounded, 2^-22), codes are exact, sums are fp32 (some hundred roundings of 2^-24 of at
          most 8 sum p|d|): 2^-16 * 16 sum p|d| covers both; a score is off by at
-         most 2^-21 max|q| sum|k| (half a step of the query's 22 bits, the step
-         being at most 2^-20 of the row's largest) in log2 units, which moves a
+         most 2^-21 max|q| sum|k| (half a step of a query of 22 bits, the step
+         being at most 2^-20 of the row's largest; it has 23) in log2 units, which moves a
          weight and the sum by ln 2 of that each.  16 bits: a weight rounds to
          fp16, 2^-11 of sum p|v|, and the query has 15 bits, 2^-14 there.
 attend   V and the weights round to fp16 (2^-11 each; a weight below 2^-14 is

@@ -9,6 +9,23 @@ from bmo_jetson_amd import KVPages, RingError
 pytestmark = pytest.mark.gpu
 
 
+def _tiles(gpu, start, lens, table, rows):
+    """The same call with as many empty entries and as large a hint as make it
+    one of tiles (few rows are taken in sets of columns): q_start, lens, table,
+    max_rows."""
+    more = 64 - len(lens)
+    assert more >= 0
+    start = np.concatenate((start, [start[-1]] * more))
+    return (i32(gpu, start), i32(gpu, np.concatenate((lens, [0] * more))),
+            i32(gpu, np.concatenate((table, np.full((more, table.shape[1]), -1)))), max(256, *rows))
+
+
+def _calls(gpu, start, lens, table, rows, tiles):
+    if tiles:
+        return _tiles(gpu, start, lens, table, rows)
+    return i32(gpu, start), i32(gpu, lens), i32(gpu, table), max(rows)
+
+
 def _run(gpu, rows, lens, page, heads, kv, dim, type_="bfloat16", causal=True, window=0, seed=0, max_rows=None, tail=3,
          table_edit=None, cache_edit=None, workspace=True, scale=0.0, gap=1, tol=True):
     pages, cache, table = pool(gpu, lens, page, kv, dim, seed + 40)
@@ -19,15 +36,20 @@ def _run(gpu, rows, lens, page, heads, kv, dim, type_="bfloat16", causal=True, w
     total = sum(rows)
     packed, x = to_type(gpu, np.random.default_rng(seed).standard_normal((total + tail, heads + gap, dim)), type_)
     q = packed[:, :heads]
-    out = gpu.full((total + tail, heads, dim), 7.0, dtype=q.dtype, device="cuda")
     start = np.concatenate(([0], np.cumsum(rows)))
     work = None
     if workspace:
         work = gpu.full((pages.workspace_bytes(heads) // 4,), float("nan"), device="cuda")
-    pages.attend(0, i32(gpu, start), i32(gpu, lens), i32(gpu, table), q, out, causal=causal, window=window, scale=scale,
-                 max_rows=max(rows) if max_rows is None else max_rows, workspace=work, stream=gpu.cuda.current_stream())
-    got = out.double().cpu().numpy()
-    assert (got[total:] == 7.0).all()  # rows behind the last
+    calls = [_calls(gpu, start, lens, table, [max(rows) if max_rows is None else max_rows], False)]
+    if len(lens) <= 64:
+        calls.append(_tiles(gpu, start, lens, table, rows))
+    results = []
+    for start_d, lens_d, table_d, most in calls:
+        out = gpu.full((total + tail, heads, dim), 7.0, dtype=q.dtype, device="cuda")
+        pages.attend(0, start_d, lens_d, table_d, q, out, causal=causal, window=window, scale=scale, max_rows=most,
+                     workspace=work, stream=gpu.cuda.current_stream())
+        results.append(out.double().cpu().numpy())
+        assert (results[-1][total:] == 7.0).all()  # rows behind the last
     refs, bounds = np.zeros((total, heads, dim)), np.zeros((total, heads, dim))
     for b, (n, L) in enumerate(zip(rows, lens)):
         L = min(L, table.shape[1] * page)
@@ -35,10 +57,11 @@ def _run(gpu, rows, lens, page, heads, kv, dim, type_="bfloat16", causal=True, w
         a, e = attention(cache, table[b], page, L, x[start[b]:start[b + 1], :heads], last, window, "attend", type_,
                          scale or None)
         refs[start[b]:start[b + 1]], bounds[start[b]:start[b + 1]] = a, e
-    if tol:
-        check(got[:total], refs, bounds, f"rows {rows} lens {lens} heads {heads}/{kv}x{dim} page {page} causal {causal}")
-        # on the whole: the output's rounding, and 16-bit operands
-        assert rel(got[:total], refs) < {"bfloat16": 2.0**-8, "float16": 2.0**-9}[type_]
+    for got in results:
+        if tol:
+            check(got[:total], refs, bounds, f"rows {rows} lens {lens} heads {heads}/{kv}x{dim} page {page} causal {causal}")
+            # on the whole: the output's rounding, and 16-bit operands
+            assert rel(got[:total], refs) < {"bfloat16": 2.0**-8, "float16": 2.0**-9}[type_]
     pages.close()
     return got[:total], refs
 
@@ -112,22 +135,23 @@ def test_what_masked_positions_hold_does_not_show(gpu, rows, window):
 
 
 @pytest.mark.parametrize("rows,at", [(150, 90), (3, 98)])
-def test_a_value_that_is_not_finite_reaches_only_rows_that_see_it(gpu, rows, at):
+@pytest.mark.parametrize("tiles", [False, True])
+def test_a_value_that_is_not_finite_reaches_only_rows_that_see_it(gpu, rows, at, tiles):
     """V block 1 of position `at` is infinite: rows before it are as they are
     without it, later ones are not finite in that block alone."""
     page, kv, dim, heads = 32, 1, 128, 2
     L = max(rows, 100)
     pages, cache, table = pool(gpu, [L], page, kv, dim, 60)
     q = gpu.randn(rows, heads, dim, device="cuda").bfloat16()
-    start, lens, t = i32(gpu, [0, rows]), i32(gpu, [L]), i32(gpu, table)
+    start, lens, t, most = _calls(gpu, [0, rows], [L], table, [rows], tiles)
     want, out = gpu.zeros_like(q), gpu.zeros_like(q)
-    pages.attend(0, start, lens, t, q, want)
+    pages.attend(0, start, lens, t, q, want, max_rows=most)
     slot = i32(gpu, [slot_of(table, 0, at, page)])
     k, v = (gpu.zeros(1, kv, dim // 32, 18, dtype=gpu.uint8, device="cuda") for _ in range(2))
     pages.gather(0, slot, k, v)
     v[0, 0, 1, :2] = gpu.tensor([0, 0x7C], dtype=gpu.uint8)
     pages.append(0, slot, k, v)
-    pages.attend(0, start, lens, t, q, out)
+    pages.attend(0, start, lens, t, q, out, max_rows=most)
     gpu.cuda.synchronize()
     sees = L - rows + np.arange(rows) >= at
     assert 0 < sees.sum() < rows
@@ -149,50 +173,54 @@ def test_bad_page_ids_are_masked(gpu, rows):
     assert not got[rows[0]:].any()
 
 
-def test_nan_in_one_query_stays_in_its_row(gpu):
+@pytest.mark.parametrize("tiles", [False, True])
+def test_nan_in_one_query_stays_in_its_row(gpu, tiles):
     pages, cache, table = pool(gpu, [100], 64, 2, 128, 5)
     q = gpu.randn(50, 4, 128, device="cuda").half()
     out, want = gpu.zeros_like(q), gpu.zeros_like(q)
-    args = (0, i32(gpu, [0, 50]), i32(gpu, [100]), i32(gpu, table))
-    pages.attend(*args, q, want)
+    *args, most = _calls(gpu, [0, 50], [100], table, [50], tiles)
+    pages.attend(0, *args, q, want, max_rows=most)
     q[7, 2, 3] = float("nan")
-    pages.attend(*args, q, out)
+    pages.attend(0, *args, q, out, max_rows=most)
     bad = gpu.zeros(50, 4, dtype=gpu.bool, device="cuda")
     bad[7, 2] = True
     assert bool(out[bad].isnan().all()) and gpu.equal(out[~bad], want[~bad])
     pages.close()
 
 
-def test_starts_that_are_no_running_sum(gpu):
+@pytest.mark.parametrize("tiles", [False, True])
+def test_starts_that_are_no_running_sum(gpu, tiles):
     """Entries whose rows are not within q are skipped."""
     pages, cache, table = pool(gpu, [50, 50, 50], 64, 2, 64, 8)
     q = gpu.randn(20, 2, 64, device="cuda").half()
     for start in ([0, 30, 5, 10], [-4, 5, 10, 20], [2**31 - 1, 0, 2**31 - 1, -2**31]):
         out = gpu.full_like(q, 7.0)
-        pages.attend(0, i32(gpu, start), i32(gpu, [50] * 3), i32(gpu, table), q, out, causal=False)
+        *args, most = _calls(gpu, start, [50] * 3, table, [20], tiles)
+        pages.attend(0, *args, q, out, causal=False, max_rows=most)
         gpu.cuda.synchronize()
         if start[0] == 0:
             assert bool((out[:5] == 7.0).all()) and bool((out[10:] == 7.0).all())
     pages.close()
 
 
-def test_replayed_from_a_graph(gpu):
+@pytest.mark.parametrize("tiles", [False, True])
+def test_replayed_from_a_graph(gpu, tiles):
     for rows, heads in (([40, 200], 4), ([1, 2], 4)):
         lens = [900, 250]
         pages, cache, table = pool(gpu, lens, 64, 2, 128, 9)
         q = gpu.randn(sum(rows), heads, 128, device="cuda").half()
-        start, ln, t = i32(gpu, [0, rows[0], sum(rows)]), i32(gpu, lens), i32(gpu, table)
+        start, ln, t, most = _calls(gpu, [0, rows[0], sum(rows)], lens, table, rows, tiles)
         work, work2 = (gpu.zeros(pages.workspace_bytes(heads), dtype=gpu.uint8, device="cuda") for _ in range(2))
         out, eager = gpu.zeros_like(q), gpu.zeros_like(q)
         graph, side = gpu.cuda.CUDAGraph(), gpu.cuda.Stream()
         side.wait_stream(gpu.cuda.current_stream())
         with gpu.cuda.stream(side), gpu.cuda.graph(graph, stream=side):
-            pages.attend(0, start, ln, t, q, out, max_rows=max(rows), workspace=work, stream=gpu.cuda.current_stream())
+            pages.attend(0, start, ln, t, q, out, max_rows=most, workspace=work, stream=gpu.cuda.current_stream())
         gpu.cuda.current_stream().wait_stream(side)
         for _ in range(4):
             q.mul_(1.05)
             graph.replay()
-            pages.attend(0, start, ln, t, q, eager, max_rows=max(rows), workspace=work2, stream=gpu.cuda.current_stream())
+            pages.attend(0, start, ln, t, q, eager, max_rows=most, workspace=work2, stream=gpu.cuda.current_stream())
             gpu.cuda.synchronize()
             assert gpu.equal(out, eager) and bool(out.any())
         pages.close()
