@@ -56,6 +56,7 @@ constexpr int kWaves = 4;  // of a workgroup, where it is not one
 constexpr int kFillWaves = 1024, kFillSteps = 4;
 constexpr int kSplitWaves = 4096, kSplitSteps = 16;
 constexpr int kMaxRuns = 128;  // of an entry
+constexpr int kLowUnits = 512, kLowSteps = 64;  // see there
 
 struct DecodeArgs {
     PagesDecodeParams p;
@@ -669,9 +670,7 @@ namespace {
 // Columns are (head, block) while there are that few heads (or rows and heads).
 bool spread(const PagesGeom &g, int heads) { return heads <= 16 / (g.dim / kQK); }
 int set_heads(const PagesGeom &g, int heads) { return spread(g, heads) ? 16 / (g.dim / kQK) : 16; }
-int64_t part_bytes(const PagesGeom &g, int heads) {
-    return (int64_t) set_heads(g, heads) * (g.dim + 2 * (g.dim / kQK)) * 4;
-}
+int64_t part_bytes(const PagesGeom &g, int hc) { return (int64_t) hc * (g.dim + 2 * (g.dim / kQK)) * 4; }
 
 template <int D, bool SPREAD, bool MULTI>
 const void *kernel_of(int nw, int type) {
@@ -701,6 +700,13 @@ hipError_t launch_of(const DecodeArgs &arg, int nw, hipStream_t stream) {
 //   one wave a unit or four:  2048 units x 16 steps 27.9 / 31.2, 8192 x 7
 //     48 / 68, 1024 x 16 18.2 / 18.7; 2048 x 32 53.9 / 54.9, x 63 100 / 97,
 //     of 3 to 63 steps 77 / 60 (a long unit's one wave is the last to end).
+//   more than 4 heads (rows) a kv head in sets of 16 or of 4, while these are no
+//     more than two workgroups a CU and 64 steps long, dim 128 (whose sets of
+//     16 hold two waves a SIMD and multiply every head with every block):  one
+//     entry, 8 heads on each of 4 kv heads, 150 positions 7.7 / 5.7, 600 11.8 /
+//     8.3, 1500 16.4 / 12.3, 12 entries of 1500 17.9 / 13.2; rows of one entry
+//     of 32 kv heads, 600 positions, 12 rows 13 / 9, 64 rows 14 / 12; past the
+//     limits 96 sets x 125 steps 18 / 21, 960 x 19 18 / 20.
 //   runs of at least 4 steps a wave, of 16, or nothing cut:  32 units x 94
 //     steps 11.2 / 21.6 / 21.6, x 250 14.5 / 16.8 / 49, 8 x 1000 17.7 / 18.7 /
 //     184; 256 x 32 13.7 / 10.7 / 10.7, 512 x 32 21.5 / 16.3 / 16.2; 96 units
@@ -711,20 +717,23 @@ hipError_t launch_units(const PagesDecodeParams &p, int heads, hipStream_t strea
     a.p = p;
     a.group = p.n_heads / p.g.n_kv;
     a.div_group = make_fastdiv((uint32_t) a.group);
-    const int hc = set_heads(p.g, heads);
-    a.n_hs = (heads + hc - 1) / hc;
-    a.units = p.g.n_kv * a.n_hs;
     a.append = p.k_new != nullptr;
     a.max_runs = 1;
-    const int64_t units = (int64_t) p.n_batch * a.units;
     int64_t longest = (int64_t) p.max_pages << p.g.page_shift;
     if (p.max_len > 0 && p.max_len < longest) longest = p.max_len;
     const int64_t seen = (int64_t) p.window + (MULTI ? p.max_rows : 0) + kStep;
     if (p.window > 0 && seen < longest) longest = seen;
     const int64_t steps = (longest + kStep - 1) / kStep;
+    const int narrow = 16 / (p.g.dim / kQK);
+    const bool low = p.g.dim == 128 && steps <= kLowSteps &&
+                     (int64_t) p.n_batch * p.g.n_kv * ((heads + narrow - 1) / narrow) <= kLowUnits;
+    const int hc = low ? narrow : set_heads(p.g, heads);
+    a.n_hs = (heads + hc - 1) / hc;
+    a.units = p.g.n_kv * a.n_hs;
+    const int64_t units = (int64_t) p.n_batch * a.units;
     const int nw = units >= 1024 && steps <= 24 ? 1 : kWaves;
     if (nw == kWaves && p.work) {
-        const int64_t room = p.work_bytes / part_bytes(p.g, heads) / units;  // runs that it holds
+        const int64_t room = p.work_bytes / part_bytes(p.g, hc) / units;  // runs that it holds
         const int64_t fill = std::min<int64_t>(kFillWaves / kWaves / units, steps / (kFillSteps * kWaves));
         const int64_t split = std::min<int64_t>(kSplitWaves / kWaves / units, steps / (kSplitSteps * kWaves));
         const int64_t runs = std::min({std::max(fill, split), room, (int64_t) kMaxRuns});
@@ -744,7 +753,7 @@ hipError_t launch_units(const PagesDecodeParams &p, int heads, hipStream_t strea
 // heads have four times as long results and a quarter of the units.
 int64_t pages_work_bytes(const PagesGeom &g, int n_heads) {
     const int group = n_heads / g.n_kv;
-    return kSplitWaves / kWaves / (spread(g, group) ? 1 : 4) * part_bytes(g, group);
+    return kSplitWaves / kWaves / (spread(g, group) ? 1 : 4) * part_bytes(g, set_heads(g, group));
 }
 
 hipError_t launch_pages_decode(const PagesDecodeParams &p, hipStream_t stream) {

@@ -41,6 +41,11 @@ def _run(gpu, rows, lens, page, heads, kv, dim, type_="bfloat16", causal=True, w
     if workspace:
         work = gpu.full((pages.workspace_bytes(heads) // 4,), float("nan"), device="cuda")
     calls = [_calls(gpu, start, lens, table, [max(rows) if max_rows is None else max_rows], False)]
+    # with a table of so many empty columns that sets of columns are shaped for long entries
+    calls.append(_calls(gpu, start, lens, np.concatenate([table, np.full((len(lens), 2100 // page), -1)], axis=1),
+                        [calls[0][3]], False))
+    if table_edit is not None:
+        calls.pop()  # (an edited table's own width counts)
     if len(lens) <= 64:
         calls.append(_tiles(gpu, start, lens, table, rows))
     results = []
