@@ -23,18 +23,25 @@
 //
 // Measured, 32 query heads on 8 of 128: eight chunks of 200 to 1024 rows over
 // 300 to 4000 positions 321 us, 763 TFLOP/s; of 1024 rows over 4096 positions
-// each about 840 (a large library product reaches 1173).  Bound by issue:
-// of a SIMD's cycles 52% are VALU (exponentials, dequantizing, masks) and 37%
-// matrix instructions, two waves a SIMD.  Eight waves a workgroup (half the
+// each 690 us, 800 TFLOP/s (a large library product reaches 1173).  Bound by
+// the card's power: the clock stands at 1.99 GHz (1.5 in that library
+// product), with 52% of a SIMD's cycles VALU (exponentials, dequantizing,
+// masks) and 37% matrix instructions, two waves a SIMD.  So less work helps
+// and another order of it does not: dequantizing and the weights between the
+// matrix instructions, or without the LDS reads, run as long; without
+// dequantizing 20% less.  Eight waves a workgroup (half the
 // dequantizing a row) win 4% with full tiles of one length and lose 10% with
 // ragged ones; stages of 32 with three waves a SIMD are 16% slower, scores one
 // stage ahead of the weights 5%.
 //
-// Precision: K and V enter as (code - 8) * d rounded to fp16, the weights as
-// fp16, sums in fp32; q enters scaled by its row's own power of two, exactly.
-// That is below the rounding of the 16-bit outputs (2e-4 against 2e-3 for
-// bf16).  K and V must lie in fp16's range; a V block whose scale is not
-// finite makes the rows that see it NaN in that block and leaves the others.
+// Precision: V enters as (code - 8) * d rounded to fp16, the weights as fp16,
+// sums in fp32; q enters scaled by its row's own power of two, exactly.  K does
+// as V for bf16 rows, whose own rounding (1.7e-3) hides it.  For fp16 rows
+// (2.1e-4) it would show where scores are large (3.2e-4 in all, and more the
+// larger they are), so K's codes enter exactly and its scales meet the products
+// of each block in fp32: 787 us where 677 were, see above.  V (and K of bf16
+// rows) must lie in fp16's range; a V block whose scale is not finite makes the
+// rows that see it NaN in that block and leaves the others.
 #include <algorithm>
 
 #include "kernels.hpp"
@@ -103,7 +110,9 @@ __device__ __forceinline__ bool finite16(uint32_t h) { return (h & 0x7C00u) != 0
 
 }  // namespace
 
-template <int D>
+// FINE (fp16 rows): K's codes enter as they are and its scales meet the
+// products of each block in fp32.
+template <int D, bool FINE>
 __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_eu(2))) void pages_attend_kernel(AttendArgs a) {
     constexpr int NW = kAttendWaves;
     constexpr int NB = D / kQK;
@@ -119,6 +128,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_
 
     __shared__ __align__(16) _Float16 s_k[2][kStage * KROW];
     __shared__ __align__(16) _Float16 s_v[2][D * VROW];
+    __shared__ __align__(8) _Float16 s_d[FINE ? 2 : 1][FINE ? NB * kStage : 4];  // K's scales, [block][key]
     __shared__ int s_flag[2][NW];  // nonzero: a bad page, or a V scale that is not finite
 
     const int lane = threadIdx.x & 63;
@@ -204,8 +214,13 @@ __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_
                 // row of the key, octet `oct` of the block
                 const int t = i / NB, blk = i % NB;
                 const _Float16 d = __builtin_bit_cast(_Float16, (uint16_t) kd[i]);
-                const pg_half8 x = k_octet(kw[i], pat) * pg_half8{d, d, d, d, d, d, d, d};
+                pg_half8 x = k_octet(kw[i], pat);
                 const int key = my_group * G + t * 16 + key16;
+                if constexpr (FINE) {
+                    if (oct == 0) s_d[buf][blk * kStage + key] = d;
+                } else {
+                    x *= pg_half8{d, d, d, d, d, d, d, d};
+                }
                 *reinterpret_cast<pg_half8 *>(&s_k[buf][key * KROW + (blk * 4 + oct) * 8]) = x;
             }
         }
@@ -299,28 +314,55 @@ __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_
     auto multiply = [&](int buf, int base, bool edge, uint32_t bad_groups) {
         constexpr int NU = kStage / 32;
         pg_float16 s[NU];
+        constexpr int N = KK * NU, AHEAD = FINE ? 4 : 8;
+        auto kx = [&](int i) {
+            return *reinterpret_cast<const pg_half8 *>(&s_k[buf][((i % NU) * 32 + n) * KROW + ((i / NU) * 2 + half) * 8]);
+        };
+        pg_half8 kring[AHEAD];
 #pragma unroll
-        for (int u = 0; u < NU; ++u)
+        for (int i = 0; i < AHEAD; ++i) kring[i] = kx(i);
+        if constexpr (!FINE) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) s[u][j] = 0.0f;
-        {
-            constexpr int N = KK * NU, AHEAD = 8;
-            auto kx = [&](int i) {
-                return *reinterpret_cast<const pg_half8 *>(&s_k[buf][((i % NU) * 32 + n) * KROW + ((i / NU) * 2 + half) * 8]);
-            };
-            pg_half8 ring[AHEAD];
+            for (int u = 0; u < NU; ++u)
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) ring[i] = kx(i);
+                for (int j = 0; j < 16; ++j) s[u][j] = 0.0f;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                s[i % NU] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[i % AHEAD], q[i / NU], s[i % NU], 0, 0, 0);
-                if (i + AHEAD < N) ring[i % AHEAD] = kx(i + AHEAD);
+                s[i % NU] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kring[i % AHEAD], q[i / NU], s[i % NU], 0, 0, 0);
+                if (i + AHEAD < N) kring[i % AHEAD] = kx(i + AHEAD);
             }
             __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 if (i + AHEAD < N) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+        } else {
+            // two products of 16 elements a block, then the block's scales
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk) {
+                pg_float16 t[NU];
+#pragma unroll
+                for (int u = 0; u < NU; ++u)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) t[u][j] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 2 * NU; ++k) {
+                    const int i = blk * 2 * NU + k;
+                    t[i % NU] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kring[i % AHEAD], q[i / NU], t[i % NU], 0, 0, 0);
+                    if (i + AHEAD < N) kring[i % AHEAD] = kx(i + AHEAD);
+                }
+#pragma unroll
+                for (int u = 0; u < NU; ++u)
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        const pg_half4 d = *reinterpret_cast<const pg_half4 *>(
+                            &s_d[buf][blk * kStage + u * 32 + 2 * j + 4 * half]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            s[u][j + e] = blk == 0 ? (float) d[e] * t[u][j + e]
+                                                   : __builtin_fmaf((float) d[e], t[u][j + e], s[u][j + e]);
+                    }
             }
         }
         // register j of tile u holds key 32 u + 8 (j / 4) + 4 half + j % 4
@@ -352,13 +394,13 @@ __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_
 #pragma unroll
                 for (int j = 0; j < 16; ++j) acc[i][j] *= alpha;
         }
-        constexpr int N = NB * 2 * NU, AHEAD = NB == 4 ? 8 : 4;
+        constexpr int NV = NB * 2 * NU, VAHEAD = NB == 4 ? 8 : 4;
         auto vx = [&](int i) {  // 2 NU runs of 16 keys, NB blocks of elements each
             return *reinterpret_cast<const pg_half8 *>(&s_v[buf][((i % NB) * kQK + n) * VROW + (i / NB) * 16 + half * 8]);
         };
-        pg_half8 ring[AHEAD], w[2 * NU];
+        pg_half8 ring[VAHEAD], w[2 * NU];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) ring[i] = vx(i);
+        for (int i = 0; i < VAHEAD; ++i) ring[i] = vx(i);
         const pg_half2 one = {(_Float16) 1.0f, (_Float16) 1.0f};
 #pragma unroll
         for (int r = 0; r < 2 * NU; ++r) {
@@ -375,9 +417,9 @@ __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_
             }
         }
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            acc[i % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[i % AHEAD], w[i / NB], acc[i % NB], 0, 0, 0);
-            if (i + AHEAD < N) ring[i % AHEAD] = vx(i + AHEAD);
+        for (int i = 0; i < NV; ++i) {
+            acc[i % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[i % VAHEAD], w[i / NB], acc[i % NB], 0, 0, 0);
+            if (i + VAHEAD < NV) ring[i % VAHEAD] = vx(i + VAHEAD);
         }
     };
 
@@ -506,9 +548,12 @@ hipError_t launch_pages_attend(const PagesAttendParams &p, hipStream_t stream) {
     const int64_t tiles = std::min(((int64_t) p.n_rows * a.group) / kTileRows + p.n_batch,
                                    p.n_batch * (((int64_t) max_rows * a.group + kTileRows - 1) / kTileRows));
     void *args[] = {&a};
-    return hipLaunchKernel(p.g.dim == 128 ? reinterpret_cast<const void *>(pages_attend_kernel<128>)
-                                          : reinterpret_cast<const void *>(pages_attend_kernel<64>),
-                           dim3((unsigned) (tiles * p.g.n_kv)), dim3(64 * kAttendWaves), args, 0, stream);
+    const bool fine = p.type == kTypeF16;
+    const void *kernel = p.g.dim == 128 ? fine ? reinterpret_cast<const void *>(pages_attend_kernel<128, true>)
+                                               : reinterpret_cast<const void *>(pages_attend_kernel<128, false>)
+                         : fine         ? reinterpret_cast<const void *>(pages_attend_kernel<64, true>)
+                                        : reinterpret_cast<const void *>(pages_attend_kernel<64, false>);
+    return hipLaunchKernel(kernel, dim3((unsigned) (tiles * p.g.n_kv)), dim3(64 * kAttendWaves), args, 0, stream);
 }
 
 }  // namespace bmo

@@ -568,8 +568,8 @@ BMO_ATTN_API int bmo_kv_pages_append_decode(bmo_kv_pages_t *pages, int layer, in
  * positions (an encoder's states, of another length).  window: as in decode,
  * counted back from the row's last position.  Rows that see nothing are
  * zeros.  max_rows: no entry has more rows (0: not known; rows past it may be
- * left as they were), max_len as in decode.  Scores and sums in fp32, K, V and
- * weights in fp16 on the matrix cores. */
+ * left as they were), max_len as in decode.  Scores and sums in fp32; V, the
+ * weights and for bf16 rows K enter the matrix cores in fp16. */
 BMO_ATTN_API int bmo_kv_pages_attend(bmo_kv_pages_t *pages, int layer, int n_batch,
                                      const int *q_start, const int *lens, const int *table,
                                      int max_pages, int n_rows, int n_heads, int type,

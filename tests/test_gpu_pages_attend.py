@@ -278,3 +278,22 @@ def test_few_and_many_rows_agree(gpu):
         # both are within a rounding (2^-11) and the operands' (2^-10) of the exact ones
         assert rel(b[rows].double().cpu().numpy(), a[rows].double().cpu().numpy()) < 2.0**-9
     pages.close()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("tiles", [False, True])
+def test_fp16_scores_are_as_exact_as_fp32(gpu, dim, tiles):
+    """Queries 16 times as large: keys rounded to fp16 would be off by 2^-12 of
+    scores around 16 to 100.  Three roundings to 11 bits remain (the output, V,
+    the weights), each at most 2^-11 / sqrt(3) of the whole in the mean square
+    when they are independent: 2^-11 together."""
+    rows, lens = [40, 300], [700, 700]
+    pages, cache, table = pool(gpu, lens, 64, 2, dim, 77)
+    q, x = to_type(gpu, 16 * np.random.default_rng(6).standard_normal((340, 4, dim)), "float16")
+    out = gpu.zeros_like(q)
+    *args, most = _calls(gpu, [0, 40, 340], lens, table, rows, tiles)
+    pages.attend(0, *args, q, out, max_rows=most, stream=gpu.cuda.current_stream())
+    ref = np.concatenate([attention(cache, table[b], 64, 700, x[at:at + n], list(range(700 - n, 700)), 0, "attend",
+                                    "float16")[0] for b, (at, n) in enumerate(((0, 40), (40, 300)))])
+    assert rel(out.double().cpu().numpy(), ref) < 2.0**-11
+    pages.close()
