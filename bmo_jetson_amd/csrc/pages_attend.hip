@@ -470,11 +470,12 @@ __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_
     }
     l += __shfl_xor(l, 32);
     if (!row_ok) return;
-    const float inv = l > 0.0f ? 1.0f / l : l * 0.0f;  // (NaN stays)
+    const float inv = l > 0.0f ? 1.0f / l : hi > lo ? l * 0.0f : 0.0f;  // (NaN stays)
     uint16_t *out = static_cast<uint16_t *>(p.out) + ((int64_t) (start + tok) * p.n_heads + head) * D;
 #pragma unroll
     for (int blk = 0; blk < NB; ++blk) {
         const float scale = (poison >> blk) & 1 ? __builtin_nanf("") : inv;
+        if (hi <= lo) acc[blk] = pg_float16{};  // sees nothing: zeros whatever the query holds
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             uint32_t w[2];

@@ -599,8 +599,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
             o = __builtin_fmaf(f, s_out[w][rr][e], o);
         }
         if (un.runs == 1) {
-            const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-            store1(p.out, column_of<MULTI, D>(a, un, b, rr).out + e, o * inv, type);
+            const Column c = column_of<MULTI, D>(a, un, b, rr);
+            // (a row that sees nothing is zeros whatever its query holds)
+            store1(p.out, c.out + e, L > 0.0f ? o * (1.0f / L) : c.hi > c.lo ? o * 0.0f : 0.0f, type);
         } else {
             float *dst = p.work + (int64_t) blockIdx.x * part_floats<D>(HC);
             dst[rr * D + e] = o;
@@ -661,7 +662,8 @@ __global__ __launch_bounds__(256) void pages_join_kernel(DecodeArgs a) {
     __syncthreads();
     if (threadIdx.x < D) {
         const int e = threadIdx.x;
-        store1(p.out, column_of<MULTI, D>(a, un, b, rr).out + e, (s_o[0][e] + s_o[1][e]) + (s_o[2][e] + s_o[3][e]), p.type);
+        const Column c = column_of<MULTI, D>(a, un, b, rr);
+        store1(p.out, c.out + e, c.hi > c.lo ? (s_o[0][e] + s_o[1][e]) + (s_o[2][e] + s_o[3][e]) : 0.0f, p.type);
     }
 }
 

@@ -297,3 +297,27 @@ def test_fp16_scores_are_as_exact_as_fp32(gpu, dim, tiles):
                                     "float16")[0] for b, (at, n) in enumerate(((0, 40), (40, 300)))])
     assert rel(out.double().cpu().numpy(), ref) < 2.0**-11
     pages.close()
+
+
+@pytest.mark.parametrize("tiles", [False, True])
+@pytest.mark.parametrize("long", [False, True])
+def test_rows_that_see_nothing_are_zeros_whatever_their_queries_hold(gpu, tiles, long):
+    """A causal chunk longer than its entry: NaN and infinities in the rows
+    before position 0, beside rows that see something."""
+    lens, rows = [3000 if long else 5, 5], [40, 40]
+    pages, cache, table = pool(gpu, lens, 64, 2, 128, 31)
+    q = gpu.randn(80, 4, 128, device="cuda").half()
+    want, out = gpu.zeros_like(q), gpu.full_like(q, 7.0)
+    *args, most = _calls(gpu, [0, 40, 80], lens, table, rows, tiles)
+    work = gpu.zeros(pages.workspace_bytes(4), dtype=gpu.uint8, device="cuda")
+    pages.attend(0, *args, q, want, max_rows=most, workspace=work)
+    blind = gpu.zeros(80, dtype=gpu.bool, device="cuda")
+    blind[40:75] = True
+    if not long:
+        blind[:35] = True
+    q[blind] = float("nan")
+    q[42] = float("inf")
+    pages.attend(0, *args, q, out, max_rows=most, workspace=work)
+    gpu.cuda.synchronize()
+    assert not bool(out[blind].any()) and gpu.equal(out[~blind], want[~blind])
+    pages.close()
