@@ -62,6 +62,7 @@ constexpr int kStage = 64;  // positions a stage
 struct AttendArgs {
     PagesAttendParams p;
     int group;          // query heads a kv head
+    int max_rows;       // of an entry
     FastDiv div_group;
 };
 
@@ -79,7 +80,9 @@ __device__ __forceinline__ bool find_tile(const AttendArgs &a, int tile, int siz
     int before = 0;
     for (int b0 = 0; b0 < a.p.n_batch; b0 += 64) {
         int b = b0 + lane;
-        int rows = b < a.p.n_batch ? entry_rows(a, b) * a.group : 0;
+        // (an entry with more rows than the call was said to have takes no
+        // tile from the others)
+        int rows = b < a.p.n_batch ? min(entry_rows(a, b), a.max_rows) * a.group : 0;
         if (a.p.n_batch <= 64) {
             const int key = rows > 0 ? max(a.p.lens[b], 0) : -1;
             int rank = 0;
@@ -543,6 +546,7 @@ hipError_t launch_pages_attend(const PagesAttendParams &p, hipStream_t stream) {
     AttendArgs a{};
     a.p = p;
     a.group = p.n_heads / p.g.n_kv;
+    a.max_rows = max_rows;
     a.div_group = make_fastdiv((uint32_t) a.group);
     // tiles: no more than the rows' and one more an entry, nor than every
     // entry's at its most rows

@@ -321,3 +321,21 @@ def test_rows_that_see_nothing_are_zeros_whatever_their_queries_hold(gpu, tiles,
     gpu.cuda.synchronize()
     assert not bool(out[blind].any()) and gpu.equal(out[~blind], want[~blind])
     pages.close()
+
+
+def test_more_rows_than_said_leave_the_others_whole(gpu):
+    for rows, said in (([300, 2, 2, 2], 2), ([2, 700, 300, 33], 40)):
+        lens = [700] * 64
+        pages, cache, table = pool(gpu, lens, 64, 8, 64, 12)
+        rows = rows + [0] * 60
+        start = np.concatenate(([0], np.cumsum(rows)))
+        q = gpu.randn(sum(rows), 16, 64, device="cuda").half()
+        want, out = gpu.zeros_like(q), gpu.full_like(q, 7.0)
+        args = (0, i32(gpu, start), i32(gpu, lens), i32(gpu, table), q)
+        pages.attend(*args, want, max_rows=max(rows), stream=gpu.cuda.current_stream())
+        pages.attend(*args, out, max_rows=said, stream=gpu.cuda.current_stream())
+        for b, n in enumerate(rows):
+            part = slice(start[b], start[b] + min(n, said))
+            # (the two calls may be shaped differently: roundings of 16-bit operands)
+            assert rel(out[part].double().cpu().numpy(), want[part].double().cpu().numpy()) < 2.0**-9
+        pages.close()
