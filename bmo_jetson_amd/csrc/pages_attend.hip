@@ -29,10 +29,10 @@
 // masks) and 37% matrix instructions, two waves a SIMD.  So less work helps
 // and another order of it does not: dequantizing and the weights between the
 // matrix instructions, or without the LDS reads, run as long; without
-// dequantizing 20% less.  Eight waves a workgroup (half the
-// dequantizing a row) win 4% with full tiles of one length and lose 10% with
-// ragged ones; stages of 32 with three waves a SIMD are 16% slower, scores one
-// stage ahead of the weights 5%.
+// dequantizing 20% less.  Eight waves a workgroup (half the dequantizing a row)
+// win 4% with full tiles of one length and lose 10% with ragged ones; stages of
+// 32 with three waves a SIMD are 16% slower, scores one stage ahead of the
+// weights 5%.
 //
 // Precision: V enters as (code - 8) * d rounded to fp16, the weights as fp16,
 // sums in fp32; q enters scaled by its row's own power of two, exactly.  K does

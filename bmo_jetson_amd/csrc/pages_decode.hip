@@ -1,4 +1,4 @@
-// pages_decode.hip -- attention of one row per entry over its pages.
+// pages_decode.hip -- attention of one or few rows per entry over its pages.
 //
 // o = sum_j p_j v_j, p = softmax(scale q . k_j) over the entry's last
 // min(len, window) positions.  HBM bounds it: 2 * 18 bytes per 32 elements of
@@ -9,7 +9,10 @@
 // operands of the matrix instructions.  The 16 columns of the products hold
 //   (head r, block b): heads of the kv head's group, up to 16 / NB of them,
 //                      each column with the query of its own block only; or
-//   head r:            up to 16 heads, when the group has more than 16 / NB.
+//   head r:            up to 16 heads, when the group has more than 16 / NB
+//                      (short calls of dim 128 take it in sets of 4 instead).
+// Ragged rows (attend's calls with few of them) are taken as heads are: a
+// column is a (token, head of the group) with limits of its own.
 // In the first form a lane has one block's products, so the block scales cost
 // one multiply a score and one a weight instead of NB each.
 //
@@ -50,7 +53,7 @@ namespace {
 
 constexpr int kStep = 32;  // positions a wave step
 constexpr int kWaves = 4;  // of a workgroup, where it is not one
-// How a launch is cut, see launch_pages_decode: waves of a launch that fills
+// How a launch is cut, see launch_units: waves of a launch that fills
 // the card once (few units) and the fewest steps of a run for each of them,
 // and the same for launches of several rounds.
 constexpr int kFillWaves = 1024, kFillSteps = 4;

@@ -12,7 +12,6 @@ namespace bmo {
 typedef _Float16 pg_half2 __attribute__((ext_vector_type(2)));
 typedef _Float16 pg_half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 pg_bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 pg_bf16x8 __attribute__((ext_vector_type(8)));
 typedef float pg_float4 __attribute__((ext_vector_type(4)));
 
 constexpr float kPagesLazy = 8.0f;       // lazy rescale threshold, log2 units
@@ -49,11 +48,6 @@ __device__ __forceinline__ pg_half8 k_octet(uint32_t w, const Patterns &p) {
     const pg_half2 a = codes_lo(w, p), b = codes_lo(y, p), c = codes_hi(w, p), d = codes_hi(y, p);
     return pg_half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
-
-template <bool B>
-struct Flag {
-    static constexpr bool value = B;
-};
 
 // p[i] at a wave-uniform index through the scalar cache, for arrays that no
 // kernel writes while the reading one runs (lengths, tables).

@@ -505,8 +505,8 @@ BMO_ATTN_API int bmo_kv_pages_list_init(bmo_kv_pages_t *pages, int *free_list, v
  *             length, longer than the table, or tokens past max_tok)
  * These five may be NULL (max_tok bounds the tokens all the same).  Table
  * columns past an entry's length, and tokens past the last, are left as they
- * were.  A page belongs to one entry.  Calls
- * on one list must be ordered.  Asynchronous, allocates nothing, one launch. */
+ * were.  A page belongs to one entry.  Calls on one list must be ordered.
+ * Asynchronous, allocates nothing, one launch. */
 BMO_ATTN_API int bmo_kv_pages_plan(bmo_kv_pages_t *pages, int *free_list, int n_batch,
                                    const int *n_new, int *lens, int *table, int max_pages,
                                    int *tok_start, int max_tok, int *tok_slot, int *tok_pos,
