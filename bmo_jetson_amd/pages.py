@@ -6,26 +6,22 @@ from __future__ import annotations
 from ._lib import lib
 from .ring import RingError, _stream
 
-_TYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "uint8": 3}
+_TYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "uint8": 3, "int32": 4}  # (int32: lengths, tables, slots)
+_CODES: dict = {}  # by dtype object (formatting one's name costs as much as a call)
 
 
-_NAMES: dict = {}  # dtype objects' names (formatting one costs as much as a call)
-
-
-def _dtype(x) -> str:
-    """The name of a tensor's element type."""
-    d = getattr(x, "dtype", None)
-    name = _NAMES.get(d)
-    if name is None:
-        name = _NAMES[d] = str(d).rsplit(".", 1)[-1]
-    return name
+def _code(x) -> int:
+    code = _CODES.get(x.dtype)
+    if code is None:
+        code = _CODES[x.dtype] = _TYPES.get(str(x.dtype).rsplit(".", 1)[-1], 5)
+    return code
 
 
 def _type(x) -> int:
-    """The element type (BMO_ATTN_F32 ..) of a tensor."""
-    code = _TYPES.get(_NAMES.get(x.dtype) or _dtype(x))
-    if code is None:
-        raise TypeError(f"expected a float32, float16, bfloat16 or uint8 tensor, got {_dtype(x)}")
+    """The element type (BMO_ATTN_F32 ..) of a tensor of rows or blocks."""
+    code = _code(x)
+    if code > 3:
+        raise TypeError(f"expected a float32, float16, bfloat16 or uint8 tensor, got {x.dtype}")
     return code
 
 
@@ -103,10 +99,10 @@ class KVPages:
         """Address of a dense int32 tensor (of n elements), or None."""
         if x is None:
             return None
-        if (_NAMES.get(x.dtype) or _dtype(x)) != "int32" or not x.is_contiguous() or (n is not None and x.numel() != n):
+        if _code(x) != 4 or not x.is_contiguous() or (n is not None and x.numel() != n):
             size = "" if n is None else f" of {n} elements"
             raise ValueError(f"{what} must be a contiguous int32 tensor{size}")
-        return self._at(x, what)
+        return x.data_ptr() if x.get_device() == self._device else self._at(x, what)
 
     def _rows(self, x, heads: int | None, what: str):
         """(address, stride, type, heads, tokens) of rows [tokens][heads][head_dim]."""
@@ -119,7 +115,8 @@ class KVPages:
             raise ValueError(f"{what}: a token's heads must be contiguous")
         if n > 1 and stride[0] < h * d:
             raise ValueError(f"{what}: rows must not overlap (an expanded tensor)")
-        return self._at(x, what), stride[0] if n > 1 else 0, _type(x), h, n
+        at = x.data_ptr() if x.get_device() == self._device else self._at(x, what)
+        return at, stride[0] if n > 1 else 0, _type(x), h, n
 
     def _out(self, x, n: int, heads: int, type_: int):
         if x.shape != (n, heads, self.head_dim) or not x.is_contiguous() or _type(x) != type_:

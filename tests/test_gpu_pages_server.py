@@ -220,3 +220,48 @@ def test_a_small_workspace_cuts_less(gpu):
                 check(got[b:b + 1], ref, bound, f"{size} bytes, entry {b}")
             assert bool((guard[size // 4:] == 5.0).all())
     s.pages.close()
+
+
+@pytest.mark.parametrize("dim,heads", [(128, 16), (64, 16)])
+def test_pages_past_32_bits_of_bytes(gpu, dim, heads):
+    """The last pages of a pool of 5 GB give the bits that the first ones of a
+    small pool give, in every kernel."""
+    kv, page, lens, stream = 8, 1024, [1500, 90], gpu.cuda.current_stream()
+    n_pages = 5 * 2**30 // (kv * page * dim * 36 // 32)
+    rows = sum(lens)
+    k, v = gpu.randn(rows, kv, dim, device="cuda"), gpu.randn(rows, kv, dim, device="cuda")
+    new = gpu.randn(2, heads + 2 * kv, dim, device="cuda")
+    results = []
+    for pages, first in ((KVPages(1, 4, page, kv, dim), 0), (KVPages(1, n_pages, page, kv, dim), n_pages - 3)):
+        table = np.array([[first + 2, first], [first + 1, -1]])
+        pos = np.concatenate([np.arange(n) for n in lens])
+        entry = np.repeat([0, 1], lens)
+        slots = table[entry, pos // page] * page + pos % page
+        table = i32(gpu, table)
+        pages.append(0, i32(gpu, slots), k, v, stream=stream)
+        got = []
+        for type_ in ("float32", "bfloat16"):
+            q = new[:, :heads].to(getattr(gpu, type_))
+            out = gpu.zeros_like(q)
+            pages.decode(0, i32(gpu, lens), table, q, out, stream=stream)
+            got.append(out)
+        x = new.half()
+        out = gpu.zeros(2, heads, dim, dtype=gpu.half, device="cuda")
+        pages.append_decode(0, i32(gpu, [n + 1 for n in lens]), table, x[:, :heads], x[:, heads:heads + kv],
+                            x[:, heads + kv:], out, stream=stream)
+        got.append(out)
+        back = [gpu.zeros(rows, kv, dim, device="cuda") for _ in range(2)]
+        pages.gather(0, i32(gpu, slots), *back, stream=stream)
+        got += back
+        q = new[:, :heads].repeat(40, 1, 1).bfloat16()
+        for batch in (2, 130):  # sets of columns, tiles
+            start = i32(gpu, [0, 40] + [80] * (batch - 1))
+            many = gpu.cat([table, table.new_full((batch - 2, 2), -1)])
+            out = gpu.zeros_like(q)
+            pages.attend(0, start, i32(gpu, lens + [0] * (batch - 2)), many, q, out, max_rows=40 if batch == 2 else 256,
+                         stream=stream)
+            got.append(out)
+        results.append([x.cpu() for x in got])
+        pages.close()
+    for a, b in zip(*results):
+        assert gpu.equal(a, b) and bool(a.any())
