@@ -40,8 +40,8 @@
 // (2.1e-4) it would show where scores are large (3.2e-4 in all, and more the
 // larger they are), so K's codes enter exactly and its scales meet the products
 // of each block in fp32: 787 us where 677 were, see above.  V (and K of bf16
-// rows) must lie in fp16's range; a V block whose scale is not finite makes the
-// rows that see it NaN in that block and leaves the others.
+// rows) must lie in fp16's range; a V block whose scale brings it past makes
+// the rows that see it NaN in that block and leaves the others.
 #include <algorithm>
 
 #include "kernels.hpp"
@@ -109,7 +109,8 @@ __device__ __forceinline__ bool find_tile(const AttendArgs &a, int tile, int siz
     return false;
 }
 
-__device__ __forceinline__ bool finite16(uint32_t h) { return (h & 0x7C00u) != 0x7C00u; }
+// Whether 8 times a scale (fp16 bits) lies in fp16's range.
+__device__ __forceinline__ bool in_range(uint32_t h) { return (h & 0x7FFFu) < 0x7000u; }
 
 }  // namespace
 
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_
     __shared__ __align__(16) _Float16 s_k[2][kStage * KROW];
     __shared__ __align__(16) _Float16 s_v[2][D * VROW];
     __shared__ __align__(8) _Float16 s_d[FINE ? 2 : 1][FINE ? NB * kStage : 4];  // K's scales, [block][key]
-    __shared__ int s_flag[2][NW];  // nonzero: a bad page, or a V scale that is not finite
+    __shared__ int s_flag[2][NW];  // nonzero: a bad page, or a V scale out of range
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
@@ -228,13 +229,17 @@ __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_
             }
         }
         if (do_v) {
+            // 16 times a scale out of range is past 2^17, which no sum of the
+            // others in range brings back (sums past the range on their own,
+            // scales beyond 500, only cost the look below)
+            const _Float16 times = (_Float16) 16.0f;
             pg_half2 check = {(_Float16) 0.0f, (_Float16) 0.0f};
 #pragma unroll
             for (int i = 0; i < TB; ++i) {
-                const pg_half2 z = {(_Float16) 0.0f, (_Float16) 0.0f};
-                check = __builtin_elementwise_fma(__builtin_bit_cast(pg_half2, vd[i].x), z, check);
-                check = __builtin_elementwise_fma(__builtin_bit_cast(pg_half2, vd[i].y), z, check);
+                check = __builtin_elementwise_fma(__builtin_bit_cast(pg_half2, vd[i].x), pg_half2{times, times}, check);
+                check = __builtin_elementwise_fma(__builtin_bit_cast(pg_half2, vd[i].y), pg_half2{times, times}, check);
             }
+            check *= pg_half2{(_Float16) 0.0f, (_Float16) 0.0f};
             const bool odd = !(check.x == (_Float16) 0.0f && check.y == (_Float16) 0.0f);
             if (__any(odd)) {  // rare: such blocks are taken as zeros here and marked
                 flag = 1;
@@ -243,8 +248,8 @@ __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_
                     uint32_t w[2] = {vd[i].x, vd[i].y};
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        if (!finite16(w[j])) w[j] &= 0xFFFF0000u;
-                        if (!finite16(w[j] >> 16)) w[j] &= 0x0000FFFFu;
+                        if (!in_range(w[j])) w[j] &= 0xFFFF0000u;
+                        if (!in_range(w[j] >> 16)) w[j] &= 0x0000FFFFu;
                     }
                     vd[i] = make_uint2(w[0], w[1]);
                 }
@@ -306,7 +311,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_
     // Running maximum (log2 units), the raw score past which it is raised, sum
     // of this lane's weights, and the outputs' transposed sums.
     float m = kPagesFloor, mt = -INFINITY, l = 0.0f;
-    int poison = 0;  // blocks whose V is not finite at a position the row sees
+    int poison = 0;  // blocks whose V is out of range at a position the row sees
     pg_float16 acc[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i)
@@ -442,7 +447,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_
             flags = __builtin_amdgcn_readfirstlane(flags);
             uint32_t bad_groups = 0;
             if (flags) {
-                // a bad page, or V scales that are not finite: look at each
+                // a bad page, or V scales out of range: look at each
                 // group of the stage again
                 for (int i = 0; i < NG; ++i) {
                     const int grp = st * NG + i;
@@ -457,7 +462,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_
                     for (int k = 0; k < G; ++k) {
                         const int pos = grp * G + k;
                         for (int blk = 0; blk < NB; ++blk)
-                            if (!finite16(*reinterpret_cast<const uint16_t *>(
+                            if (!in_range(*reinterpret_cast<const uint16_t *>(
                                     at + page_scale_offset((k >> 4) * NB + blk, k & 15, 1))) &&
                                 pos >= lo && pos < hi)
                                 poison |= 1 << blk;

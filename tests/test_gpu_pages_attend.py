@@ -9,20 +9,24 @@ from bmo_jetson_amd import KVPages, RingError
 pytestmark = pytest.mark.gpu
 
 
-def _tiles(gpu, start, lens, table, rows):
+MORE = 256  # rows behind the last, so that a call can be said to have so many an entry
+
+
+def _tiles(gpu, start, lens, table, rows, group, kv):
     """The same call with as many empty entries and as large a hint as make it
     one of tiles (few rows are taken in sets of columns): q_start, lens, table,
-    max_rows."""
-    more = 64 - len(lens)
-    assert more >= 0
+    max_rows.  q has MORE rows behind the last."""
+    more, most = 64 - len(lens), max(MORE, *rows)
+    units = 64 * kv
+    assert more >= 0 and -(-most * group // 16) * units >= max(1024, 2 * -(-most * group // 128) * units + 1)
     start = np.concatenate((start, [start[-1]] * more))
     return (i32(gpu, start), i32(gpu, np.concatenate((lens, [0] * more))),
-            i32(gpu, np.concatenate((table, np.full((more, table.shape[1]), -1)))), max(256, *rows))
+            i32(gpu, np.concatenate((table, np.full((more, table.shape[1]), -1)))), most)
 
 
-def _calls(gpu, start, lens, table, rows, tiles):
+def _calls(gpu, start, lens, table, rows, tiles, group=1, kv=1):
     if tiles:
-        return _tiles(gpu, start, lens, table, rows)
+        return _tiles(gpu, start, lens, table, rows, group, kv)
     return i32(gpu, start), i32(gpu, lens), i32(gpu, table), max(rows)
 
 
@@ -34,8 +38,7 @@ def _run(gpu, rows, lens, page, heads, kv, dim, type_="bfloat16", causal=True, w
     if table_edit is not None:
         table = table_edit(table)
     total = sum(rows)
-    packed, x = to_type(gpu, np.random.default_rng(seed).standard_normal((total + tail, heads + gap, dim)), type_)
-    q = packed[:, :heads]
+    packed, x = to_type(gpu, np.random.default_rng(seed).standard_normal((total + tail + MORE, heads + gap, dim)), type_)
     start = np.concatenate(([0], np.cumsum(rows)))
     work = None
     if workspace:
@@ -47,10 +50,11 @@ def _run(gpu, rows, lens, page, heads, kv, dim, type_="bfloat16", causal=True, w
     if table_edit is not None:
         calls.pop()  # (an edited table's own width counts)
     if len(lens) <= 64:
-        calls.append(_tiles(gpu, start, lens, table, rows))
+        calls.append(_tiles(gpu, start, lens, table, rows, heads // kv, kv))
     results = []
     for start_d, lens_d, table_d, most in calls:
-        out = gpu.full((total + tail, heads, dim), 7.0, dtype=q.dtype, device="cuda")
+        q = packed[:, :heads] if len(lens_d) > len(lens) else packed[:total + tail, :heads]
+        out = gpu.full(q.shape, 7.0, dtype=q.dtype, device="cuda")
         pages.attend(0, start_d, lens_d, table_d, q, out, causal=causal, window=window, scale=scale, max_rows=most,
                      workspace=work, stream=gpu.cuda.current_stream())
         results.append(out.double().cpu().numpy())
@@ -147,8 +151,8 @@ def test_a_value_that_is_not_finite_reaches_only_rows_that_see_it(gpu, rows, at,
     page, kv, dim, heads = 32, 1, 128, 2
     L = max(rows, 100)
     pages, cache, table = pool(gpu, [L], page, kv, dim, 60)
-    q = gpu.randn(rows, heads, dim, device="cuda").bfloat16()
-    start, lens, t, most = _calls(gpu, [0, rows], [L], table, [rows], tiles)
+    q = gpu.randn(rows + MORE * tiles, heads, dim, device="cuda").bfloat16()
+    start, lens, t, most = _calls(gpu, [0, rows], [L], table, [rows], tiles, 2)
     want, out = gpu.zeros_like(q), gpu.zeros_like(q)
     pages.attend(0, start, lens, t, q, want, max_rows=most)
     slot = i32(gpu, [slot_of(table, 0, at, page)])
@@ -158,6 +162,7 @@ def test_a_value_that_is_not_finite_reaches_only_rows_that_see_it(gpu, rows, at,
     pages.append(0, slot, k, v)
     pages.attend(0, start, lens, t, q, out, max_rows=most)
     gpu.cuda.synchronize()
+    out, want = out[:rows], want[:rows]
     sees = L - rows + np.arange(rows) >= at
     assert 0 < sees.sum() < rows
     sees = gpu.from_numpy(sees).cuda()
@@ -181,13 +186,13 @@ def test_bad_page_ids_are_masked(gpu, rows):
 @pytest.mark.parametrize("tiles", [False, True])
 def test_nan_in_one_query_stays_in_its_row(gpu, tiles):
     pages, cache, table = pool(gpu, [100], 64, 2, 128, 5)
-    q = gpu.randn(50, 4, 128, device="cuda").half()
+    q = gpu.randn(50 + MORE * tiles, 4, 128, device="cuda").half()
     out, want = gpu.zeros_like(q), gpu.zeros_like(q)
-    *args, most = _calls(gpu, [0, 50], [100], table, [50], tiles)
+    *args, most = _calls(gpu, [0, 50], [100], table, [50], tiles, 2, 2)
     pages.attend(0, *args, q, want, max_rows=most)
     q[7, 2, 3] = float("nan")
     pages.attend(0, *args, q, out, max_rows=most)
-    bad = gpu.zeros(50, 4, dtype=gpu.bool, device="cuda")
+    bad = gpu.zeros(q.shape[:2], dtype=gpu.bool, device="cuda")
     bad[7, 2] = True
     assert bool(out[bad].isnan().all()) and gpu.equal(out[~bad], want[~bad])
     pages.close()
@@ -197,10 +202,11 @@ def test_nan_in_one_query_stays_in_its_row(gpu, tiles):
 def test_starts_that_are_no_running_sum(gpu, tiles):
     """Entries whose rows are not within q are skipped."""
     pages, cache, table = pool(gpu, [50, 50, 50], 64, 2, 64, 8)
-    q = gpu.randn(20, 2, 64, device="cuda").half()
-    for start in ([0, 30, 5, 10], [-4, 5, 10, 20], [2**31 - 1, 0, 2**31 - 1, -2**31]):
+    n = 20 + MORE * tiles
+    q = gpu.randn(n, 2, 64, device="cuda").half()
+    for start in ([0, n + 10, 5, 10], [-4, 5, 10, 20], [2**31 - 1, 0, 2**31 - 1, -2**31]):
         out = gpu.full_like(q, 7.0)
-        *args, most = _calls(gpu, start, [50] * 3, table, [20], tiles)
+        *args, most = _calls(gpu, start, [50] * 3, table, [20], tiles, 1, 2)
         pages.attend(0, *args, q, out, causal=False, max_rows=most)
         gpu.cuda.synchronize()
         if start[0] == 0:
@@ -213,8 +219,8 @@ def test_replayed_from_a_graph(gpu, tiles):
     for rows, heads in (([40, 200], 4), ([1, 2], 4)):
         lens = [900, 250]
         pages, cache, table = pool(gpu, lens, 64, 2, 128, 9)
-        q = gpu.randn(sum(rows), heads, 128, device="cuda").half()
-        start, ln, t, most = _calls(gpu, [0, rows[0], sum(rows)], lens, table, rows, tiles)
+        q = gpu.randn(sum(rows) + MORE * tiles, heads, 128, device="cuda").half()
+        start, ln, t, most = _calls(gpu, [0, rows[0], sum(rows)], lens, table, rows, tiles, 2, 2)
         work, work2 = (gpu.zeros(pages.workspace_bytes(heads), dtype=gpu.uint8, device="cuda") for _ in range(2))
         out, eager = gpu.zeros_like(q), gpu.zeros_like(q)
         graph, side = gpu.cuda.CUDAGraph(), gpu.cuda.Stream()
@@ -291,7 +297,7 @@ def test_fp16_scores_are_as_exact_as_fp32(gpu, dim, tiles):
     pages, cache, table = pool(gpu, lens, 64, 2, dim, 77)
     q, x = to_type(gpu, 16 * np.random.default_rng(6).standard_normal((340, 4, dim)), "float16")
     out = gpu.zeros_like(q)
-    *args, most = _calls(gpu, [0, 40, 340], lens, table, rows, tiles)
+    *args, most = _calls(gpu, [0, 40, 340], lens, table, rows, tiles, 2, 2)
     pages.attend(0, *args, q, out, max_rows=most, stream=gpu.cuda.current_stream())
     ref = np.concatenate([attention(cache, table[b], 64, 700, x[at:at + n], list(range(700 - n, 700)), 0, "attend",
                                     "float16")[0] for b, (at, n) in enumerate(((0, 40), (40, 300)))])
@@ -306,12 +312,12 @@ def test_rows_that_see_nothing_are_zeros_whatever_their_queries_hold(gpu, tiles,
     before position 0, beside rows that see something."""
     lens, rows = [3000 if long else 5, 5], [40, 40]
     pages, cache, table = pool(gpu, lens, 64, 2, 128, 31)
-    q = gpu.randn(80, 4, 128, device="cuda").half()
+    q = gpu.randn(80 + MORE * tiles, 4, 128, device="cuda").half()
     want, out = gpu.zeros_like(q), gpu.full_like(q, 7.0)
-    *args, most = _calls(gpu, [0, 40, 80], lens, table, rows, tiles)
+    *args, most = _calls(gpu, [0, 40, 80], lens, table, rows, tiles, 2, 2)
     work = gpu.zeros(pages.workspace_bytes(4), dtype=gpu.uint8, device="cuda")
     pages.attend(0, *args, q, want, max_rows=most, workspace=work)
-    blind = gpu.zeros(80, dtype=gpu.bool, device="cuda")
+    blind = gpu.zeros(len(q), dtype=gpu.bool, device="cuda")
     blind[40:75] = True
     if not long:
         blind[:35] = True
@@ -319,7 +325,9 @@ def test_rows_that_see_nothing_are_zeros_whatever_their_queries_hold(gpu, tiles,
     q[42] = float("inf")
     pages.attend(0, *args, q, out, max_rows=most, workspace=work)
     gpu.cuda.synchronize()
-    assert not bool(out[blind].any()) and gpu.equal(out[~blind], want[~blind])
+    sees = ~blind
+    sees[80:] = False
+    assert not bool(out[blind].any()) and gpu.equal(out[sees], want[sees])
     pages.close()
 
 
@@ -339,3 +347,35 @@ def test_more_rows_than_said_leave_the_others_whole(gpu):
             # (the two calls may be shaped differently: roundings of 16-bit operands)
             assert rel(out[part].double().cpu().numpy(), want[part].double().cpu().numpy()) < 2.0**-9
         pages.close()
+
+
+@pytest.mark.parametrize("tiles", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("value", [65520.0, 7e4, 5e5, float("inf")])
+def test_values_past_fp16_at_masked_positions_do_not_show(gpu, tiles, dim, value):
+    """What an fp32 request may have left in a page: scales within fp16 whose
+    values are not.  A row that sees one is not finite in that block."""
+    page, kv, heads, rows = 64, 1, 2, 60
+    pages, cache, table = pool(gpu, [200], page, kv, dim, 4)
+    q = gpu.randn(rows + MORE * tiles, heads, dim, device="cuda").bfloat16()
+    *args, most = _calls(gpu, [0, rows], [150], table, [rows], tiles, 2)
+    want, out = gpu.zeros_like(q), gpu.zeros_like(q)
+    pages.attend(0, *args, q, want, max_rows=most)
+    far = np.array([slot_of(table, 0, p, page) for p in range(150, 200)])
+    x = gpu.full((len(far), kv, dim), value, device="cuda")
+    x[::2] *= -1
+    pages.append(0, i32(gpu, far), x, x)
+    pages.attend(0, *args, q, out, max_rows=most)
+    assert bool(want.any()) and gpu.equal(out, want)
+    # at position 120, in V's last block alone: rows 0..29 end before it
+    k, v = gpu.zeros(1, kv, dim, device="cuda"), gpu.zeros(1, kv, dim, device="cuda")
+    at = i32(gpu, [slot_of(table, 0, 120, page)])
+    pages.append(0, at, k, v)
+    pages.attend(0, *args, q, want, max_rows=most)
+    v[0, 0, -3] = value
+    pages.append(0, at, k, v)
+    pages.attend(0, *args, q, out, max_rows=most)
+    assert gpu.equal(out[:30], want[:30]) and gpu.equal(out[:, :, :-32], want[:, :, :-32])
+    if tiles or not np.isfinite(value):
+        assert not bool(out[30:rows, :, -32:].isfinite().all(-1).any())
+    pages.close()
