@@ -134,10 +134,11 @@ def test_lengths_and_requests_out_of_range(gpu):
     pages.close()
 
 
-def test_replayed_from_a_graph(gpu):
+@pytest.mark.parametrize("n,width,n_pages", [(30, 10, 120), (2400, 4, 3500)])  # one workgroup, several
+def test_replayed_from_a_graph(gpu, n, width, n_pages):
     """A captured step: every replay grows the entries from where the last one
     left them, with eager plans of the program's own in between."""
-    n, page, width, n_pages = 30, 32, 10, 120
+    page = 32
     pages = KVPages(1, n_pages, page, 1, 64)
     m = Model(n_pages, page, n, width)
     free, lens, table = _device(gpu, pages, n, width)
