@@ -313,7 +313,7 @@ int bmo_kv_pages_gather(bmo_kv_pages_t *h, int layer, int n_tok, const int *slot
 
 int64_t bmo_kv_pages_workspace_bytes(const bmo_kv_pages_t *h, int n_heads) {
     if (!h || n_heads <= 0 || n_heads % h->g.n_kv != 0) return 0;
-    return bmo::pages_work_bytes(h->g, n_heads);
+    return bmo::pages_work_bytes(h->g);
 }
 
 int bmo_kv_pages_decode(bmo_kv_pages_t *h, int layer, int n_batch, const int *lens, const int *table, int max_pages,

@@ -82,8 +82,8 @@ struct PagesDecodeParams {
 hipError_t launch_pages_decode(const PagesDecodeParams &p, hipStream_t stream);
 // Ragged rows, no more than max_rows an entry, in 16 bits, by the same kernel.
 hipError_t launch_pages_few_rows(const PagesDecodeParams &p, hipStream_t stream);
-// Bytes of partial results that a split launch of n_heads query heads needs.
-int64_t pages_work_bytes(const PagesGeom &g, int n_heads);
+// Bytes of partial results that a launch may keep.
+int64_t pages_work_bytes(const PagesGeom &g);
 
 // Attention of ragged rows.
 struct PagesAttendParams {

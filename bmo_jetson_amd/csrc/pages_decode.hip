@@ -685,6 +685,11 @@ namespace {
 bool spread(const PagesGeom &g, int heads) { return heads <= 16 / (g.dim / kQK); }
 int set_heads(const PagesGeom &g, int heads) { return spread(g, heads) ? 16 / (g.dim / kQK) : 16; }
 int64_t part_bytes(const PagesGeom &g, int hc) { return (int64_t) hc * (g.dim + 2 * (g.dim / kQK)) * 4; }
+// Workgroups of a launch whose long entries are cut (sets of 16 of dim 128
+// leave room for half as many at a time).
+int64_t split_workgroups(const PagesGeom &g, int hc) {
+    return kSplitWaves / kWaves / (hc == 16 && g.dim == 128 ? 2 : 1);
+}
 
 template <int D, bool SPREAD, bool MULTI>
 const void *kernel_of(int nw, int type) {
@@ -723,8 +728,13 @@ hipError_t launch_of(const DecodeArgs &arg, int nw, hipStream_t stream) {
 //     limits 96 sets x 125 steps 18 / 21, 960 x 19 18 / 20.
 //   runs of at least 4 steps a wave, of 16, or nothing cut:  32 units x 94
 //     steps 11.2 / 21.6 / 21.6, x 250 14.5 / 16.8 / 49, 8 x 1000 17.7 / 18.7 /
-//     184; 256 x 32 13.7 / 10.7 / 10.7, 512 x 32 21.5 / 16.3 / 16.2; 96 units
-//     of 62 to 1000 steps 56 / 54 / 183.
+//     184; 128 units of up to 250 steps in 3 or 2 runs 35.4 / 32.5, 24 of up to
+//     1000 in 15 or 10 27 / 25, 80 of up to 282 in 4 or 3 39 / 34 (past two
+//     workgroups a CU the entries' own lengths decide: 96 of 62 to 1000 in 10
+//     or 8 52.5 / 57.5, all of 1000 84 / 78); 256 x 32 13.7 / 10.7 / 10.7, 512 x 32 21.5 / 16.3 / 16.2; 96 units
+//     of 62 to 1000 steps 56 / 54 / 183.  Sets of 16 rows, bf16, cut for 1024
+//     workgroups, for 512, or not:  132 x 204 steps 46 / 45 / 54, 128 x 500
+//     82 / 66 / 72.
 template <bool MULTI>
 hipError_t launch_units(const PagesDecodeParams &p, int heads, hipStream_t stream) {
     DecodeArgs a{};
@@ -749,8 +759,12 @@ hipError_t launch_units(const PagesDecodeParams &p, int heads, hipStream_t strea
     if (nw == kWaves && p.work) {
         const int64_t room = p.work_bytes / part_bytes(p.g, hc) / units;  // runs that it holds
         const int64_t fill = std::min<int64_t>(kFillWaves / kWaves / units, steps / (kFillSteps * kWaves));
-        const int64_t split = std::min<int64_t>(kSplitWaves / kWaves / units, steps / (kSplitSteps * kWaves));
-        const int64_t runs = std::min({std::max(fill, split), room, (int64_t) kMaxRuns});
+        const int64_t split = std::min<int64_t>(split_workgroups(p.g, hc) / units, steps / (kSplitSteps * kWaves));
+        const int64_t most = std::min({std::max(fill, split), room, (int64_t) kMaxRuns});
+        int64_t runs = std::max<int64_t>(most, 1);
+        if (units * runs <= 512)  // as many as load 256 CUs most evenly
+            for (int64_t r = runs - 1; r > 0; --r)
+                if ((units * r + 255) / 256 * runs < (units * runs + 255) / 256 * r) runs = r;
         if (runs > 1) {
             a.max_runs = (int) runs;
             a.run = (int) ((steps + runs - 1) / runs);
@@ -763,12 +777,9 @@ hipError_t launch_units(const PagesDecodeParams &p, int heads, hipStream_t strea
 
 }  // namespace
 
-// Every workgroup that a split launch of one-row entries can have; sets of 16
-// heads have four times as long results and a quarter of the units.
-int64_t pages_work_bytes(const PagesGeom &g, int n_heads) {
-    const int group = n_heads / g.n_kv;
-    return kSplitWaves / kWaves / (spread(g, group) ? 1 : 4) * part_bytes(g, set_heads(g, group));
-}
+// Every workgroup that a launch of sets of 16 may have (sets of fewer have
+// smaller results).
+int64_t pages_work_bytes(const PagesGeom &g) { return split_workgroups(g, 16) * part_bytes(g, 16); }
 
 hipError_t launch_pages_decode(const PagesDecodeParams &p, hipStream_t stream) {
     return launch_units<false>(p, p.n_heads / p.g.n_kv, stream);
