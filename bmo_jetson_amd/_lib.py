@@ -72,6 +72,8 @@ SIGNATURES = {
     "bmo_kv_pages_decode": (i32, [P, i32, i32, P, P, i32, i32, i32, P, i64, P, f32, i32, i32, P, i64, P]),
     "bmo_kv_pages_append_decode": (i32, [P, i32, i32, P, P, i32, i32, i32, P, i64, P, P, i64, P, f32, i32, i32, P,
                                          i64, P]),
+    "bmo_kv_pages_append_decode_granted": (i32, [P, i32, i32, P, P, P, P, i32, i32, i32, P, i64, P, P, i64, P, f32, i32,
+                                                 i32, P, i64, P]),
     "bmo_kv_pages_attend": (i32, [P, i32, i32, P, P, P, i32, i32, i32, i32, P, i64, P, f32, i32, i32, i32, i32, P,
                                   i64, P]),
 }

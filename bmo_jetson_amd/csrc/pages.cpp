@@ -142,12 +142,20 @@ int slots_call(bmo_kv_pages_t *h, const char *fn, bool append, int layer, int n_
     });
 }
 
-int decode_call(bmo_kv_pages_t *h, const char *fn, bool append, int layer, int n_batch, const int *lens, const int *table,
-                int max_pages, int n_heads, int type, const void *q, int64_t q_stride, const void *k_new,
+// What a plan was asked for and answered, of the calls that are told.
+struct Granted {
+    bool told;
+    const int *n_new, *status;
+};
+
+int decode_call(bmo_kv_pages_t *h, const char *fn, bool append, Granted granted, int layer, int n_batch, const int *lens,
+                const int *table, int max_pages, int n_heads, int type, const void *q, int64_t q_stride, const void *k_new,
                 const void *v_new, int64_t kv_stride, void *out, float scale, int window, int max_len, void *work,
                 int64_t work_bytes, void *stream) {
     return guarded(h, fn, [&](Call &c) {
-        if (!lens || !table || !q || !out || (append && (!k_new || !v_new))) return c.null();
+        if (!lens || !table || !q || !out || (append && (!k_new || !v_new)) ||
+            (granted.told && (!granted.n_new || !granted.status)))
+            return c.null();
         if (int rc = check_layer(c, layer)) return rc;
         if (int rc = check_table(c, n_batch, max_pages)) return rc;
         if (int rc = check_heads(c, n_heads)) return rc;
@@ -173,6 +181,8 @@ int decode_call(bmo_kv_pages_t *h, const char *fn, bool append, int layer, int n
         p.n_batch = n_batch;
         p.n_heads = n_heads;
         p.lens = lens;
+        p.n_new = granted.n_new;
+        p.status = granted.status;
         p.table = table;
         p.max_pages = max_pages;
         p.window = (int64_t) window >= (int64_t) max_pages << g.page_shift ? 0 : window;
@@ -319,7 +329,7 @@ int64_t bmo_kv_pages_workspace_bytes(const bmo_kv_pages_t *h, int n_heads) {
 int bmo_kv_pages_decode(bmo_kv_pages_t *h, int layer, int n_batch, const int *lens, const int *table, int max_pages,
                         int n_heads, int type, const void *q, int64_t q_stride, void *out, float scale, int window,
                         int max_len, void *workspace, int64_t workspace_bytes, void *stream) {
-    return decode_call(h, "bmo_kv_pages_decode", false, layer, n_batch, lens, table, max_pages, n_heads, type, q, q_stride,
+    return decode_call(h, "bmo_kv_pages_decode", false, {}, layer, n_batch, lens, table, max_pages, n_heads, type, q, q_stride,
                        nullptr, nullptr, 0, out, scale, window, max_len, workspace, workspace_bytes, stream);
 }
 
@@ -327,8 +337,18 @@ int bmo_kv_pages_append_decode(bmo_kv_pages_t *h, int layer, int n_batch, const 
                                int n_heads, int type, const void *q, int64_t q_stride, const void *k_new,
                                const void *v_new, int64_t kv_stride, void *out, float scale, int window, int max_len,
                                void *workspace, int64_t workspace_bytes, void *stream) {
-    return decode_call(h, "bmo_kv_pages_append_decode", true, layer, n_batch, lens, table, max_pages, n_heads, type, q,
+    return decode_call(h, "bmo_kv_pages_append_decode", true, {}, layer, n_batch, lens, table, max_pages, n_heads, type, q,
                        q_stride, k_new, v_new, kv_stride, out, scale, window, max_len, workspace, workspace_bytes, stream);
+}
+
+int bmo_kv_pages_append_decode_granted(bmo_kv_pages_t *h, int layer, int n_batch, const int *n_new, const int *status,
+                                       const int *lens, const int *table, int max_pages, int n_heads, int type,
+                                       const void *q, int64_t q_stride, const void *k_new, const void *v_new,
+                                       int64_t kv_stride, void *out, float scale, int window, int max_len, void *workspace,
+                                       int64_t workspace_bytes, void *stream) {
+    return decode_call(h, "bmo_kv_pages_append_decode_granted", true, {true, n_new, status}, layer, n_batch, lens, table,
+                       max_pages, n_heads, type, q, q_stride, k_new, v_new, kv_stride, out, scale, window, max_len,
+                       workspace, workspace_bytes, stream);
 }
 
 int bmo_kv_pages_attend(bmo_kv_pages_t *h, int layer, int n_batch, const int *q_start, const int *lens, const int *table,

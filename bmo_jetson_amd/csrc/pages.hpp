@@ -59,6 +59,8 @@ struct PagesDecodeParams {
     int n_batch;
     int n_heads;
     const int *lens;
+    const int *n_new;  // what a plan was asked for and its status, nullable: entries
+    const int *status; // that did not grow have no positions here
     const int *table;
     int max_pages;
     int window;  // 0: none

@@ -101,7 +101,7 @@ __device__ __forceinline__ Unit unit_of(const DecodeArgs &a, int b, int unit) {
     const int64_t room = (int64_t) a.p.max_pages << a.p.g.page_shift;
     u.kvh = unit / a.n_hs;
     u.row0 = (unit - u.kvh * a.n_hs) * HC;
-    u.entry_len = (int) min((int64_t) max(uniform_int(a.p.lens, b), 0), room);
+    u.entry_len = (int) min((int64_t) max(granted_len(a.p.lens, a.p.n_new, a.p.status, b), 0), room);
     if constexpr (MULTI) {
         u.start = uniform_int(a.p.q_start, b);
         const int end = uniform_int(a.p.q_start, b + 1);

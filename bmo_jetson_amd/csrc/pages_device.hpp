@@ -55,6 +55,15 @@ __device__ __forceinline__ int uniform_int(const int *p, int i) {
     return ((const __attribute__((address_space(4))) int *) p)[i];
 }
 
+// The length of entry b; 0 for one that a plan did not let grow: it asked for
+// nothing (n_new) or was refused (status), each array nullable.
+__device__ __forceinline__ int granted_len(const int *lens, const int *n_new, const int *status, int b) {
+    // (an absent array is read as lens, so that no load waits for another)
+    const int len = uniform_int(lens, b);
+    const int asked = uniform_int(n_new ? n_new : lens, b), state = uniform_int(status ? status : lens, b);
+    return (n_new && asked <= 0) || (status && state != 0) ? 0 : len;
+}
+
 // 16 bytes that a launch reads once.
 __device__ __forceinline__ uint4 stream16(const uint8_t *p) {
     typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));

@@ -33,10 +33,11 @@ class KVPages:
     on the pool's device): ``free`` [n_pages + 2], which ``list_init`` fills,
     ``table`` [n_batch][max_pages] and ``lens`` [n_batch], which ``plan`` keeps.
     A server's step plans the new tokens' slots once and then runs, per layer,
-    ``append`` and ``attend`` for prompts or ``append_decode`` for single tokens;
-    the calls run on ``stream`` and can be captured in a HIP graph.  For cross
-    attention the encoder's K and V are appended once, and ``attend`` with
-    ``causal=False`` (or ``decode``) reads them."""
+    ``append`` and ``attend`` for prompts or ``append_decode`` for single tokens
+    (with the plan's ``n_new`` and ``status``, so that entries that it refused
+    keep what they have); the calls run on ``stream`` and can be captured in a
+    HIP graph.  For cross attention the encoder's K and V are appended once, and
+    ``attend`` with ``causal=False`` (or ``decode``) reads them."""
 
     def __init__(self, n_layers: int, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int):
         L = lib()
@@ -204,17 +205,25 @@ class KVPages:
             float(scale), int(window), int(max_len), *self._work(workspace), _stream(stream)))
 
     def append_decode(self, layer: int, lens, table, q, k, v, out, scale: float = 0.0, window: int = 0,
-                      max_len: int = 0, workspace=None, stream=None) -> None:
+                      max_len: int = 0, workspace=None, stream=None, n_new=None, status=None) -> None:
         """decode with k and v [n_batch][n_kv_heads][head_dim] appended at each
-        entry's last position (lens counts it already)."""
+        entry's last position (lens counts it already).  With the n_new and
+        status [n_batch] of the plan before, entries that it did not let grow are
+        left as they are and get zeros; without them every entry with positions
+        must have grown."""
         n, lens_p, table_p, width = self._table(lens, table)
         qp, stride, type_, heads, nq = self._rows(q, None, "q")
         kp, kstride, ktype, _, nk = self._rows(k, self.n_kv_heads, "k")
         vp, vstride, vtype, _, nv = self._rows(v, self.n_kv_heads, "v")
         if nq != n or nk != n or nv != n or kstride != vstride or ktype != type_ or vtype != type_:
             raise ValueError("q, k and v must have one row an entry and one type, k and v the same stride")
-        self._check("bmo_kv_pages_append_decode", lib().bmo_kv_pages_append_decode(
-            self._h, int(layer), n, lens_p, table_p, width, heads, type_, qp, stride, kp, vp, kstride,
+        fn, granted = "bmo_kv_pages_append_decode", ()
+        if n_new is not None or status is not None:
+            if n_new is None or status is None:
+                raise ValueError("n_new and status come together")
+            fn, granted = fn + "_granted", (self._ints(n_new, "n_new", n), self._ints(status, "status", n))
+        self._check(fn, getattr(lib(), fn)(
+            self._h, int(layer), n, *granted, lens_p, table_p, width, heads, type_, qp, stride, kp, vp, kstride,
             self._out(out, n, heads, type_), float(scale), int(window), int(max_len), *self._work(workspace),
             _stream(stream)))
 

@@ -549,7 +549,9 @@ BMO_ATTN_API int bmo_kv_pages_decode(bmo_kv_pages_t *pages, int layer, int n_bat
 /* The same with the append of the newest position: k_new and v_new
  * [n_batch][n_kv_heads][head_dim] are quantized into position lens[b] - 1 and
  * attended to with their quantized values.  Entries must not share the page of
- * that position. */
+ * that position.  Every entry with positions must have grown by its token: one
+ * that did not would lose the newest token that it has.  Behind a plan that
+ * may refuse an entry, or with entries that pause, call _granted. */
 BMO_ATTN_API int bmo_kv_pages_append_decode(bmo_kv_pages_t *pages, int layer, int n_batch,
                                             const int *lens, const int *table, int max_pages,
                                             int n_heads, int type, const void *q,
@@ -558,6 +560,16 @@ BMO_ATTN_API int bmo_kv_pages_append_decode(bmo_kv_pages_t *pages, int layer, in
                                             float scale, int window, int max_len,
                                             void *workspace, int64_t workspace_bytes,
                                             void *stream);
+
+/* bmo_kv_pages_append_decode behind a plan: n_new and status [n_batch] (device)
+ * as the plan took and wrote them.  Entries with n_new[b] > 0 and status[b] == 0
+ * are appended to and attended; what every other entry holds is left as it is,
+ * and its row of out is zeros (try again once pages are free). */
+BMO_ATTN_API int bmo_kv_pages_append_decode_granted(
+    bmo_kv_pages_t *pages, int layer, int n_batch, const int *n_new, const int *status,
+    const int *lens, const int *table, int max_pages, int n_heads, int type, const void *q,
+    int64_t q_stride, const void *k_new, const void *v_new, int64_t kv_stride, void *out,
+    float scale, int window, int max_len, void *workspace, int64_t workspace_bytes, void *stream);
 
 /* Attention of ragged rows: entry b has rows q_start[b] .. q_start[b + 1] - 1
  * of q and out [n_rows][n_heads][head_dim] (type F16 or BF16; q_start
