@@ -76,6 +76,8 @@ SIGNATURES = {
                                                  i32, P, i64, P]),
     "bmo_kv_pages_attend": (i32, [P, i32, i32, P, P, P, i32, i32, i32, i32, P, i64, P, f32, i32, i32, i32, i32, P,
                                   i64, P]),
+    "bmo_kv_pages_attend_granted": (i32, [P, i32, i32, P, P, P, P, i32, i32, i32, i32, P, i64, P, f32, i32, i32, i32,
+                                          i32, P, i64, P]),
 }
 
 

@@ -201,6 +201,56 @@ int decode_call(bmo_kv_pages_t *h, const char *fn, bool append, Granted granted,
     });
 }
 
+int attend_call(bmo_kv_pages_t *h, const char *fn, Granted granted, int layer, int n_batch, const int *q_start,
+                const int *lens, const int *table, int max_pages, int n_rows, int n_heads, int type, const void *q,
+                int64_t q_stride, void *out, float scale, int causal, int window, int max_rows, int max_len,
+                void *workspace, int64_t workspace_bytes, void *stream) {
+    return guarded(h, fn, [&](Call &c) {
+        if (!q_start || !lens || !table || (n_rows != 0 && (!q || !out)) || (granted.told && !granted.status))
+            return c.null();
+        if (int rc = check_layer(c, layer)) return rc;
+        if (int rc = check_table(c, n_batch, max_pages)) return rc;
+        if (int rc = check_heads(c, n_heads)) return rc;
+        const bmo::PagesGeom &g = c.h->g;
+        if (type != bmo::kTypeF16 && type != bmo::kTypeBF16) return c.arg("rows must be fp16 or bf16");
+        if (n_rows < 0 || (int64_t) n_rows * n_heads > (1 << 30))
+            return c.arg("n_rows must not be negative, n_rows * n_heads at most 2^30");
+        // (tiles: 2^23 of rows and one an entry and kv head, 256 threads each)
+        if ((int64_t) n_batch * g.n_kv > (1 << 22)) return c.arg("n_batch * n_kv_heads must be at most 2^22");
+        if (const char *why = row_fault(q, q_stride, (int64_t) n_heads * g.dim, type)) return c.arg(why);
+        if (!aligned(out, 16) || !aligned(workspace, 16)) return c.arg("out and workspace must be aligned to 16 bytes");
+        if (window < 0 || max_rows < 0 || max_len < 0 || workspace_bytes < 0)
+            return c.arg("window, max_rows, max_len and sizes must not be negative");
+        if (!(scale > 0.0f)) scale = 1.0f / std::sqrt((float) g.dim);
+        if (!std::isfinite(scale)) return c.arg("scale must be finite");
+        if (n_rows == 0) return c.done(hipSuccess);
+        c.enter();
+        bmo::PagesAttendParams p{};
+        p.base = c.h->mem + layer * g.layer_bytes;
+        p.g = g;
+        p.n_batch = n_batch;
+        p.n_heads = n_heads;
+        p.q_start = q_start;
+        p.lens = lens;
+        p.status = granted.status;
+        p.table = table;
+        p.max_pages = max_pages;
+        p.n_rows = n_rows;
+        p.causal = causal != 0;
+        p.window = (int64_t) window >= (int64_t) max_pages << g.page_shift ? 0 : window;
+        p.type = type;
+        p.q = q;
+        p.q_stride = q_stride;
+        p.out = out;
+        p.qscale = scale * kLog2e;
+        p.max_rows = max_rows;
+        p.max_len = max_len;
+        p.work = static_cast<float *>(workspace);
+        p.work_bytes = workspace_bytes;
+        return c.done(bmo::launch_pages_attend(p, (hipStream_t) stream));
+    });
+}
+
 }  // namespace
 
 extern "C" {
@@ -355,48 +405,17 @@ int bmo_kv_pages_attend(bmo_kv_pages_t *h, int layer, int n_batch, const int *q_
                         int max_pages, int n_rows, int n_heads, int type, const void *q, int64_t q_stride, void *out,
                         float scale, int causal, int window, int max_rows, int max_len, void *workspace,
                         int64_t workspace_bytes, void *stream) {
-    return guarded(h, "bmo_kv_pages_attend", [&](Call &c) {
-        if (!q_start || !lens || !table || (n_rows != 0 && (!q || !out))) return c.null();
-        if (int rc = check_layer(c, layer)) return rc;
-        if (int rc = check_table(c, n_batch, max_pages)) return rc;
-        if (int rc = check_heads(c, n_heads)) return rc;
-        const bmo::PagesGeom &g = c.h->g;
-        if (type != bmo::kTypeF16 && type != bmo::kTypeBF16) return c.arg("rows must be fp16 or bf16");
-        if (n_rows < 0 || (int64_t) n_rows * n_heads > (1 << 30))
-            return c.arg("n_rows must not be negative, n_rows * n_heads at most 2^30");
-        // (tiles: 2^23 of rows and one an entry and kv head, 256 threads each)
-        if ((int64_t) n_batch * g.n_kv > (1 << 22)) return c.arg("n_batch * n_kv_heads must be at most 2^22");
-        if (const char *why = row_fault(q, q_stride, (int64_t) n_heads * g.dim, type)) return c.arg(why);
-        if (!aligned(out, 16) || !aligned(workspace, 16)) return c.arg("out and workspace must be aligned to 16 bytes");
-        if (window < 0 || max_rows < 0 || max_len < 0 || workspace_bytes < 0)
-            return c.arg("window, max_rows, max_len and sizes must not be negative");
-        if (!(scale > 0.0f)) scale = 1.0f / std::sqrt((float) g.dim);
-        if (!std::isfinite(scale)) return c.arg("scale must be finite");
-        if (n_rows == 0) return c.done(hipSuccess);
-        c.enter();
-        bmo::PagesAttendParams p{};
-        p.base = c.h->mem + layer * g.layer_bytes;
-        p.g = g;
-        p.n_batch = n_batch;
-        p.n_heads = n_heads;
-        p.q_start = q_start;
-        p.lens = lens;
-        p.table = table;
-        p.max_pages = max_pages;
-        p.n_rows = n_rows;
-        p.causal = causal != 0;
-        p.window = (int64_t) window >= (int64_t) max_pages << g.page_shift ? 0 : window;
-        p.type = type;
-        p.q = q;
-        p.q_stride = q_stride;
-        p.out = out;
-        p.qscale = scale * kLog2e;
-        p.max_rows = max_rows;
-        p.max_len = max_len;
-        p.work = static_cast<float *>(workspace);
-        p.work_bytes = workspace_bytes;
-        return c.done(bmo::launch_pages_attend(p, (hipStream_t) stream));
-    });
+    return attend_call(h, "bmo_kv_pages_attend", {}, layer, n_batch, q_start, lens, table, max_pages, n_rows, n_heads, type,
+                       q, q_stride, out, scale, causal, window, max_rows, max_len, workspace, workspace_bytes, stream);
+}
+
+int bmo_kv_pages_attend_granted(bmo_kv_pages_t *h, int layer, int n_batch, const int *status, const int *q_start,
+                                const int *lens, const int *table, int max_pages, int n_rows, int n_heads, int type,
+                                const void *q, int64_t q_stride, void *out, float scale, int causal, int window,
+                                int max_rows, int max_len, void *workspace, int64_t workspace_bytes, void *stream) {
+    return attend_call(h, "bmo_kv_pages_attend_granted", {true, nullptr, status}, layer, n_batch, q_start, lens, table,
+                       max_pages, n_rows, n_heads, type, q, q_stride, out, scale, causal, window, max_rows, max_len,
+                       workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

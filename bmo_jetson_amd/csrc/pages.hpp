@@ -95,6 +95,7 @@ struct PagesAttendParams {
     int n_heads;
     const int *q_start;  // [n_batch + 1]
     const int *lens;
+    const int *status;  // a plan's, nullable: entries that it refused have no positions here
     const int *table;
     int max_pages;
     int n_rows;  // rows of q and out

@@ -147,7 +147,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_
     const int start = p.q_start[b];
     const int n_tok = entry_rows(a, b);
     const int64_t room = (int64_t) p.max_pages << g.page_shift;
-    const int len = (int) min((int64_t) max(uniform_int(p.lens, b), 0), room);
+    const int len = (int) min((int64_t) max(granted_len(p.lens, nullptr, p.status, b), 0), room);
     const int *table = p.table + (int64_t) b * p.max_pages;
 
     // This lane's row, and the positions [lo, hi) it sees.
@@ -531,6 +531,7 @@ hipError_t launch_pages_attend(const PagesAttendParams &p, hipStream_t stream) {
         d.n_batch = p.n_batch;
         d.n_heads = p.n_heads;
         d.lens = p.lens;
+        d.status = p.status;
         d.table = p.table;
         d.max_pages = p.max_pages;
         d.window = p.window;

@@ -34,8 +34,8 @@ class KVPages:
     ``table`` [n_batch][max_pages] and ``lens`` [n_batch], which ``plan`` keeps.
     A server's step plans the new tokens' slots once and then runs, per layer,
     ``append`` and ``attend`` for prompts or ``append_decode`` for single tokens
-    (with the plan's ``n_new`` and ``status``, so that entries that it refused
-    keep what they have); the calls run on ``stream`` and can be captured in a
+    (with the plan's ``status``, and ``n_new``, so that entries that it refused
+    keep what they have and get zeros); the calls run on ``stream`` and can be captured in a
     HIP graph.  For cross attention the encoder's K and V are appended once, and
     ``attend`` with ``causal=False`` (or ``decode``) reads them."""
 
@@ -228,13 +228,18 @@ class KVPages:
             _stream(stream)))
 
     def attend(self, layer: int, q_start, lens, table, q, out, causal: bool = True, scale: float = 0.0,
-               window: int = 0, max_rows: int = 0, max_len: int = 0, workspace=None, stream=None) -> None:
+               window: int = 0, max_rows: int = 0, max_len: int = 0, workspace=None, stream=None,
+               status=None) -> None:
         """Ragged rows q and out [n_rows][n_heads][head_dim] (fp16 or bf16), entry
         b's from q_start[b] to q_start[b + 1]: its last positions (causal), or
-        rows that see all of its positions (cross attention)."""
+        rows that see all of its positions (cross attention).  With the status
+        [n_batch] of the plan before, rows of entries that it refused are zeros."""
         n, lens_p, table_p, width = self._table(lens, table)
         qp, stride, type_, heads, rows = self._rows(q, None, "q")
-        self._check("bmo_kv_pages_attend", lib().bmo_kv_pages_attend(
-            self._h, int(layer), n, self._ints(q_start, "q_start", n + 1), lens_p, table_p, width, rows, heads, type_, qp,
+        fn, granted = "bmo_kv_pages_attend", ()
+        if status is not None:
+            fn, granted = fn + "_granted", (self._ints(status, "status", n),)
+        self._check(fn, getattr(lib(), fn)(
+            self._h, int(layer), n, *granted, self._ints(q_start, "q_start", n + 1), lens_p, table_p, width, rows, heads, type_, qp,
             stride, self._out(out, rows, heads, type_), float(scale), int(bool(causal)), int(window), int(max_rows),
             int(max_len), *self._work(workspace), _stream(stream)))

@@ -589,6 +589,19 @@ BMO_ATTN_API int bmo_kv_pages_attend(bmo_kv_pages_t *pages, int layer, int n_bat
                                      int causal, int window, int max_rows, int max_len,
                                      void *workspace, int64_t workspace_bytes, void *stream);
 
+/* bmo_kv_pages_attend behind a plan that may refuse entries: status [n_batch]
+ * (device) as the plan wrote it.  A refused entry's rows are in q (the plan's
+ * tok_start counts them) but have no positions, as its length tells nothing of
+ * them: rows of entries with status[b] != 0 are zeros. */
+BMO_ATTN_API int bmo_kv_pages_attend_granted(bmo_kv_pages_t *pages, int layer, int n_batch,
+                                             const int *status, const int *q_start,
+                                             const int *lens, const int *table, int max_pages,
+                                             int n_rows, int n_heads, int type, const void *q,
+                                             int64_t q_stride, void *out, float scale, int causal,
+                                             int window, int max_rows, int max_len,
+                                             void *workspace, int64_t workspace_bytes,
+                                             void *stream);
+
 /* ---- node-level drop-in ------------------------------------------------------ */
 
 /* Same signature and semantics as the reference's launch_decode_attention

@@ -123,3 +123,61 @@ def test_granted_refusals(gpu):
     gpu.cuda.synchronize()
     s.check_slots("nothing granted")
     s.pages.close()
+
+
+@pytest.mark.parametrize("tiles", [False, True])
+@pytest.mark.parametrize("dim,type_", [(64, "float16"), (128, "bfloat16")])
+def test_chunks_of_which_a_plan_refuses_some(gpu, tiles, dim, type_):
+    """A step of prompt pieces into a pool that runs out: refused entries' rows
+    are zeros, the others' what they are among themselves, and nothing that was
+    there is overwritten."""
+    heads, kv, width, more = 4, 2, 3, 250
+    lens = [32, 40, 20, 3, 90] + [0] * (59 if tiles else 0)  # (many entries: tiles of rows)
+    n = len(lens)
+    s = Pool(gpu, lens, width, kv, dim, 3)
+    new = [1, 0, 12, 9, 40] + [0] * (n - 5)  # refused: 0 finds no page, 4 passes its table
+    total = sum(new)
+    start, slots, status = i32(gpu, np.zeros(n + 1)), i32(gpu, np.full(total, -1)), i32(gpu, np.full(n, -1))
+    s.pages.plan(s.free, i32(gpu, new), s.lens, s.table, start, slots, status=status, stream=gpu.cuda.current_stream())
+    states = [1, 0, 0, 0, 2] + [0] * (n - 5)
+    assert status.tolist() == states
+    x = np.concatenate([np.random.default_rng(8).standard_normal((total + more, heads, dim)),
+                        kv_rows(9, total + more, 2 * kv, dim)], axis=1)
+    t, x = to_type(gpu, x, type_)
+    q, k, v = t.split([heads, kv, kv], dim=1)
+    out = gpu.full((total + more, heads, dim), 7.0, dtype=q.dtype, device="cuda")
+    most = 256 if tiles else max(new)
+    if tiles:
+        assert -(-most * 2 // 16) * n * kv >= max(1024, 2 * -(-most * 2 // 128) * n * kv + 1)
+    s.pages.append(1, slots, k[:total], v[:total], stream=gpu.cuda.current_stream())
+    s.pages.attend(1, start, s.lens, s.table, q, out, max_rows=most, status=status, stream=gpu.cuda.current_stream())
+    got, at = out.double().cpu().numpy(), np.concatenate(([0], np.cumsum(new)))
+    for b in range(5):
+        if states[b] == 0:
+            lens[b] += new[b]
+            where = [slot_of(s.host_table, b, p, PAGE) for p in range(lens[b] - new[b], lens[b])]
+            if where:
+                s.cache[1].put(where, x[at[b]:at[b + 1], heads:heads + kv], x[at[b]:at[b + 1], heads + kv:])
+    s.check_slots("chunks")
+    for b in range(5):
+        part = slice(at[b], at[b + 1])
+        if states[b]:
+            assert not got[part].any()
+        elif new[b]:
+            ref, bound = attention(s.cache[1], s.host_table[b], PAGE, lens[b], x[part, :heads],
+                                   list(range(lens[b] - new[b], lens[b])), 0, "attend", type_)
+            check(got[part], ref, bound, f"entry {b}")
+    assert (got[total:] == 7.0).all()
+    # cross attention likewise: a refused entry has nothing that is read
+    s.pages.attend(1, start, s.lens, s.table, q, out, causal=False, max_rows=most, status=status,
+                   stream=gpu.cuda.current_stream())
+    assert not out[at[0]:at[1]].any() and not out[at[4]:at[5]].any() and bool(out[at[2]:at[4]].any(-1).all())
+    with pytest.raises(ValueError, match="status"):
+        s.pages.attend(1, start, s.lens, s.table, q, out, status=status[:-1])
+    from bmo_jetson_amd import lib
+    P = lambda z: z.data_ptr()
+    assert lib().bmo_kv_pages_attend_granted(s.pages.handle, 0, n, None, P(start), P(s.lens), P(s.table), width, total, heads,
+                                             1, P(q), 0, P(out), 0.0, 1, 0, 0, 0, None, 0, None) == 1
+    assert lib().bmo_kv_pages_attend_granted(None, 0, 1, None, None, None, None, 1, 1, 1, 1, None, 0, None, 0.0, 1, 0, 0, 0,
+                                             None, 0, None) == 1
+    s.pages.close()
