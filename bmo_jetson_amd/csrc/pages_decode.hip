@@ -86,6 +86,7 @@ struct Unit {
     int start, n_tok, entry_len;  // several rows
     int lo, len, lo_max, hi_min;
     int step0, n, runs;  // steps and runs
+    bool whole;          // the table reaches the entry's last position
 };
 // Positions that the token of a multi-row entry sees end before hi_of, and
 // begin with lo_of that.
@@ -101,7 +102,9 @@ __device__ __forceinline__ Unit unit_of(const DecodeArgs &a, int b, int unit) {
     const int64_t room = (int64_t) a.p.max_pages << a.p.g.page_shift;
     u.kvh = unit / a.n_hs;
     u.row0 = (unit - u.kvh * a.n_hs) * HC;
-    u.entry_len = (int) min((int64_t) max(granted_len(a.p.lens, a.p.n_new, a.p.status, b), 0), room);
+    const int given = granted_len(a.p.lens, a.p.n_new, a.p.status, b);
+    u.entry_len = (int) min((int64_t) max(given, 0), room);
+    u.whole = given <= room;
     if constexpr (MULTI) {
         u.start = uniform_int(a.p.q_start, b);
         const int end = uniform_int(a.p.q_start, b + 1);
@@ -203,8 +206,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
     }
 
     // The new token's row goes to its slot before the wave that will read it
-    // starts on its steps (of several head sets each writes the same bytes).
-    if (!MULTI && a.append && un.len > 0 && s_end == un.step0 + un.n && wave == (s_end - 1 - s_begin) % NW) {
+    // starts on its steps (of several head sets each writes the same bytes).  A
+    // last position past the table is in no page: its row is dropped.
+    if (!MULTI && a.append && un.len > 0 && un.whole && s_end == un.step0 + un.n && wave == (s_end - 1 - s_begin) % NW) {
         constexpr int BL = 32 / NB, NE = NB, HE = NE / 2, LPD = 4 / HE;
         const int nb = lane / BL, gi = lane % BL;
         const int64_t src = (int64_t) b * p.kv_stride + kvh * D + (nb % NB) * kQK + gi * HE;

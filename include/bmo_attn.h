@@ -549,9 +549,10 @@ BMO_ATTN_API int bmo_kv_pages_decode(bmo_kv_pages_t *pages, int layer, int n_bat
 /* The same with the append of the newest position: k_new and v_new
  * [n_batch][n_kv_heads][head_dim] are quantized into position lens[b] - 1 and
  * attended to with their quantized values.  Entries must not share the page of
- * that position.  Every entry with positions must have grown by its token: one
- * that did not would lose the newest token that it has.  Behind a plan that
- * may refuse an entry, or with entries that pause, call _granted. */
+ * that position; one past the table is dropped, as with a page id out of
+ * range.  Every entry with positions must have grown by its token: one that
+ * did not would lose the newest token that it has.  Behind a plan that may
+ * refuse an entry, or with entries that pause, call _granted. */
 BMO_ATTN_API int bmo_kv_pages_append_decode(bmo_kv_pages_t *pages, int layer, int n_batch,
                                             const int *lens, const int *table, int max_pages,
                                             int n_heads, int type, const void *q,
