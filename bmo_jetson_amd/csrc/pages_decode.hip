@@ -16,13 +16,14 @@
 // In the first form a lane has one block's products, so the block scales cost
 // one multiply a score and one a weight instead of NB each.
 //
-// K side, first form: q becomes a whole number of 23 bits (fp32; 15 bits for
-// 16-bit rows) times a power of two per row, in signed base-256 digits, and
-// the codes 0..15 enter v_mfma_i32_16x16x64_i8 as the bytes that a mask
-// leaves; the digits' sums and the -8 of every code join exactly in 32 bits.
-// Second form: q as two fp16 parts (16-bit rows: one, exactly), the codes
-// minus 8 exact in fp16.  Either way a query is within 2^-22 (2^-14) of its
-// row's largest element, and a block's product meets its scale in fp32.
+// K side: q as two fp16 parts times a power of two of its row (16-bit rows: one
+// part, exactly), the codes minus 8 exact in fp16, so a query is within 2^-22 of
+// each of its elements, however far apart these are, and a block's product meets
+// its scale in fp32.  (Whole numbers of 23 bits of the row's largest element, 15
+// for 16-bit rows, in base-256 digits on v_mfma_i32_16x16x64_i8 take 3 VALU
+// instructions a dword of codes, not 9: 6% less time in fp32, 2 to 4% in 16
+// bits.  But a channel 300 times the rest left the others so few bits that
+// outputs were 7e-5 off in fp32 and 8e-3 in fp16.)
 //
 // V side: weight times V scale, brought to fp16's range by a power of two per
 // column (from the largest scale so far), enters as two fp16 parts, exact to
@@ -164,8 +165,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
     constexpr int HC = 16 / CB;             // heads a head set
     constexpr int PB = NB / CB;             // blocks a column
     constexpr int QP = F32 ? 2 : 1;         // fp16 parts of the query
-    constexpr int QD = F32 ? 3 : 2;         // or base-256 digits
-    constexpr int QBITS = F32 ? 22 : 14;    // |Q| <= 2^QBITS
     constexpr int WP = F32 ? 2 : 1;         // parts of a weight
     constexpr int BUF = 2;  // steps resident in registers
     const PagesDecodeParams &p = a.p;
@@ -292,12 +291,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
     for (int j = 0; j < BUF - 1; ++j) load(min(first + j * NW, last), ids[j], buf[j]);
     __builtin_amdgcn_sched_barrier(0);
 
-    // The query, of every block (zero outside the column's own when columns are
-    // blocks); what the products make of it is multiplied by sq.
-    typedef int int4_t __attribute__((ext_vector_type(4)));
-    pg_half8 qp[SPREAD ? 1 : QP][SPREAD ? 1 : NB];
-    int4_t qd[SPREAD ? QD : 1][NB / 2];  // digits of blocks 2 i, 2 i + 1
-    int q8 = 0;                          // -8 times the sum of the row's Q in the column's block
+    // The query as fp16 parts, times a power of two of its row (of every block;
+    // zero outside the column's own when columns are blocks); what the products
+    // make of it is multiplied by sq.
+    pg_half8 qp[QP][NB];
     float sq;
     {
         float amax = 0.0f, bad = 0.0f;
@@ -306,7 +303,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
         for (int i = 0; i < PB; ++i) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int e = SPREAD ? (j & 3) + (j & 4) * 4 : octet_elem(0, j);  // 0..3, 16..19
+                const int e = octet_elem(0, j);  // 0..3, 16..19
                 x[i][j] = r >= un.cols ? 0.0f : e < 16 ? qx[i][0][e & 3] : qx[i][1][e & 3];
                 amax = fmaxf(amax, __builtin_fabsf(x[i][j]));
                 bad += x[i][j] * 0.0f;  // NaN if it is not finite
@@ -326,46 +323,21 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
         bad += __shfl_xor(bad, 32);
         // (rows below 2^-90 count as zeros: their scores do)
         const int ex = max(__builtin_amdgcn_frexp_expf(amax), -90);
-        constexpr int shift = SPREAD ? QBITS : 15;
         // (never 0: masked scores are -inf times it)
-        sq = bad == 0.0f ? fmaxf(__builtin_amdgcn_ldexpf(p.qscale, ex - shift), 1e-37f) : __builtin_nanf("");
-        if constexpr (SPREAD) {
-            uint32_t dig[QD][2];
+        sq = bad == 0.0f ? fmaxf(__builtin_amdgcn_ldexpf(p.qscale, ex - 15), 1e-37f) : __builtin_nanf("");
 #pragma unroll
-            for (int k = 0; k < QD; ++k) dig[k][0] = dig[k][1] = 0;
+        for (int blk = 0; blk < NB; ++blk)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                int Q = (int) __builtin_rintf(__builtin_amdgcn_ldexpf(x[0][j], shift - ex));
-                q8 -= 8 * Q;
+                float y = __builtin_amdgcn_ldexpf(x[SPREAD ? 0 : blk][j], 15 - ex);
+                if (SPREAD && blk != cb) y = 0.0f;
 #pragma unroll
-                for (int k = 0; k < QD; ++k) {
-                    const int low = k + 1 < QD ? (int) (int8_t) Q : Q;
-                    dig[k][j >> 2] |= (uint32_t) (low & 0xFF) << (8 * (j & 3));
-                    Q = (Q - low) >> 8;
+                for (int i = 0; i < QP; ++i) {
+                    const _Float16 h = (_Float16) y;
+                    qp[i][blk][j] = h;
+                    y -= (float) h;
                 }
             }
-            q8 += __shfl_xor(q8, 16);
-            q8 += __shfl_xor(q8, 32);
-#pragma unroll
-            for (int k = 0; k < QD; ++k)
-#pragma unroll
-                for (int i = 0; i < NB / 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) qd[k][i][e] = cb == 2 * i + (e >> 1) ? (int) dig[k][e & 1] : 0;
-        } else {
-#pragma unroll
-            for (int blk = 0; blk < NB; ++blk)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float y = __builtin_amdgcn_ldexpf(x[SPREAD ? 0 : blk][j], shift - ex);
-#pragma unroll
-                    for (int i = 0; i < QP; ++i) {
-                        const _Float16 h = (_Float16) y;
-                        qp[i][blk][j] = h;
-                        y -= (float) h;
-                    }
-                }
-        }
     }
 
     // A column's running maximum m (log2 units), the raw score past which it
@@ -377,7 +349,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
     uint32_t dt[PB];  // fp16 bits of the largest scale that kd allows for
     pg_float4 acc[NB][2];
     const pg_float4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    const int4_t izero = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < NB; ++i) acc[i][0] = acc[i][1] = zero;
 #pragma unroll
@@ -400,55 +371,30 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
 
     auto compute = [&](int step, Tile &t) {
         float s[8];  // scores, to be multiplied by sq
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = 0.0f;
+        pg_float4 d[2] = {zero, zero};
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk) {
+            pg_half8 kc[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) kc[u] = k_octet(word(t.k[u / T], (u % T) * NB + blk), pat);
+            if (!SPREAD) d[0] = d[1] = zero;
+#pragma unroll
+            for (int i = 0; i < QP; ++i)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) d[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[u], qp[i][blk], d[u], 0, 0, 0);
+            if (!SPREAD)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[i] = times_scale(d[i >> 2][i & 3], t.sc[i >> 2][SPREAD ? 0 : blk], 0, i & 3, s[i]);
+        }
         if constexpr (SPREAD) {
-            int4_t d[2][QD];
-            const int4_t start = {q8, q8, q8, q8};
-#pragma unroll
-            for (int i = 0; i < NB / 2; ++i) {
-                int4_t kc[2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const uint32_t w0 = word(t.k[u / T], (u % T) * NB + 2 * i);
-                    const uint32_t w1 = word(t.k[u / T], (u % T) * NB + 2 * i + 1);
-                    kc[u] = int4_t{(int) (w0 & 0x0F0F0F0Fu), (int) ((w0 >> 4) & 0x0F0F0F0Fu), (int) (w1 & 0x0F0F0F0Fu),
-                                   (int) ((w1 >> 4) & 0x0F0F0F0Fu)};
-                }
-#pragma unroll
-                for (int k = 0; k < QD; ++k)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        d[u][k] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-                            kc[u], qd[k][i], i > 0 ? d[u][k] : k == 0 ? start : izero, 0, 0, 0);
-            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int u = i >> 2, e = i & 3;
-                // sum (c - 8) Q, below 2^31 (the way there may wrap)
-                uint32_t sum = (uint32_t) d[u][QD - 1][e];
-#pragma unroll
-                for (int k = QD - 2; k >= 0; --k) sum = (sum << 8) + (uint32_t) d[u][k][e];
-                float x = times_scale((float) (int) sum, t.sc[u][0], 0, e, 0.0f);
+                float x = times_scale(d[i >> 2][i & 3], t.sc[i >> 2][0], 0, i & 3, 0.0f);
                 x += pg_dpp<0xB1>(x);
                 if constexpr (NB == 4) x += pg_dpp<0x4E>(x);
                 s[i] = x;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] = 0.0f;
-#pragma unroll
-            for (int blk = 0; blk < NB; ++blk) {
-                pg_float4 d[2] = {zero, zero};
-                pg_half8 kc[2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) kc[u] = k_octet(word(t.k[u / T], (u % T) * NB + blk), pat);
-#pragma unroll
-                for (int i = 0; i < QP; ++i)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        d[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc[u], qp[SPREAD ? 0 : i][SPREAD ? 0 : blk], d[u], 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    s[i] = times_scale(d[i >> 2][i & 3], t.sc[i >> 2][SPREAD ? 0 : blk], 0, i & 3, s[i]);
             }
         }
         if (!(step * kStep >= un.lo_max && step * kStep + kStep <= un.hi_min && t.ok == (1 << TG) - 1)) {

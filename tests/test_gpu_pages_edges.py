@@ -2,9 +2,53 @@
 import numpy as np
 import pytest
 
-from _pages import attention, check, i32, kv_rows, pool, to_type
+from _pages import HALF_STEP, attention, check, i32, kv_rows, pool, rel, slot_of, to_type
 
 pytestmark = pytest.mark.gpu
+
+# A result as a whole, in the mean square.  A rounding is at most half a step,
+# relative to the value, and 1 / sqrt(3) of that in the mean square.  fp16 rows:
+# the output's rounding and the weight's, 2^-11 sqrt(2 / 3); bf16 rows: 2^-8 /
+# sqrt(3) and the weight's 2^-11.  fp32: sums of some hundred roundings of 2^-24.
+WHOLE = {"float32": 5e-6, "float16": 2.0**-11, "bfloat16": 2.0**-8}
+
+
+def decode_reference(cache, table_row, page, length, q, type_, scale=None):
+    """(out, bound) of rows q that see all of an entry's positions, in 64 bits.
+    A query is within 2^-22 of each of its own elements (fp32: two fp16 parts,
+    each rounded, 2^-11 of 2^-11; 16-bit rows are exact) and within 2^-39 of its
+    largest (the parts end at 2^-24, half a step of that is 2^-25, the largest
+    is scaled past 2^14); a score sums 32 products in a block and up to 4 blocks
+    in fp32, 40 roundings of 2^-24, scaled, shifted by the maximum and raised
+    (4 more).  So it is off by e = (2^-22 + 44 2^-24) sum|q k| + 2^-39 max|q|
+    sum|k|, which moves a weight by e of itself and the sum by as much.  The
+    weighted sum itself: two parts of a weight (2^-22) and sums in fp32, within
+    2^-16 of 16 sum p|d| as in _pages; of 16-bit rows one part, 2^-11."""
+    n, heads, dim = q.shape
+    group = heads // cache.k.shape[1]
+    scale = dim**-0.5 if scale is None else scale
+    at = np.array([slot_of([table_row], 0, p, page) for p in range(length)])
+    out, bound = np.zeros(q.shape), np.zeros(q.shape)
+    for i in range(n):
+        for h in range(heads):
+            k, v, d = cache.k[at, h // group], cache.v[at, h // group], np.abs(cache.d[at, h // group])
+            s = k @ q[i, h] * scale
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            off = (2.0**-22 + 44 * 2.0**-24) * (np.abs(k) @ np.abs(q[i, h])).max() * scale
+            off += 2.0**-39 * np.abs(q[i, h]).max() * np.abs(k).sum(axis=1).max() * scale
+            b = (2 * off + (0 if type_ == "float32" else 2.0**-11)) * (p @ np.abs(v))
+            b += 2.0**-16 * 16 * np.repeat(p @ d, 32)
+            out[i, h] = p @ v
+            bound[i, h] = b + HALF_STEP[type_] * (np.abs(out[i, h]) + b)
+    return out, bound
+
+
+def refill(gpu, pages, cache, k, v):
+    """Every slot of layer 0 anew."""
+    every = np.arange(len(cache.k))
+    cache.put(every, k, v)
+    pages.append(0, i32(gpu, every), *(gpu.from_numpy(x).cuda() for x in (k, v)), stream=gpu.cuda.current_stream())
 
 
 @pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (2, 2, 128), (16, 1, 128), (16, 1, 64)])
@@ -32,4 +76,44 @@ def test_a_token_past_the_table_is_dropped(gpu, heads, kv, dim, past):
         check(out[b:b + 1].cpu().numpy(), ref, bound, f"entry {b}")
     pages.decode(0, i32(gpu, long), i32(gpu, table), q, plain, stream=stream)
     assert gpu.equal(out, plain)
+    pages.close()
+
+
+@pytest.mark.parametrize("type_", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 128), (3, 1, 64), (16, 1, 128), (16, 1, 64)])
+@pytest.mark.parametrize("big", [30, 300, 3000])
+def test_a_query_channel_far_above_the_rest(gpu, type_, heads, kv, dim, big):
+    """One channel of the query `big` times the others, against keys that hold
+    nothing there: the other channels keep their own precision, in decode, in
+    few rows and in tiles."""
+    page, length = 64, 600
+    pages, cache, table = pool(gpu, [length], page, kv, dim, 5)
+    k, v = kv_rows(3, len(cache.k), kv, dim), kv_rows(4, len(cache.k), kv, dim)
+    k[:, :, 41] = 0.0
+    refill(gpu, pages, cache, k, v)
+    x = np.random.default_rng(1).standard_normal((1, heads, dim))
+    x[:, :, 41] = big
+    q, x = to_type(gpu, x, type_)
+    lens, t, stream = i32(gpu, [length]), i32(gpu, table), gpu.cuda.current_stream()
+    ref, bound = decode_reference(cache, table[0], page, length, x, type_)
+    out = gpu.zeros_like(q)
+    pages.decode(0, lens, t, q, out, stream=stream)
+    got = out.double().cpu().numpy()
+    check(got, ref, bound, "decode")
+    assert rel(got, ref) < WHOLE[type_]
+    if type_ != "float32":
+        out.zero_()
+        pages.attend(0, i32(gpu, [0, 1]), lens, t, q, out, max_rows=1, stream=stream)
+        got = out.double().cpu().numpy()
+        check(got, ref, bound, "few rows")
+        assert rel(got, ref) < WHOLE[type_]
+        # and as one of so many entries and rows that they are taken in tiles
+        q = gpu.cat([q, q.new_zeros(2000, heads, dim)])
+        out, n = gpu.zeros_like(q), 64
+        pages.attend(0, i32(gpu, [0] + [1] * n), i32(gpu, [length] + [0] * (n - 1)),
+                     gpu.cat([t, t.new_full((n - 1, t.shape[1]), -1)]), q, out, max_rows=2000, stream=stream)
+        got = out[:1].double().cpu().numpy()
+        ref, bound = attention(cache, table[0], page, length, x, [length - 1], 0, "attend", type_)
+        check(got, ref, bound, "tiles")
+        assert rel(got, ref) < 2.0**-11 * (1 if type_ == "float16" else 8)
     pages.close()
