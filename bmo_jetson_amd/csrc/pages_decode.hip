@@ -25,24 +25,29 @@
 // bits.  But a channel 300 times the rest left the others so few bits that
 // outputs were 7e-5 off in fp32 and 8e-3 in fp16.)
 //
-// V side: weight times V scale, brought to fp16's range by a power of two per
-// column (from the largest scale so far), enters as two fp16 parts, exact to
-// 2^-22 (16-bit rows: one part), against the codes minus 8,
-// exact in fp16, sums in fp32.  An fp32 call is as close as fp32 sums; the
-// 16-bit parts stay below the outputs' own rounding.
-//
-// Softmax is online with a running maximum per column, raised only when a
-// score passes it by 8 (log2 units), so that the exchange between the four
-// lanes of a column and the rescaling are rare.  Masked positions get weight
-// 0 by select, whatever their slots hold.
+// V side: weight times V scale enters as two fp16 parts (16-bit rows: one)
+// against the codes minus 8, exact in fp16, sums in fp32.  Softmax is online.
+// What the weights are taken down by in a block follows the largest product of
+// weight and scale there, not the largest score: it is put at 2^2 and none
+// passes 2^15, so the parts are exact to 2^-22 of a product, or to 2^-27 of the
+// largest, whatever scales and weights unimportant positions have.  (Taken from
+// the largest score and the largest scale, a position of no weight with a scale
+// 2^20 times the others' left these 2e-3 off.)  So an fp32 call is as close as
+// fp32 sums; the 16-bit parts stay below the outputs' own rounding.  The four
+// lanes of a column look at the products, and rescale, only when a scale passes
+// four times the largest so far or a score the room that this leaves: once or
+// twice a run, unless positions of little weight have scales 2^8 times the
+// important ones'.  Masked positions get weight 0 by select, whatever their
+// slots hold.
 //
 // Work: an item is a run of steps of one (entry, kv head, head set), walked
 // by the NW waves of a workgroup in turn and joined in LDS.  The host knows
 // how long an entry can be, not how long each is: where that is long for the
 // units there are, an entry of n steps has ceil(n / c) even runs, up to a
 // number of them for which the grid has workgroups (those of shorter entries
-// end at once); results of entries that have several are kept as (max, sum,
-// row) in the workspace and joined by a second kernel in the order of the runs.
+// end at once); results of entries that have several are kept in the workspace,
+// with their sums and what both were taken down by, and joined by a second
+// kernel in the order of the runs.
 //
 // Measured, graph replays, every page from HBM, 32 query heads of 128: 64
 // entries of 3000 positions on 32 kv heads, fp32, 167 us, 5.3 TB/s (VALU 61% of
@@ -66,6 +71,13 @@ constexpr int kWaves = 4;  // of a workgroup, where it is not one
 constexpr int kFillWaves = 1024, kFillSteps = 4;
 constexpr int kSplitWaves = 4096, kSplitSteps = 16;
 constexpr int kMaxRuns = 128;  // of an entry
+// Softmax, in log2 units: how far a score may pass the one that the weights'
+// sum is taken from; and weight times V scale, which enters as fp16: where the
+// largest is put, what it has to pass to be put there again when a look is
+// taken, and what none passes between two looks.  A scale of zero counts as
+// 2^kZeroScale, so that weights stay finite.
+constexpr float kScoreLimit = 8.0f;
+constexpr float kProductTop = 2.0f, kProductRaise = 4.0f, kProductLimit = 15.0f, kZeroScale = -100.0f;
 constexpr int kLowUnits = 512, kLowSteps = 64;  // see there
 
 struct DecodeArgs {
@@ -146,10 +158,10 @@ __device__ __forceinline__ Column column_of(const DecodeArgs &a, const Unit &u, 
     return c;
 }
 
-// Floats of a partial result of HC heads: their rows, and maximum and sum of
-// every block (whose weights have a scale of their own).
+// Floats of a partial result of HC heads: their rows, what each block's weights
+// were taken down by, and each head's score that the sum is taken from, and sum.
 template <int D>
-__host__ __device__ constexpr int part_floats(int hc) { return hc * (D + 2 * (D / kQK)); }
+__host__ __device__ constexpr int part_floats(int hc) { return hc * (D + D / kQK + 2); }
 
 }  // namespace
 
@@ -171,7 +183,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
     const PagesGeom &g = p.g;
 
     __shared__ __align__(16) float s_out[NW][HC][D];
-    __shared__ float s_m[NW][HC][NB], s_l[NW][HC][NB];
+    __shared__ float s_mm[NW][HC][NB], s_m[NW][HC], s_l[NW][HC];
 
     // (16-bit kernels: known not to be fp32)
     const int type = F32 ? (int) kTypeF32 : p.type == kTypeF16 ? (int) kTypeF16 : (int) kTypeBF16;
@@ -340,13 +352,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
             }
     }
 
-    // A column's running maximum m (log2 units), the raw score past which it
-    // is raised, and per block the power of two 2^kd that its scales are
-    // brought up by (mm = m - kd) and the scale past which that changes.  l
-    // is the sum of this lane's weights times 2^kd of block 0.
-    float m = kPagesFloor, mt = -INFINITY, l = 0.0f;
-    float mm[PB], kd[PB];
-    uint32_t dt[PB];  // fp16 bits of the largest scale that kd allows for
+    // In log2 units, m is the column's largest score (lazily: none has passed it
+    // by kScoreLimit) and mm what its weights are taken down by in each block:
+    // the largest weight times V scale there, less kProductTop, lazily too.  No
+    // raw score has passed mt and no scale dt (fp16 bits, four times the largest
+    // so far), which together keep the products below kProductLimit.
+    // to_m = 2^(mm - m) of the first block; l is the sum of this lane's weights
+    // from m.
+    float m = kPagesFloor, mt = -INFINITY, to_m = 1.0f, l = 0.0f;
+    float mm[PB];
+    uint32_t dt[PB];
     pg_float4 acc[NB][2];
     const pg_float4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -354,7 +369,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
 #pragma unroll
     for (int i = 0; i < PB; ++i) {
         mm[i] = kPagesFloor;
-        kd[i] = 0.0f;
         dt[i] = 0;
     }
     const Patterns pat;
@@ -431,45 +445,66 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
             raise = raise || dx[j] > dt[j];
         }
         if (__any(raise)) {
+            // (what is changed follows from the column's own scores and scales,
+            // whichever asked, so that no column's rounding depends on another's)
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            // (a maximum that is not past its limit stays, so that lanes of
-            // one column agree whichever of them asked)
-            const float m_new = mx > mt ? fmaxf(m, mx * sq) : m;
-            float alpha[PB];
+            bool own = mx > mt;
+            float top[PB];  // the largest weight, from the largest score here, times scale
+            const float most = mx * sq;
+            {
+                float e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sq, -most));
+#pragma unroll
+                for (int j = 0; j < PB; ++j) {
+                    top[j] = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        // (not known to be the words below, whose conversions
+                        // would then be made up here for both)
+                        uint32_t d = word(t.sc[i >> 2][j], 2 + ((i & 2) >> 1));
+                        asm volatile("" : "+v"(d));
+                        const pg_half2 d2 = __builtin_bit_cast(pg_half2, d);
+                        top[j] = fmaxf(top[j], __builtin_fabsf(e[i] * (float) d2.x));
+                        top[j] = fmaxf(top[j], __builtin_fabsf(e[i + 1] * (float) d2.y));
+                    }
+                    top[j] = fmaxf(top[j], __shfl_xor(top[j], 16));
+                    top[j] = fmaxf(top[j], __shfl_xor(top[j], 32));
+                    dx[j] = max(dx[j], (uint32_t) __shfl_xor((int) dx[j], 16));
+                    dx[j] = max(dx[j], (uint32_t) __shfl_xor((int) dx[j], 32));
+                    own = own || dx[j] > dt[j];
+                }
+            }
+            const float m_old = m;
+            m = own ? fmaxf(m, most) : m;
+            l *= __builtin_amdgcn_exp2f(m_old - m);
+            float alpha[PB], room = m + kScoreLimit;
 #pragma unroll
             for (int j = 0; j < PB; ++j) {
-                dx[j] = max(dx[j], (uint32_t) __shfl_xor((int) dx[j], 16));
-                dx[j] = max(dx[j], (uint32_t) __shfl_xor((int) dx[j], 32));
-                // weights are below 2^8 and scales below 2^(ex + 1), so that
-                // their product times 2^kd stays below 2^15
-                if (dx[j] > dt[j] || dt[j] == 0) {
-                    const float d = f16_bits_to_f32(dx[j]);
-                    const int ex = d == 0.0f ? -24 : __builtin_amdgcn_frexp_expf(d);
-                    kd[j] = (float) (6 - ex);
-                    // 2^(ex + 1), or infinity: then nothing is past it but NaN
-                    dt[j] = f32_to_f16_bits(__builtin_amdgcn_ldexpf(1.0f, ex + 1));
-                }
-                alpha[j] = __builtin_amdgcn_exp2f(mm[j] - (m_new - kd[j]));
-                mm[j] = m_new - kd[j];
+                // (infinity counts as the largest scale: what it reaches is not
+                // finite, and nothing else is shifted for it)
+                const float at = most + fmaxf(__builtin_amdgcn_logf(fminf(top[j], 65504.0f)), kZeroScale);
+                const float mm_old = mm[j];
+                mm[j] = own && at > mm_old + kProductRaise ? at - kProductTop : mm_old;
+                alpha[j] = __builtin_amdgcn_exp2f(mm_old - mm[j]);
+                if (dx[j] > dt[j]) dt[j] = min(dx[j] + 0x800u, 0x7C00u);  // four times the scale
+                room = fminf(room, mm[j] + kProductLimit - __builtin_amdgcn_logf(fminf(f16_bits_to_f32(dt[j]), 65504.0f)));
             }
-            if (mx > mt) {
-                m = m_new;
-                mt = (m_new + kPagesLazy) / sq;
-            }
-            l *= alpha[0];
+            if (own) mt = room / sq;
+            to_m = __builtin_amdgcn_exp2f(mm[0] - m);
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
                 acc[i][0] *= alpha[SPREAD ? 0 : i];
                 acc[i][1] *= alpha[SPREAD ? 0 : i];
             }
         }
-        // weights times 2^kd of block 0; the other blocks' come by a factor
+        // weights of the first block; the other blocks' come by a factor
         float w[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sq, -mm[0]));
-            l += w[i];
+            l = __builtin_fmaf(w[i], to_m, l);
         }
 #pragma unroll
         for (int j = 0; j < PB; ++j) {
@@ -542,23 +577,27 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
     }
     if (oct == 0) {
 #pragma unroll
-        for (int j = 0; j < PB; ++j) {
-            s_m[wave][r][SPREAD ? cb : j] = mm[j];
-            s_l[wave][r][SPREAD ? cb : j] = j == 0 ? l : l * __builtin_amdgcn_exp2f(mm[0] - mm[j]);
+        for (int j = 0; j < PB; ++j) s_mm[wave][r][SPREAD ? cb : j] = mm[j];
+        if (cb == 0) {
+            s_m[wave][r] = m;
+            s_l[wave][r] = l;
         }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < un.cols * D; i += 64 * NW) {
         const int rr = i / D, e = i % D, blk = e / kQK;
-        float M = s_m[0][rr][blk];
+        float M = s_m[0][rr], MM = s_mm[0][rr][blk];
 #pragma unroll
-        for (int w = 1; w < NW; ++w) M = fmaxf(M, s_m[w][rr][blk]);
+        for (int w = 1; w < NW; ++w) {
+            M = fmaxf(M, s_m[w][rr]);
+            MM = fmaxf(MM, s_mm[w][rr][blk]);
+        }
+        const float base = un.runs == 1 ? M : MM;
         float L = 0.0f, o = 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-            const float f = __builtin_amdgcn_exp2f(s_m[w][rr][blk] - M);
-            L = __builtin_fmaf(f, s_l[w][rr][blk], L);
-            o = __builtin_fmaf(f, s_out[w][rr][e], o);
+            L = __builtin_fmaf(__builtin_amdgcn_exp2f(s_m[w][rr] - M), s_l[w][rr], L);
+            o = __builtin_fmaf(__builtin_amdgcn_exp2f(s_mm[w][rr][blk] - base), s_out[w][rr][e], o);
         }
         if (un.runs == 1) {
             const Column c = column_of<MULTI, D>(a, un, b, rr);
@@ -567,9 +606,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(SPREAD 
         } else {
             float *dst = p.work + (int64_t) blockIdx.x * part_floats<D>(HC);
             dst[rr * D + e] = o;
-            if (e % kQK == 0) {
-                dst[HC * D + rr * NB + blk] = M;
-                dst[HC * (D + NB) + rr * NB + blk] = L;
+            if (e % kQK == 0) dst[HC * D + rr * NB + blk] = MM;
+            if (e == 0) {
+                dst[HC * (D + NB) + rr] = M;
+                dst[HC * (D + NB + 1) + rr] = L;
             }
         }
     }
@@ -598,15 +638,14 @@ __global__ __launch_bounds__(256) void pages_join_kernel(DecodeArgs a) {
     for (int e = 0; e < E; ++e) o[e] = 0.0f;
     // block `wave`: every run's share of the whole, a run a lane
     if (wave < NB) {
-        const float *q = src + HC * D + rr * NB + wave;
+        const float *q = src + HC * D + rr * NB + wave, *ml = src + HC * (D + NB) + rr;
         float M = kPagesFloor, L = 0.0f;
-        for (int i = lane; i < runs; i += 64) M = fmaxf(M, q[i * stride]);
+        for (int i = lane; i < runs; i += 64) M = fmaxf(M, ml[i * stride]);
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
         for (int i = lane; i < runs; i += 64) {
-            const float f = __builtin_amdgcn_exp2f(q[i * stride] - M);
-            s_w[i][wave] = f;
-            L = __builtin_fmaf(f, q[i * stride + HC * NB], L);
+            s_w[i][wave] = __builtin_amdgcn_exp2f(q[i * stride] - M);
+            L = __builtin_fmaf(__builtin_amdgcn_exp2f(ml[i * stride] - M), ml[i * stride + HC], L);
         }
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) L += __shfl_xor(L, d);
@@ -634,7 +673,9 @@ namespace {
 // Columns are (head, block) while there are that few heads (or rows and heads).
 bool spread(const PagesGeom &g, int heads) { return heads <= 16 / (g.dim / kQK); }
 int set_heads(const PagesGeom &g, int heads) { return spread(g, heads) ? 16 / (g.dim / kQK) : 16; }
-int64_t part_bytes(const PagesGeom &g, int hc) { return (int64_t) hc * (g.dim + 2 * (g.dim / kQK)) * 4; }
+int64_t part_bytes(const PagesGeom &g, int hc) {
+    return (int64_t) (g.dim == 128 ? part_floats<128>(hc) : part_floats<64>(hc)) * 4;
+}
 // Workgroups of a launch whose long entries are cut (sets of 16 of dim 128
 // leave room for half as many at a time).
 int64_t split_workgroups(const PagesGeom &g, int hc) {

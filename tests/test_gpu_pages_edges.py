@@ -11,6 +11,14 @@ pytestmark = pytest.mark.gpu
 # the output's rounding and the weight's, 2^-11 sqrt(2 / 3); bf16 rows: 2^-8 /
 # sqrt(3) and the weight's 2^-11.  fp32: sums of some hundred roundings of 2^-24.
 WHOLE = {"float32": 5e-6, "float16": 2.0**-11, "bfloat16": 2.0**-8}
+# An output below the type's normal range ends at a fixed step, half of which is
+# what rounding can cost there whatever the value: fp16's step is 2^-24.
+LEAST = {"float32": 0.0, "float16": 2.0**-25, "bfloat16": 0.0}
+
+
+def check_whole(got, ref, type_):
+    off = np.linalg.norm(got - ref)
+    assert off < WHOLE[type_] * np.linalg.norm(ref) + LEAST[type_] * ref.size**0.5, rel(got, ref)
 
 
 def decode_reference(cache, table_row, page, length, q, type_, scale=None):
@@ -40,7 +48,7 @@ def decode_reference(cache, table_row, page, length, q, type_, scale=None):
             b = (2 * off + (0 if type_ == "float32" else 2.0**-11)) * (p @ np.abs(v))
             b += 2.0**-16 * 16 * np.repeat(p @ d, 32)
             out[i, h] = p @ v
-            bound[i, h] = b + HALF_STEP[type_] * (np.abs(out[i, h]) + b)
+            bound[i, h] = b + HALF_STEP[type_] * (np.abs(out[i, h]) + b) + LEAST[type_]
     return out, bound
 
 
@@ -100,13 +108,13 @@ def test_a_query_channel_far_above_the_rest(gpu, type_, heads, kv, dim, big):
     pages.decode(0, lens, t, q, out, stream=stream)
     got = out.double().cpu().numpy()
     check(got, ref, bound, "decode")
-    assert rel(got, ref) < WHOLE[type_]
+    check_whole(got, ref, type_)
     if type_ != "float32":
         out.zero_()
         pages.attend(0, i32(gpu, [0, 1]), lens, t, q, out, max_rows=1, stream=stream)
         got = out.double().cpu().numpy()
         check(got, ref, bound, "few rows")
-        assert rel(got, ref) < WHOLE[type_]
+        check_whole(got, ref, type_)
         # and as one of so many entries and rows that they are taken in tiles
         q = gpu.cat([q, q.new_zeros(2000, heads, dim)])
         out, n = gpu.zeros_like(q), 64
@@ -116,4 +124,61 @@ def test_a_query_channel_far_above_the_rest(gpu, type_, heads, kv, dim, big):
         ref, bound = attention(cache, table[0], page, length, x, [length - 1], 0, "attend", type_)
         check(got, ref, bound, "tiles")
         assert rel(got, ref) < 2.0**-11 * (1 if type_ == "float16" else 8)
+    pages.close()
+
+
+@pytest.mark.parametrize("type_", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 128), (3, 1, 64), (16, 1, 128), (16, 1, 64)])
+@pytest.mark.parametrize("ratio", [10, 20, 24])
+def test_unimportant_positions_with_large_values(gpu, type_, heads, kv, dim, ratio):
+    """Every 40th position has V scales 2^ratio times the others' and almost no
+    weight: the others keep their precision, whole and cut in runs."""
+    page, length = 64, 2300
+    pages, cache, table = pool(gpu, [length], page, kv, dim, 5)
+    k, v = kv_rows(3, len(cache.k), kv, dim), kv_rows(4, len(cache.k), kv, dim)
+    far = [slot_of(table, 0, p, page) for p in range(7, length, 40)]
+    k[:, :, 0], k[far, :, :] = 0.0, 0.0
+    k[far, :, 0] = -60.0
+    v *= 2.0**-12
+    v[far] *= 2.0**ratio
+    refill(gpu, pages, cache, k, v)
+    x = np.random.default_rng(1).standard_normal((1, heads, dim))
+    x[:, :, 0] = 8.0  # scores of -42 (-60 where the heads are 64 wide)
+    q, x = to_type(gpu, x, type_)
+    ref, bound = decode_reference(cache, table[0], page, length, x, type_)
+    work = gpu.zeros(pages.workspace_bytes(heads), dtype=gpu.uint8, device="cuda")
+    for w in (None, work):
+        out = gpu.zeros_like(q)
+        pages.decode(0, i32(gpu, [length]), i32(gpu, table), q, out, workspace=w, stream=gpu.cuda.current_stream())
+        got = out.double().cpu().numpy()
+        check(got, ref, bound, f"decode, workspace {w is not None}")
+        check_whole(got, ref, type_)
+    pages.close()
+
+
+@pytest.mark.parametrize("type_", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 128), (3, 1, 64), (16, 1, 128), (16, 1, 64)])
+@pytest.mark.parametrize("down", [12, 20, 30, 100])
+def test_a_position_that_takes_the_weight_and_holds_nothing(gpu, type_, heads, kv, dim, down):
+    """One position's weight is about 2^down times any other's and its V is
+    zero: what the others add up to is small and as exact as ever."""
+    page, length = 64, 700
+    pages, cache, table = pool(gpu, [length], page, kv, dim, 5)
+    k, v = np.zeros((len(cache.k), kv, dim)), kv_rows(4, len(cache.k), kv, dim)
+    sink = slot_of(table, 0, 130, page)
+    k[:, :, 40] = np.random.default_rng(2).standard_normal((len(k), kv)) / 50  # a factor of 2 or so between weights
+    k[sink, :, :], v[sink] = 0.0, 0.0
+    k[sink, :, 0] = 8.0
+    refill(gpu, pages, cache, k.astype(np.float32), v)
+    x = np.zeros((1, heads, dim))
+    x[:, :, 0] = (down + 0.3) * np.log(2) / 8 * dim**0.5
+    x[:, :, 40] = 30.0
+    q, x = to_type(gpu, x, type_)
+    ref, bound = decode_reference(cache, table[0], page, length, x, type_)
+    assert 0 < np.abs(ref).max() < 2.0**-down * length * 8
+    out = gpu.zeros_like(q)
+    pages.decode(0, i32(gpu, [length]), i32(gpu, table), q, out, stream=gpu.cuda.current_stream())
+    got = out.double().cpu().numpy()
+    check(got, ref, bound, "decode")
+    check_whole(got, ref, type_)
     pages.close()
