@@ -34,8 +34,8 @@
 // 32 with three waves a SIMD are 16% slower, scores one stage ahead of the
 // weights 5%.
 //
-// Precision: V enters as (code - 8) * d rounded to fp16, the weights as fp16,
-// sums in fp32; q enters scaled by its row's own power of two, exactly.  K does
+// Precision: V enters as (code - 8) * d rounded to fp16, the weights as fp16
+// (with all its bits down to 2^-21 of the row's largest), sums in fp32; q enters scaled by its row's own power of two, exactly.  K does
 // as V for bf16 rows, whose own rounding (1.7e-3) hides it.  For fp16 rows
 // (2.1e-4) it would show where scores are large (3.2e-4 in all, and more the
 // larger they are), so K's codes enter exactly and its scales meet the products
@@ -58,6 +58,11 @@ constexpr int kAttendWaves = 4;
 constexpr int kWaveRows = 32;
 constexpr int kTileRows = kWaveRows * kAttendWaves;
 constexpr int kStage = 64;  // positions a stage
+// Softmax, in log2 units: the running maximum is raised when a score passes it
+// by kLazy, and its weight is 2^kTop, so that none passes 2^15 and fp16 holds
+// weights down to 2^-21 of it with all their bits (those of 2^-32 are still
+// some).  4 and 11 would hold 2^-25, for 2 to 3% more time in raising it.
+constexpr float kLazy = 8.0f, kTop = 7.0f;
 
 struct AttendArgs {
     PagesAttendParams p;
@@ -394,7 +399,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_
             mx = fmaxf(mx, __shfl_xor(mx, 32));
             const float m_new = mx > mt ? fmaxf(m, mx * f) : m;
             const float alpha = __builtin_amdgcn_exp2f(m - m_new);
-            if (mx > mt) mt = (m_new + kPagesLazy) / f;
+            if (mx > mt) mt = (m_new + kLazy) / f;
             m = m_new;
             l *= alpha;
 #pragma unroll
@@ -410,6 +415,7 @@ __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_
 #pragma unroll
         for (int i = 0; i < VAHEAD; ++i) ring[i] = vx(i);
         const pg_half2 one = {(_Float16) 1.0f, (_Float16) 1.0f};
+        const float up = kTop - m;
 #pragma unroll
         for (int r = 0; r < 2 * NU; ++r) {
             // keys 0, 2, 1, 3 of each quad, as V's rows hold them; their sum is
@@ -417,8 +423,8 @@ __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
                 const int u = r / 2, k = 8 * (r & 1) + (j & 4) + ((j >> 1) & 1);
-                const pg_half2 h = {(_Float16) __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][k], f, -m)),
-                                    (_Float16) __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][k + 2], f, -m))};
+                const pg_half2 h = {(_Float16) __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][k], f, up)),
+                                    (_Float16) __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][k + 2], f, up))};
                 w[r][j] = h.x;
                 w[r][j + 1] = h.y;
                 l = __builtin_amdgcn_fdot2(h, one, l, false);

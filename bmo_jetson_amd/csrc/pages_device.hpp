@@ -14,7 +14,6 @@ typedef _Float16 pg_half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 pg_bf16x2 __attribute__((ext_vector_type(2)));
 typedef float pg_float4 __attribute__((ext_vector_type(4)));
 
-constexpr float kPagesLazy = 8.0f;       // lazy rescale threshold, log2 units
 constexpr float kPagesFloor = -1.0e30f;  // running-max floor, finite
 
 // Element of its block that slot r of octet c of a dequantized K dword holds

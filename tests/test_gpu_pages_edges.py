@@ -182,3 +182,35 @@ def test_a_position_that_takes_the_weight_and_holds_nothing(gpu, type_, heads, k
     check(got, ref, bound, "decode")
     check_whole(got, ref, type_)
     pages.close()
+
+
+@pytest.mark.parametrize("type_", ["float16", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("down", [12, 16, 19])
+def test_tiles_keep_small_weights(gpu, type_, dim, down):
+    """Tiles of rows, one position with about 2^down times any other's weight
+    and V of zero: the weights of the others (down to 2^-21 of the largest) have
+    all of fp16's bits (2^-11), as V has, so the whole is off by their roundings and the output's alone."""
+    page, length, heads, kv = 64, 700, 4, 2
+    pages, cache, table = pool(gpu, [length], page, kv, dim, 5)
+    k, v = np.zeros((len(cache.k), kv, dim)), 256 * kv_rows(4, len(cache.k), kv, dim)
+    sink = slot_of(table, 0, 130, page)
+    k[:, :, 40] = np.random.default_rng(2).standard_normal((len(k), kv)) / 50
+    k[sink, :, :], v[sink] = 0.0, 0.0
+    k[sink, :, 0] = 8.0
+    refill(gpu, pages, cache, k.astype(np.float32), v)
+    x = np.zeros((1, heads, dim))
+    x[:, :, 0] = (down + 0.3) * np.log(2) / 8 * dim**0.5
+    x[:, :, 40] = 30.0
+    q, x = to_type(gpu, x, type_)
+    q = gpu.cat([q, q.new_zeros(2000, heads, dim)])
+    out, n, t = gpu.zeros_like(q), 64, i32(gpu, table)
+    pages.attend(0, i32(gpu, [0] + [1] * n), i32(gpu, [length] + [0] * (n - 1)),
+                 gpu.cat([t, t.new_full((n - 1, t.shape[1]), -1)]), q, out, max_rows=2000, stream=gpu.cuda.current_stream())
+    got = out[:1].double().cpu().numpy()
+    ref, _ = attention(cache, table[0], page, length, x, [length - 1], 0, "attend", type_)
+    # three roundings, each 1 / sqrt(3) of its half step in the mean square
+    off = np.linalg.norm(got - ref)
+    three = ((HALF_STEP[type_]**2 + 2 * 2.0**-22) / 3)**0.5
+    assert off < three * np.linalg.norm(ref) + LEAST[type_] * ref.size**0.5, (rel(got, ref), np.abs(ref).max())
+    pages.close()
