@@ -12,11 +12,13 @@
 //
 // The entries pass in chunks of 1024, one a thread: one block-wide pass of
 // three prefix sums (lane shifts, no LDS but for the waves' sums), then the
-// workgroup's share of the chunk's new tokens, each finding
-// its entry by binary search in LDS.  The token on a page's first position
-// also enters the page in the table.  With many tokens several workgroups do
-// the same scans and share the tokens; lengths, list and counts are replaced
-// by the workgroup that arrives last, when every other has read them.
+// workgroup's share of the chunk's new tokens, each finding its entry by binary
+// search in LDS.  The token on a page's first position also enters the page in
+// the table; where no call asks for the tokens' places, granted pages are
+// walked instead, so that what is refused costs nothing.  With many tokens
+// several workgroups do the same scans and share the tokens; lengths, list and
+// counts are replaced by the workgroup that arrives last, when every other has
+// read them.
 //
 // Latency bounds it, load after load (lengths, list, table) and the code's own
 // fetch: 48 entries with a token each 4.4 us, 256 entries with 64 k tokens of
@@ -171,6 +173,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanParams p) {
     const int64_t n_free = min(max(p.list[0], 0), p.n_pages);
     const int *ids = p.list + kListHead;
 
+    const bool places = p.tok_slot || p.tok_pos || p.tok_entry;
     Carry c;
     Entry e{};
     for (int b0 = 0; b0 < p.n_batch; b0 += kPlanThreads) {
@@ -178,11 +181,23 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanParams p) {
         e = scan_chunk(p, b0, n_free, c, s_sums);
         const int n = min(kPlanThreads, p.n_batch - b0);
         __syncthreads();  // the last chunk's tokens are placed
-        s_start[tid] = clamp_int(e.start);
+        // (pages before the entry's: of granted ones only these are walked)
+        s_start[tid] = clamp_int(places ? e.start : e.upto - e.need - before.need);
         s_len[tid] = (int) e.len;
         s_have[tid] = (int) e.have_pages;
         s_taken[tid] = e.state == 0 ? clamp_int(n_free - 1 - (e.upto - e.need)) : INT32_MIN;
         __syncthreads();
+        if (!places) {
+            // pages of this chunk, shared like tokens: the k-th in the order of
+            // the entries comes k-th from the end of the list
+            for (int64_t k = (int64_t) blockIdx.x * kPlanThreads + tid; k < c.given - before.need;
+                 k += (int64_t) gridDim.x * kPlanThreads) {
+                const int i = find(s_start, n, (int) k);
+                p.table[(int64_t) (b0 + i) * p.max_pages + s_have[i] + ((int) k - s_start[i])] =
+                    ids[n_free - 1 - (before.need + k)];
+            }
+            continue;
+        }
         // tokens of this chunk, every gridDim.x-th run of them this workgroup's
         const int64_t end = min(c.tokens, (int64_t) p.max_tok);
         for (int64_t t = before.tokens + (int64_t) blockIdx.x * kPlanThreads + tid; t < end;
