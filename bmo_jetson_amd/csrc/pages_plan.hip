@@ -187,26 +187,18 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanParams p) {
         s_have[tid] = (int) e.have_pages;
         s_taken[tid] = e.state == 0 ? clamp_int(n_free - 1 - (e.upto - e.need)) : INT32_MIN;
         __syncthreads();
-        if (!places) {
-            // pages of this chunk, shared like tokens: the k-th in the order of
-            // the entries comes k-th from the end of the list
-            for (int64_t k = (int64_t) blockIdx.x * kPlanThreads + tid; k < c.given - before.need;
-                 k += (int64_t) gridDim.x * kPlanThreads) {
-                const int i = find(s_start, n, (int) k);
-                p.table[(int64_t) (b0 + i) * p.max_pages + s_have[i] + ((int) k - s_start[i])] =
-                    ids[n_free - 1 - (before.need + k)];
-            }
-            continue;
-        }
-        // tokens of this chunk, every gridDim.x-th run of them this workgroup's
-        const int64_t end = min(c.tokens, (int64_t) p.max_tok);
-        for (int64_t t = before.tokens + (int64_t) blockIdx.x * kPlanThreads + tid; t < end;
+        // tokens (or granted pages, by their first positions) of this chunk, every
+        // gridDim.x-th run of them this workgroup's
+        const int64_t begin = places ? before.tokens : 0;
+        const int64_t end = places ? min(c.tokens, (int64_t) p.max_tok) : c.given - before.need;
+        for (int64_t t = begin + (int64_t) blockIdx.x * kPlanThreads + tid; t < end;
              t += (int64_t) gridDim.x * kPlanThreads) {
             const int i = find(s_start, n, (int) t);
             const int taken = s_taken[i];
             int pos = -1, slot = -1;
             if (taken != INT32_MIN) {
-                pos = s_len[i] + ((int) t - s_start[i]);
+                pos = (int) t - s_start[i];
+                pos = places ? s_len[i] + pos : (s_have[i] + pos) << p.page_shift;
                 const int col = pos >> p.page_shift, off = pos & (page - 1);
                 int *entry = p.table + (int64_t) (b0 + i) * p.max_pages + col;
                 int id;
