@@ -21,27 +21,29 @@
 // that 16 lanes reading 16 bytes each from consecutive rows meet every LDS
 // bank once.
 //
-// Measured, 32 query heads on 8 of 128: eight chunks of 200 to 1024 rows over
-// 300 to 4000 positions 321 us, 763 TFLOP/s; of 1024 rows over 4096 positions
-// each 690 us, 800 TFLOP/s (a large library product reaches 1173).  Bound by
-// the card's power: the clock stands at 1.99 GHz (1.5 in that library
-// product), with 52% of a SIMD's cycles VALU (exponentials, dequantizing,
-// masks) and 37% matrix instructions, two waves a SIMD.  So less work helps
-// and another order of it does not: dequantizing and the weights between the
-// matrix instructions, or without the LDS reads, run as long; without
+// Measured in a graph, 32 query heads on 8 of 128, bf16: eight chunks of 200 to
+// 1024 rows over 300 to 4000 positions 325 us, 755 TFLOP/s; of 1024 rows that all
+// see 4096 positions 638 us, 862 TFLOP/s (a large library product reaches 1211).
+// Bound by the card's power: with such full tiles the clock stands at 2.02 GHz
+// (1.5 in that library product), with 53% of a SIMD's cycles VALU (exponentials,
+// dequantizing, masks) and 38% matrix instructions, two waves a SIMD (46% and
+// 32% in the eight chunks, whose last workgroups leave CUs idle).  So less work
+// helps and another order of it does not: dequantizing and the weights between
+// the matrix instructions, or without the LDS reads, run as long; without
 // dequantizing 20% less.  Eight waves a workgroup (half the dequantizing a row)
 // win 4% with full tiles of one length and lose 10% with ragged ones; stages of
 // 32 with three waves a SIMD are 16% slower, scores one stage ahead of the
 // weights 5%.
 //
 // Precision: V enters as (code - 8) * d rounded to fp16, the weights as fp16
-// (with all its bits down to 2^-21 of the row's largest), sums in fp32; q enters scaled by its row's own power of two, exactly.  K does
-// as V for bf16 rows, whose own rounding (1.7e-3) hides it.  For fp16 rows
-// (2.1e-4) it would show where scores are large (3.2e-4 in all, and more the
-// larger they are), so K's codes enter exactly and its scales meet the products
-// of each block in fp32: 787 us where 677 were, see above.  V (and K of bf16
-// rows) must lie in fp16's range; a V block whose scale brings it past makes
-// the rows that see it NaN in that block and leaves the others.
+// (with all its bits down to 2^-21 of the row's largest), sums in fp32; q enters
+// scaled by its row's own power of two, exactly.  K does as V for bf16 rows,
+// whose own rounding (1.7e-3) hides it.  For fp16 rows (2.1e-4) it would show
+// where scores are large (3.2e-4 in all, and more the larger they are), so K's
+// codes enter exactly and its scales meet the products of each block in fp32:
+// 754 us where 638 are, see above.  V (and K of bf16 rows) must lie in fp16's
+// range; a V block whose scale brings it past makes the rows that see it NaN in
+// that block and leaves the others.
 #include <algorithm>
 
 #include "kernels.hpp"
@@ -510,16 +512,16 @@ __global__ __launch_bounds__(64 * kAttendWaves) __attribute__((amdgpu_waves_per_
 
 // Calls with few rows are taken a column a row (pages_decode.hip), 16 columns a
 // workgroup and an entry's positions shared among workgroups.  A tile's
-// workgroup goes over its entry alone, 34 ns a position (23 with every wave
-// full), 95 ps of the whole chip's time; a set of 16 columns takes 30 ps.  So
-// sets win until they fill the chip as tiles do not (1024 of them), and past
-// that where a tile is no more than two sets.  us in a graph, tiles / sets:
-//   32 kv heads of 128, one entry of 4000: 1 row 148 / 12, 16 rows 147 / 19,
-//     64 rows 109 / 33; 64 entries of 1000: 4 rows 193 / 49, 16 rows 195 / 85,
-//     24 rows 195 / 163, 48 rows 197 / 240.
-//   8 kv heads of 128, 32 heads, 16 entries of 8000: 4 rows 283 / 47, 16 rows
-//     (512 sets) 204 / 123, 24 (768) 208 / 186, 32 (1024) 213 / 238.
-//   16 kv heads of 64, 64 entries of 1000: 16 rows 73 / 25, 32 rows 52 / 42.
+// workgroup goes over its entry alone, 37 ns a position (27 with every wave
+// full), 98 ps of the whole chip's time; a set of 16 columns takes 30 to 40 ps.
+// So sets win until they fill the chip as tiles do not (1024 of them), and past
+// that where a tile is no more than two sets.  us in a graph, bf16, tiles / sets:
+//   32 kv heads of 128, one entry of 4000: 1 row 149 / 13, 16 rows 149 / 20,
+//     64 rows 110 / 34; 64 entries of 1000: 4 rows 203 / 53, 16 rows 197 / 90,
+//     24 rows 199 / 169, 48 rows 204 / 247.
+//   8 kv heads of 128, 32 heads, 16 entries of 8000: 4 rows 286 / 50, 16 rows
+//     (512 sets) 220 / 123, 24 (768) 230 / 187, 32 (1024) 242 / 255.
+//   16 kv heads of 64, 64 entries of 1000: 16 rows 75 / 26, 32 rows 53 / 44.
 static bool few_rows(const PagesAttendParams &p, int max_rows) {
     const int64_t rows = (int64_t) max_rows * (p.n_heads / p.g.n_kv);
     const int64_t units = (int64_t) p.n_batch * p.g.n_kv;

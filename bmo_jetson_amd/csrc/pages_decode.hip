@@ -50,10 +50,10 @@
 // kernel in the order of the runs.
 //
 // Measured, graph replays, every page from HBM, 32 query heads of 128: 64
-// entries of 3000 positions on 32 kv heads, fp32, 167 us, 5.3 TB/s (VALU 61% of
-// the cycles; the loads alone take 136); 12 entries of 32000 on 8, bf16, 81 us,
-// 5.5 TB/s (the loads alone 76: HBM in this page order); one entry of 700 on
-// 32, fp32, 8.7 us, six steps a wave one after the other.
+// entries of 3000 positions on 32 kv heads, fp32, 167 us, 5.3 TB/s (VALU 62% of
+// the cycles; the loads alone take 136), bf16 143; 12 entries of 32000 on 8,
+// bf16, 84 us, 5.3 TB/s (the loads alone 76: HBM in this page order); one entry
+// of 700 on 32, fp32, 9.1 us, six steps a wave one after the other.
 #include <algorithm>
 
 #include "kernels.hpp"
@@ -706,26 +706,29 @@ hipError_t launch_of(const DecodeArgs &arg, int nw, hipStream_t stream) {
 }
 
 // Shape of a launch, from its units and the steps that its longest entry can
-// have.  us a launch in a graph, dim 128, fp32, 32 heads:
-//   one wave a unit or four:  2048 units x 16 steps 27.9 / 31.2, 8192 x 7
-//     48 / 68, 1024 x 16 18.2 / 18.7; 2048 x 32 53.9 / 54.9, x 63 100 / 97,
-//     of 3 to 63 steps 77 / 60 (a long unit's one wave is the last to end).
+// have.  us a launch in a graph, pages from HBM, dim 128, 32 heads:
+//   one wave a unit or four, fp32:  2048 units x 16 steps 38 / 42, 8192 x 7
+//     56 / 87, 1024 x 16 19.7 / 19.2; 2048 x 32 63 / 62, x 63 116 / 109, of 3 to
+//     63 steps 85 / 65 (a long unit's one wave is the last to end).
 //   more than 4 heads (rows) a kv head in sets of 16 or of 4, while these are no
 //     more than two workgroups a CU and 64 steps long, dim 128 (whose sets of
 //     16 hold two waves a SIMD and multiply every head with every block):  one
-//     entry, 8 heads on each of 4 kv heads, 150 positions 7.7 / 5.7, 600 11.8 /
-//     8.3, 1500 16.4 / 12.3, 12 entries of 1500 17.9 / 13.2; rows of one entry
-//     of 32 kv heads, 600 positions, 12 rows 13 / 9, 64 rows 14 / 12; past the
-//     limits 96 sets x 125 steps 18 / 21, 960 x 19 18 / 20.
-//   runs of at least 4 steps a wave, of 16, or nothing cut:  32 units x 94
-//     steps 11.2 / 21.6 / 21.6, x 250 14.5 / 16.8 / 49, 8 x 1000 17.7 / 18.7 /
-//     184; 128 units of up to 250 steps in 3 or 2 runs 35.4 / 32.5, 24 of up to
-//     1000 in 15 or 10 27 / 25, 80 of up to 282 in 4 or 3 39 / 34 (past two
-//     workgroups a CU the entries' own lengths decide: 96 of 62 to 1000 in 10
-//     or 8 52.5 / 57.5, all of 1000 84 / 78); 256 x 32 13.7 / 10.7 / 10.7, 512 x 32 21.5 / 16.3 / 16.2; 96 units
-//     of 62 to 1000 steps 56 / 54 / 183.  Sets of 16 rows, bf16, cut for 1024
-//     workgroups, for 512, or not:  132 x 204 steps 46 / 45 / 54, 128 x 500
-//     82 / 66 / 72.
+//     entry, 8 heads on each of 4 kv heads, fp32, 150 positions 8.3 / 6.1, 600
+//     11.8 / 8.5, 1500 17.1 / 13.1, 12 entries of 1500 18.5 / 14.3; rows of one
+//     entry of 32 kv heads, 600 positions, bf16, 12 rows 13.1 / 8.9, 64 rows
+//     14.8 / 12.4; past the limits 96 sets x 125 steps 20.8 / 23.3, 960 x 19
+//     20.4 / 23.1.
+//   long entries cut for 256 workgroups (runs of at least 4 steps a wave), for
+//     1024 (of 16), or not; the rule takes the more runs of the first two:  fp32,
+//     32 units x 94 steps 12.8 / 23 / 23, x 250 15.8 / 24.4 / 52, 8 x 1000
+//     16.6 / 23.7 / 192; bf16, 96 units of 62 to 1000 steps 95 / 61 / 169.  Fewer
+//     steps a wave lose:  fp32, 256 x 32 in two runs or one 15.7 / 11.0, 512 x 32
+//     25.2 / 17.3.  Sets of 16 rows, bf16, cut for 1024 workgroups, for 512, or
+//     not:  132 x 204 steps 52 / 46 / 56, 128 x 500 79 / 71 / 125.
+//   runs that load the CUs evenly, bf16:  128 units of up to 250 steps in 3 or 2
+//     runs 33.5 / 31.7, 24 of up to 1000 in 15 or 10 29.6 / 26.9, 80 of up to 282
+//     in 4 or 3 28.8 / 25.6; past two workgroups a CU it hardly matters (96 of 62
+//     to 1000 in 10 or 8 61.0 / 60.0, all of 1000 83 / 81).
 template <bool MULTI>
 hipError_t launch_units(const PagesDecodeParams &p, int heads, hipStream_t stream) {
     DecodeArgs a{};

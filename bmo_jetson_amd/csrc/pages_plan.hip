@@ -21,8 +21,8 @@
 // read them.
 //
 // Latency bounds it, load after load (lengths, list, table) and the code's own
-// fetch: 48 entries with a token each 4.4 us, 256 entries with 64 k tokens of
-// prompts 7.1 us in a graph (one workgroup per 1024 tokens; per 4096 8.7 us,
+// fetch: 48 entries with a token each 4.8 us, 256 entries with 64 k tokens of
+// prompts 7.2 us in a graph (one workgroup per 1024 tokens; per 4096 8.7 us,
 // waves of a quarter as many threads 13 us).  Four returned pages a thread at
 // a time cost a token's step 0.5 us more than they save.
 #include <algorithm>

@@ -503,7 +503,8 @@ BMO_ATTN_API int bmo_kv_pages_list_init(bmo_kv_pages_t *pages, int *free_list, v
  *             entry: its slot and position (-1 for a refused entry) and entry
  *   status [n_batch]: 0 done, 1 no free pages, 2 out of range (a negative
  *             length, longer than the table, or tokens past max_tok)
- * These five may be NULL (max_tok bounds the tokens all the same).  Table
+ * These five may be NULL (max_tok bounds the tokens all the same); what reads
+ * the pages next takes n_new and status, see the _granted calls.  Table
  * columns past an entry's length, and tokens past the last, are left as they
  * were.  A page belongs to one entry.  Calls on one list must be ordered.
  * Asynchronous, allocates nothing, one launch. */
@@ -539,7 +540,9 @@ BMO_ATTN_API int64_t bmo_kv_pages_workspace_bytes(const bmo_kv_pages_t *pages, i
  * without positions gets zeros.  max_len: no entry is longer (0: not known);
  * it only chooses how the call is cut.  fp32 results are as close as fp32
  * arithmetic.  An entry's result depends on no other entry's; its rounding
- * depends on how it is cut (n_batch, max_len, the table's width). */
+ * depends on how it is cut (n_batch, max_len, the table's width).  Queries
+ * enter within 2^-22 of each element (16-bit ones exactly); in 16 bits the
+ * weights, times V's scales, are rounded to fp16. */
 BMO_ATTN_API int bmo_kv_pages_decode(bmo_kv_pages_t *pages, int layer, int n_batch,
                                      const int *lens, const int *table, int max_pages,
                                      int n_heads, int type, const void *q, int64_t q_stride,
@@ -582,7 +585,9 @@ BMO_ATTN_API int bmo_kv_pages_append_decode_granted(
  * counted back from the row's last position.  Rows that see nothing are
  * zeros.  max_rows: no entry has more rows (0: not known; rows past it may be
  * left as they were), max_len as in decode.  Scores and sums in fp32; V, the
- * weights and for bf16 rows K enter the matrix cores in fp16. */
+ * weights and for bf16 rows K enter the matrix cores in fp16 (in calls of few
+ * rows the weights alone, times V's scales).  K and V past fp16's range (scales
+ * from 8192 on) may make the rows that see them NaN, by the call's shape. */
 BMO_ATTN_API int bmo_kv_pages_attend(bmo_kv_pages_t *pages, int layer, int n_batch,
                                      const int *q_start, const int *lens, const int *table,
                                      int max_pages, int n_rows, int n_heads, int type,
