@@ -463,7 +463,9 @@ BMO_ATTN_API int bmo_launch_gemv_q4_0_q8_1(const void *W_dev, const float *x_dev
  * `stride` elements apart from token to token (0: dense; a packed QKV row has
  * a longer one), 16-byte aligned.  Calls that write slots must be ordered with
  * the calls that read them, as for the ring.  K and V must be finite and, for
- * attend, lie in fp16 range; what masked positions hold never shows.
+ * attend, lie in fp16 range; what masked positions hold never shows.  Scores,
+ * scale q . k, are taken up to 10^6 in magnitude; far past that, where fp32 no
+ * longer tells neighbours apart (from 10^7 on), rows can come out as NaN.
  */
 typedef struct bmo_kv_pages bmo_kv_pages_t;
 
