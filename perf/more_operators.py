@@ -152,7 +152,7 @@ def _weights(g, outs, cols):
     return codes, scales.half()
 
 
-def _matrix(codes, scales, gated=False):
+def _matrix(codes, scales):
     """What a program keeps of its weights: the library's, or their values."""
     outs, blocks, _ = codes.shape
     if own:
@@ -160,7 +160,7 @@ def _matrix(codes, scales, gated=False):
         packed = torch.empty(outs, blocks, 18, dtype=torch.uint8, device="cuda")
         packed[:, :, :2] = scales.view(torch.uint8).view(outs, blocks, 2)
         packed[:, :, 2:] = codes[:, :, :16] | (codes[:, :, 16:] << 4)
-        w = Q4Weights(outs, blocks * 32, gated=gated)
+        w = Q4Weights(outs, blocks * 32)
         w.load(packed, stream=torch.cuda.current_stream())
         torch.cuda.synchronize()
         return w
@@ -274,7 +274,7 @@ def _ffn_inputs(c, seed):
 def _prepare_ffn(c, seed):
     into, down, (codes, scales) = _ffn_inputs(c, seed)
     m, h = c["rows"], c["hidden"]
-    return {"kind": "ffn", "in": _matrix(*into, gated=True), "down": _matrix(*down), "codes": codes, "scales": scales,
+    return {"kind": "ffn", "in": _matrix(*into), "down": _matrix(*down), "codes": codes, "scales": scales,
             "act": c["act"], "hidden": torch.empty(m, h, dtype=torch.int8, device="cuda"),
             "hidden_scales": torch.empty(m, h // 32, dtype=torch.float16, device="cuda"),
             "out": torch.empty(m, c["dim"], dtype=_type(c["type"]), device="cuda")}
