@@ -22,10 +22,15 @@ from .ring import (  # noqa: F401
     BLOCK_Q4_0_BYTES,
 )
 from .pages import KVPages  # noqa: F401
+from .rows import Q4Weights, Rope, quantize_rows, rms_norm  # noqa: F401
 
 __all__ = [
     "KVRing",
     "KVPages",
+    "Q4Weights",
+    "Rope",
+    "quantize_rows",
+    "rms_norm",
     "RingError",
     "Session",
     "launch_decode_attention",

@@ -18,6 +18,7 @@ P = ctypes.c_void_p
 i32 = ctypes.c_int
 i64 = ctypes.c_int64
 f32 = ctypes.c_float
+f64 = ctypes.c_double
 
 SIGNATURES = {
     "bmo_kv_ring_stripe_bytes": (i64, [i32, i32]),
@@ -78,6 +79,22 @@ SIGNATURES = {
                                   i64, P]),
     "bmo_kv_pages_attend_granted": (i32, [P, i32, i32, P, P, P, P, i32, i32, i32, i32, P, i64, P, f32, i32, i32, i32,
                                           i32, P, i64, P]),
+    "bmo_rows_last_error": (ctypes.c_char_p, []),
+    "bmo_rms_norm": (i32, [i32, i32, i32, P, i64, i32, P, i64, i32, P, f32, i32, P, i64, P, P, P]),
+    "bmo_quantize_rows": (i32, [i32, i32, i32, P, i64, P, P, P]),
+    "bmo_rope_create": (P, [i32, i32, i32, f64, f64, i32, f64, f64, f64, P]),
+    "bmo_rope_free": (None, [P]),
+    "bmo_rope_device": (i32, [P]),
+    "bmo_rope_last_error": (ctypes.c_char_p, [P]),
+    "bmo_rope_apply": (i32, [P, i32, P, i32, i32, P, i64, P, i64, i32, P, i64, P, i64, P]),
+    "bmo_weights_create": (P, [i32, i32]),
+    "bmo_weights_free": (None, [P]),
+    "bmo_weights_bytes": (i64, [P]),
+    "bmo_weights_device": (i32, [P]),
+    "bmo_weights_last_error": (ctypes.c_char_p, [P]),
+    "bmo_weights_load": (i32, [P, i32, i32, P, P]),
+    "bmo_weights_product": (i32, [P, i32, P, P, i32, P, i64, P]),
+    "bmo_weights_gated": (i32, [P, i32, P, P, i32, i32, P, i64, P, P, P]),
 }
 
 

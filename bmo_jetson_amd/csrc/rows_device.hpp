@@ -1,0 +1,102 @@
+// rows_device.hpp -- what the operators on rows share.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "pages_device.hpp"
+#include "rows.hpp"
+
+namespace bmo {
+
+typedef float rw_float4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ uint32_t bf16_bits(float x) {
+    const __bf16 h = (__bf16) x;
+    return __builtin_bit_cast(uint16_t, h);
+}
+
+// Eight elements as they lie in memory; the second 16 bytes are fp32's.
+struct Raw8 {
+    uint4 a, b;
+};
+__device__ __forceinline__ Raw8 load_raw8(const void *p, int64_t i, int type) {
+    const uint8_t *src = static_cast<const uint8_t *>(p) + i * type_bytes(type);
+    Raw8 r;
+    r.a = *reinterpret_cast<const uint4 *>(src);
+    r.b = r.a;
+    if (type == kTypeF32) r.b = *reinterpret_cast<const uint4 *>(src + 16);
+    return r;
+}
+__device__ __forceinline__ void widen8(const Raw8 &r, int type, float (&x)[8]) {
+    const uint32_t u[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+    if (type == kTypeF32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = __builtin_bit_cast(float, u[j]);
+    } else if (type == kTypeF16) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = f16_bits_to_f32(j & 1 ? u[j >> 1] >> 16 : u[j >> 1] & 0xFFFFu);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = __builtin_bit_cast(float, j & 1 ? u[j >> 1] & 0xFFFF0000u : u[j >> 1] << 16);
+    }
+}
+// Rounds x to the type, as its stored value reads.
+__device__ __forceinline__ float round_to(float x, int type) {
+    if (type == kTypeF16) return f16_bits_to_f32(f32_to_f16_bits(x));
+    if (type == kTypeBF16) return __builtin_bit_cast(float, bf16_bits(x) << 16);
+    return x;
+}
+__device__ __forceinline__ void store8(void *p, int64_t i, const float (&x)[8], int type) {
+    if (type == kTypeF32) {
+        rw_float4 *dst = reinterpret_cast<rw_float4 *>(static_cast<float *>(p) + i);
+        dst[0] = rw_float4{x[0], x[1], x[2], x[3]};
+        dst[1] = rw_float4{x[4], x[5], x[6], x[7]};
+        return;
+    }
+    uint32_t u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        u[j] = type == kTypeF16 ? f32_to_f16_bits(x[2 * j]) | ((uint32_t) f32_to_f16_bits(x[2 * j + 1]) << 16)
+                                : bf16_bits(x[2 * j]) | (bf16_bits(x[2 * j + 1]) << 16);
+    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + i) = make_uint4(u[0], u[1], u[2], u[3]);
+}
+
+// The scale of a block whose largest magnitude is amax: the least fp16 that is
+// not below amax / 127, so that no code passes 127.  NaN where that is none (a
+// NaN or an infinity in the block, magnitudes past 127 * 65504), with codes 0.
+struct Scale8 {
+    uint32_t bits;
+    float inv;  // 1 / scale, 0 for codes that are 0
+};
+__device__ __forceinline__ Scale8 scale_of(float amax) {
+    const float d = amax / 127.0f;
+    uint32_t h = f32_to_f16_bits(d);
+    if (f16_bits_to_f32(h) * 127.0f < amax) ++h;  // (18 bits, exact: also where the quotient was rounded, or is 0)
+    if (!(d <= 65504.0f)) return {0x7E00u, 0.0f};
+    return {h, h ? 1.0f / f16_bits_to_f32(h) : 0.0f};
+}
+// Four codes as bytes: the integers nearest to x * inv (codes of a block whose
+// scale is NaN are 0 whatever it holds).
+__device__ __forceinline__ uint32_t codes4(const float *x, float inv) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float q = inv != 0.0f ? __builtin_rintf(x[j] * inv) : 0.0f;
+        w |= ((uint32_t) (int) q & 0xFFu) << (8 * j);
+    }
+    return w;
+}
+__device__ __forceinline__ float max_abs8(const float (&x)[8]) {
+    float m = __builtin_fabsf(x[0]);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) m = __builtin_elementwise_maximum(m, __builtin_fabsf(x[j]));  // NaN if any is
+    return m;
+}
+// The largest of a quad's lanes.
+__device__ __forceinline__ float quad_max(float v) {
+    v = __builtin_elementwise_maximum(v, pg_dpp<0xB1>(v));
+    return __builtin_elementwise_maximum(v, pg_dpp<0x4E>(v));
+}
+
+}  // namespace bmo

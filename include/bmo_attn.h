@@ -17,10 +17,9 @@
  *   - Every call is asynchronous on its stream unless it says otherwise.  A
  *     call that writes slots (append, fused append+decode, write, reset,
  *     import) must be ordered with the calls that read those slots, as on one
- *     stream; decode calls alone may overlap.  Only bmo_kv_ring_create,
- *     bmo_attn_session_create and bmo_kv_ring_prefill (its staging buffer,
- *     when a staged call needs a larger one than the ring holds) allocate
- *     device memory.
+ *     stream; decode calls alone may overlap.  Only the _create calls and
+ *     bmo_kv_ring_prefill (its staging buffer, when a staged call needs a
+ *     larger one than the ring holds) allocate device memory.
  *   - Functions returning int return BMO_ATTN_OK (0) or an error code below;
  *     bmo_kv_ring_last_error() then describes the most recent failure on that
  *     ring (as bmo_last_error does per handle, src/bmo_api.h:145).
@@ -609,6 +608,124 @@ BMO_ATTN_API int bmo_kv_pages_attend_granted(bmo_kv_pages_t *pages, int layer, i
                                              int window, int max_rows, int max_len,
                                              void *workspace, int64_t workspace_bytes,
                                              void *stream);
+
+/* ---- rows between two attentions ------------------------------------------------ */
+/*
+ * What a transformer layer does to the rows of many sessions before and after
+ * the paged cache's attention: norm, projections, rotary positions, gated
+ * feed-forward (for one session the reference has rmsnorm_kernel,
+ * residual_add_kernel, rope_interleaved_kernel and swiglu_split_kernel,
+ * src/bmo_cuda_kernels.cu:244-387).  Inference only: the weights are 4-bit
+ * codes, there is no backward pass.
+ *
+ * Rows are F32, F16 or BF16, `stride` elements apart (0: dense), aligned to
+ * their elements; 16-byte aligned rows of a multiple of 8 elements are
+ * fastest.
+ *
+ * 8-bit rows are what the products take: int8 codes [rows][cols], 16-byte
+ * aligned, and fp16 scales [rows][cols / 32], both dense.  A block of 32
+ * elements has d = the least fp16 that is not below its largest magnitude /
+ * 127, and codes q = the integer nearest to x / d (x / d within fp32's
+ * rounding), so that no code passes 127; its elements stand for q * d.  A
+ * block of zeros has d = 0.  One that holds a NaN, an infinity or a magnitude
+ * past 127 * 65504 has d = NaN: what is computed from it is NaN.
+ *
+ * Calls allocate nothing and can be captured.  Calls without a handle run on
+ * the current device.
+ */
+
+/* Message of this thread's last failed call of bmo_rms_norm or
+ * bmo_quantize_rows; NULL if the last one succeeded. */
+BMO_ATTN_API const char *bmo_rows_last_error(void);
+
+/* RMS norm of rows x [n_rows][dim], dim at most 32768:
+ *   h = residual + x, stored in the residual rounded to its type (residual
+ *       NULL: h = x; the norm is that of the stored values)
+ *   y = h / sqrt(mean(h^2) + eps) * weight
+ * y goes to out, to 8-bit rows (dim a multiple of 32), or to both; what is
+ * NULL is not written.  out may be x with the same type and stride.  fp32
+ * inside; the squares of a row have to sum below fp32's range. */
+BMO_ATTN_API int bmo_rms_norm(int n_rows, int dim, int type, const void *x, int64_t x_stride,
+                              int residual_type, void *residual, int64_t residual_stride,
+                              int weight_type, const void *weight, float eps, int out_type,
+                              void *out, int64_t out_stride, void *codes, void *scales,
+                              void *stream);
+
+/* Rows x [n_rows][cols] as 8-bit rows (cols a multiple of 32). */
+BMO_ATTN_API int bmo_quantize_rows(int n_rows, int cols, int type, const void *x, int64_t stride,
+                                   void *codes, void *scales, void *stream);
+
+/* Rotary positions: pair i of the first rot_dim elements of a head, elements
+ * (2i, 2i + 1) if interleaved, else (i, i + rot_dim / 2), turns by position *
+ * rate_i and is multiplied by `magnitude`; elements from rot_dim on stay.
+ *   rate_i = theta^(-2i / rot_dim) / factor, or with a trained length (> 0)
+ *            YaRN's blend: as it is for pairs that turn more than beta_fast
+ *            times over that length, divided by factor for those that turn
+ *            less than beta_slow times, linear in i between;
+ *            divided by divisors[i] (host, [rot_dim / 2]; NULL: 1)
+ * beta_fast, beta_slow <= 0: 32, 1.  magnitude <= 0: 0.1 ln(factor) + 1 with a
+ * trained length and a factor above 1, else 1.  theta > 1; no rate may pass 1.
+ * The rates are kept on the device current at create.  NULL on failure
+ * (bmo_rope_last_error(NULL) has the calling thread's reason). */
+typedef struct bmo_rope bmo_rope_t;
+BMO_ATTN_API bmo_rope_t *bmo_rope_create(int head_dim, int rot_dim, int interleaved, double theta,
+                                         double factor, int trained, double beta_fast,
+                                         double beta_slow, double magnitude,
+                                         const double *divisors);
+/* NULL-safe. */
+BMO_ATTN_API void bmo_rope_free(bmo_rope_t *rope);
+BMO_ATTN_API int bmo_rope_device(const bmo_rope_t *rope);
+BMO_ATTN_API const char *bmo_rope_last_error(const bmo_rope_t *rope);
+
+/* Turns rows q [n_tok][n_heads][head_dim] and k [n_tok][n_kv_heads][head_dim]
+ * (n_kv_heads 0: none) by positions [n_tok] (device, any int: a plan's
+ * tok_pos) into q_out and k_out, which may be q and k with their strides but
+ * must not overlap them otherwise.  Cosines and sines are the exact ones
+ * rounded to fp32, each product and sum is rounded to fp32, the result to the
+ * type. */
+BMO_ATTN_API int bmo_rope_apply(bmo_rope_t *rope, int n_tok, const int *positions, int type,
+                                int n_heads, const void *q, int64_t q_stride, void *q_out,
+                                int64_t q_out_stride, int n_kv_heads, const void *k,
+                                int64_t k_stride, void *k_out, int64_t k_out_stride,
+                                void *stream);
+
+/* A Q4_0 weight matrix [rows][cols] (cols a multiple of 32) on the current
+ * device, laid out for the matrix cores; zeros at first.  NULL on failure
+ * (bmo_weights_last_error(NULL) has the calling thread's reason). */
+typedef struct bmo_weights bmo_weights_t;
+BMO_ATTN_API bmo_weights_t *bmo_weights_create(int rows, int cols);
+/* NULL-safe. */
+BMO_ATTN_API void bmo_weights_free(bmo_weights_t *weights);
+BMO_ATTN_API int64_t bmo_weights_bytes(const bmo_weights_t *weights);
+BMO_ATTN_API int bmo_weights_device(const bmo_weights_t *weights);
+BMO_ATTN_API const char *bmo_weights_last_error(const bmo_weights_t *weights);
+
+/* Rows row .. row + n_rows - 1 of the matrix from ggml blocks [n_rows]
+ * [cols / 32] of 18 bytes (device).  Must be ordered with the products. */
+BMO_ATTN_API int bmo_weights_load(bmo_weights_t *weights, int row, int n_rows, const void *blocks,
+                                  void *stream);
+
+/* out [n_rows][rows] = 8-bit rows [n_rows][cols] times the matrix:
+ *   out[m][n] = sum over blocks of d4 * d8 * sum((code - 8) * q),
+ * a block's sum an exact integer, blocks added in fp32; the order, and with it
+ * the rounding, depends on the sizes alone.  n_rows at most 2^20. */
+BMO_ATTN_API int bmo_weights_product(bmo_weights_t *weights, int n_rows, const void *codes,
+                                     const void *scales, int type, void *out, int64_t out_stride,
+                                     void *stream);
+
+/* Activations of a gated feed-forward. */
+#define BMO_ATTN_SILU 1
+#define BMO_ATTN_GELU 2 /* by its tanh form */
+
+/* The first half of a gated feed-forward: with G the first half of the
+ * matrix's rows and U the second (rows a multiple of 64),
+ *   h = act(G x) * (U x), [n_rows][rows / 2],
+ * in one launch, into out, into 8-bit rows for the projection down, or both;
+ * what is NULL is not written. */
+BMO_ATTN_API int bmo_weights_gated(bmo_weights_t *weights, int n_rows, const void *codes,
+                                   const void *scales, int activation, int type, void *out,
+                                   int64_t out_stride, void *out_codes, void *out_scales,
+                                   void *stream);
 
 /* ---- node-level drop-in ------------------------------------------------------ */
 
