@@ -19,6 +19,8 @@ namespace bmo {
 namespace {
 
 typedef int wt_int4 __attribute__((ext_vector_type(4)));
+typedef int wt_int16 __attribute__((ext_vector_type(16)));
+typedef float wt_float16 __attribute__((ext_vector_type(16)));
 
 constexpr int kMagicBits = 0x4B400000;       // 1.5 * 2^23
 constexpr float kMagic = 12582912.0f;
@@ -193,9 +195,226 @@ hipError_t run_few(const ProductParams &p, hipStream_t stream) {
                            dim3(64 * KW), args, 0, stream);
 }
 
+// Many rows: a wave takes 64 rows and two tiles of 32 outputs (of a gated
+// product one of gates and the one that they let through), a workgroup's waves
+// WM x WN such pieces, or KW waves share one and take every KW-th unit of it.
+constexpr int kManyThreads = 256;
+
+// Two units' codes of 16 rows each to a 32-row operand: lanes 16 to 31 and 48
+// to 63 of the first change places with lanes 0 to 15 and 32 to 47 of the
+// second.  (Wait states before the first: the compiler's hazard pass does not
+// see inside.)
+__device__ __forceinline__ void pair_rows(uint4 &a, uint4 &b) {
+    asm volatile(
+        "s_nop 3\n"
+        "v_permlane16_swap_b32 %0, %4\n"
+        "v_permlane16_swap_b32 %1, %5\n"
+        "v_permlane16_swap_b32 %2, %6\n"
+        "v_permlane16_swap_b32 %3, %7\n"
+        "s_nop 3"
+        : "+v"(a.x), "+v"(a.y), "+v"(a.z), "+v"(a.w), "+v"(b.x), "+v"(b.y), "+v"(b.z), "+v"(b.w));
+}
+
+__device__ __forceinline__ uint32_t dword(const uint4 &v, int t) { return t == 0 ? v.x : t == 1 ? v.y : t == 2 ? v.z : v.w; }
+
+template <int KW, bool GATED, bool EVEN>
+__global__ __launch_bounds__(kManyThreads, 2) void many_rows_kernel(ProductParams p, int n_pairs) {
+    constexpr int WN = KW == 4 ? 1 : 2, WM = 4 / KW / WN, MT = 2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kw = wave % KW, wn = wave / KW % WN, wm = wave / KW / WN;
+    const int m32 = lane & 31, h = lane >> 5;
+    const int m0 = ((int) blockIdx.y * WM + wm) * 32 * MT;
+    const int pair = (int) blockIdx.x * WN + wn;
+    const int nb = p.g.cols / 32;
+    // (tiles of 32 rows; a pair past the last reads the last and stores nothing)
+    auto unit = [&](int n, int u) {
+        const int tile = GATED ? pair + n * (p.g.tiles / 4) : 2 * pair + n;
+        return p.w + (int64_t) min(2 * tile + u, p.g.tiles - 1) * p.g.chunks * kUnitBytes;
+    };
+    const uint8_t *w[2][2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) w[n][u] = unit(n, u) + lane * 16;
+    // A lane carries the scales of four rows in one block: tile lane / 32, unit
+    // lane / 16 % 2, rows 4g .., g = lane / 4 % 4, block t = lane % 4.
+    const uint8_t *ws = unit(lane >> 5, (lane >> 4) & 1) + kUnitScales + (lane & 15) * 8;
+    __shared__ uint4 s_scale[4][2][4][2][2];  // [wave][tile][block][half][32 bytes]
+    uint2 *scale_to = reinterpret_cast<uint2 *>(s_scale[wave]) + (lane >> 5) * 32 + (lane & 3) * 8 + ((lane >> 2) & 1) * 4 +
+                      ((lane >> 4) & 1) * 2 + ((lane >> 3) & 1);
+    const int8_t *x[MT];
+    const uint16_t *d[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int row = min(m0 + 32 * m + m32, p.n_rows - 1);
+        x[m] = p.codes + (int64_t) row * p.g.cols + h * 16;
+        d[m] = p.scales + (int64_t) row * nb;
+    }
+    auto load_x = [&](int m, int c, int t) {  // (past the last block: weights are zeros)
+        return *reinterpret_cast<const wt_int4 *>(x[m] + min(4 * c + t, nb - 1) * 32);
+    };
+    auto load_d = [&](int m, int c) {
+        if constexpr (EVEN) return *reinterpret_cast<const uint2 *>(d[m] + 4 * c);
+        uint32_t v[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) v[t] = d[m][min(4 * c + t, nb - 1)];
+        return make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
+    };
+    wt_float16 acc[2][MT];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[n][m][i] = 0.0f;
+    wt_int16 magic;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) magic[i] = kMagicBits;
+    const int last = p.g.chunks - 1;
+    int c = min(kw, last);
+    uint4 q[2][2], q1[2][2];
+    uint2 sc, sc1, dd[MT], dd1[MT];
+    wt_int4 xv[4][MT];
+    auto load_chunk = [&](int at, uint4 (&qq)[2][2], uint2 &s, uint2 (&e)[MT]) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) qq[n][u] = *reinterpret_cast<const uint4 *>(w[n][u] + (int64_t) at * kUnitBytes);
+        s = *reinterpret_cast<const uint2 *>(ws + (int64_t) at * kUnitBytes);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) e[m] = load_d(m, at);
+    };
+    load_chunk(c, q, sc, dd);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) xv[t][m] = load_x(m, c, t);
+    for (int k = kw; k <= last; k += KW) {
+        const int next = min(k + KW, last);
+        load_chunk(next, q1, sc1, dd1);
+        *scale_to = sc;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) pair_rows(q[n][0], q[n][1]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            float d8[MT], off[MT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const uint32_t v = t < 2 ? dd[m].x : dd[m].y;
+                d8[m] = t & 1 ? half_hi(v) : half_lo(v);
+                off[m] = -kMagic * d8[m];
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const uint32_t a = dword(q[n][0], t), b = dword(q[n][1], t);
+                const wt_int4 av = {(int) (a << 4 & 0xF0F0F0F0u), (int) (a & 0xF0F0F0F0u), (int) (b << 4 & 0xF0F0F0F0u),
+                                    (int) (b & 0xF0F0F0F0u)};
+                const uint4 s0 = s_scale[wave][n][t][h][0], s1 = s_scale[wave][n][t][h][1];
+                const uint32_t sv[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const wt_float16 f = __builtin_bit_cast(
+                        wt_float16, __builtin_amdgcn_mfma_i32_32x32x32_i8(av, xv[t][m], magic, 0, 0, 0));
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float part = __builtin_fmaf(f[i], d8[m], off[m]);
+                        acc[n][m][i] = __builtin_fmaf(i & 1 ? half_hi(sv[i >> 1]) : half_lo(sv[i >> 1]), part, acc[n][m][i]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m) xv[t][m] = load_x(m, next, t);
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) q[n][u] = q1[n][u];
+        sc = sc1;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) dd[m] = dd1[m];
+    }
+    if constexpr (KW > 1) {
+        // the waves of a piece add up in the order of their units
+        __shared__ rw_float4 s_acc[4][4][64];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    s_acc[wave][j][lane] = rw_float4{acc[n][m][4 * j], acc[n][m][4 * j + 1], acc[n][m][4 * j + 2],
+                                                     acc[n][m][4 * j + 3]};
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    rw_float4 v = s_acc[wave - kw][j][lane];
+#pragma unroll
+                    for (int k = 1; k < KW; ++k) v += s_acc[wave - kw + k][j][lane];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[n][m][4 * j + r] = v[r];
+                }
+            }
+    }
+    if (pair >= n_pairs) return;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        if (KW > 1 && m % KW != kw) continue;  // each stores a part
+        const int64_t row = m0 + 32 * m + m32;
+        if constexpr (GATED) {
+            const int n_out = p.g.rows / 2, n0 = pair * 32 + 4 * h;
+            float v[16], amax = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                v[i] = gate(acc[0][m][i] * kCodeStep, acc[1][m][i] * kCodeStep, p.activation);
+                amax = __builtin_elementwise_maximum(amax, __builtin_fabsf(v[i]));
+            }
+            if (p.out && row < p.n_rows) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    store_quad(p, row, n0 + 8 * j, n_out, rw_float4{v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]});
+            }
+            if (p.out_codes) {
+                const Scale8 s = scale_of(__builtin_elementwise_maximum(amax, __shfl_xor(amax, 32)));
+                if (row < p.n_rows) {
+                    uint32_t *dst = reinterpret_cast<uint32_t *>(p.out_codes + row * n_out + n0);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) dst[2 * j] = codes4(v + 4 * j, s.inv);
+                    if (h == 0) p.out_scales[row * (n_out / 32) + pair] = (uint16_t) s.bits;
+                }
+            }
+        } else if (row < p.n_rows) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    store_quad(p, row, (2 * pair + n) * 32 + 8 * j + 4 * h, p.g.rows,
+                               rw_float4{acc[n][m][4 * j], acc[n][m][4 * j + 1], acc[n][m][4 * j + 2], acc[n][m][4 * j + 3]} *
+                                   kCodeStep);
+        }
+    }
+}
+
+template <int KW, bool GATED>
+hipError_t run_many(const ProductParams &p, hipStream_t stream) {
+    constexpr int WN = KW == 4 ? 1 : 2, WM = 4 / KW / WN;
+    ProductParams q = p;
+    int pairs = GATED ? p.g.rows / 64 : (p.g.rows + 63) / 64;
+    void *args[] = {&q, &pairs};
+    const bool even = p.g.cols % 128 == 0 && reinterpret_cast<uintptr_t>(p.scales) % 8 == 0;
+    return hipLaunchKernel(even ? reinterpret_cast<const void *>(many_rows_kernel<KW, GATED, true>)
+                                : reinterpret_cast<const void *>(many_rows_kernel<KW, GATED, false>),
+                           dim3((unsigned) ((pairs + WN - 1) / WN), (unsigned) ((p.n_rows + 64 * WM - 1) / (64 * WM))),
+                           dim3(kManyThreads), args, 0, stream);
+}
+
 }  // namespace
 
 hipError_t launch_product(const ProductParams &p, hipStream_t stream) {
+    if (p.n_rows > 64) {
+        if (p.activation) return run_many<1, true>(p, stream);
+        return run_many<1, false>(p, stream);
+    }
     if (p.activation) return p.n_rows <= 16 ? run_few<1, 4, 8, true>(p, stream) : run_few<2, 4, 4, true>(p, stream);
     return p.n_rows <= 16 ? run_few<1, 1, 8, false>(p, stream) : run_few<4, 2, 4, false>(p, stream);
 }
