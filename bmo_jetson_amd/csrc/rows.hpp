@@ -78,13 +78,11 @@ hipError_t launch_rope(const RopeParams &p, hipStream_t stream);
 //   [0, 1024)     codes: dword ((g * 16 + i) * 4 + t) holds elements 8g .. 8g+7
 //                 of block t of row i, each code - 8 as a signed nibble, byte j
 //                 element 8g + j (low) and 8g + 4 + j (high)
-//   [1024, 1152)  scales, fp16: element (g * 4 + t) * 4 + r is that of block t
-//                 of row 4g + r
+//   [1024, 1152)  scales, fp16: element i * 4 + t is that of block t of row i
 //
 // The 16 bytes at lane * 16 are what lane (g, i) of a 16x16x32 integer matrix
-// instruction takes of four blocks (the high nibbles of a dword in place and
-// the low ones shifted are 16 (code - 8) as bytes), and the 32 bytes of scales
-// at 1024 + 32 g belong to the four rows of its results.
+// instruction takes of four blocks: the high nibbles of a dword in place and
+// the low ones shifted are 16 (code - 8) as bytes.
 constexpr int kUnitRows = 16, kUnitCols = 128, kUnitBytes = 1152, kUnitScales = 1024;
 
 struct WeightsGeom {

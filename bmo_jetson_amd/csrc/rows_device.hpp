@@ -76,15 +76,13 @@ __device__ __forceinline__ Scale8 scale_of(float amax) {
     if (!(d <= 65504.0f)) return {0x7E00u, 0.0f};
     return {h, h ? 1.0f / f16_bits_to_f32(h) : 0.0f};
 }
-// Four codes as bytes: the integers nearest to x * inv (codes of a block whose
-// scale is NaN are 0 whatever it holds).
+// The integer nearest to x * inv (codes of a block whose scale is NaN are 0
+// whatever it holds), and four as bytes.
+__device__ __forceinline__ int code1(float x, float inv) { return inv != 0.0f ? (int) __builtin_rintf(x * inv) : 0; }
 __device__ __forceinline__ uint32_t codes4(const float *x, float inv) {
     uint32_t w = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float q = inv != 0.0f ? __builtin_rintf(x[j] * inv) : 0.0f;
-        w |= ((uint32_t) (int) q & 0xFFu) << (8 * j);
-    }
+    for (int j = 0; j < 4; ++j) w |= ((uint32_t) code1(x[j], inv) & 0xFFu) << (8 * j);
     return w;
 }
 __device__ __forceinline__ float max_abs8(const float (&x)[8]) {
@@ -97,6 +95,13 @@ __device__ __forceinline__ float max_abs8(const float (&x)[8]) {
 __device__ __forceinline__ float quad_max(float v) {
     v = __builtin_elementwise_maximum(v, pg_dpp<0xB1>(v));
     return __builtin_elementwise_maximum(v, pg_dpp<0x4E>(v));
+}
+
+// The largest of a row's 16 lanes.
+__device__ __forceinline__ float row16_max(float v) {
+    v = quad_max(v);
+    v = __builtin_elementwise_maximum(v, pg_dpp<0x124>(v));         // row_ror:4
+    return __builtin_elementwise_maximum(v, pg_dpp<0x128>(v));      // row_ror:8
 }
 
 }  // namespace bmo

@@ -19,6 +19,8 @@ namespace bmo {
 namespace {
 
 typedef int wt_int4 __attribute__((ext_vector_type(4)));
+typedef uint32_t wt_uint2 __attribute__((ext_vector_type(2)));
+typedef uint32_t wt_uint4 __attribute__((ext_vector_type(4)));
 typedef int wt_int16 __attribute__((ext_vector_type(16)));
 typedef float wt_float16 __attribute__((ext_vector_type(16)));
 
@@ -48,11 +50,13 @@ __global__ __launch_bounds__(256) void pack_kernel(PackParams p, FastDiv div_blo
         const uint32_t hi = (((qs[at + 2] | qs[at + 3] << 16) >> sh) & 0x0F0F0F0Fu);
         reinterpret_cast<uint32_t *>(unit)[(g * kUnitRows + ri) * 4 + t] = (lo | hi << 4) ^ 0x88888888u;
     }
-    reinterpret_cast<uint16_t *>(unit + kUnitScales)[((ri / 4) * 4 + t) * 4 + ri % 4] = src[0];
+    reinterpret_cast<uint16_t *>(unit + kUnitScales)[ri * 4 + t] = src[0];
 }
 
 __device__ __forceinline__ float half_lo(uint32_t u) { return f16_bits_to_f32(u & 0xFFFFu); }
 __device__ __forceinline__ float half_hi(uint32_t u) { return f16_bits_to_f32(u >> 16); }
+
+__device__ __forceinline__ uint32_t dword(const uint4 &v, int t) { return t == 0 ? v.x : t == 1 ? v.y : t == 2 ? v.z : v.w; }
 
 // The activation of a gate times what it lets through.
 __device__ __forceinline__ float gate(float g, float u, int activation) {
@@ -69,16 +73,22 @@ __device__ __forceinline__ void store_quad(const ProductParams &p, int64_t m, in
         if (n + j < n_out) store1(p.out, at + j, v[j], p.type);
 }
 
-// Few rows: a workgroup takes 16 * MT rows and NT tiles of 16 outputs, its KW
-// waves every KW-th unit of the tiles; their sums are joined in LDS, wave after
-// wave.
-template <int MT, int NT, int KW, bool GATED>
+constexpr int kRowStride = 144;  // of 128 codes in LDS: 16 rows' octets lie in different banks
+
+// Few rows: a workgroup takes 16 * MT rows and NT tiles of 16 outputs (of a
+// gated product two tiles of gates and the two that they let through), its KW
+// waves a run of the tiles' units each; their sums are joined in LDS, wave after
+// wave.  The 8-bit rows are the rows of the result here: a lane has one output
+// of four rows, with the output's scales its own and the rows' read from LDS,
+// where the wave puts them.  PF units are under way at once.
+template <int MT, int NT, int KW, int PF, bool GATED>
 __global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p) {
     static_assert(!GATED || NT == 4, "two tiles of gates and the two that they let through");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i16 = lane & 15, g = lane >> 4;
     const int m0 = blockIdx.y * 16 * MT;
-    const int nb = p.g.cols / 32;
+    const int nb = p.g.cols / 32, last = p.g.chunks - 1;
+    const int per = (p.g.chunks + KW - 1) / KW, c0 = wave * per, c1 = min(c0 + per, p.g.chunks);
     const uint8_t *w[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -86,55 +96,91 @@ __global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p) {
         tile = min(tile, p.g.tiles - 1);
         w[n] = p.w + (int64_t) tile * p.g.chunks * kUnitBytes;
     }
-    const int8_t *x[MT];
-    const uint16_t *d[MT];
+    // The rows' offsets from the workgroup's first fit 32 bits: 63 * 2^24.  (A
+    // unit's 128 codes of a row are read by eight lanes, and go through LDS to
+    // the lanes that multiply them.)
+    const int8_t *codes = p.codes + (int64_t) m0 * p.g.cols;
+    const uint16_t *scales = p.scales + (int64_t) m0 * nb;
+    uint32_t x_at[MT][2], d_at[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-        const int row = min(m0 + 16 * m + i16, p.n_rows - 1);
-        x[m] = p.codes + (int64_t) row * p.g.cols;
-        d[m] = p.scales + (int64_t) row * nb;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            x_at[m][i] = (uint32_t) min(16 * m + 8 * i + (lane >> 3), p.n_rows - 1 - m0) * (uint32_t) p.g.cols;
+        d_at[m] = (uint32_t) min(16 * m + i16, p.n_rows - 1 - m0) * (uint32_t) nb;
     }
+    wt_uint4 q[PF][NT], x[PF][MT][2];
+    wt_uint2 d4[PF][NT];
+    uint32_t d8[PF][MT];
+    auto load = [&](int j, int c) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const uint8_t *u = w[n] + (uint32_t) c * (uint32_t) kUnitBytes;
+            q[j][n] = __builtin_nontemporal_load(reinterpret_cast<const wt_uint4 *>(u + lane * 16));
+            d4[j][n] = *reinterpret_cast<const wt_uint2 *>(u + kUnitScales + i16 * 8);
+        }
+        // (past the last block weights are zeros)
+        const uint32_t e = (uint32_t) min(c * kUnitCols + (lane & 7) * 16, p.g.cols - 16), b = (uint32_t) min(4 * c + g, nb - 1);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) x[j][m][i] = *reinterpret_cast<const wt_uint4 *>(codes + (x_at[m][i] + e));
+            d8[j][m] = scales[d_at[m] + b];
+        }
+    };
+    __shared__ rw_float4 s_acc[KW][MT][NT][64];
+    __shared__ float s_d8[KW][MT][4][16];
+    __shared__ uint8_t s_x[KW][MT][16][kRowStride];
     rw_float4 acc[MT][NT];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[m][n] = rw_float4{0, 0, 0, 0};
     const wt_int4 magic = {kMagicBits, kMagicBits, kMagicBits, kMagicBits};
-    for (int c = wave; c < p.g.chunks; c += KW) {
-        uint4 q[NT], s0[NT], s1[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const uint8_t *u = w[n] + (int64_t) c * kUnitBytes;
-            q[n] = *reinterpret_cast<const uint4 *>(u + lane * 16);
-            s0[n] = *reinterpret_cast<const uint4 *>(u + kUnitScales + g * 32);
-            s1[n] = *reinterpret_cast<const uint4 *>(u + kUnitScales + g * 32 + 16);
-        }
+    for (int j = 0; j < PF; ++j) load(j, min(c0 + j, last));
+    for (int c = c0; c < c1; c += PF) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int b = min(4 * c + t, nb - 1);  // (past the last: weights are zeros)
+        for (int j = 0; j < PF; ++j) {
+            if (c + j >= c1) break;
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                const long xa = *reinterpret_cast<const long *>(x[m] + b * 32 + g * 8);
-                const float d8 = f16_bits_to_f32(d[m][b]), off = -kMagic * d8;
+                s_d8[wave][m][g][i16] = half_lo(d8[j][m]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    *reinterpret_cast<wt_uint4 *>(&s_x[wave][m][8 * i + (lane >> 3)][(lane & 7) * 16]) = x[j][m][i];
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                long wv[NT];
+                float ds[NT], off[NT];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const uint32_t v = (&q[n].x)[t];
-                    const uint2 wv = make_uint2(v << 4 & 0xF0F0F0F0u, v & 0xF0F0F0F0u);
-                    const wt_int4 z =
-                        __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, wv), xa, magic, 0, 0, 0);
-                    const rw_float4 f = __builtin_bit_cast(rw_float4, z);
-                    const uint32_t sc[2] = {(&(t < 2 ? s0[n] : s1[n]).x)[2 * (t & 1)],
-                                            (&(t < 2 ? s0[n] : s1[n]).x)[2 * (t & 1) + 1]};
+                    const uint32_t v = q[j][n][t], s = d4[j][n][t >> 1];
+                    wv[n] = __builtin_bit_cast(long, wt_uint2{v << 4 & 0xF0F0F0F0u, v & 0xF0F0F0F0u});
+                    ds[n] = t & 1 ? half_hi(s) : half_lo(s);
+                    asm volatile("" : "+v"(ds[n]));  // (in fp32: an fma that widens an operand takes twice the time)
+                    off[n] = -kMagic * ds[n];
+                }
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float part = __builtin_fmaf(f[r], d8, off);
-                        acc[m][n][r] = __builtin_fmaf(r & 1 ? half_hi(sc[r >> 1]) : half_lo(sc[r >> 1]), part, acc[m][n][r]);
+                for (int m = 0; m < MT; ++m) {
+                    const rw_float4 dr = *reinterpret_cast<const rw_float4 *>(&s_d8[wave][m][t][4 * g]);
+                    const long xv = *reinterpret_cast<const long *>(&s_x[wave][m][i16][t * 32 + g * 8]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const rw_float4 f = __builtin_bit_cast(
+                            rw_float4, __builtin_amdgcn_mfma_i32_16x16x32_i8(xv, wv[n], magic, 0, 0, 0));
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float part = __builtin_fmaf(f[r], ds[n], off[n]);
+                            acc[m][n][r] = __builtin_fmaf(dr[r], part, acc[m][n][r]);
+                        }
                     }
                 }
             }
+            if (c + j + PF < c1) load(j, c + j + PF);
         }
     }
-    __shared__ rw_float4 s_acc[KW][MT][NT][64];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -142,127 +188,152 @@ __global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p) {
     __syncthreads();
     auto joined = [&](int m, int n) {
         rw_float4 v = s_acc[0][m][n][lane];
+#pragma unroll
         for (int k = 1; k < KW; ++k) v += s_acc[k][m][n][lane];
         return v * kCodeStep;
     };
     if constexpr (GATED) {
-        const int n_out = p.g.rows / 2;
+        const int n_out = p.g.rows / 2, n0 = (int) blockIdx.x * 32 + i16;
         for (int m = wave; m < MT; m += KW) {
-            const int64_t row = m0 + 16 * m + i16;
-            float h[8];
+            const int64_t row0 = m0 + 16 * m + 4 * g;
+            float h[2][4];
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const rw_float4 a = joined(m, n), b = joined(m, n + 2);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) h[4 * n + r] = gate(a[r], b[r], p.activation);
+                for (int r = 0; r < 4; ++r) h[n][r] = gate(a[r], b[r], p.activation);
             }
-            const int n0 = (int) blockIdx.x * 32 + 4 * g;
-            if (p.out && row < p.n_rows) {
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
-                    store_quad(p, row, n0 + 16 * n, n_out, rw_float4{h[4 * n], h[4 * n + 1], h[4 * n + 2], h[4 * n + 3]});
-            }
-            if (p.out_codes) {
-                float amax = max_abs8(h);
-                amax = __builtin_elementwise_maximum(amax, __shfl_xor(amax, 16));
-                amax = __builtin_elementwise_maximum(amax, __shfl_xor(amax, 32));
-                const Scale8 s = scale_of(amax);
-                if (row < p.n_rows) {
-                    uint32_t *dst = reinterpret_cast<uint32_t *>(p.out_codes + row * n_out + n0);
-                    dst[0] = codes4(h, s.inv);
-                    dst[4] = codes4(h + 4, s.inv);
-                    if (g == 0) p.out_scales[row * (n_out / 32) + blockIdx.x] = (uint16_t) s.bits;
+            for (int r = 0; r < 4; ++r) {
+                const int64_t row = row0 + r;
+                if (p.out && row < p.n_rows) {
+                    store1(p.out, row * p.out_stride + n0, h[0][r], p.type);
+                    store1(p.out, row * p.out_stride + n0 + 16, h[1][r], p.type);
+                }
+                if (p.out_codes) {
+                    const Scale8 s =
+                        scale_of(row16_max(__builtin_elementwise_maximum(__builtin_fabsf(h[0][r]), __builtin_fabsf(h[1][r]))));
+                    if (row < p.n_rows) {
+                        p.out_codes[row * n_out + n0] = (int8_t) code1(h[0][r], s.inv);
+                        p.out_codes[row * n_out + n0 + 16] = (int8_t) code1(h[1][r], s.inv);
+                        if (i16 == 0) p.out_scales[row * (n_out / 32) + blockIdx.x] = (uint16_t) s.bits;
+                    }
                 }
             }
         }
     } else {
         for (int i = wave; i < MT * NT; i += KW) {
-            const int m = i / NT, n = i % NT;
-            const int64_t row = m0 + 16 * m + i16;
+            const int m = i / NT, n = i % NT, col = ((int) blockIdx.x * NT + n) * 16 + i16;
+            const int64_t row0 = m0 + 16 * m + 4 * g;
             const rw_float4 v = joined(m, n);
-            if (row < p.n_rows) store_quad(p, row, ((int) blockIdx.x * NT + n) * 16 + 4 * g, p.g.rows, v);
+            if (col < p.g.rows) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (row0 + r < p.n_rows) store1(p.out, (row0 + r) * p.out_stride + col, v[r], p.type);
+            }
         }
     }
 }
 
-template <int MT, int NT, int KW, bool GATED>
+template <int MT, int NT, int KW, int PF, bool GATED>
 hipError_t run_few(const ProductParams &p, hipStream_t stream) {
     ProductParams q = p;
     void *args[] = {&q};
     const int per = GATED ? 2 : NT, tiles = GATED ? p.g.tiles / 2 : p.g.tiles;
-    return hipLaunchKernel(reinterpret_cast<const void *>(few_rows_kernel<MT, NT, KW, GATED>),
+    return hipLaunchKernel(reinterpret_cast<const void *>(few_rows_kernel<MT, NT, KW, PF, GATED>),
                            dim3((unsigned) ((tiles + per - 1) / per), (unsigned) ((p.n_rows + 16 * MT - 1) / (16 * MT))),
                            dim3(64 * KW), args, 0, stream);
 }
 
-// Many rows: a wave takes 64 rows and two tiles of 32 outputs (of a gated
-// product one of gates and the one that they let through), a workgroup's waves
-// WM x WN such pieces, or KW waves share one and take every KW-th unit of it.
-constexpr int kManyThreads = 256;
+// Many rows: a wave takes MT * 32 rows and NT tiles of 32 outputs (of a gated
+// product one of gates and the one that they let through), a workgroup WM * WN
+// such pieces, each shared by KW waves, which take every KW-th unit of it and
+// join their sums in LDS.  The outputs are the rows of the results here: a lane
+// has 16 outputs of one row, its scale is the lane's own and the outputs' are
+// read from LDS, where the wave puts them.  The rows' codes go through LDS too,
+// a unit ahead: eight lanes read a row's 128, which costs the loads a quarter of
+// what reading them as the matrix cores take them does.
 
 // Two units' codes of 16 rows each to a 32-row operand: lanes 16 to 31 and 48
 // to 63 of the first change places with lanes 0 to 15 and 32 to 47 of the
-// second.  (Wait states before the first: the compiler's hazard pass does not
-// see inside.)
-__device__ __forceinline__ void pair_rows(uint4 &a, uint4 &b) {
+// second.  (Wait states: the compiler's hazard pass does not see inside.)
+__device__ __forceinline__ void pair_rows(wt_uint4 &a, wt_uint4 &b) {
+    uint32_t a0 = a[0], a1 = a[1], a2 = a[2], a3 = a[3], b0 = b[0], b1 = b[1], b2 = b[2], b3 = b[3];
     asm volatile(
-        "s_nop 3\n"
-        "v_permlane16_swap_b32 %0, %4\n"
-        "v_permlane16_swap_b32 %1, %5\n"
-        "v_permlane16_swap_b32 %2, %6\n"
-        "v_permlane16_swap_b32 %3, %7\n"
+        "s_nop 3\n\t"
+        "v_permlane16_swap_b32 %0, %4\n\t"
+        "v_permlane16_swap_b32 %1, %5\n\t"
+        "v_permlane16_swap_b32 %2, %6\n\t"
+        "v_permlane16_swap_b32 %3, %7\n\t"
         "s_nop 3"
-        : "+v"(a.x), "+v"(a.y), "+v"(a.z), "+v"(a.w), "+v"(b.x), "+v"(b.y), "+v"(b.z), "+v"(b.w));
+        : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3), "+v"(b0), "+v"(b1), "+v"(b2), "+v"(b3));
+    a = wt_uint4{a0, a1, a2, a3};
+    b = wt_uint4{b0, b1, b2, b3};
 }
 
-__device__ __forceinline__ uint32_t dword(const uint4 &v, int t) { return t == 0 ? v.x : t == 1 ? v.y : t == 2 ? v.z : v.w; }
+// A barrier that waits for LDS alone, not for loads under way.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <int KW, bool GATED, bool EVEN>
-__global__ __launch_bounds__(kManyThreads, 2) void many_rows_kernel(ProductParams p, int n_pairs) {
-    constexpr int WN = KW == 4 ? 1 : 2, WM = 4 / KW / WN, MT = 2;
+template <int MT, int NT, int WM, int WN, int KW, bool GATED, bool EVEN>
+__global__ __launch_bounds__(64 * WM * WN * KW, 2) void many_rows_kernel(ProductParams p, int n_pieces) {
+    static_assert(!GATED || NT == 2, "a tile of gates and the one that they let through");
+    constexpr int WAVES = WM * WN * KW, ROWS = 32 * MT * WM, XL = 4 * MT / WN;  // rows of a workgroup; loads of a lane
+    constexpr bool ALONE = WM * WN == 1;  // a wave reads only the codes that it puts into LDS itself
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kw = wave % KW, wn = wave / KW % WN, wm = wave / KW / WN;
     const int m32 = lane & 31, h = lane >> 5;
     const int m0 = ((int) blockIdx.y * WM + wm) * 32 * MT;
-    const int pair = (int) blockIdx.x * WN + wn;
-    const int nb = p.g.cols / 32;
-    // (tiles of 32 rows; a pair past the last reads the last and stores nothing)
+    const int piece = (int) blockIdx.x * WN + wn;
+    const int nb = p.g.cols / 32, last = p.g.chunks - 1;
+    // (tiles of 32 outputs; a piece past the last reads the last and stores nothing)
     auto unit = [&](int n, int u) {
-        const int tile = GATED ? pair + n * (p.g.tiles / 4) : 2 * pair + n;
+        const int tile = GATED ? piece + n * (p.g.tiles / 4) : NT * piece + n;
         return p.w + (int64_t) min(2 * tile + u, p.g.tiles - 1) * p.g.chunks * kUnitBytes;
     };
-    const uint8_t *w[2][2];
+    const uint8_t *w[NT][2];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) w[n][u] = unit(n, u) + lane * 16;
-    // A lane carries the scales of four rows in one block: tile lane / 32, unit
-    // lane / 16 % 2, rows 4g .., g = lane / 4 % 4, block t = lane % 4.
-    const uint8_t *ws = unit(lane >> 5, (lane >> 4) & 1) + kUnitScales + (lane & 15) * 8;
-    __shared__ uint4 s_scale[4][2][4][2][2];  // [wave][tile][block][half][32 bytes]
-    uint2 *scale_to = reinterpret_cast<uint2 *>(s_scale[wave]) + (lane >> 5) * 32 + (lane & 3) * 8 + ((lane >> 2) & 1) * 4 +
-                      ((lane >> 4) & 1) * 2 + ((lane >> 3) & 1);
-    const int8_t *x[MT];
-    const uint16_t *d[MT];
+        for (int u = 0; u < 2; ++u) w[n][u] = unit(n, u);
+    // A lane carries the scales of row lane % 32 of tile lane / 32 to where the
+    // lanes of the row's half take them: results 4j + i are rows 8j + 4h + i.
+    const uint8_t *ws = unit(NT == 2 ? lane >> 5 : 0, (lane >> 4) & 1) + kUnitScales + (lane & 15) * 8;
+    __shared__ rw_float4 s_scale[WAVES][2][4][2][4];  // [tile][block][half][16 rows]
+    float *scale_to = reinterpret_cast<float *>(s_scale[wave][lane >> 5]) + ((lane >> 2) & 1) * 16 + ((lane >> 3) & 3) * 4 +
+                      (lane & 3);
+    // (the rows' offsets from the workgroup's first fit 32 bits: 127 * 2^24)
+    const int first = (int) blockIdx.y * ROWS;
+    const int8_t *codes = p.codes + (int64_t) first * p.g.cols;
+    const uint16_t *scales = p.scales + (int64_t) first * nb;
+    uint32_t d_at[MT], x_at[XL];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int row = min(m0 + 32 * m + m32, p.n_rows - 1);
-        x[m] = p.codes + (int64_t) row * p.g.cols + h * 16;
-        d[m] = p.scales + (int64_t) row * nb;
-    }
-    auto load_x = [&](int m, int c, int t) {  // (past the last block: weights are zeros)
-        return *reinterpret_cast<const wt_int4 *>(x[m] + min(4 * c + t, nb - 1) * 32);
+    for (int m = 0; m < MT; ++m) d_at[m] = (uint32_t) min(wm * 32 * MT + 32 * m + m32, p.n_rows - 1 - first) * (uint32_t) nb;
+    const int x_row = wave / KW * (8 * XL) + (lane >> 3), piece16 = lane & 7;
+#pragma unroll
+    for (int i = 0; i < XL; ++i) x_at[i] = (uint32_t) min(x_row + 8 * i, p.n_rows - 1 - first) * (uint32_t) p.g.cols;
+    // (a row's sixteens change places by the row, so that eight rows' lie in
+    // different banks)
+    __shared__ wt_int4 s_x[KW][ALONE ? 1 : 2][ROWS][8];
+    wt_int4 xr[XL];
+    auto load_x = [&](int c) {  // (past the last block weights are zeros)
+        const uint32_t e = (uint32_t) min(c * kUnitCols + piece16 * 16, p.g.cols - 16);
+#pragma unroll
+        for (int i = 0; i < XL; ++i) xr[i] = *reinterpret_cast<const wt_int4 *>(codes + (x_at[i] + e));
+    };
+    auto put_x = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < XL; ++i) s_x[kw][buffer][x_row + 8 * i][piece16 ^ (x_row & 7)] = xr[i];
     };
     auto load_d = [&](int m, int c) {
-        if constexpr (EVEN) return *reinterpret_cast<const uint2 *>(d[m] + 4 * c);
+        if constexpr (EVEN) return *reinterpret_cast<const wt_uint2 *>(scales + (d_at[m] + 4 * (uint32_t) c));
         uint32_t v[4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) v[t] = d[m][min(4 * c + t, nb - 1)];
-        return make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
+        for (int t = 0; t < 4; ++t) v[t] = scales[d_at[m] + (uint32_t) min(4 * c + t, nb - 1)];
+        return wt_uint2{v[0] | v[1] << 16, v[2] | v[3] << 16};
     };
-    wt_float16 acc[2][MT];
+    wt_float16 acc[NT][MT];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -270,63 +341,86 @@ __global__ __launch_bounds__(kManyThreads, 2) void many_rows_kernel(ProductParam
     wt_int16 magic;
 #pragma unroll
     for (int i = 0; i < 16; ++i) magic[i] = kMagicBits;
-    const int last = p.g.chunks - 1;
-    int c = min(kw, last);
-    uint4 q[2][2], q1[2][2];
-    uint2 sc, sc1, dd[MT], dd1[MT];
-    wt_int4 xv[4][MT];
-    auto load_chunk = [&](int at, uint4 (&qq)[2][2], uint2 &s, uint2 (&e)[MT]) {
+    asm volatile("" : "+v"(magic));  // (kept, not made again before each use)
+    wt_uint4 q[NT][2], q1[NT][2];
+    wt_uint2 sc, sc1, dd[MT], dd1[MT];
+    auto load_units = [&](int c, wt_uint4 (&qq)[NT][2], wt_uint2 &s, wt_uint2 (&e)[MT]) {
+        const uint32_t at = (uint32_t) c * (uint32_t) kUnitBytes;
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) qq[n][u] = *reinterpret_cast<const uint4 *>(w[n][u] + (int64_t) at * kUnitBytes);
-        s = *reinterpret_cast<const uint2 *>(ws + (int64_t) at * kUnitBytes);
+            for (int u = 0; u < 2; ++u) qq[n][u] = *reinterpret_cast<const wt_uint4 *>(w[n][u] + at + lane * 16);
+        s = *reinterpret_cast<const wt_uint2 *>(ws + at);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) e[m] = load_d(m, at);
+        for (int m = 0; m < MT; ++m) e[m] = load_d(m, c);
     };
-    load_chunk(c, q, sc, dd);
+    load_x(min(kw, last));
+    load_units(min(kw, last), q, sc, dd);
+    const int steps = (last + KW) / KW;
+    for (int step = 0; step < steps; ++step) {
+        const int next = min((step + 1) * KW + kw, last), at = ALONE ? 0 : step & 1;
+        if (ALONE && KW > 1 && step * KW + kw > last) break;
+        put_x(at);
+        if (!ALONE) lds_barrier();
+        load_x(next);
+        load_units(next, q1, sc1, dd1);
+        if (ALONE || KW == 1 || step * KW + kw <= last) {  // (else a unit that another wave has)
+            scale_to[0] = half_lo(sc[0]);
+            scale_to[32] = half_hi(sc[0]);
+            scale_to[64] = half_lo(sc[1]);
+            scale_to[96] = half_hi(sc[1]);
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+            for (int n = 0; n < NT; ++n) pair_rows(q[n][0], q[n][1]);
+            // What a block needs of LDS is read while the one before it is
+            // multiplied.
+            wt_int4 xv[2][MT];
+            rw_float4 d4[2][4];
+            auto read_x = [&](int t) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) xv[t][m] = load_x(m, c, t);
-    for (int k = kw; k <= last; k += KW) {
-        const int next = min(k + KW, last);
-        load_chunk(next, q1, sc1, dd1);
-        *scale_to = sc;
+                for (int m = 0; m < MT; ++m)
+                    xv[t & 1][m] = s_x[kw][at][wm * 32 * MT + 32 * m + m32][(2 * t + h) ^ (m32 & 7)];
+            };
+            auto read_d4 = [&](int e) {  // e: tile e % NT of block e / NT
 #pragma unroll
-        for (int n = 0; n < 2; ++n) pair_rows(q[n][0], q[n][1]);
+                for (int j = 0; j < 4; ++j) d4[e & 1][j] = s_scale[wave][e % NT][e / NT][h][j];
+            };
+            read_x(0);
+            read_d4(0);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            float d8[MT], off[MT];
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const uint32_t v = t < 2 ? dd[m].x : dd[m].y;
-                d8[m] = t & 1 ? half_hi(v) : half_lo(v);
-                off[m] = -kMagic * d8[m];
-            }
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const uint32_t a = dword(q[n][0], t), b = dword(q[n][1], t);
-                const wt_int4 av = {(int) (a << 4 & 0xF0F0F0F0u), (int) (a & 0xF0F0F0F0u), (int) (b << 4 & 0xF0F0F0F0u),
-                                    (int) (b & 0xF0F0F0F0u)};
-                const uint4 s0 = s_scale[wave][n][t][h][0], s1 = s_scale[wave][n][t][h][1];
-                const uint32_t sv[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+            for (int t = 0; t < 4; ++t) {
+                float d8[MT], off[MT];
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    const wt_float16 f = __builtin_bit_cast(
-                        wt_float16, __builtin_amdgcn_mfma_i32_32x32x32_i8(av, xv[t][m], magic, 0, 0, 0));
+                    d8[m] = t & 1 ? half_hi(dd[m][t >> 1]) : half_lo(dd[m][t >> 1]);
+                    asm volatile("" : "+v"(d8[m]));  // (in fp32: an fma that widens an operand takes twice the time)
+                    off[m] = -kMagic * d8[m];
+                }
+                if (t < 3) read_x(t + 1);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float part = __builtin_fmaf(f[i], d8[m], off[m]);
-                        acc[n][m][i] = __builtin_fmaf(i & 1 ? half_hi(sv[i >> 1]) : half_lo(sv[i >> 1]), part, acc[n][m][i]);
+                for (int n = 0; n < NT; ++n) {
+                    const int e = t * NT + n;
+                    const uint32_t a = q[n][0][t], b = q[n][1][t];
+                    const wt_int4 av = {(int) (a << 4 & 0xF0F0F0F0u), (int) (a & 0xF0F0F0F0u), (int) (b << 4 & 0xF0F0F0F0u),
+                                        (int) (b & 0xF0F0F0F0u)};
+                    wt_int16 z[MT];
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+                        z[m] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av, xv[t & 1][m], magic, 0, 0, 0);
+                    if (e + 1 < 4 * NT) read_d4(e + 1);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        const wt_float16 f = __builtin_bit_cast(wt_float16, z[m]);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            acc[n][m][r] =
+                                __builtin_fmaf(d4[e & 1][r >> 2][r & 3], __builtin_fmaf(f[r], d8[m], off[m]), acc[n][m][r]);
                     }
+
                 }
             }
-#pragma unroll
-            for (int m = 0; m < MT; ++m) xv[t][m] = load_x(m, next, t);
         }
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int u = 0; u < 2; ++u) q[n][u] = q1[n][u];
         sc = sc1;
@@ -335,9 +429,9 @@ __global__ __launch_bounds__(kManyThreads, 2) void many_rows_kernel(ProductParam
     }
     if constexpr (KW > 1) {
         // the waves of a piece add up in the order of their units
-        __shared__ rw_float4 s_acc[4][4][64];
+        __shared__ rw_float4 s_acc[WAVES][4][64];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 __syncthreads();
@@ -356,13 +450,13 @@ __global__ __launch_bounds__(kManyThreads, 2) void many_rows_kernel(ProductParam
                 }
             }
     }
-    if (pair >= n_pairs) return;
+    if (piece >= n_pieces) return;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         if (KW > 1 && m % KW != kw) continue;  // each stores a part
         const int64_t row = m0 + 32 * m + m32;
         if constexpr (GATED) {
-            const int n_out = p.g.rows / 2, n0 = pair * 32 + 4 * h;
+            const int n_out = p.g.rows / 2, n0 = piece * 32 + 4 * h;
             float v[16], amax = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -380,43 +474,42 @@ __global__ __launch_bounds__(kManyThreads, 2) void many_rows_kernel(ProductParam
                     uint32_t *dst = reinterpret_cast<uint32_t *>(p.out_codes + row * n_out + n0);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) dst[2 * j] = codes4(v + 4 * j, s.inv);
-                    if (h == 0) p.out_scales[row * (n_out / 32) + pair] = (uint16_t) s.bits;
+                    if (h == 0) p.out_scales[row * (n_out / 32) + piece] = (uint16_t) s.bits;
                 }
             }
         } else if (row < p.n_rows) {
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    store_quad(p, row, (2 * pair + n) * 32 + 8 * j + 4 * h, p.g.rows,
+                    store_quad(p, row, (NT * piece + n) * 32 + 8 * j + 4 * h, p.g.rows,
                                rw_float4{acc[n][m][4 * j], acc[n][m][4 * j + 1], acc[n][m][4 * j + 2], acc[n][m][4 * j + 3]} *
                                    kCodeStep);
         }
     }
 }
 
-template <int KW, bool GATED>
+template <int MT, int NT, int WM, int WN, int KW, bool GATED>
 hipError_t run_many(const ProductParams &p, hipStream_t stream) {
-    constexpr int WN = KW == 4 ? 1 : 2, WM = 4 / KW / WN;
     ProductParams q = p;
-    int pairs = GATED ? p.g.rows / 64 : (p.g.rows + 63) / 64;
-    void *args[] = {&q, &pairs};
+    int pieces = GATED ? p.g.rows / 64 : (p.g.rows + 32 * NT - 1) / (32 * NT);
+    void *args[] = {&q, &pieces};
     const bool even = p.g.cols % 128 == 0 && reinterpret_cast<uintptr_t>(p.scales) % 8 == 0;
-    return hipLaunchKernel(even ? reinterpret_cast<const void *>(many_rows_kernel<KW, GATED, true>)
-                                : reinterpret_cast<const void *>(many_rows_kernel<KW, GATED, false>),
-                           dim3((unsigned) ((pairs + WN - 1) / WN), (unsigned) ((p.n_rows + 64 * WM - 1) / (64 * WM))),
-                           dim3(kManyThreads), args, 0, stream);
+    return hipLaunchKernel(even ? reinterpret_cast<const void *>(many_rows_kernel<MT, NT, WM, WN, KW, GATED, true>)
+                                : reinterpret_cast<const void *>(many_rows_kernel<MT, NT, WM, WN, KW, GATED, false>),
+                           dim3((unsigned) ((pieces + WN - 1) / WN), (unsigned) ((p.n_rows + 32 * MT * WM - 1) / (32 * MT * WM))),
+                           dim3(64 * WM * WN * KW), args, 0, stream);
 }
 
 }  // namespace
 
 hipError_t launch_product(const ProductParams &p, hipStream_t stream) {
     if (p.n_rows > 64) {
-        if (p.activation) return run_many<1, true>(p, stream);
-        return run_many<1, false>(p, stream);
+        if (p.activation) return run_many<2, 2, 2, 2, 1, true>(p, stream);
+        return run_many<2, 2, 2, 2, 1, false>(p, stream);
     }
-    if (p.activation) return p.n_rows <= 16 ? run_few<1, 4, 8, true>(p, stream) : run_few<2, 4, 4, true>(p, stream);
-    return p.n_rows <= 16 ? run_few<1, 1, 8, false>(p, stream) : run_few<4, 2, 4, false>(p, stream);
+    if (p.activation) return p.n_rows <= 16 ? run_few<1, 4, 8, 2, true>(p, stream) : run_few<2, 4, 4, 2, true>(p, stream);
+    return p.n_rows <= 16 ? run_few<1, 1, 8, 4, false>(p, stream) : run_few<4, 2, 4, 2, false>(p, stream);
 }
 
 hipError_t launch_weights_pack(const PackParams &p, hipStream_t stream) {
