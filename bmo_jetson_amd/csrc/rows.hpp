@@ -87,11 +87,11 @@ constexpr int kUnitRows = 16, kUnitCols = 128, kUnitBytes = 1152, kUnitScales = 
 
 struct WeightsGeom {
     int rows, cols;
-    int tiles;   // of 16 rows
+    int tiles;   // of 16 rows, an even number
     int chunks;  // of 128 columns
 };
 inline WeightsGeom make_weights_geom(int rows, int cols) {
-    return {rows, cols, (rows + kUnitRows - 1) / kUnitRows, (cols + kUnitCols - 1) / kUnitCols};
+    return {rows, cols, (rows + 2 * kUnitRows - 1) / (2 * kUnitRows) * 2, (cols + kUnitCols - 1) / kUnitCols};
 }
 inline int64_t weights_bytes(const WeightsGeom &g) { return (int64_t) g.tiles * g.chunks * kUnitBytes; }
 

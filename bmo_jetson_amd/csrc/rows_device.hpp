@@ -104,4 +104,10 @@ __device__ __forceinline__ float row16_max(float v) {
     return __builtin_elementwise_maximum(v, pg_dpp<0x128>(v));      // row_ror:8
 }
 
+// The largest of a half's 32 lanes.
+__device__ __forceinline__ float half_max(float v) {
+    v = row16_max(v);
+    return __builtin_elementwise_maximum(v, __shfl_xor(v, 16));
+}
+
 }  // namespace bmo

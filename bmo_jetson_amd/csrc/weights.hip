@@ -65,14 +65,6 @@ __device__ __forceinline__ float gate(float g, float u, int activation) {
     return g / (1.0f + expf(-a)) * u;
 }
 
-// Outputs n .. n + 3 of row m.
-__device__ __forceinline__ void store_quad(const ProductParams &p, int64_t m, int n, int n_out, rw_float4 v) {
-    const int64_t at = m * p.out_stride + n;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (n + j < n_out) store1(p.out, at + j, v[j], p.type);
-}
-
 constexpr int kRowStride = 144;  // of 128 codes in LDS: 16 rows' octets lie in different banks
 
 // Few rows: a workgroup takes 16 * MT rows and NT tiles of 16 outputs (of a
@@ -248,16 +240,16 @@ hipError_t run_few(const ProductParams &p, hipStream_t stream) {
 // Many rows: a wave takes MT * 32 rows and NT tiles of 32 outputs (of a gated
 // product one of gates and the one that they let through), a workgroup WM * WN
 // such pieces, each shared by KW waves, which take every KW-th unit of it and
-// join their sums in LDS.  The outputs are the rows of the results here: a lane
-// has 16 outputs of one row, its scale is the lane's own and the outputs' are
-// read from LDS, where the wave puts them.  The rows' codes go through LDS too,
-// a unit ahead: eight lanes read a row's 128, which costs the loads a quarter of
-// what reading them as the matrix cores take them does.
+// join their sums in LDS.  As with few rows a lane has one output, here of 16
+// rows, whose scales are read from LDS.  The rows' codes and scales go there a
+// unit ahead: eight lanes read a row's 128 codes, which costs the loads a
+// quarter of what reading them as the matrix cores take them does.  D units'
+// weights and DX units' codes are under way at once.
 
-// Two units' codes of 16 rows each to a 32-row operand: lanes 16 to 31 and 48
-// to 63 of the first change places with lanes 0 to 15 and 32 to 47 of the
-// second.  (Wait states: the compiler's hazard pass does not see inside.)
-__device__ __forceinline__ void pair_rows(wt_uint4 &a, wt_uint4 &b) {
+// Two units' codes of 16 outputs each to a 32-column operand: lanes 16 to 31
+// and 48 to 63 of the first change places with lanes 0 to 15 and 32 to 47 of
+// the second.  (Wait states: the compiler's hazard pass does not see inside.)
+__device__ __forceinline__ void pair_units(wt_uint4 &a, wt_uint4 &b) {
     uint32_t a0 = a[0], a1 = a[1], a2 = a[2], a3 = a[3], b0 = b[0], b1 = b[1], b2 = b[2], b3 = b[3];
     asm volatile(
         "s_nop 3\n\t"
@@ -274,62 +266,62 @@ __device__ __forceinline__ void pair_rows(wt_uint4 &a, wt_uint4 &b) {
 // A barrier that waits for LDS alone, not for loads under way.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <int MT, int NT, int WM, int WN, int KW, bool GATED, bool EVEN>
+template <int MT, int NT, int WM, int WN, int KW, int D, int DX, bool GATED>
 __global__ __launch_bounds__(64 * WM * WN * KW, 2) void many_rows_kernel(ProductParams p, int n_pieces) {
     static_assert(!GATED || NT == 2, "a tile of gates and the one that they let through");
+    static_assert(D % DX == 0, "a slot of codes belongs to one of units");
     constexpr int WAVES = WM * WN * KW, ROWS = 32 * MT * WM, XL = 4 * MT / WN;  // rows of a workgroup; loads of a lane
-    constexpr bool ALONE = WM * WN == 1;  // a wave reads only the codes that it puts into LDS itself
+    constexpr bool ALONE = WM * WN == 1;  // a wave reads only what it puts into LDS itself
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kw = wave % KW, wn = wave / KW % WN, wm = wave / KW / WN;
-    const int m32 = lane & 31, h = lane >> 5;
-    const int m0 = ((int) blockIdx.y * WM + wm) * 32 * MT;
+    const int l32 = lane & 31, h = lane >> 5;
     const int piece = (int) blockIdx.x * WN + wn;
     const int nb = p.g.cols / 32, last = p.g.chunks - 1;
-    // (tiles of 32 outputs; a piece past the last reads the last and stores nothing)
-    auto unit = [&](int n, int u) {
+    // (a tile past the last reads the last and stores nothing)
+    const uint32_t tile_bytes = (uint32_t) p.g.chunks * (uint32_t) kUnitBytes;
+    const uint8_t *w[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
         const int tile = GATED ? piece + n * (p.g.tiles / 4) : NT * piece + n;
-        return p.w + (int64_t) min(2 * tile + u, p.g.tiles - 1) * p.g.chunks * kUnitBytes;
-    };
-    const uint8_t *w[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) w[n][u] = unit(n, u);
-    // A lane carries the scales of row lane % 32 of tile lane / 32 to where the
-    // lanes of the row's half take them: results 4j + i are rows 8j + 4h + i.
-    const uint8_t *ws = unit(NT == 2 ? lane >> 5 : 0, (lane >> 4) & 1) + kUnitScales + (lane & 15) * 8;
-    __shared__ rw_float4 s_scale[WAVES][2][4][2][4];  // [tile][block][half][16 rows]
-    float *scale_to = reinterpret_cast<float *>(s_scale[wave][lane >> 5]) + ((lane >> 2) & 1) * 16 + ((lane >> 3) & 3) * 4 +
-                      (lane & 3);
+        w[n] = p.w + (int64_t) min(2 * tile, p.g.tiles - 2) * tile_bytes;
+    }
+    const uint32_t scales_at = ((lane >> 4) & 1) * tile_bytes + kUnitScales + (lane & 15) * 8;
     // (the rows' offsets from the workgroup's first fit 32 bits: 127 * 2^24)
     const int first = (int) blockIdx.y * ROWS;
     const int8_t *codes = p.codes + (int64_t) first * p.g.cols;
     const uint16_t *scales = p.scales + (int64_t) first * nb;
-    uint32_t d_at[MT], x_at[XL];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) d_at[m] = (uint32_t) min(wm * 32 * MT + 32 * m + m32, p.n_rows - 1 - first) * (uint32_t) nb;
     const int x_row = wave / KW * (8 * XL) + (lane >> 3), piece16 = lane & 7;
+    uint32_t x_at[XL], d_at[XL];
 #pragma unroll
-    for (int i = 0; i < XL; ++i) x_at[i] = (uint32_t) min(x_row + 8 * i, p.n_rows - 1 - first) * (uint32_t) p.g.cols;
-    // (a row's sixteens change places by the row, so that eight rows' lie in
-    // different banks)
+    for (int i = 0; i < XL; ++i) {
+        const uint32_t row = (uint32_t) min(x_row + 8 * i, p.n_rows - 1 - first);
+        x_at[i] = row * (uint32_t) p.g.cols;
+        d_at[i] = row * (uint32_t) nb;
+    }
+    // A row's sixteens change places by the row, so that eight rows' lie in
+    // different banks.  Results 4j + i of a lane are rows 8j + 4h + i: a half's
+    // scales lie together.
     __shared__ wt_int4 s_x[KW][ALONE ? 1 : 2][ROWS][8];
-    wt_int4 xr[XL];
-    auto load_x = [&](int c) {  // (past the last block weights are zeros)
+    __shared__ float s_d8[KW][ALONE ? 1 : 2][ROWS / 32][4][2][16];
+    wt_int4 xr[DX][XL];
+    uint32_t dr[DX][XL];
+    auto load_x = [&](int j, int c) {  // (past the last block weights are zeros)
         const uint32_t e = (uint32_t) min(c * kUnitCols + piece16 * 16, p.g.cols - 16);
+        const uint32_t b = (uint32_t) min(4 * c + (lane & 3), nb - 1);
 #pragma unroll
-        for (int i = 0; i < XL; ++i) xr[i] = *reinterpret_cast<const wt_int4 *>(codes + (x_at[i] + e));
+        for (int i = 0; i < XL; ++i) {
+            xr[j][i] = *reinterpret_cast<const wt_int4 *>(codes + (x_at[i] + e));
+            dr[j][i] = scales[d_at[i] + b];
+        }
     };
-    auto put_x = [&](int buffer) {
+    auto put_x = [&](int j, int buffer) {
 #pragma unroll
-        for (int i = 0; i < XL; ++i) s_x[kw][buffer][x_row + 8 * i][piece16 ^ (x_row & 7)] = xr[i];
-    };
-    auto load_d = [&](int m, int c) {
-        if constexpr (EVEN) return *reinterpret_cast<const wt_uint2 *>(scales + (d_at[m] + 4 * (uint32_t) c));
-        uint32_t v[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) v[t] = scales[d_at[m] + (uint32_t) min(4 * c + t, nb - 1)];
-        return wt_uint2{v[0] | v[1] << 16, v[2] | v[3] << 16};
+        for (int i = 0; i < XL; ++i) {
+            const int row = x_row + 8 * i;
+            s_x[kw][buffer][row][piece16 ^ (x_row & 7)] = xr[j][i];
+            // (lanes 4 apart write the same)
+            s_d8[kw][buffer][row >> 5][lane & 3][(row >> 2) & 1][((row >> 3) & 3) * 4 + (row & 3)] = half_lo(dr[j][i]);
+        }
     };
     wt_float16 acc[NT][MT];
 #pragma unroll
@@ -342,90 +334,85 @@ __global__ __launch_bounds__(64 * WM * WN * KW, 2) void many_rows_kernel(Product
 #pragma unroll
     for (int i = 0; i < 16; ++i) magic[i] = kMagicBits;
     asm volatile("" : "+v"(magic));  // (kept, not made again before each use)
-    wt_uint4 q[NT][2], q1[NT][2];
-    wt_uint2 sc, sc1, dd[MT], dd1[MT];
-    auto load_units = [&](int c, wt_uint4 (&qq)[NT][2], wt_uint2 &s, wt_uint2 (&e)[MT]) {
+    wt_uint4 q[D][NT][2];
+    wt_uint2 d4[D][NT];
+    auto load_units = [&](int j, int c) {
         const uint32_t at = (uint32_t) c * (uint32_t) kUnitBytes;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) qq[n][u] = *reinterpret_cast<const wt_uint4 *>(w[n][u] + at + lane * 16);
-        s = *reinterpret_cast<const wt_uint2 *>(ws + at);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) e[m] = load_d(m, c);
+            for (int u = 0; u < 2; ++u)
+                q[j][n][u] = *reinterpret_cast<const wt_uint4 *>(w[n] + (u * tile_bytes + at) + lane * 16);
+            d4[j][n] = *reinterpret_cast<const wt_uint2 *>(w[n] + at + scales_at);
+        }
     };
-    load_x(min(kw, last));
-    load_units(min(kw, last), q, sc, dd);
+    // Step s takes unit s * KW + kw.  Its weights lie in slot s % D, read after
+    // step s - D's were used; its rows' codes in slot s % DX, read once those
+    // of step s - DX are in LDS.
     const int steps = (last + KW) / KW;
-    for (int step = 0; step < steps; ++step) {
-        const int next = min((step + 1) * KW + kw, last), at = ALONE ? 0 : step & 1;
-        if (ALONE && KW > 1 && step * KW + kw > last) break;
-        put_x(at);
-        if (!ALONE) lds_barrier();
-        load_x(next);
-        load_units(next, q1, sc1, dd1);
-        if (ALONE || KW == 1 || step * KW + kw <= last) {  // (else a unit that another wave has)
-            scale_to[0] = half_lo(sc[0]);
-            scale_to[32] = half_hi(sc[0]);
-            scale_to[64] = half_lo(sc[1]);
-            scale_to[96] = half_hi(sc[1]);
+    auto unit_of = [&](int step) { return min(step * KW + kw, last); };
 #pragma unroll
-            for (int n = 0; n < NT; ++n) pair_rows(q[n][0], q[n][1]);
-            // What a block needs of LDS is read while the one before it is
-            // multiplied.
-            wt_int4 xv[2][MT];
-            rw_float4 d4[2][4];
-            auto read_x = [&](int t) {
+    for (int j = 0; j < D; ++j) {
+        if (j < DX) load_x(j, unit_of(j));
+        load_units(j, unit_of(j));
+    }
+    for (int step0 = 0; step0 < steps; step0 += D) {
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
-                    xv[t & 1][m] = s_x[kw][at][wm * 32 * MT + 32 * m + m32][(2 * t + h) ^ (m32 & 7)];
-            };
-            auto read_d4 = [&](int e) {  // e: tile e % NT of block e / NT
+        for (int j = 0; j < D; ++j) {
+            const int step = step0 + j, at = ALONE ? 0 : step & 1, jx = j % DX;
+            if (step >= steps || (ALONE && step * KW + kw > last)) break;
+            put_x(jx, at);
+            if (!ALONE) lds_barrier();
+            load_x(jx, unit_of(step + DX));
+            if (ALONE || KW == 1 || step * KW + kw <= last) {  // (else a unit that another wave has)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) d4[e & 1][j] = s_scale[wave][e % NT][e / NT][h][j];
-            };
-            read_x(0);
-            read_d4(0);
+                for (int n = 0; n < NT; ++n) pair_units(q[j][n][0], q[j][n][1]);
+                // What a block of rows needs of LDS is read while the one before
+                // it is multiplied.
+                wt_int4 xv[2];
+                rw_float4 d8[2][4];
+                auto read_rows = [&](int e) {  // e: rows e % MT, block e / MT
+                    const int t = e / MT, m = wm * MT + e % MT;
+                    xv[e & 1] = s_x[kw][at][32 * m + l32][(2 * t + h) ^ (l32 & 7)];
+                    const rw_float4 *src = reinterpret_cast<const rw_float4 *>(s_d8[kw][at][m][t][h]);
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                float d8[MT], off[MT];
+                    for (int i = 0; i < 4; ++i) d8[e & 1][i] = src[i];
+                };
+                read_rows(0);
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    d8[m] = t & 1 ? half_hi(dd[m][t >> 1]) : half_lo(dd[m][t >> 1]);
-                    asm volatile("" : "+v"(d8[m]));  // (in fp32: an fma that widens an operand takes twice the time)
-                    off[m] = -kMagic * d8[m];
-                }
-                if (t < 3) read_x(t + 1);
+                for (int t = 0; t < 4; ++t) {
+                    wt_int4 wv[NT];
+                    float ds[NT], off[NT];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const int e = t * NT + n;
-                    const uint32_t a = q[n][0][t], b = q[n][1][t];
-                    const wt_int4 av = {(int) (a << 4 & 0xF0F0F0F0u), (int) (a & 0xF0F0F0F0u), (int) (b << 4 & 0xF0F0F0F0u),
+                    for (int n = 0; n < NT; ++n) {
+                        const uint32_t a = q[j][n][0][t], b = q[j][n][1][t];
+                        wv[n] = wt_int4{(int) (a << 4 & 0xF0F0F0F0u), (int) (a & 0xF0F0F0F0u), (int) (b << 4 & 0xF0F0F0F0u),
                                         (int) (b & 0xF0F0F0F0u)};
-                    wt_int16 z[MT];
-#pragma unroll
-                    for (int m = 0; m < MT; ++m)
-                        z[m] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av, xv[t & 1][m], magic, 0, 0, 0);
-                    if (e + 1 < 4 * NT) read_d4(e + 1);
+                        ds[n] = t & 1 ? half_hi(d4[j][n][t >> 1]) : half_lo(d4[j][n][t >> 1]);
+                        asm volatile("" : "+v"(ds[n]));  // (in fp32: an fma that widens an operand takes twice the time)
+                        off[n] = -kMagic * ds[n];
+                    }
 #pragma unroll
                     for (int m = 0; m < MT; ++m) {
-                        const wt_float16 f = __builtin_bit_cast(wt_float16, z[m]);
+                        const int e = t * MT + m;
+                        wt_int16 z[NT];
 #pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            acc[n][m][r] =
-                                __builtin_fmaf(d4[e & 1][r >> 2][r & 3], __builtin_fmaf(f[r], d8[m], off[m]), acc[n][m][r]);
+                        for (int n = 0; n < NT; ++n)
+                            z[n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xv[e & 1], wv[n], magic, 0, 0, 0);
+                        if (e + 1 < 4 * MT) read_rows(e + 1);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            const wt_float16 f = __builtin_bit_cast(wt_float16, z[n]);
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                acc[n][m][r] =
+                                    __builtin_fmaf(d8[e & 1][r >> 2][r & 3], __builtin_fmaf(f[r], ds[n], off[n]), acc[n][m][r]);
+                        }
                     }
-
                 }
             }
+            load_units(j, unit_of(step + D));
         }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) q[n][u] = q1[n][u];
-        sc = sc1;
-#pragma unroll
-        for (int m = 0; m < MT; ++m) dd[m] = dd1[m];
     }
     if constexpr (KW > 1) {
         // the waves of a piece add up in the order of their units
@@ -451,52 +438,40 @@ __global__ __launch_bounds__(64 * WM * WN * KW, 2) void many_rows_kernel(Product
             }
     }
     if (piece >= n_pieces) return;
+    // (the waves of a piece store a part each: results r with r % KW == kw)
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        if (KW > 1 && m % KW != kw) continue;  // each stores a part
-        const int64_t row = m0 + 32 * m + m32;
-        if constexpr (GATED) {
-            const int n_out = p.g.rows / 2, n0 = piece * 32 + 4 * h;
-            float v[16], amax = 0.0f;
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                v[i] = gate(acc[0][m][i] * kCodeStep, acc[1][m][i] * kCodeStep, p.activation);
-                amax = __builtin_elementwise_maximum(amax, __builtin_fabsf(v[i]));
-            }
-            if (p.out && row < p.n_rows) {
+        for (int r = 0; r < 16; ++r) {
+            const int64_t row = (int64_t) first + (wm * MT + m) * 32 + 8 * (r >> 2) + 4 * h + (r & 3);
+            if (KW > 1 && r % KW != kw) continue;
+            if constexpr (GATED) {
+                const int n_out = p.g.rows / 2, col = piece * 32 + l32;
+                const float v = gate(acc[0][m][r] * kCodeStep, acc[1][m][r] * kCodeStep, p.activation);
+                if (p.out && row < p.n_rows) store1(p.out, row * p.out_stride + col, v, p.type);
+                if (p.out_codes) {
+                    const Scale8 s = scale_of(half_max(__builtin_fabsf(v)));
+                    if (row < p.n_rows) {
+                        p.out_codes[row * n_out + col] = (int8_t) code1(v, s.inv);
+                        if (l32 == 0) p.out_scales[row * (n_out / 32) + piece] = (uint16_t) s.bits;
+                    }
+                }
+            } else if (row < p.n_rows) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    store_quad(p, row, n0 + 8 * j, n_out, rw_float4{v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]});
-            }
-            if (p.out_codes) {
-                const Scale8 s = scale_of(__builtin_elementwise_maximum(amax, __shfl_xor(amax, 32)));
-                if (row < p.n_rows) {
-                    uint32_t *dst = reinterpret_cast<uint32_t *>(p.out_codes + row * n_out + n0);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) dst[2 * j] = codes4(v + 4 * j, s.inv);
-                    if (h == 0) p.out_scales[row * (n_out / 32) + piece] = (uint16_t) s.bits;
+                for (int n = 0; n < NT; ++n) {
+                    const int col = (NT * piece + n) * 32 + l32;
+                    if (col < p.g.rows) store1(p.out, row * p.out_stride + col, acc[n][m][r] * kCodeStep, p.type);
                 }
             }
-        } else if (row < p.n_rows) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    store_quad(p, row, (NT * piece + n) * 32 + 8 * j + 4 * h, p.g.rows,
-                               rw_float4{acc[n][m][4 * j], acc[n][m][4 * j + 1], acc[n][m][4 * j + 2], acc[n][m][4 * j + 3]} *
-                                   kCodeStep);
         }
-    }
 }
 
-template <int MT, int NT, int WM, int WN, int KW, bool GATED>
+template <int MT, int NT, int WM, int WN, int KW, int D, int DX, bool GATED>
 hipError_t run_many(const ProductParams &p, hipStream_t stream) {
     ProductParams q = p;
     int pieces = GATED ? p.g.rows / 64 : (p.g.rows + 32 * NT - 1) / (32 * NT);
     void *args[] = {&q, &pieces};
-    const bool even = p.g.cols % 128 == 0 && reinterpret_cast<uintptr_t>(p.scales) % 8 == 0;
-    return hipLaunchKernel(even ? reinterpret_cast<const void *>(many_rows_kernel<MT, NT, WM, WN, KW, GATED, true>)
-                                : reinterpret_cast<const void *>(many_rows_kernel<MT, NT, WM, WN, KW, GATED, false>),
+    return hipLaunchKernel(reinterpret_cast<const void *>(many_rows_kernel<MT, NT, WM, WN, KW, D, DX, GATED>),
                            dim3((unsigned) ((pieces + WN - 1) / WN), (unsigned) ((p.n_rows + 32 * MT * WM - 1) / (32 * MT * WM))),
                            dim3(64 * WM * WN * KW), args, 0, stream);
 }
@@ -505,8 +480,8 @@ hipError_t run_many(const ProductParams &p, hipStream_t stream) {
 
 hipError_t launch_product(const ProductParams &p, hipStream_t stream) {
     if (p.n_rows > 64) {
-        if (p.activation) return run_many<2, 2, 2, 2, 1, true>(p, stream);
-        return run_many<2, 2, 2, 2, 1, false>(p, stream);
+        if (p.activation) return run_many<2, 2, 2, 2, 1, 2, 1, true>(p, stream);
+        return run_many<2, 2, 2, 2, 1, 2, 1, false>(p, stream);
     }
     if (p.activation) return p.n_rows <= 16 ? run_few<1, 4, 8, 2, true>(p, stream) : run_few<2, 4, 4, 2, true>(p, stream);
     return p.n_rows <= 16 ? run_few<1, 1, 8, 4, false>(p, stream) : run_few<4, 2, 4, 2, false>(p, stream);
