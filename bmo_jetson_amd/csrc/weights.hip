@@ -65,6 +65,134 @@ __device__ __forceinline__ float gate(float g, float u, int activation) {
     return g / (1.0f + expf(-a)) * u;
 }
 
+// A barrier that waits for LDS alone, not for loads under way.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// One row: vector units alone, which spend half the instructions on it that the
+// matrix cores' sixteen rows take.  A workgroup takes NT tiles of 16 outputs (of
+// a gated product two of gates and the two that they let through), its KW waves
+// a run of their units each.  Lane (g, i) multiplies block g of a unit's four of
+// output i, for which the four octets change places between lanes: eight dot
+// products that begin with the float's bits, as the matrix instructions do.  The
+// row lies in LDS, its scales in fp32.
+constexpr int kOneRowChunks = 256;  // of a row in LDS, 144 bytes each
+
+// Dword t of lanes 16 g .. to dword g of lanes 16 t ..: from octet g of four
+// blocks to four octets of block g.  (Wait states: the compiler's hazard pass
+// does not see inside.)
+__device__ __forceinline__ wt_uint4 turn_octets(const wt_uint4 &v) {
+    uint32_t a = v[0], b = v[1], c = v[2], d = v[3];
+    asm volatile(
+        "s_nop 3\n\t"
+        "v_permlane32_swap_b32 %0, %2\n\t"
+        "v_permlane32_swap_b32 %1, %3\n\t"
+        "s_nop 3\n\t"
+        "v_permlane16_swap_b32 %0, %1\n\t"
+        "v_permlane16_swap_b32 %2, %3\n\t"
+        "s_nop 3"
+        : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
+    return wt_uint4{a, b, c, d};
+}
+
+template <int NT, int KW, int PF, bool GATED>
+__global__ __launch_bounds__(64 * KW) void one_row_kernel(ProductParams p) {
+    static_assert(!GATED || NT == 4, "two tiles of gates and the two that they let through");
+    extern __shared__ uint8_t s_row[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i16 = lane & 15, g = lane >> 4;
+    const int nb = p.g.cols / 32, last = p.g.chunks - 1;
+    const int per = (p.g.chunks + KW - 1) / KW, c0 = wave * per, c1 = min(c0 + per, p.g.chunks);
+    const uint8_t *w[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int tile = GATED ? (int) blockIdx.x * 2 + (n & 1) + (n & 2 ? p.g.tiles / 2 : 0) : (int) blockIdx.x * NT + n;
+        w[n] = p.w + (int64_t) min(tile, p.g.tiles - 1) * p.g.chunks * kUnitBytes;
+    }
+    wt_uint4 q[PF][NT];
+    uint32_t d4[PF][NT];
+    auto load = [&](int j, int c) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const uint8_t *u = w[n] + (uint32_t) c * (uint32_t) kUnitBytes;
+            q[j][n] = __builtin_nontemporal_load(reinterpret_cast<const wt_uint4 *>(u + lane * 16));
+            d4[j][n] = *reinterpret_cast<const uint16_t *>(u + kUnitScales + i16 * 8 + g * 2);
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < PF; ++j) load(j, min(c0 + j, last));
+    float *s_d8 = reinterpret_cast<float *>(s_row + p.g.chunks * kUnitCols);
+    for (int o = threadIdx.x; o < nb * 2; o += 64 * KW)
+        reinterpret_cast<wt_uint4 *>(s_row)[o] = reinterpret_cast<const wt_uint4 *>(p.codes)[o];
+    // (past the last block weights are zeros, the codes whatever lies there)
+    for (int b = threadIdx.x; b < p.g.chunks * 4; b += 64 * KW) s_d8[b] = b < nb ? half_lo(p.scales[b]) : 0.0f;
+    lds_barrier();
+    float acc[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n] = 0.0f;
+    for (int c = c0; c < c1; c += PF) {
+#pragma unroll
+        for (int j = 0; j < PF; ++j) {
+            if (c + j >= c1) break;
+            const wt_uint4 *x = reinterpret_cast<const wt_uint4 *>(s_row + (c + j) * kUnitCols + g * 32);
+            const wt_uint4 xa = x[0], xb = x[1];
+            const float d8 = s_d8[4 * (c + j) + g];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const wt_uint4 v = turn_octets(q[j][n]);
+                float ds = half_lo(d4[j][n]);
+                asm volatile("" : "+v"(ds));  // (in fp32: an fma that widens an operand takes twice the time)
+                int z = kMagicBits;
+#pragma unroll
+                for (int o = 0; o < 4; ++o) {
+                    z = __builtin_amdgcn_sdot4((int) (v[o] << 4 & 0xF0F0F0F0u), (int) (o < 2 ? xa : xb)[2 * (o & 1)], z, false);
+                    z = __builtin_amdgcn_sdot4((int) (v[o] & 0xF0F0F0F0u), (int) (o < 2 ? xa : xb)[2 * (o & 1) + 1], z, false);
+                }
+                acc[n] = __builtin_fmaf(d8, __builtin_fmaf(__builtin_bit_cast(float, z), ds, -kMagic * ds), acc[n]);
+            }
+            if (c + j + PF < c1) load(j, c + j + PF);
+        }
+    }
+    __shared__ float s_acc[KW][NT][16];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        acc[n] += __shfl_xor(acc[n], 16);
+        acc[n] += __shfl_xor(acc[n], 32);
+        if (g == 0) s_acc[wave][n][i16] = acc[n];
+    }
+    __syncthreads();
+    auto joined = [&](int n, int i) {
+        float v = s_acc[0][n][i];
+#pragma unroll
+        for (int k = 1; k < KW; ++k) v += s_acc[k][n][i];
+        return v * kCodeStep;
+    };
+    const int t = threadIdx.x;
+    if constexpr (GATED) {
+        if (t >= 32) return;
+        const int col = (int) blockIdx.x * 32 + t;
+        const float v = gate(joined(t >> 4, t & 15), joined(2 + (t >> 4), t & 15), p.activation);
+        if (p.out) store1(p.out, col, v, p.type);
+        if (p.out_codes) {
+            const Scale8 s = scale_of(half_max(__builtin_fabsf(v)));
+            p.out_codes[col] = (int8_t) code1(v, s.inv);
+            if (t == 0) p.out_scales[col / 32] = (uint16_t) s.bits;
+        }
+    } else {
+        const int col = (int) blockIdx.x * 16 * NT + t;
+        if (t < 16 * NT && col < p.g.rows) store1(p.out, col, joined(t >> 4, t & 15), p.type);
+    }
+}
+
+template <int NT, int KW, int PF, bool GATED>
+hipError_t run_one(const ProductParams &p, hipStream_t stream) {
+    ProductParams q = p;
+    void *args[] = {&q};
+    const int per = GATED ? 2 : NT, tiles = GATED ? p.g.tiles / 2 : p.g.tiles;
+    return hipLaunchKernel(reinterpret_cast<const void *>(one_row_kernel<NT, KW, PF, GATED>),
+                           dim3((unsigned) ((tiles + per - 1) / per)), dim3(64 * KW), args,
+                           (size_t) p.g.chunks * (kUnitCols + 16), stream);
+}
+
 constexpr int kRowStride = 144;  // of 128 codes in LDS: 16 rows' octets lie in different banks
 
 // Few rows: a workgroup takes 16 * MT rows and NT tiles of 16 outputs (of a
@@ -263,9 +391,6 @@ __device__ __forceinline__ void pair_units(wt_uint4 &a, wt_uint4 &b) {
     b = wt_uint4{b0, b1, b2, b3};
 }
 
-// A barrier that waits for LDS alone, not for loads under way.
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
 template <int MT, int NT, int WM, int WN, int KW, int D, int DX, bool GATED>
 __global__ __launch_bounds__(64 * WM * WN * KW, 2) void many_rows_kernel(ProductParams p, int n_pieces) {
     static_assert(!GATED || NT == 2, "a tile of gates and the one that they let through");
@@ -395,14 +520,11 @@ __global__ __launch_bounds__(64 * WM * WN * KW, 2) void many_rows_kernel(Product
 #pragma unroll
                     for (int m = 0; m < MT; ++m) {
                         const int e = t * MT + m;
-                        wt_int16 z[NT];
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-                            z[n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xv[e & 1], wv[n], magic, 0, 0, 0);
                         if (e + 1 < 4 * MT) read_rows(e + 1);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            const wt_float16 f = __builtin_bit_cast(wt_float16, z[n]);
+                            const wt_float16 f = __builtin_bit_cast(
+                                wt_float16, __builtin_amdgcn_mfma_i32_32x32x32_i8(xv[e & 1], wv[n], magic, 0, 0, 0));
 #pragma unroll
                             for (int r = 0; r < 16; ++r)
                                 acc[n][m][r] =
@@ -479,6 +601,8 @@ hipError_t run_many(const ProductParams &p, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_product(const ProductParams &p, hipStream_t stream) {
+    if (p.n_rows == 1 && p.g.chunks <= kOneRowChunks)
+        return p.activation ? run_one<4, 8, 2, true>(p, stream) : run_one<1, 8, 2, false>(p, stream);
     if (p.n_rows > 64) {
         if (p.activation) return run_many<2, 2, 2, 2, 1, 2, 1, true>(p, stream);
         return run_many<2, 2, 2, 2, 1, 2, 1, false>(p, stream);
