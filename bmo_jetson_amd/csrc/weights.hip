@@ -12,6 +12,7 @@
 // d8.  A second one adds d4 times that, so an output is off by the roundings
 // of an fp32 sum of its blocks' parts only.
 #include "kernels.hpp"
+#include "product_shape.hpp"
 #include "rows_device.hpp"
 
 namespace bmo {
@@ -263,6 +264,7 @@ __global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p) {
 #pragma unroll
         for (int j = 0; j < PF; ++j) {
             if (c + j >= c1) break;
+            __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses stay in order)
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 s_d8[wave][m][g][i16] = half_lo(d8[j][m]);
@@ -270,6 +272,7 @@ __global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p) {
                 for (int i = 0; i < 2; ++i)
                     *reinterpret_cast<wt_uint4 *>(&s_x[wave][m][8 * i + (lane >> 3)][(lane & 7) * 16]) = x[j][m][i];
             }
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 long wv[NT];
@@ -355,14 +358,17 @@ __global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p) {
     }
 }
 
-template <int MT, int NT, int KW, int PF, bool GATED>
+// The shape's numbers are those of product_shape.hpp.
+template <int SHAPE, int PF, bool GATED>
 hipError_t run_few(const ProductParams &p, hipStream_t stream) {
+    constexpr ProductShape S = GATED ? kGatedShapes[SHAPE] : kProductShapes[SHAPE];
+    constexpr int MT = S.rows / 16, NT = GATED ? 4 : S.outs / 16;
     ProductParams q = p;
     void *args[] = {&q};
-    const int per = GATED ? 2 : NT, tiles = GATED ? p.g.tiles / 2 : p.g.tiles;
-    return hipLaunchKernel(reinterpret_cast<const void *>(few_rows_kernel<MT, NT, KW, PF, GATED>),
-                           dim3((unsigned) ((tiles + per - 1) / per), (unsigned) ((p.n_rows + 16 * MT - 1) / (16 * MT))),
-                           dim3(64 * KW), args, 0, stream);
+    const int outs = GATED ? p.g.rows / 2 : p.g.rows;
+    return hipLaunchKernel(reinterpret_cast<const void *>(few_rows_kernel<MT, NT, S.waves, PF, GATED>),
+                           dim3((unsigned) ((outs + S.outs - 1) / S.outs), (unsigned) ((p.n_rows + S.rows - 1) / S.rows)),
+                           dim3(64 * S.waves), args, 0, stream);
 }
 
 // Many rows: a wave takes MT * 32 rows and NT tiles of 32 outputs (of a gated
@@ -486,8 +492,12 @@ __global__ __launch_bounds__(64 * WM * WN * KW, 2) void many_rows_kernel(Product
         for (int j = 0; j < D; ++j) {
             const int step = step0 + j, at = ALONE ? 0 : step & 1, jx = j % DX;
             if (step >= steps || (ALONE && step * KW + kw > last)) break;
+            if (ALONE) __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses stay in order)
             put_x(jx, at);
-            if (!ALONE) lds_barrier();
+            if (ALONE)
+                __builtin_amdgcn_wave_barrier();
+            else
+                lds_barrier();
             load_x(jx, unit_of(step + DX));
             if (ALONE || KW == 1 || step * KW + kw <= last) {  // (else a unit that another wave has)
 #pragma unroll
@@ -588,27 +598,40 @@ __global__ __launch_bounds__(64 * WM * WN * KW, 2) void many_rows_kernel(Product
         }
 }
 
-template <int MT, int NT, int WM, int WN, int KW, int D, int DX, bool GATED>
+template <int SHAPE, int WM, int WN, int D, int DX, bool GATED>
 hipError_t run_many(const ProductParams &p, hipStream_t stream) {
+    constexpr ProductShape S = GATED ? kGatedShapes[SHAPE] : kProductShapes[SHAPE];
+    constexpr int MT = S.rows / (32 * WM), NT = GATED ? 2 : S.outs / (32 * WN), PIECE = GATED ? 32 : 32 * NT;
+    static_assert(S.outs == PIECE * WN && S.rows == 32 * MT * WM, "the shape's sizes");
     ProductParams q = p;
-    int pieces = GATED ? p.g.rows / 64 : (p.g.rows + 32 * NT - 1) / (32 * NT);
+    int pieces = ((GATED ? p.g.rows / 2 : p.g.rows) + PIECE - 1) / PIECE;
     void *args[] = {&q, &pieces};
-    return hipLaunchKernel(reinterpret_cast<const void *>(many_rows_kernel<MT, NT, WM, WN, KW, D, DX, GATED>),
-                           dim3((unsigned) ((pieces + WN - 1) / WN), (unsigned) ((p.n_rows + 32 * MT * WM - 1) / (32 * MT * WM))),
-                           dim3(64 * WM * WN * KW), args, 0, stream);
+    return hipLaunchKernel(reinterpret_cast<const void *>(many_rows_kernel<MT, NT, WM, WN, S.waves, D, DX, GATED>),
+                           dim3((unsigned) ((pieces + WN - 1) / WN), (unsigned) ((p.n_rows + S.rows - 1) / S.rows)),
+                           dim3(64 * WM * WN * S.waves), args, 0, stream);
 }
 
 }  // namespace
 
 hipError_t launch_product(const ProductParams &p, hipStream_t stream) {
     if (p.n_rows == 1 && p.g.chunks <= kOneRowChunks)
-        return p.activation ? run_one<4, 8, 2, true>(p, stream) : run_one<1, 8, 2, false>(p, stream);
-    if (p.n_rows > 64) {
-        if (p.activation) return run_many<2, 2, 2, 2, 1, 2, 1, true>(p, stream);
-        return run_many<2, 2, 2, 2, 1, 2, 1, false>(p, stream);
+        return p.activation ? run_one<4, 8, 1, true>(p, stream) : run_one<1, 8, 2, false>(p, stream);
+    if (p.activation) {
+        switch (product_shape(true, p.n_rows, p.g.rows / 2, p.g.chunks)) {
+        case 0: return run_few<0, 1, true>(p, stream);
+        case 1: return run_few<1, 1, true>(p, stream);
+        case 2: return run_many<2, 1, 1, 1, 1, true>(p, stream);
+        default: return run_many<3, 2, 2, 1, 1, true>(p, stream);
+        }
     }
-    if (p.activation) return p.n_rows <= 16 ? run_few<1, 4, 8, 2, true>(p, stream) : run_few<2, 4, 4, 2, true>(p, stream);
-    return p.n_rows <= 16 ? run_few<1, 1, 8, 4, false>(p, stream) : run_few<4, 2, 4, 2, false>(p, stream);
+    switch (product_shape(false, p.n_rows, p.g.rows, p.g.chunks)) {
+    case 0: return run_few<0, 2, false>(p, stream);
+    case 1: return run_few<1, 1, false>(p, stream);
+    case 2: return run_many<2, 1, 1, 2, 1, false>(p, stream);
+    case 3: return run_many<3, 1, 1, 1, 1, false>(p, stream);
+    case 4: return run_many<4, 2, 2, 2, 1, false>(p, stream);
+    default: return run_many<5, 2, 2, 2, 1, false>(p, stream);
+    }
 }
 
 hipError_t launch_weights_pack(const PackParams &p, hipStream_t stream) {

@@ -1,6 +1,6 @@
-"""Test helper: the workgroup shapes of decode and staged prefill calls, from the
-rules that the library is compiled with (bmo_jetson_amd/csrc/decode_shape.hpp
-and prefill_shape.hpp)."""
+"""Test helper: the workgroup shapes of decode and staged prefill calls and of
+products, from the rules that the library is compiled with
+(bmo_jetson_amd/csrc/decode_shape.hpp, prefill_shape.hpp and product_shape.hpp)."""
 import os
 import subprocess
 
@@ -29,3 +29,9 @@ def staged_shapes(calls):
     """(units in full rounds of 16 waves x 16 queries, waves per workgroup and
     per block of queries of the rest) of each (units, tokens, slots)."""
     return _ask("prefill_shape_check", ["%d %d %d" % c for c in calls])
+
+
+def product_shapes(calls):
+    """(rows and outputs of a workgroup, waves of a piece) of each (gated, rows,
+    outputs, columns)."""
+    return _ask("product_shape_check", ["%d %d %d %d" % (bool(g), m, n, -(-k // 128)) for g, m, n, k in calls])

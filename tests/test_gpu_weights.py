@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+from _shapes import product_shapes
 from _rows import blocks_of, check, check8, gated, product, q4_0, rounded, split8
 
 pytestmark = pytest.mark.gpu
@@ -62,6 +63,22 @@ def test_numbers_of_columns(gpu, cols):
 @pytest.mark.parametrize("n,rows,cols", [(1, 4096, 4096), (5, 1001, 512), (40, 2050, 640), (150, 515, 1024), (700, 384, 512)])
 def test_types_and_larger_sizes(gpu, n, rows, cols, type_):
     _product(gpu, n, rows, cols, type_)
+
+
+# rows, outputs, columns and the kernel that takes them (workgroup's rows, outputs; waves of a piece)
+SHAPES = [(2, 97, 416, (16, 16, 8)), (37, 161, 1120, (16, 16, 8)), (37, 4097, 416, (16, 32, 8)), (69, 1001, 1120, (16, 32, 8)),
+          (197, 1001, 96, (32, 32, 4)), (261, 1001, 416, (32, 32, 4)), (131, 8193, 736, (32, 64, 4)),
+          (197, 6001, 736, (32, 64, 4)), (901, 2049, 96, (64, 128, 1)), (901, 4097, 736, (64, 128, 1)),
+          (515, 12001, 1120, (128, 128, 1)), (3001, 2049, 1120, (128, 128, 1))]
+GATED_SHAPES = [(2, 32, 96, (16, 32, 8)), (69, 160, 416, (16, 32, 8)), (131, 1024, 736, (32, 32, 8)),
+                (69, 2080, 736, (32, 32, 8)), (131, 1024, 96, (32, 32, 4)), (69, 2080, 160, (32, 32, 4)),
+                (515, 6016, 96, (128, 64, 1)), (901, 4128, 96, (128, 64, 1)), (1101, 3104, 736, (128, 64, 1))]
+
+
+@pytest.mark.parametrize("n,rows,cols,shape", SHAPES)
+def test_every_kernel(gpu, n, rows, cols, shape):
+    assert product_shapes([(False, n, rows, cols)]) == [shape]
+    _product(gpu, n, rows, cols, seed=n)
 
 
 def test_gemv_of_each_row(gpu):
@@ -130,10 +147,13 @@ def test_extreme_codes_and_scales(gpu, n):
 
 
 @pytest.mark.parametrize("activation", ["silu", "gelu"])
-@pytest.mark.parametrize("n,hidden,cols", [(1, 32, 32), (1, 1056, 416), (7, 64, 256), (16, 96, 1024), (17, 512, 96), (33, 32, 640),
+@pytest.mark.parametrize("n,hidden,cols", [c[:3] for c in GATED_SHAPES] + [
+                                           (1, 32, 32), (1, 1056, 416), (7, 64, 256), (16, 96, 1024), (17, 512, 96), (33, 32, 640),
                                            (64, 160, 256), (65, 288, 256), (129, 64, 512), (300, 96, 160), (2, 5632, 4096)])
 def test_gated(gpu, n, hidden, cols, activation):
     torch = gpu
+    assert (n, hidden, cols, product_shapes([(True, n, hidden, cols)])[0]) in GATED_SHAPES or (n, hidden, cols) not in [
+        c[:3] for c in GATED_SHAPES]
     blocks, wc, ws = q4_0(n, 2 * hidden, cols)
     ws = (ws.astype(np.float32) * 3).astype(np.float16)
     w = _weights(torch, blocks_of(wc, ws))
