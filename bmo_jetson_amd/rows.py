@@ -21,64 +21,86 @@ from __future__ import annotations
 import ctypes
 
 from ._lib import lib
-from .pages import _code, _type
+from .pages import _code
 from .ring import RingError, _stream
 
 _ACTIVATIONS = {"silu": 1, "gelu": 2}
-_SMALL: dict = {}  # dtype objects of codes and scales, by their size (formatting a name costs as much as a call)
+_SMALL: dict = {}  # what is asked of torch: the dtype objects of codes and scales, the current device
+
+
+def _small(name: str):
+    known = _SMALL.get(name)
+    if known is None:
+        import torch
+        known = _SMALL[name] = getattr(torch, name)
+    return known
 
 
 def _current() -> int:
-    import torch
-    return torch.cuda.current_device()
+    """The current device."""
+    known = _SMALL.get("device")
+    if known is None:
+        import torch
+        known = _SMALL["device"] = torch.cuda.current_device
+    return known()
 
+
+def _shape(what: str, shape, n, cols) -> ValueError:
+    want = f"[{'rows' if n is None else n}][{'columns' if cols is None else cols}]"
+    return ValueError(f"{what} must be {want}, got {tuple(shape)}")
+
+
+def _on(x, device: int, what: str) -> ValueError:
+    return ValueError(f"{what} must be on device {device}, not on {x.device}")
+
+
+# (The checks below cost as much as the launch of a short kernel: each asks a
+# tensor as little as it can.)
 
 def _rows(x, device: int, what: str, n=None, cols=None):
     """(address, stride, type, rows, columns) of a 2-d tensor of values."""
     shape = x.shape
-    if len(shape) != 2 or (n is not None and shape[0] != n) or (cols is not None and shape[1] != cols):
-        want = f"[{'rows' if n is None else n}][{'columns' if cols is None else cols}]"
-        raise ValueError(f"{what} must be {want}, got {tuple(shape)}")
+    if len(shape) != 2:
+        raise _shape(what, shape, n, cols)
+    rows, width = shape
+    if (n is not None and rows != n) or (cols is not None and width != cols):
+        raise _shape(what, shape, n, cols)
     type_ = _code(x)
     if type_ > 2:
         raise TypeError(f"{what} must be float32, float16 or bfloat16, got {x.dtype}")
-    stride = x.stride()
-    if shape[1] > 1 and shape[0] and stride[1] != 1:
-        raise ValueError(f"{what}: a row's elements must be contiguous")
-    if shape[0] > 1 and stride[0] < shape[1]:
-        raise ValueError(f"{what}: rows must not overlap (an expanded tensor)")
-    _on(x, device, what)
-    return x.data_ptr(), stride[0] if shape[0] > 1 else 0, type_, shape[0], shape[1]
-
-
-def _on(x, device: int, what: str) -> None:
+    stride = 0
+    if not x.is_contiguous():
+        stride, inner = x.stride()
+        if width > 1 and inner != 1:
+            raise ValueError(f"{what}: a row's elements must be contiguous")
+        if rows > 1 and stride < width:
+            raise ValueError(f"{what}: rows must not overlap (an expanded tensor)")
+        if rows == 1:
+            stride = 0
     if x.get_device() != device:
-        raise ValueError(f"{what} must be on device {device}, not on {x.device}")
-
-
-def _small(x, name: str) -> bool:
-    """Whether x has the dtype of that name."""
-    known = _SMALL.get(name)
-    if known is None and str(x.dtype) == "torch." + name:
-        known = _SMALL[name] = x.dtype
-    return x.dtype is known
+        raise _on(x, device, what)
+    return x.data_ptr(), stride, type_, rows, width
 
 
 def _rows8(codes, scales, device: int, what: str, n=None, cols=None):
     """(codes, scales, rows, columns) of 8-bit rows: addresses and sizes."""
     shape = codes.shape
-    if len(shape) != 2 or (n is not None and shape[0] != n) or (cols is not None and shape[1] != cols):
-        want = f"[{'rows' if n is None else n}][{'columns' if cols is None else cols}]"
-        raise ValueError(f"{what}: codes must be {want}, got {tuple(shape)}")
-    if scales.shape != (shape[0], shape[1] // 32) or shape[1] % 32:
+    if len(shape) != 2:
+        raise _shape(f"{what}: codes", shape, n, cols)
+    rows, width = shape
+    if (n is not None and rows != n) or (cols is not None and width != cols):
+        raise _shape(f"{what}: codes", shape, n, cols)
+    if scales.shape != (rows, width // 32) or width % 32:
         raise ValueError(f"{what}: scales must be one for each 32 codes of a row, got {tuple(scales.shape)}")
-    if not (_small(codes, "int8") and _small(scales, "float16")):
+    if codes.dtype is not _small("int8") or scales.dtype is not _small("float16"):
         raise TypeError(f"{what} must be int8 and float16, got {codes.dtype} and {scales.dtype}")
     if not (codes.is_contiguous() and scales.is_contiguous()):
         raise ValueError(f"{what}: codes and scales must be contiguous")
-    _on(codes, device, what)
-    _on(scales, device, what)
-    return codes.data_ptr(), scales.data_ptr(), shape[0], shape[1]
+    if codes.get_device() != device:
+        raise _on(codes, device, what)
+    if scales.get_device() != device:
+        raise _on(scales, device, what)
+    return codes.data_ptr(), scales.data_ptr(), rows, width
 
 
 def _check(fn: str, rc: int) -> None:
@@ -98,7 +120,8 @@ def rms_norm(x, weight, eps: float = 1e-5, residual=None, out=None, codes=None, 
     op, o_stride, o_type, _, _ = _rows(out, device, "out", n, dim) if out is not None else (None, 0, 0, 0, 0)
     if weight.shape != (dim,) or not weight.is_contiguous() or _code(weight) > 2:
         raise ValueError(f"weight must be a contiguous float tensor of {dim} elements")
-    _on(weight, device, "weight")
+    if weight.get_device() != device:
+        raise _on(weight, device, "weight")
     if (codes is None) != (scales is None):
         raise ValueError("codes and scales come together")
     if out is None and codes is None:
@@ -190,16 +213,21 @@ class Rope(_Handle):
         if len(shape) != 3 or shape[0] != n or shape[2] != self.head_dim or (like is not None and shape != like.shape):
             raise ValueError(f"{what} must be [{n}][{'heads' if like is None else like.shape[1]}][{self.head_dim}], "
                              f"got {tuple(shape)}")
-        stride, heads = x.stride(), shape[1]
-        if n and (stride[2] != 1 or (heads > 1 and stride[1] != self.head_dim)):
-            raise ValueError(f"{what}: a token's heads must be contiguous")
-        if n > 1 and stride[0] < heads * self.head_dim:
-            raise ValueError(f"{what}: rows must not overlap (an expanded tensor)")
-        type_ = _type(x)
+        heads, stride = shape[1], 0
+        if not x.is_contiguous():
+            stride, per_head, inner = x.stride()
+            if n and (inner != 1 or (heads > 1 and per_head != self.head_dim)):
+                raise ValueError(f"{what}: a token's heads must be contiguous")
+            if n > 1 and stride < heads * self.head_dim:
+                raise ValueError(f"{what}: rows must not overlap (an expanded tensor)")
+            if n <= 1:
+                stride = 0
+        type_ = _code(x)
         if type_ > 2:
             raise TypeError(f"{what} must be float32, float16 or bfloat16, got {x.dtype}")
-        _on(x, self._device, what)
-        return x.data_ptr(), stride[0] if n > 1 else 0, type_, heads
+        if x.get_device() != self._device:
+            raise _on(x, self._device, what)
+        return x.data_ptr(), stride, type_, heads
 
     def apply(self, positions, q, k=None, q_out=None, k_out=None, stream=None) -> None:
         """Turns q [n_tok][heads][head_dim], and k, by positions [n_tok] (int32),
@@ -207,7 +235,8 @@ class Rope(_Handle):
         n = positions.numel()
         if _code(positions) != 4 or not positions.is_contiguous():
             raise ValueError("positions must be a contiguous int32 tensor")
-        _on(positions, self._device, "positions")
+        if positions.get_device() != self._device:
+            raise _on(positions, self._device, "positions")
         qp, q_stride, type_, heads = self._heads(q, n, "q")
         parts = [(qp, q_stride) if q_out is None else self._heads(q_out, n, "q_out", q)]
         kp, k_stride, k_type, k_heads = (None, 0, type_, 0) if k is None else self._heads(k, n, "k")
@@ -239,7 +268,8 @@ class Q4Weights(_Handle):
         shape = (blocks.shape[0], self.cols // 32, 18)
         if tuple(blocks.shape) != shape or _code(blocks) != 3 or not blocks.is_contiguous():
             raise ValueError(f"blocks must be a contiguous uint8 tensor {shape}")
-        _on(blocks, self._device, "blocks")
+        if blocks.get_device() != self._device:
+            raise _on(blocks, self._device, "blocks")
         self._check("bmo_weights_load", lib().bmo_weights_load(self._h, int(row), shape[0], blocks.data_ptr(),
                                                                _stream(stream)))
 
