@@ -207,7 +207,8 @@ int bmo_rms_norm(int n_rows, int dim, int type, const void *x, int64_t x_stride,
     return guarded(nullptr, "bmo_rms_norm", [&](Call &c) {
         if (!weight || (n_rows != 0 && (!x || (!out && !codes)))) return c.null();
         if (!codes != !scales) return c.arg("codes and scales come together");
-        if (n_rows < 0) return c.arg("n_rows must not be negative");
+        // (a workgroup of up to 1024 a row: the grid's threads stay below 2^32)
+        if (n_rows < 0 || n_rows >= (1 << 22)) return c.arg("n_rows must be at least 0 and below 2^22");
         if (dim <= 0 || dim > bmo::kNormMaxDim) return c.arg("dim must be positive and at most 32768");
         if (codes && dim % 32 != 0) return c.arg("8-bit rows need a dim that is a multiple of 32");
         if (!(eps >= 0.0f) || !std::isfinite(eps)) return c.arg("eps must be finite and not negative");
@@ -328,6 +329,8 @@ int bmo_rope_apply(bmo_rope_t *h, int n_tok, const int *positions, int type, int
         if (n_tok < 0) return c.arg("n_tok must not be negative");
         if (n_heads <= 0 || n_kv_heads < 0 || n_heads > 4096 || n_kv_heads > 4096)
             return c.arg("n_heads must be positive, n_kv_heads not negative, both at most 4096");
+        // (a workgroup takes at least 512 elements, or a whole token: their number stays below 2^24)
+        if ((int64_t) n_tok * (n_heads + n_kv_heads) * h->dim > (int64_t(1) << 32)) return c.arg("too large (2^32 elements)");
         const int64_t q_dense = (int64_t) n_heads * h->dim, k_dense = (int64_t) n_kv_heads * h->dim;
         if (const char *why = row_fault(q, q_stride, q_dense, type)) return c.arg(why);
         if (const char *why = row_fault(q_out, q_out_stride, q_dense, type)) return c.arg(why);

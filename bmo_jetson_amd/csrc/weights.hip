@@ -267,7 +267,7 @@ __global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p) {
             __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses stay in order)
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                s_d8[wave][m][g][i16] = half_lo(d8[j][m]);
+                s_d8[wave][m][g][i16] = 4 * (c + j) + g < nb ? half_lo(d8[j][m]) : 0.0f;  // (past the last block nothing)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
                     *reinterpret_cast<wt_uint4 *>(&s_x[wave][m][8 * i + (lane >> 3)][(lane & 7) * 16]) = x[j][m][i];
@@ -445,13 +445,15 @@ __global__ __launch_bounds__(64 * WM * WN * KW, 2) void many_rows_kernel(Product
             dr[j][i] = scales[d_at[i] + b];
         }
     };
-    auto put_x = [&](int j, int buffer) {
+    auto put_x = [&](int j, int buffer, int c) {
+        const bool real = 4 * c + (lane & 3) < nb;  // (past the last block nothing)
 #pragma unroll
         for (int i = 0; i < XL; ++i) {
             const int row = x_row + 8 * i;
             s_x[kw][buffer][row][piece16 ^ (x_row & 7)] = xr[j][i];
             // (lanes 4 apart write the same)
-            s_d8[kw][buffer][row >> 5][lane & 3][(row >> 2) & 1][((row >> 3) & 3) * 4 + (row & 3)] = half_lo(dr[j][i]);
+            s_d8[kw][buffer][row >> 5][lane & 3][(row >> 2) & 1][((row >> 3) & 3) * 4 + (row & 3)] =
+                real ? half_lo(dr[j][i]) : 0.0f;
         }
     };
     wt_float16 acc[NT][MT];
@@ -493,7 +495,7 @@ __global__ __launch_bounds__(64 * WM * WN * KW, 2) void many_rows_kernel(Product
             const int step = step0 + j, at = ALONE ? 0 : step & 1, jx = j % DX;
             if (step >= steps || (ALONE && step * KW + kw > last)) break;
             if (ALONE) __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses stay in order)
-            put_x(jx, at);
+            put_x(jx, at, unit_of(step));
             if (ALONE)
                 __builtin_amdgcn_wave_barrier();
             else

@@ -644,14 +644,16 @@ BMO_ATTN_API const char *bmo_rows_last_error(void);
  *   y = h / sqrt(mean(h^2) + eps) * weight
  * y goes to out, to 8-bit rows (dim a multiple of 32), or to both; what is
  * NULL is not written.  out may be x with the same type and stride.  fp32
- * inside; the squares of a row have to sum below fp32's range. */
+ * inside; the squares of a row have to sum below fp32's range.  n_rows below
+ * 2^22. */
 BMO_ATTN_API int bmo_rms_norm(int n_rows, int dim, int type, const void *x, int64_t x_stride,
                               int residual_type, void *residual, int64_t residual_stride,
                               int weight_type, const void *weight, float eps, int out_type,
                               void *out, int64_t out_stride, void *codes, void *scales,
                               void *stream);
 
-/* Rows x [n_rows][cols] as 8-bit rows (cols a multiple of 32). */
+/* Rows x [n_rows][cols] as 8-bit rows (cols a multiple of 32; at most 2^33
+ * elements). */
 BMO_ATTN_API int bmo_quantize_rows(int n_rows, int cols, int type, const void *x, int64_t stride,
                                    void *codes, void *scales, void *stream);
 
@@ -682,7 +684,7 @@ BMO_ATTN_API const char *bmo_rope_last_error(const bmo_rope_t *rope);
  * tok_pos) into q_out and k_out, which may be q and k with their strides but
  * must not overlap them otherwise.  Cosines and sines are the exact ones
  * rounded to fp32, each product and sum is rounded to fp32, the result to the
- * type. */
+ * type.  At most 2^32 elements. */
 BMO_ATTN_API int bmo_rope_apply(bmo_rope_t *rope, int n_tok, const int *positions, int type,
                                 int n_heads, const void *q, int64_t q_stride, void *q_out,
                                 int64_t q_out_stride, int n_kv_heads, const void *k,

@@ -146,6 +146,22 @@ def test_extreme_codes_and_scales(gpu, n):
     assert np.isnan(got[n // 2]).all() and np.isnan(got[:, 7]).all()
 
 
+@pytest.mark.parametrize("n", [1, 5, 100])
+@pytest.mark.parametrize("cols", [32, 96, 160])
+def test_an_infinite_scale_in_the_last_block(gpu, n, cols):
+    """What lies past the last block adds nothing, whatever that block's scale."""
+    torch = gpu
+    wc = np.full((40, cols // 32, 32), 9, np.uint8)
+    w = _weights(torch, blocks_of(wc, np.full((40, cols // 32), -2.0, np.float16)))
+    scales = np.ones((n, cols // 32), np.float16)
+    scales[n // 2, -1] = np.inf
+    out = torch.empty(n, 40, device="cuda")
+    w.product(torch.ones(n, cols, dtype=torch.int8, device="cuda"), torch.from_numpy(scales).cuda(), out,
+              stream=torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    assert (out[n // 2] == -np.inf).all() and torch.isfinite(torch.cat((out[:n // 2], out[n // 2 + 1:]))).all()
+
+
 @pytest.mark.parametrize("activation", ["silu", "gelu"])
 @pytest.mark.parametrize("n,hidden,cols", [c[:3] for c in GATED_SHAPES] + [
                                            (1, 32, 32), (1, 1056, 416), (7, 64, 256), (16, 96, 1024), (17, 512, 96), (33, 32, 640),

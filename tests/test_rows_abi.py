@@ -21,7 +21,7 @@ def _norm(**k):
 
 @pytest.mark.parametrize("args,rc,why", [
     (dict(x=None), 1, "null"), (dict(w=None), 1, "null"), (dict(out=None), 1, "null"), (dict(codes=A), 2, "together"),
-    (dict(n=-1), 2, "n_rows"), (dict(dim=0), 2, "dim"), (dict(dim=32769), 2, "dim"),
+    (dict(n=-1), 2, "n_rows"), (dict(n=1 << 22), 2, "n_rows"), (dict(dim=0), 2, "dim"), (dict(dim=32769), 2, "dim"),
     (dict(dim=48, codes=A, scales=A), 2, "multiple of 32"), (dict(eps=-1.0), 2, "eps"), (dict(eps=float("nan")), 2, "eps"),
     (dict(type=3), 2, "fp32"), (dict(wt=9), 2, "fp32"), (dict(ot=-1), 2, "fp32"), (dict(res=A, rt=4), 2, "fp32"),
     (dict(xs=63), 2, "shorter"), (dict(res=A, rs=1), 2, "shorter"), (dict(os=TOO_LONG), 2, "long"),
