@@ -18,13 +18,17 @@ struct ProductShape {
 // Few rows (16 x 16 matrix instructions) and many (32 x 32).  The times are
 // fitted to calls with weights from HBM, 2 to 3000 rows by 512 to 32001 outputs
 // of 1024 to 11264 columns (gated: 2048 rows by 512 to 5632 outputs of 1024 to
-// 8192), to 10 to 16% in the mean.  Against the fastest of 10 shapes (7 gated)
-// the choice costs 2.8% in the mean over the 126 (64) of them, 20% at worst (512
-// rows x 1000 outputs x 11264: 29.8 us, 25.6 with 32 rows x 64 outputs in 16 x
-// 16); one shape for all of few or many would cost up to 5 times as much.
+// 8192), and the product's moved by up to 15% to where they choose best.  Against
+// the fastest of 10 shapes (7 gated) the choice costs 1.6% in the mean over the
+// 126 calls, 15% at worst (48 rows x 4096 outputs x 5632: 10.7 us, 9.3 with 8
+// waves to 32 x 32); gated 1.2% over 64, 16% at worst.  What a shape is worth:
+// 16 x 16 at 2 x 512 x 4096 3.5 us, 16 x 32 there 5.8; 16 x 64 at 64 x 4096 x
+// 4096 8.1, 32 x 32 there 9.2; 128 x 128 at 2048 x 12288 x 4096 267, 64 x 128
+// there 303.
 constexpr ProductShape kProductShapes[] = {
-    {16, 16, 8, 2.30, 0.45, 0.66},  {16, 32, 8, 2.83, 0.85, 0.89},   {32, 32, 4, 3.75, 0.63, 0.57},
-    {32, 64, 4, 4.59, 1.11, 0.99},  {64, 128, 1, 7.19, 1.04, 0.80},  {128, 128, 1, 10.29, 1.83, 1.40},
+    {16, 16, 8, 2.34, 0.54, 0.77}, {16, 32, 8, 3.02, 0.93, 1.00},  {16, 64, 8, 3.00, 0.69, 1.49},
+    {32, 32, 4, 4.17, 0.75, 0.55}, {32, 64, 4, 4.26, 1.31, 0.95},  {64, 128, 1, 6.47, 1.03, 0.74},
+    {128, 128, 1, 9.82, 1.84, 1.19},
 };
 constexpr ProductShape kGatedShapes[] = {
     {16, 32, 8, 3.62, 1.49, 1.67},

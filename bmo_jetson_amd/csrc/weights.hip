@@ -629,10 +629,11 @@ hipError_t launch_product(const ProductParams &p, hipStream_t stream) {
     switch (product_shape(false, p.n_rows, p.g.rows, p.g.chunks)) {
     case 0: return run_few<0, 2, false>(p, stream);
     case 1: return run_few<1, 1, false>(p, stream);
-    case 2: return run_many<2, 1, 1, 2, 1, false>(p, stream);
-    case 3: return run_many<3, 1, 1, 1, 1, false>(p, stream);
-    case 4: return run_many<4, 2, 2, 2, 1, false>(p, stream);
-    default: return run_many<5, 2, 2, 2, 1, false>(p, stream);
+    case 2: return run_few<2, 1, false>(p, stream);
+    case 3: return run_many<3, 1, 1, 2, 1, false>(p, stream);
+    case 4: return run_many<4, 1, 1, 1, 1, false>(p, stream);
+    case 5: return run_many<5, 2, 2, 2, 1, false>(p, stream);
+    default: return run_many<6, 2, 2, 2, 1, false>(p, stream);
     }
 }
 

@@ -66,8 +66,9 @@ def test_types_and_larger_sizes(gpu, n, rows, cols, type_):
 
 
 # rows, outputs, columns and the kernel that takes them (workgroup's rows, outputs; waves of a piece)
-SHAPES = [(2, 97, 416, (16, 16, 8)), (37, 161, 1120, (16, 16, 8)), (37, 4097, 416, (16, 32, 8)), (69, 1001, 1120, (16, 32, 8)),
-          (197, 1001, 96, (32, 32, 4)), (261, 1001, 416, (32, 32, 4)), (131, 8193, 736, (32, 64, 4)),
+SHAPES = [(2, 97, 416, (16, 16, 8)), (37, 161, 1120, (16, 16, 8)), (37, 4097, 416, (16, 64, 8)), (69, 1001, 1120, (16, 32, 8)),
+          (17, 8161, 1248, (16, 64, 8)), (33, 2001, 1120, (16, 32, 8)), (325, 1057, 1120, (32, 32, 4)),
+          (197, 1001, 96, (16, 64, 8)), (261, 1001, 416, (32, 32, 4)), (131, 8193, 736, (32, 64, 4)),
           (197, 6001, 736, (32, 64, 4)), (901, 2049, 96, (64, 128, 1)), (901, 4097, 736, (64, 128, 1)),
           (515, 12001, 1120, (128, 128, 1)), (3001, 2049, 1120, (128, 128, 1))]
 GATED_SHAPES = [(2, 32, 96, (16, 32, 8)), (69, 160, 416, (16, 32, 8)), (131, 1024, 736, (32, 32, 8)),

@@ -2,7 +2,7 @@
 import test_gpu_weights
 from _shapes import product_shapes
 
-PRODUCT = {(16, 16, 8), (16, 32, 8), (32, 32, 4), (32, 64, 4), (64, 128, 1), (128, 128, 1)}
+PRODUCT = {(16, 16, 8), (16, 32, 8), (16, 64, 8), (32, 32, 4), (32, 64, 4), (64, 128, 1), (128, 128, 1)}
 GATED = {(16, 32, 8), (32, 32, 8), (32, 32, 4), (128, 64, 1)}
 
 
