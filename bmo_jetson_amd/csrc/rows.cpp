@@ -6,6 +6,7 @@
 
 #include <cmath>
 #include <cstdio>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -122,6 +123,38 @@ const char *rows8_fault(const void *codes, const void *scales) {
                                                     : "codes must be aligned to 16 bytes, scales to their elements";
 }
 
+// What a call reads or writes: n rows of `dense` bytes, `stride` bytes apart.
+struct Span {
+    const void *p;
+    int64_t n, dense, stride;
+    bool operator==(const Span &o) const { return p == o.p && dense == o.dense && (n == 1 || stride == o.stride); }
+};
+Span span(const void *p, int64_t n, int64_t elements, int64_t stride, int size) {
+    return {p, n, elements * size, stride * size};
+}
+Span span8(const void *codes, int64_t n, int64_t cols) { return {codes, 1, n * cols, 0}; }
+Span span_scales(const void *scales, int64_t n, int64_t cols) { return {scales, 1, n * (cols / 32) * 2, 0}; }
+
+// Whether two of them share bytes, as far as it can be told at once: rows that
+// lie apart may have others between them, so of those only the starts count.
+bool meet(const Span &a, const Span &b) {
+    if (!a.p || !b.p) return false;
+    if (a.p == b.p) return true;
+    if ((a.n > 1 && a.stride != a.dense) || (b.n > 1 && b.stride != b.dense)) return false;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return x < y ? y - x < (uintptr_t) (a.n * a.dense) : x - y < (uintptr_t) (b.n * b.dense);
+}
+// Whether anything written meets what else is written or read.
+bool overlap(std::initializer_list<Span> written, std::initializer_list<Span> read) {
+    for (const Span *w = written.begin(); w != written.end(); ++w) {
+        for (const Span *o = w + 1; o != written.end(); ++o)
+            if (meet(*w, *o)) return true;
+        for (const Span &r : read)
+            if (meet(*w, r)) return true;
+    }
+    return false;
+}
+
 // A create that failed: says why and returns nullptr.
 std::nullptr_t refused(std::string &error, const char *fn, const std::string &why) {
     error = std::string(fn) + ": " + why;
@@ -178,6 +211,10 @@ int product_call(bmo_weights_t *h, const char *fn, bool gated, int n_rows, const
         if (const char *why = rows8_fault(codes, scales)) return c.arg(why);
         if (const char *why = rows8_fault(out_codes, out_scales)) return c.arg(why);
         if (n_rows == 0) return c.done(hipSuccess);
+        if (overlap({span(out, n_rows, n_out, out_stride, bmo::type_bytes(type)), span8(out_codes, n_rows, n_out),
+                     span_scales(out_scales, n_rows, n_out)},
+                    {span8(codes, n_rows, h->g.cols), span_scales(scales, n_rows, h->g.cols)}))
+            return c.arg("what is written overlaps what is read, or something else that is written");
         c.enter();
         bmo::ProductParams p{};
         p.w = h->mem;
@@ -223,6 +260,15 @@ int bmo_rms_norm(int n_rows, int dim, int type, const void *x, int64_t x_stride,
         }
         if (const char *why = rows8_fault(codes, scales)) return c.arg(why);
         if (n_rows == 0) return c.done(hipSuccess);
+        const Span rows = span(x, n_rows, dim, x_stride, bmo::type_bytes(type));
+        const Span sums = span(residual, n_rows, dim, residual_stride, bmo::type_bytes(residual_type));
+        const Span result = span(out, n_rows, dim, out_stride, bmo::type_bytes(out_type));
+        const Span w = span(weight, 1, dim, dim, bmo::type_bytes(weight_type));
+        const bool in_place = result == rows && out_type == type, doubled = sums == rows && residual_type == type;
+        if (overlap({sums, result, span8(codes, n_rows, dim), span_scales(scales, n_rows, dim)}, {w}) ||
+            overlap({span8(codes, n_rows, dim), span_scales(scales, n_rows, dim)}, {rows}) ||
+            (!in_place && meet(result, rows)) || (!doubled && meet(sums, rows)))
+            return c.arg("what is written overlaps what is read, or something else that is written");
         bmo::NormParams p{};
         p.n_rows = n_rows;
         p.dim = dim;
@@ -255,6 +301,9 @@ int bmo_quantize_rows(int n_rows, int cols, int type, const void *x, int64_t str
         if (const char *why = row_fault(x, stride, cols, type)) return c.arg(why);
         if (const char *why = rows8_fault(codes, scales)) return c.arg(why);
         if (n_rows == 0) return c.done(hipSuccess);
+        if (overlap({span8(codes, n_rows, cols), span_scales(scales, n_rows, cols)},
+                    {span(x, n_rows, cols, stride, bmo::type_bytes(type))}))
+            return c.arg("what is written overlaps what is read, or something else that is written");
         bmo::QuantizeParams p{};
         p.n_rows = n_rows;
         p.cols = cols;
@@ -341,6 +390,14 @@ int bmo_rope_apply(bmo_rope_t *h, int n_tok, const int *positions, int type, int
         if ((q == q_out && q_stride != q_out_stride) || (n_kv_heads && k == k_out && k_stride != k_out_stride))
             return c.arg("rows turned in place keep their stride");
         if (n_tok == 0) return c.done(hipSuccess);
+        const int size = bmo::type_bytes(type);
+        const Span qs = span(q, n_tok, q_dense, q_stride, size), qo = span(q_out, n_tok, q_dense, q_out_stride, size);
+        const Span none = {nullptr, 0, 0, 0};
+        const Span ks = n_kv_heads ? span(k, n_tok, k_dense, k_stride, size) : none;
+        const Span ko = n_kv_heads ? span(k_out, n_tok, k_dense, k_out_stride, size) : none;
+        if (overlap({qo, ko}, {{positions, 1, (int64_t) n_tok * 4, 0}}) || meet(qo, ks) || meet(ko, qs) ||
+            (q != q_out && meet(qo, qs)) || (k != k_out && meet(ko, ks)))
+            return c.arg("what is written overlaps what is read, or something else that is written");
         c.enter();
         bmo::RopeParams p{};
         p.rates = h->rates;

@@ -630,8 +630,11 @@ BMO_ATTN_API int bmo_kv_pages_attend_granted(bmo_kv_pages_t *pages, int layer, i
  * block of zeros has d = 0.  One that holds a NaN, an infinity or a magnitude
  * past 127 * 65504 has d = NaN: what is computed from it is NaN.
  *
- * Calls allocate nothing and can be captured.  Calls without a handle run on
- * the current device.
+ * What a call writes must not overlap what it reads or something else that it
+ * writes, other than where it says so; what can be told from addresses is
+ * refused.  Calls keep nothing between them: they may run at once, also on one
+ * handle.  They allocate nothing and can be captured.  Calls without a handle
+ * run on the current device.
  */
 
 /* Message of this thread's last failed call of bmo_rms_norm or
@@ -643,9 +646,9 @@ BMO_ATTN_API const char *bmo_rows_last_error(void);
  *       NULL: h = x; the norm is that of the stored values)
  *   y = h / sqrt(mean(h^2) + eps) * weight
  * y goes to out, to 8-bit rows (dim a multiple of 32), or to both; what is
- * NULL is not written.  out may be x with the same type and stride.  fp32
- * inside; the squares of a row have to sum below fp32's range.  n_rows below
- * 2^22. */
+ * NULL is not written.  out may be x, and x the residual (h = 2 x), with the
+ * same type and stride.  fp32 inside; the squares of a row have to sum below
+ * fp32's range.  n_rows below 2^22. */
 BMO_ATTN_API int bmo_rms_norm(int n_rows, int dim, int type, const void *x, int64_t x_stride,
                               int residual_type, void *residual, int64_t residual_stride,
                               int weight_type, const void *weight, float eps, int out_type,
@@ -710,7 +713,8 @@ BMO_ATTN_API int bmo_weights_load(bmo_weights_t *weights, int row, int n_rows, c
 /* out [n_rows][rows] = 8-bit rows [n_rows][cols] times the matrix:
  *   out[m][n] = sum over blocks of d4 * d8 * sum((code - 8) * q),
  * a block's sum an exact integer, blocks added in fp32; the order, and with it
- * the rounding, depends on the sizes alone.  n_rows at most 2^20. */
+ * the rounding, depends on the sizes alone.  A scale that is NaN or infinite
+ * makes NaN of the outputs that it takes part in.  n_rows at most 2^20. */
 BMO_ATTN_API int bmo_weights_product(bmo_weights_t *weights, int n_rows, const void *codes,
                                      const void *scales, int type, void *out, int64_t out_stride,
                                      void *stream);

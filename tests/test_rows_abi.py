@@ -33,6 +33,27 @@ def test_norm_refuses(args, rc, why):
     assert err.startswith("bmo_rms_norm:") and why in err
 
 
+# (2 rows of 64: 512 bytes of fp32, 128 of codes, 8 of scales)
+B, C, D = A + 4096, A + 8192, A + 12288
+
+
+@pytest.mark.parametrize("args", [
+    dict(x=A, out=A + 256, w=B), dict(x=A, out=A, ot=1, w=B), dict(x=A, out=A, xs=128, w=B), dict(x=A, out=B, w=B + 508),
+    dict(x=A, res=B, out=B, w=C), dict(x=A, res=A + 4, out=B, w=C), dict(x=A, res=A, rt=1, out=B, w=C),
+    dict(x=A, res=B, out=C, w=B + 4), dict(x=A, out=None, codes=A + 496, scales=B, w=C),
+    dict(x=A, out=None, codes=B, scales=A + 510, w=C), dict(x=A, out=C, codes=B, scales=B + 126, w=D),
+    dict(x=A, out=B, codes=B + 496, scales=C, w=D)])
+def test_norm_refuses_overlaps(args):
+    assert _norm(**args) == 2
+    assert "overlaps" in bmo.lib().bmo_rows_last_error().decode()
+
+
+@pytest.mark.parametrize("x,codes,scales", [(A, A, B), (A, A + 496, B), (A, B, A + 510), (A, B, B + 126), (A + 64, A, B)])
+def test_quantize_refuses_overlaps(x, codes, scales):
+    assert bmo.lib().bmo_quantize_rows(2, 64, 0, x, 0, codes, scales, None) == 2
+    assert "overlaps" in bmo.lib().bmo_rows_last_error().decode()
+
+
 @pytest.mark.parametrize("args,rc,why", [
     ((2, 64, 0, None, 0, A, A), 1, "null"), ((2, 64, 0, A, 0, None, A), 1, "null"), ((2, 64, 0, A, 0, A, None), 1, "null"),
     ((-1, 64, 0, A, 0, A, A), 2, "n_rows"), ((2, 48, 0, A, 0, A, A), 2, "multiple"), ((2, 0, 0, A, 0, A, A), 2, "multiple"),
