@@ -10,7 +10,13 @@
 // float, are that plus the sum, exactly (sums stay below 2^20), and one fma
 // with d8 takes the offset out again: -1.5 * 2^23 * d8 is exact for an fp16
 // d8.  A second one adds d4 times that, so an output is off by the roundings
-// of an fp32 sum of its blocks' parts only.
+// of an fp32 sum of its blocks' parts only.  (Converting the integer takes as
+// long as seven fmas.)
+//
+// Few rows are bound by reading the weights once, many by those two fmas: a
+// 32 x 32 tile of a block takes 32 of them a lane and 10 other vector
+// instructions beside the one matrix instruction, about 4 clocks each with the
+// matrix cores in turn.
 #include "kernels.hpp"
 #include "product_shape.hpp"
 #include "rows_device.hpp"
@@ -75,7 +81,9 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // a run of their units each.  Lane (g, i) multiplies block g of a unit's four of
 // output i, for which the four octets change places between lanes: eight dot
 // products that begin with the float's bits, as the matrix instructions do.  The
-// row lies in LDS, its scales in fp32.
+// row lies in LDS, its scales in fp32.  Bound by the weights' bytes and the
+// launch: 12288 x 4096 in 6.6 us, 4.3 TB/s (a large copy: 5.1), with the matrix
+// cores 8.1; gated 2 x 5632 x 4096 8.0 against 9.5.
 constexpr int kOneRowChunks = 256;  // of a row in LDS, 144 bytes each
 
 // Dword t of lanes 16 g .. to dword g of lanes 16 t ..: from octet g of four
@@ -201,7 +209,11 @@ constexpr int kRowStride = 144;  // of 128 codes in LDS: 16 rows' octets lie in 
 // waves a run of the tiles' units each; their sums are joined in LDS, wave after
 // wave.  The 8-bit rows are the rows of the result here: a lane has one output
 // of four rows, with the output's scales its own and the rows' read from LDS,
-// where the wave puts them.  PF units are under way at once.
+// where the wave puts them.  PF units are under way at once (2 of the narrowest
+// shape: its waves wait for loads; of the others, whose registers they cost
+// waves, 1: 64 x 4096 x 4096 8.1 against 8.4 us, gated 17 x 5632 x 4096 15.6
+// against 17.8).  Bound by a load, its use and the joining in turn: 64 x 4096 x
+// 4096 takes 8.1 us, where the bytes alone take 2 and a launch 1.6.
 template <int MT, int NT, int KW, int PF, bool GATED>
 __global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p) {
     static_assert(!GATED || NT == 4, "two tiles of gates and the two that they let through");
@@ -379,6 +391,13 @@ hipError_t run_few(const ProductParams &p, hipStream_t stream) {
 // unit ahead: eight lanes read a row's 128 codes, which costs the loads a
 // quarter of what reading them as the matrix cores take them does.  D units'
 // weights and DX units' codes are under way at once.
+//
+// 2048 x 12288 x 4096 takes 262 us, 785 TFLOP/s.  In a copy that skips work the
+// vector and matrix instructions alone take 205, the accesses to LDS 25 and the
+// loads from memory 40 more.  With the next tile's matrix instruction put ahead
+// of a tile's fmas it takes 258 to 272: the two waves of a SIMD issue more than
+// half of the time as it is.  Three or four waves a SIMD, in 168 or 128
+// registers, need narrower pieces: 287 and 292.
 
 // Two units' codes of 16 outputs each to a 32-column operand: lanes 16 to 31
 // and 48 to 63 of the first change places with lanes 0 to 15 and 32 to 47 of

@@ -72,7 +72,7 @@ def _run(torch, dim, rot, interleaved, type_, n=5, heads=3, kv=2, pos=None, seed
 
 @pytest.mark.parametrize("type_", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("interleaved", [True, False])
-@pytest.mark.parametrize("dim,rot", [(128, 128), (128, 64), (64, 64), (96, 24), (80, 40), (256, 64), (6, 4), (2, 2),
+@pytest.mark.parametrize("dim,rot", [(128, 128), (128, 64), (64, 64), (96, 24), (80, 40), (80, 20), (96, 48), (20, 12), (256, 64), (6, 4), (2, 2),
                                      (128, 2), (130, 126), (1024, 1024)])
 def test_layouts_sizes_types(gpu, dim, rot, interleaved, type_):
     _run(gpu, dim, rot, interleaved, type_)
