@@ -635,8 +635,13 @@ hipError_t run_many(const ProductParams &p, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_product(const ProductParams &p, hipStream_t stream) {
-    if (p.n_rows == 1 && p.g.chunks <= kOneRowChunks)
-        return p.activation ? run_one<4, 8, 1, true>(p, stream) : run_one<1, 8, 2, false>(p, stream);
+    if (p.n_rows == 1 && p.g.chunks <= kOneRowChunks) {
+        if (p.activation) return run_one<4, 8, 1, true>(p, stream);
+        // Rows past 4096 columns with no more tiles than CUs: 16 waves to a tile (4096 x
+        // 5632 4.8 against 5.2 us, 4096 x 11264 6.8 against 7.8, 2048 x 8192 4.8 against
+        // 5.5; else 8: 12288 x 4096 6.7 against 8.2, 5120 x 5120 5.5 against 5.7).
+        return p.g.tiles <= 256 && p.g.chunks > 32 ? run_one<1, 16, 2, false>(p, stream) : run_one<1, 8, 2, false>(p, stream);
+    }
     if (p.activation) {
         switch (product_shape(true, p.n_rows, p.g.rows / 2, p.g.chunks)) {
         case 0: return run_few<0, 1, true>(p, stream);
