@@ -383,21 +383,22 @@ hipError_t run_few(const ProductParams &p, hipStream_t stream) {
                            dim3(64 * S.waves), args, 0, stream);
 }
 
-// Many rows: a wave takes MT * 32 rows and NT tiles of 32 outputs (of a gated
-// product one of gates and the one that they let through), a workgroup WM * WN
-// such pieces, each shared by KW waves, which take every KW-th unit of it and
+// Many rows: a workgroup takes MT * 32 rows, a wave NT tiles of 32 outputs (of a
+// gated product one of gates and the one that they let through), WN such pieces
+// to a workgroup, each shared by KW waves, which take every KW-th unit of it and
 // join their sums in LDS.  As with few rows a lane has one output, here of 16
 // rows, whose scales are read from LDS.  The rows' codes and scales go there a
 // unit ahead: eight lanes read a row's 128 codes, which costs the loads a
 // quarter of what reading them as the matrix cores take them does.  D units'
 // weights and DX units' codes are under way at once.
 //
-// 2048 x 12288 x 4096 takes 262 us, 785 TFLOP/s.  In a copy that skips work the
-// vector and matrix instructions alone take 205, the accesses to LDS 25 and the
-// loads from memory 40 more.  With the next tile's matrix instruction put ahead
-// of a tile's fmas it takes 258 to 272: the two waves of a SIMD issue more than
-// half of the time as it is.  Three or four waves a SIMD, in 168 or 128
-// registers, need narrower pieces: 287 and 292.
+// 2048 x 12288 x 4096 takes 257 us, 800 TFLOP/s (64 x 256 outputs a workgroup).
+// In a copy of 128 x 128 (265) that skips work the vector and matrix
+// instructions alone take 205, the accesses to LDS 25 and the loads from memory
+// 40 more.  With the next tile's matrix instruction put ahead of a tile's fmas
+// that took 258 to 272: the two waves of a SIMD issue more than half of the time
+// as it is.  Three or four waves a SIMD, in 168 or 128 registers, need narrower
+// pieces: 287 and 292.
 
 // Two units' codes of 16 outputs each to a 32-column operand: lanes 16 to 31
 // and 48 to 63 of the first change places with lanes 0 to 15 and 32 to 47 of
@@ -416,14 +417,14 @@ __device__ __forceinline__ void pair_units(wt_uint4 &a, wt_uint4 &b) {
     b = wt_uint4{b0, b1, b2, b3};
 }
 
-template <int MT, int NT, int WM, int WN, int KW, int D, int DX, bool GATED>
-__global__ __launch_bounds__(64 * WM * WN * KW, 2) void many_rows_kernel(ProductParams p, int n_pieces) {
+template <int MT, int NT, int WN, int KW, int D, int DX, bool GATED>
+__global__ __launch_bounds__(64 * WN * KW, 2) void many_rows_kernel(ProductParams p, int n_pieces) {
     static_assert(!GATED || NT == 2, "a tile of gates and the one that they let through");
     static_assert(D % DX == 0, "a slot of codes belongs to one of units");
-    constexpr int WAVES = WM * WN * KW, ROWS = 32 * MT * WM, XL = 4 * MT / WN;  // rows of a workgroup; loads of a lane
-    constexpr bool ALONE = WM * WN == 1;  // a wave reads only what it puts into LDS itself
+    constexpr int WAVES = WN * KW, ROWS = 32 * MT, XL = 4 * MT / WN;  // rows of a workgroup; loads of a lane
+    constexpr bool ALONE = WN == 1;  // a wave reads only what it puts into LDS itself
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kw = wave % KW, wn = wave / KW % WN, wm = wave / KW / WN;
+    const int kw = wave % KW, wn = wave / KW;
     const int l32 = lane & 31, h = lane >> 5;
     const int piece = (int) blockIdx.x * WN + wn;
     const int nb = p.g.cols / 32, last = p.g.chunks - 1;
@@ -436,11 +437,11 @@ __global__ __launch_bounds__(64 * WM * WN * KW, 2) void many_rows_kernel(Product
         w[n] = p.w + (int64_t) min(2 * tile, p.g.tiles - 2) * tile_bytes;
     }
     const uint32_t scales_at = ((lane >> 4) & 1) * tile_bytes + kUnitScales + (lane & 15) * 8;
-    // (the rows' offsets from the workgroup's first fit 32 bits: 127 * 2^24)
+    // (the rows' offsets from the workgroup's first fit 32 bits: 63 * 2^24)
     const int first = (int) blockIdx.y * ROWS;
     const int8_t *codes = p.codes + (int64_t) first * p.g.cols;
     const uint16_t *scales = p.scales + (int64_t) first * nb;
-    const int x_row = wave / KW * (8 * XL) + (lane >> 3), piece16 = lane & 7;
+    const int x_row = wn * (8 * XL) + (lane >> 3), piece16 = lane & 7;
     uint32_t x_at[XL], d_at[XL];
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
@@ -528,7 +529,7 @@ __global__ __launch_bounds__(64 * WM * WN * KW, 2) void many_rows_kernel(Product
                 wt_int4 xv[2];
                 rw_float4 d8[2][4];
                 auto read_rows = [&](int e) {  // e: rows e % MT, block e / MT
-                    const int t = e / MT, m = wm * MT + e % MT;
+                    const int t = e / MT, m = e % MT;
                     xv[e & 1] = s_x[kw][at][32 * m + l32][(2 * t + h) ^ (l32 & 7)];
                     const rw_float4 *src = reinterpret_cast<const rw_float4 *>(s_d8[kw][at][m][t][h]);
 #pragma unroll
@@ -596,7 +597,7 @@ __global__ __launch_bounds__(64 * WM * WN * KW, 2) void many_rows_kernel(Product
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const int64_t row = (int64_t) first + (wm * MT + m) * 32 + 8 * (r >> 2) + 4 * h + (r & 3);
+            const int64_t row = (int64_t) first + m * 32 + 8 * (r >> 2) + 4 * h + (r & 3);
             if (KW > 1 && r % KW != kw) continue;
             if constexpr (GATED) {
                 const int n_out = p.g.rows / 2, col = piece * 32 + l32;
@@ -619,17 +620,17 @@ __global__ __launch_bounds__(64 * WM * WN * KW, 2) void many_rows_kernel(Product
         }
 }
 
-template <int SHAPE, int WM, int WN, int D, int DX, bool GATED>
+template <int SHAPE, int WN, int D, int DX, bool GATED>
 hipError_t run_many(const ProductParams &p, hipStream_t stream) {
     constexpr ProductShape S = GATED ? kGatedShapes[SHAPE] : kProductShapes[SHAPE];
-    constexpr int MT = S.rows / (32 * WM), NT = GATED ? 2 : S.outs / (32 * WN), PIECE = GATED ? 32 : 32 * NT;
-    static_assert(S.outs == PIECE * WN && S.rows == 32 * MT * WM, "the shape's sizes");
+    constexpr int MT = S.rows / 32, NT = GATED ? 2 : S.outs / (32 * WN), PIECE = GATED ? 32 : 32 * NT;
+    static_assert(S.outs == PIECE * WN && S.rows == 32 * MT, "the shape's sizes");
     ProductParams q = p;
     int pieces = ((GATED ? p.g.rows / 2 : p.g.rows) + PIECE - 1) / PIECE;
     void *args[] = {&q, &pieces};
-    return hipLaunchKernel(reinterpret_cast<const void *>(many_rows_kernel<MT, NT, WM, WN, S.waves, D, DX, GATED>),
+    return hipLaunchKernel(reinterpret_cast<const void *>(many_rows_kernel<MT, NT, WN, S.waves, D, DX, GATED>),
                            dim3((unsigned) ((pieces + WN - 1) / WN), (unsigned) ((p.n_rows + S.rows - 1) / S.rows)),
-                           dim3(64 * WM * WN * S.waves), args, 0, stream);
+                           dim3(64 * WN * S.waves), args, 0, stream);
 }
 
 }  // namespace
@@ -645,19 +646,22 @@ hipError_t launch_product(const ProductParams &p, hipStream_t stream) {
     if (p.activation) {
         switch (product_shape(true, p.n_rows, p.g.rows / 2, p.g.chunks)) {
         case 0: return run_few<0, 1, true>(p, stream);
-        case 1: return run_few<1, 1, true>(p, stream);
-        case 2: return run_many<2, 1, 1, 1, 1, true>(p, stream);
-        default: return run_many<3, 2, 2, 1, 1, true>(p, stream);
+        case 1: return run_many<1, 1, 1, 1, true>(p, stream);
+        case 2: return run_many<2, 1, 1, 1, true>(p, stream);
+        case 3: return run_many<3, 2, 2, 1, true>(p, stream);
+        case 4: return run_many<4, 2, 2, 1, true>(p, stream);
+        default: return run_many<5, 4, 1, 1, true>(p, stream);
         }
     }
     switch (product_shape(false, p.n_rows, p.g.rows, p.g.chunks)) {
     case 0: return run_few<0, 2, false>(p, stream);
     case 1: return run_few<1, 1, false>(p, stream);
     case 2: return run_few<2, 1, false>(p, stream);
-    case 3: return run_many<3, 1, 1, 2, 1, false>(p, stream);
-    case 4: return run_many<4, 1, 1, 1, 1, false>(p, stream);
-    case 5: return run_many<5, 2, 2, 2, 1, false>(p, stream);
-    default: return run_many<6, 2, 2, 2, 1, false>(p, stream);
+    case 3: return run_many<3, 1, 2, 1, false>(p, stream);
+    case 4: return run_many<4, 1, 1, 1, false>(p, stream);
+    case 5: return run_many<5, 2, 2, 1, false>(p, stream);
+    case 6: return run_many<6, 2, 2, 1, false>(p, stream);
+    default: return run_many<7, 4, 1, 1, false>(p, stream);
     }
 }
 

@@ -2,8 +2,9 @@
 import test_gpu_weights
 from _shapes import product_shapes
 
-PRODUCT = {(16, 16, 8), (16, 32, 8), (16, 64, 8), (32, 32, 4), (32, 64, 4), (64, 128, 1), (128, 128, 1)}
-GATED = {(16, 32, 8), (32, 32, 8), (32, 32, 4), (128, 64, 1)}
+PRODUCT = {(16, 16, 8), (16, 32, 8), (16, 64, 8), (32, 32, 4), (32, 64, 4), (32, 128, 2), (64, 128, 2),
+           (64, 256, 1)}
+GATED = {(16, 32, 8), (32, 32, 8), (32, 32, 4), (32, 64, 2), (64, 64, 2), (64, 128, 1)}
 
 
 def test_the_gpu_tests_meet_every_kernel():
@@ -22,5 +23,5 @@ def test_launches_stay_within_their_limits():
 
 
 def test_few_rows_take_small_pieces_and_many_large_ones():
-    assert product_shapes([(False, 2, 4096, 4096), (False, 4096, 12288, 4096)]) == [(16, 16, 8), (128, 128, 1)]
-    assert product_shapes([(True, 2, 5632, 4096), (True, 4096, 5632, 4096)]) == [(16, 32, 8), (128, 64, 1)]
+    assert product_shapes([(False, 2, 4096, 4096), (False, 4096, 12288, 4096)]) == [(16, 16, 8), (64, 256, 1)]
+    assert product_shapes([(True, 2, 5632, 4096), (True, 4096, 5632, 4096)]) == [(16, 32, 8), (64, 128, 1)]
