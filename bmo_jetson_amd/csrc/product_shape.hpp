@@ -19,22 +19,21 @@ struct ProductShape {
 // Few rows (16 x 16 matrix instructions) and many (32 x 32).  The times are
 // fitted to calls with weights from HBM, 2 to 3000 rows by 512 to 32001 outputs
 // of 640 to 11264 columns (gated: 2048 rows by 512 to 11264 outputs of 640 to
-// 8192), and moved by up to 15% to where they choose best.  Against the fastest
-// of 13 shapes (8 gated) the choice costs 1.6% in the mean over the 162 calls, 18%
-// at worst (32 rows x 11264 outputs x 640: 6.4 us, 5.4 with 32 x 32); gated 0.4%
-// over 80, 9% at worst.  What a shape is worth: 16 x 16 at 2 x 512 x 4096 3.5 us,
-// 16 x 32 there 5.8; 16 x 64 at 64 x 4096 x 4096 8.1, 32 x 32 there 9.2; 64 x 128
-// with two waves to a piece at 1500 x 11264 x 4096 203, 64 x 256 there 223, at 2048
-// x 12288 x 4096 274 and 257.  Both read a unit's weights once for 64 rows; 128 x
-// 128 takes 226 and 265, for its workgroups fill fewer last rounds.
+// 8192), and moved by up to 15% to where they choose best: against the fastest
+// shape 0.7% in the mean over the 162 calls, 16% at worst (32 rows x 32001 outputs
+// x 1024: 11.2 us, 9.7 with 32 x 64); gated 0.2% over 80, 8% at worst.  What a
+// shape is worth: 16 x 16 at 2 x 512 x 4096 3.5 us, 16 x 32 there 5.7; 16 x 64 at 64 x
+// 4096 x 4096 8.1, 32 x 32 there 9.0; 32 x 32 with eight waves at 48 x 4096 x 5632 9.1,
+// with four 11.1; 64 x 128 with two waves to a piece at 1500 x 12288 x 4096 201, 64 x
+// 256 there 213, at 2048 x 12288 x 4096 267 and 250.
 constexpr ProductShape kProductShapes[] = {
-    {16, 16, 8, 1, 2.45, 0.76, 0},    {16, 32, 8, 1, 2.96, 1.05, 0},    {16, 64, 8, 1, 2.61, 1.58, 0},
-    {32, 32, 4, 3, 3.30, 0.80, 0.62}, {32, 64, 4, 2, 4.41, 1.21, 0.99}, {32, 128, 2, 2, 4.20, 1.13, 0.93},
-    {64, 128, 2, 2, 7.01, 1.81, 1.47}, {64, 256, 1, 2, 9.10, 2.05, 1.18},
+    {16, 16, 8, 1, 2.50, 0.81, 0},     {16, 32, 8, 1, 3.15, 1.00, 0},    {16, 64, 8, 1, 2.90, 1.74, 0},
+    {32, 32, 4, 2, 3.68, 0.75, 0.59},  {32, 32, 8, 1, 3.88, 1.32, 0},    {32, 64, 4, 2, 3.96, 1.25, 1.11},
+    {32, 128, 2, 2, 4.75, 1.30, 1.01}, {64, 128, 2, 2, 6.95, 1.98, 1.29}, {64, 256, 1, 2, 9.38, 1.66, 1.12},
 };
 constexpr ProductShape kGatedShapes[] = {
-    {16, 32, 8, 1, 4.23, 1.76, 0},    {32, 32, 8, 1, 5.18, 2.28, 0},     {32, 32, 4, 2, 4.33, 1.42, 1.04},
-    {32, 64, 2, 2, 4.90, 1.35, 0.94}, {64, 64, 2, 2, 11.23, 1.72, 1.40}, {64, 128, 1, 2, 15.59, 1.69, 1.23},
+    {16, 32, 8, 1, 3.84, 1.72, 0},    {32, 32, 8, 1, 5.06, 2.10, 0},     {32, 32, 4, 2, 4.59, 1.31, 0.94},
+    {32, 64, 2, 2, 4.71, 1.34, 0.92}, {64, 64, 2, 2, 10.18, 2.07, 1.43}, {64, 128, 1, 2, 13.18, 1.52, 1.38},
 };
 constexpr int kProductKinds = sizeof(kProductShapes) / sizeof(ProductShape);
 constexpr int kGatedKinds = sizeof(kGatedShapes) / sizeof(ProductShape);

@@ -390,15 +390,18 @@ hipError_t run_few(const ProductParams &p, hipStream_t stream) {
 // rows, whose scales are read from LDS.  The rows' codes and scales go there a
 // unit ahead: eight lanes read a row's 128 codes, which costs the loads a
 // quarter of what reading them as the matrix cores take them does.  D units'
-// weights and DX units' codes are under way at once.
+// weights and DX units' codes are under way at once.  AHEAD: a tile's matrix
+// instruction stands before the fmas of the tile before it, which takes the
+// registers of a second unit (64 x 128, D 1 against D 2 without: 1000 x 4096 x 5632
+// 66 against 71 us, 48 x 4096 x 5632 48.0 against 49.6; gated 1000 x 5632 x 4096 140
+// against 144; 64 x 256 plain 250 against 248 at 2048 x 12288 x 4096, narrower ones
+// the same either way).
 //
-// 2048 x 12288 x 4096 takes 257 us, 800 TFLOP/s (64 x 256 outputs a workgroup).
+// 2048 x 12288 x 4096 takes 249 us, 828 TFLOP/s (64 x 256 outputs a workgroup).
 // In a copy of 128 x 128 (265) that skips work the vector and matrix
 // instructions alone take 205, the accesses to LDS 25 and the loads from memory
-// 40 more.  With the next tile's matrix instruction put ahead of a tile's fmas
-// that took 258 to 272: the two waves of a SIMD issue more than half of the time
-// as it is.  Three or four waves a SIMD, in 168 or 128 registers, need narrower
-// pieces: 287 and 292.
+// 40 more: the two waves of a SIMD issue more than half of the time.  Three or
+// four waves a SIMD, in 168 or 128 registers, need narrower pieces: 287 and 292.
 
 // Two units' codes of 16 outputs each to a 32-column operand: lanes 16 to 31
 // and 48 to 63 of the first change places with lanes 0 to 15 and 32 to 47 of
@@ -417,7 +420,7 @@ __device__ __forceinline__ void pair_units(wt_uint4 &a, wt_uint4 &b) {
     b = wt_uint4{b0, b1, b2, b3};
 }
 
-template <int MT, int NT, int WN, int KW, int D, int DX, bool GATED>
+template <int MT, int NT, int WN, int KW, int D, int DX, bool AHEAD, bool GATED>
 __global__ __launch_bounds__(64 * WN * KW, 2) void many_rows_kernel(ProductParams p, int n_pieces) {
     static_assert(!GATED || NT == 2, "a tile of gates and the one that they let through");
     static_assert(D % DX == 0, "a slot of codes belongs to one of units");
@@ -526,43 +529,52 @@ __global__ __launch_bounds__(64 * WN * KW, 2) void many_rows_kernel(ProductParam
                 for (int n = 0; n < NT; ++n) pair_units(q[j][n][0], q[j][n][1]);
                 // What a block of rows needs of LDS is read while the one before
                 // it is multiplied.
-                wt_int4 xv[2];
+                constexpr int TILES = 4 * MT * NT;  // of a unit: block e / MT, rows e % MT, outputs n
+                wt_int4 xv[2], wv[NT];
                 rw_float4 d8[2][4];
-                auto read_rows = [&](int e) {  // e: rows e % MT, block e / MT
+                float ds[2][NT], off[2][NT];
+                wt_float16 f[2];
+                auto read_rows = [&](int e) {
                     const int t = e / MT, m = e % MT;
                     xv[e & 1] = s_x[kw][at][32 * m + l32][(2 * t + h) ^ (l32 & 7)];
                     const rw_float4 *src = reinterpret_cast<const rw_float4 *>(s_d8[kw][at][m][t][h]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) d8[e & 1][i] = src[i];
                 };
-                read_rows(0);
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    wt_int4 wv[NT];
-                    float ds[NT], off[NT];
+                auto unpack = [&](int t) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         const uint32_t a = q[j][n][0][t], b = q[j][n][1][t];
                         wv[n] = wt_int4{(int) (a << 4 & 0xF0F0F0F0u), (int) (a & 0xF0F0F0F0u), (int) (b << 4 & 0xF0F0F0F0u),
                                         (int) (b & 0xF0F0F0F0u)};
-                        ds[n] = t & 1 ? half_hi(d4[j][n][t >> 1]) : half_lo(d4[j][n][t >> 1]);
-                        asm volatile("" : "+v"(ds[n]));  // (in fp32: an fma that widens an operand takes twice the time)
-                        off[n] = -kMagic * ds[n];
+                        float &d = ds[t & 1][n];
+                        d = t & 1 ? half_hi(d4[j][n][t >> 1]) : half_lo(d4[j][n][t >> 1]);
+                        asm volatile("" : "+v"(d));  // (in fp32: an fma that widens an operand takes twice the time)
+                        off[t & 1][n] = -kMagic * d;
                     }
+                };
+                auto multiply = [&](int i) {
+                    const int e = i / NT;
+                    if (i % (NT * MT) == 0) unpack(e / MT);
+                    f[i & 1] = __builtin_bit_cast(
+                        wt_float16, __builtin_amdgcn_mfma_i32_32x32x32_i8(xv[e & 1], wv[i % NT], magic, 0, 0, 0));
+                };
+                read_rows(0);
+                if (AHEAD) multiply(0);
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        const int e = t * MT + m;
-                        if (e + 1 < 4 * MT) read_rows(e + 1);
+                for (int i = 0; i < TILES; ++i) {
+                    const int e = i / NT, t = e / MT, m = e % MT, n = i % NT;
+                    if (n == 0 && e + 1 < 4 * MT) read_rows(e + 1);
+                    if (!AHEAD)
+                        multiply(i);
+                    else if (i + 1 < TILES)
+                        multiply(i + 1);
+                    if (AHEAD) __builtin_amdgcn_sched_barrier(0);  // (else the compiler moves it down to its fmas)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            const wt_float16 f = __builtin_bit_cast(
-                                wt_float16, __builtin_amdgcn_mfma_i32_32x32x32_i8(xv[e & 1], wv[n], magic, 0, 0, 0));
-#pragma unroll
-                            for (int r = 0; r < 16; ++r)
-                                acc[n][m][r] =
-                                    __builtin_fmaf(d8[e & 1][r >> 2][r & 3], __builtin_fmaf(f[r], ds[n], off[n]), acc[n][m][r]);
-                        }
-                    }
+                    for (int r = 0; r < 16; ++r)
+                        acc[n][m][r] = __builtin_fmaf(d8[e & 1][r >> 2][r & 3],
+                                                      __builtin_fmaf(f[i & 1][r], ds[t & 1][n], off[t & 1][n]), acc[n][m][r]);
+                    if (AHEAD) __builtin_amdgcn_sched_barrier(0);
                 }
             }
             load_units(j, unit_of(step + D));
@@ -620,7 +632,7 @@ __global__ __launch_bounds__(64 * WN * KW, 2) void many_rows_kernel(ProductParam
         }
 }
 
-template <int SHAPE, int WN, int D, int DX, bool GATED>
+template <int SHAPE, int WN, int D, int DX, bool AHEAD, bool GATED>
 hipError_t run_many(const ProductParams &p, hipStream_t stream) {
     constexpr ProductShape S = GATED ? kGatedShapes[SHAPE] : kProductShapes[SHAPE];
     constexpr int MT = S.rows / 32, NT = GATED ? 2 : S.outs / (32 * WN), PIECE = GATED ? 32 : 32 * NT;
@@ -628,7 +640,7 @@ hipError_t run_many(const ProductParams &p, hipStream_t stream) {
     ProductParams q = p;
     int pieces = ((GATED ? p.g.rows / 2 : p.g.rows) + PIECE - 1) / PIECE;
     void *args[] = {&q, &pieces};
-    return hipLaunchKernel(reinterpret_cast<const void *>(many_rows_kernel<MT, NT, WN, S.waves, D, DX, GATED>),
+    return hipLaunchKernel(reinterpret_cast<const void *>(many_rows_kernel<MT, NT, WN, S.waves, D, DX, AHEAD, GATED>),
                            dim3((unsigned) ((pieces + WN - 1) / WN), (unsigned) ((p.n_rows + S.rows - 1) / S.rows)),
                            dim3(64 * WN * S.waves), args, 0, stream);
 }
@@ -646,22 +658,23 @@ hipError_t launch_product(const ProductParams &p, hipStream_t stream) {
     if (p.activation) {
         switch (product_shape(true, p.n_rows, p.g.rows / 2, p.g.chunks)) {
         case 0: return run_few<0, 1, true>(p, stream);
-        case 1: return run_many<1, 1, 1, 1, true>(p, stream);
-        case 2: return run_many<2, 1, 1, 1, true>(p, stream);
-        case 3: return run_many<3, 2, 2, 1, true>(p, stream);
-        case 4: return run_many<4, 2, 2, 1, true>(p, stream);
-        default: return run_many<5, 4, 1, 1, true>(p, stream);
+        case 1: return run_many<1, 1, 1, 1, false, true>(p, stream);
+        case 2: return run_many<2, 1, 1, 1, false, true>(p, stream);
+        case 3: return run_many<3, 2, 2, 1, false, true>(p, stream);
+        case 4: return run_many<4, 2, 1, 1, true, true>(p, stream);
+        default: return run_many<5, 4, 1, 1, true, true>(p, stream);
         }
     }
     switch (product_shape(false, p.n_rows, p.g.rows, p.g.chunks)) {
     case 0: return run_few<0, 2, false>(p, stream);
     case 1: return run_few<1, 1, false>(p, stream);
     case 2: return run_few<2, 1, false>(p, stream);
-    case 3: return run_many<3, 1, 2, 1, false>(p, stream);
-    case 4: return run_many<4, 1, 1, 1, false>(p, stream);
-    case 5: return run_many<5, 2, 2, 1, false>(p, stream);
-    case 6: return run_many<6, 2, 2, 1, false>(p, stream);
-    default: return run_many<7, 4, 1, 1, false>(p, stream);
+    case 3: return run_many<3, 1, 2, 1, false, false>(p, stream);
+    case 4: return run_many<4, 1, 2, 1, false, false>(p, stream);
+    case 5: return run_many<5, 1, 1, 1, false, false>(p, stream);
+    case 6: return run_many<6, 2, 2, 1, false, false>(p, stream);
+    case 7: return run_many<7, 2, 1, 1, true, false>(p, stream);
+    default: return run_many<8, 4, 2, 1, false, false>(p, stream);
     }
 }
 

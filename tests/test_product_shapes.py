@@ -2,8 +2,8 @@
 import test_gpu_weights
 from _shapes import product_shapes
 
-PRODUCT = {(16, 16, 8), (16, 32, 8), (16, 64, 8), (32, 32, 4), (32, 64, 4), (32, 128, 2), (64, 128, 2),
-           (64, 256, 1)}
+PRODUCT = {(16, 16, 8), (16, 32, 8), (16, 64, 8), (32, 32, 4), (32, 32, 8), (32, 64, 4), (32, 128, 2),
+           (64, 128, 2), (64, 256, 1)}
 GATED = {(16, 32, 8), (32, 32, 8), (32, 32, 4), (32, 64, 2), (64, 64, 2), (64, 128, 1)}
 
 
