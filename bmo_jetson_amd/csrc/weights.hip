@@ -204,7 +204,7 @@ hipError_t run_one(const ProductParams &p, hipStream_t stream) {
 
 constexpr int kRowStride = 144;  // of 128 codes in LDS: 16 rows' octets lie in different banks
 
-// Few rows: a workgroup takes 16 * MT rows and NT tiles of 16 outputs (of a
+// Few rows: a workgroup takes 16 rows and NT tiles of 16 outputs (of a
 // gated product two tiles of gates and the two that they let through), its KW
 // waves a run of the tiles' units each; their sums are joined in LDS, wave after
 // wave.  The 8-bit rows are the rows of the result here: a lane has one output
@@ -214,12 +214,12 @@ constexpr int kRowStride = 144;  // of 128 codes in LDS: 16 rows' octets lie in 
 // waves, 1: 64 x 4096 x 4096 8.1 against 8.4 us, gated 17 x 5632 x 4096 15.6
 // against 17.8).  Bound by a load, its use and the joining in turn: 64 x 4096 x
 // 4096 takes 8.1 us, where the bytes alone take 2 and a launch 1.6.
-template <int MT, int NT, int KW, int PF, bool GATED>
+template <int NT, int KW, int PF, bool GATED>
 __global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p) {
     static_assert(!GATED || NT == 4, "two tiles of gates and the two that they let through");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i16 = lane & 15, g = lane >> 4;
-    const int m0 = blockIdx.y * 16 * MT;
+    const int m0 = blockIdx.y * 16;
     const int nb = p.g.cols / 32, last = p.g.chunks - 1;
     const int per = (p.g.chunks + KW - 1) / KW, c0 = wave * per, c1 = min(c0 + per, p.g.chunks);
     const uint8_t *w[NT];
@@ -229,22 +229,18 @@ __global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p) {
         tile = min(tile, p.g.tiles - 1);
         w[n] = p.w + (int64_t) tile * p.g.chunks * kUnitBytes;
     }
-    // The rows' offsets from the workgroup's first fit 32 bits: 63 * 2^24.  (A
+    // The rows' offsets from the workgroup's first fit 32 bits: 15 * 2^24.  (A
     // unit's 128 codes of a row are read by eight lanes, and go through LDS to
     // the lanes that multiply them.)
     const int8_t *codes = p.codes + (int64_t) m0 * p.g.cols;
     const uint16_t *scales = p.scales + (int64_t) m0 * nb;
-    uint32_t x_at[MT][2], d_at[MT];
+    uint32_t x_at[2];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            x_at[m][i] = (uint32_t) min(16 * m + 8 * i + (lane >> 3), p.n_rows - 1 - m0) * (uint32_t) p.g.cols;
-        d_at[m] = (uint32_t) min(16 * m + i16, p.n_rows - 1 - m0) * (uint32_t) nb;
-    }
-    wt_uint4 q[PF][NT], x[PF][MT][2];
+    for (int i = 0; i < 2; ++i) x_at[i] = (uint32_t) min(8 * i + (lane >> 3), p.n_rows - 1 - m0) * (uint32_t) p.g.cols;
+    const uint32_t d_at = (uint32_t) min(i16, p.n_rows - 1 - m0) * (uint32_t) nb;
+    wt_uint4 q[PF][NT], x[PF][2];
     wt_uint2 d4[PF][NT];
-    uint32_t d8[PF][MT];
+    uint32_t d8[PF];
     auto load = [&](int j, int c) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -255,20 +251,15 @@ __global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p) {
         // (past the last block weights are zeros)
         const uint32_t e = (uint32_t) min(c * kUnitCols + (lane & 7) * 16, p.g.cols - 16), b = (uint32_t) min(4 * c + g, nb - 1);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) x[j][m][i] = *reinterpret_cast<const wt_uint4 *>(codes + (x_at[m][i] + e));
-            d8[j][m] = scales[d_at[m] + b];
-        }
+        for (int i = 0; i < 2; ++i) x[j][i] = *reinterpret_cast<const wt_uint4 *>(codes + (x_at[i] + e));
+        d8[j] = scales[d_at + b];
     };
-    __shared__ rw_float4 s_acc[KW][MT][NT][64];
-    __shared__ float s_d8[KW][MT][4][16];
-    __shared__ uint8_t s_x[KW][MT][16][kRowStride];
-    rw_float4 acc[MT][NT];
+    __shared__ rw_float4 s_acc[KW][NT][64];
+    __shared__ float s_d8[KW][4][16];
+    __shared__ uint8_t s_x[KW][16][kRowStride];
+    rw_float4 acc[NT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[m][n] = rw_float4{0, 0, 0, 0};
+    for (int n = 0; n < NT; ++n) acc[n] = rw_float4{0, 0, 0, 0};
     const wt_int4 magic = {kMagicBits, kMagicBits, kMagicBits, kMagicBits};
 #pragma unroll
     for (int j = 0; j < PF; ++j) load(j, min(c0 + j, last));
@@ -277,13 +268,10 @@ __global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p) {
         for (int j = 0; j < PF; ++j) {
             if (c + j >= c1) break;
             __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses stay in order)
+            s_d8[wave][g][i16] = 4 * (c + j) + g < nb ? half_lo(d8[j]) : 0.0f;  // (past the last block nothing)
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                s_d8[wave][m][g][i16] = 4 * (c + j) + g < nb ? half_lo(d8[j][m]) : 0.0f;  // (past the last block nothing)
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    *reinterpret_cast<wt_uint4 *>(&s_x[wave][m][8 * i + (lane >> 3)][(lane & 7) * 16]) = x[j][m][i];
-            }
+            for (int i = 0; i < 2; ++i)
+                *reinterpret_cast<wt_uint4 *>(&s_x[wave][8 * i + (lane >> 3)][(lane & 7) * 16]) = x[j][i];
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -297,76 +285,64 @@ __global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p) {
                     asm volatile("" : "+v"(ds[n]));  // (in fp32: an fma that widens an operand takes twice the time)
                     off[n] = -kMagic * ds[n];
                 }
+                const rw_float4 dr = *reinterpret_cast<const rw_float4 *>(&s_d8[wave][t][4 * g]);
+                const long xv = *reinterpret_cast<const long *>(&s_x[wave][i16][t * 32 + g * 8]);
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const rw_float4 dr = *reinterpret_cast<const rw_float4 *>(&s_d8[wave][m][t][4 * g]);
-                    const long xv = *reinterpret_cast<const long *>(&s_x[wave][m][i16][t * 32 + g * 8]);
+                for (int n = 0; n < NT; ++n) {
+                    const rw_float4 f =
+                        __builtin_bit_cast(rw_float4, __builtin_amdgcn_mfma_i32_16x16x32_i8(xv, wv[n], magic, 0, 0, 0));
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const rw_float4 f = __builtin_bit_cast(
-                            rw_float4, __builtin_amdgcn_mfma_i32_16x16x32_i8(xv, wv[n], magic, 0, 0, 0));
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const float part = __builtin_fmaf(f[r], ds[n], off[n]);
-                            acc[m][n][r] = __builtin_fmaf(dr[r], part, acc[m][n][r]);
-                        }
-                    }
+                    for (int r = 0; r < 4; ++r) acc[n][r] = __builtin_fmaf(dr[r], __builtin_fmaf(f[r], ds[n], off[n]), acc[n][r]);
                 }
             }
             if (c + j + PF < c1) load(j, c + j + PF);
         }
     }
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) s_acc[wave][m][n][lane] = acc[m][n];
+    for (int n = 0; n < NT; ++n) s_acc[wave][n][lane] = acc[n];
     __syncthreads();
-    auto joined = [&](int m, int n) {
-        rw_float4 v = s_acc[0][m][n][lane];
+    auto joined = [&](int n) {
+        rw_float4 v = s_acc[0][n][lane];
 #pragma unroll
-        for (int k = 1; k < KW; ++k) v += s_acc[k][m][n][lane];
+        for (int k = 1; k < KW; ++k) v += s_acc[k][n][lane];
         return v * kCodeStep;
     };
+    const int64_t row0 = m0 + 4 * g;
     if constexpr (GATED) {
+        if (wave != 0) return;
         const int n_out = p.g.rows / 2, n0 = (int) blockIdx.x * 32 + i16;
-        for (int m = wave; m < MT; m += KW) {
-            const int64_t row0 = m0 + 16 * m + 4 * g;
-            float h[2][4];
+        float h[2][4];
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const rw_float4 a = joined(m, n), b = joined(m, n + 2);
+        for (int n = 0; n < 2; ++n) {
+            const rw_float4 a = joined(n), b = joined(n + 2);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) h[n][r] = gate(a[r], b[r], p.activation);
+            for (int r = 0; r < 4; ++r) h[n][r] = gate(a[r], b[r], p.activation);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int64_t row = row0 + r;
+            if (p.out && row < p.n_rows) {
+                store1(p.out, row * p.out_stride + n0, h[0][r], p.type);
+                store1(p.out, row * p.out_stride + n0 + 16, h[1][r], p.type);
             }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int64_t row = row0 + r;
-                if (p.out && row < p.n_rows) {
-                    store1(p.out, row * p.out_stride + n0, h[0][r], p.type);
-                    store1(p.out, row * p.out_stride + n0 + 16, h[1][r], p.type);
-                }
-                if (p.out_codes) {
-                    const Scale8 s =
-                        scale_of(row16_max(__builtin_elementwise_maximum(__builtin_fabsf(h[0][r]), __builtin_fabsf(h[1][r]))));
-                    if (row < p.n_rows) {
-                        p.out_codes[row * n_out + n0] = (int8_t) code1(h[0][r], s.inv);
-                        p.out_codes[row * n_out + n0 + 16] = (int8_t) code1(h[1][r], s.inv);
-                        if (i16 == 0) p.out_scales[row * (n_out / 32) + blockIdx.x] = (uint16_t) s.bits;
-                    }
+            if (p.out_codes) {
+                const Scale8 s =
+                    scale_of(row16_max(__builtin_elementwise_maximum(__builtin_fabsf(h[0][r]), __builtin_fabsf(h[1][r]))));
+                if (row < p.n_rows) {
+                    p.out_codes[row * n_out + n0] = (int8_t) code1(h[0][r], s.inv);
+                    p.out_codes[row * n_out + n0 + 16] = (int8_t) code1(h[1][r], s.inv);
+                    if (i16 == 0) p.out_scales[row * (n_out / 32) + blockIdx.x] = (uint16_t) s.bits;
                 }
             }
         }
     } else {
-        for (int i = wave; i < MT * NT; i += KW) {
-            const int m = i / NT, n = i % NT, col = ((int) blockIdx.x * NT + n) * 16 + i16;
-            const int64_t row0 = m0 + 16 * m + 4 * g;
-            const rw_float4 v = joined(m, n);
-            if (col < p.g.rows) {
+        static_assert(NT <= KW, "a wave joins one tile at most");
+        const int n = wave, col = ((int) blockIdx.x * NT + n) * 16 + i16;
+        if (n >= NT || col >= p.g.rows) return;
+        const rw_float4 v = joined(n);
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (row0 + r < p.n_rows) store1(p.out, (row0 + r) * p.out_stride + col, v[r], p.type);
-            }
-        }
+        for (int r = 0; r < 4; ++r)
+            if (row0 + r < p.n_rows) store1(p.out, (row0 + r) * p.out_stride + col, v[r], p.type);
     }
 }
 
@@ -374,11 +350,12 @@ __global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p) {
 template <int SHAPE, int PF, bool GATED>
 hipError_t run_few(const ProductParams &p, hipStream_t stream) {
     constexpr ProductShape S = GATED ? kGatedShapes[SHAPE] : kProductShapes[SHAPE];
-    constexpr int MT = S.rows / 16, NT = GATED ? 4 : S.outs / 16;
+    constexpr int NT = GATED ? 4 : S.outs / 16;
+    static_assert(S.rows == 16, "the shape's rows");
     ProductParams q = p;
     void *args[] = {&q};
     const int outs = GATED ? p.g.rows / 2 : p.g.rows;
-    return hipLaunchKernel(reinterpret_cast<const void *>(few_rows_kernel<MT, NT, S.waves, PF, GATED>),
+    return hipLaunchKernel(reinterpret_cast<const void *>(few_rows_kernel<NT, S.waves, PF, GATED>),
                            dim3((unsigned) ((outs + S.outs - 1) / S.outs), (unsigned) ((p.n_rows + S.rows - 1) / S.rows)),
                            dim3(64 * S.waves), args, 0, stream);
 }
@@ -390,7 +367,7 @@ hipError_t run_few(const ProductParams &p, hipStream_t stream) {
 // rows, whose scales are read from LDS.  The rows' codes and scales go there a
 // unit ahead: eight lanes read a row's 128 codes, which costs the loads a
 // quarter of what reading them as the matrix cores take them does.  D units'
-// weights and DX units' codes are under way at once.  AHEAD: a tile's matrix
+// weights are under way at once.  AHEAD: a tile's matrix
 // instruction stands before the fmas of the tile before it, which takes the
 // registers of a second unit (64 x 128, D 1 against D 2 without: 1000 x 4096 x 5632
 // 66 against 71 us, 48 x 4096 x 5632 48.0 against 49.6; gated 1000 x 5632 x 4096 140
@@ -420,10 +397,9 @@ __device__ __forceinline__ void pair_units(wt_uint4 &a, wt_uint4 &b) {
     b = wt_uint4{b0, b1, b2, b3};
 }
 
-template <int MT, int NT, int WN, int KW, int D, int DX, bool AHEAD, bool GATED>
+template <int MT, int NT, int WN, int KW, int D, bool AHEAD, bool GATED>
 __global__ __launch_bounds__(64 * WN * KW, 2) void many_rows_kernel(ProductParams p, int n_pieces) {
     static_assert(!GATED || NT == 2, "a tile of gates and the one that they let through");
-    static_assert(D % DX == 0, "a slot of codes belongs to one of units");
     constexpr int WAVES = WN * KW, ROWS = 32 * MT, XL = 4 * MT / WN;  // rows of a workgroup; loads of a lane
     constexpr bool ALONE = WN == 1;  // a wave reads only what it puts into LDS itself
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -457,26 +433,26 @@ __global__ __launch_bounds__(64 * WN * KW, 2) void many_rows_kernel(ProductParam
     // scales lie together.
     __shared__ wt_int4 s_x[KW][ALONE ? 1 : 2][ROWS][8];
     __shared__ float s_d8[KW][ALONE ? 1 : 2][ROWS / 32][4][2][16];
-    wt_int4 xr[DX][XL];
-    uint32_t dr[DX][XL];
-    auto load_x = [&](int j, int c) {  // (past the last block weights are zeros)
+    wt_int4 xr[XL];
+    uint32_t dr[XL];
+    auto load_x = [&](int c) {  // (past the last block weights are zeros)
         const uint32_t e = (uint32_t) min(c * kUnitCols + piece16 * 16, p.g.cols - 16);
         const uint32_t b = (uint32_t) min(4 * c + (lane & 3), nb - 1);
 #pragma unroll
         for (int i = 0; i < XL; ++i) {
-            xr[j][i] = *reinterpret_cast<const wt_int4 *>(codes + (x_at[i] + e));
-            dr[j][i] = scales[d_at[i] + b];
+            xr[i] = *reinterpret_cast<const wt_int4 *>(codes + (x_at[i] + e));
+            dr[i] = scales[d_at[i] + b];
         }
     };
-    auto put_x = [&](int j, int buffer, int c) {
+    auto put_x = [&](int buffer, int c) {
         const bool real = 4 * c + (lane & 3) < nb;  // (past the last block nothing)
 #pragma unroll
         for (int i = 0; i < XL; ++i) {
             const int row = x_row + 8 * i;
-            s_x[kw][buffer][row][piece16 ^ (x_row & 7)] = xr[j][i];
+            s_x[kw][buffer][row][piece16 ^ (x_row & 7)] = xr[i];
             // (lanes 4 apart write the same)
             s_d8[kw][buffer][row >> 5][lane & 3][(row >> 2) & 1][((row >> 3) & 3) * 4 + (row & 3)] =
-                real ? half_lo(dr[j][i]) : 0.0f;
+                real ? half_lo(dr[i]) : 0.0f;
         }
     };
     wt_float16 acc[NT][MT];
@@ -503,27 +479,25 @@ __global__ __launch_bounds__(64 * WN * KW, 2) void many_rows_kernel(ProductParam
         }
     };
     // Step s takes unit s * KW + kw.  Its weights lie in slot s % D, read after
-    // step s - D's were used; its rows' codes in slot s % DX, read once those
-    // of step s - DX are in LDS.
+    // step s - D's were used; its rows' codes are read once those of the step
+    // before are in LDS.
     const int steps = (last + KW) / KW;
     auto unit_of = [&](int step) { return min(step * KW + kw, last); };
+    load_x(unit_of(0));
 #pragma unroll
-    for (int j = 0; j < D; ++j) {
-        if (j < DX) load_x(j, unit_of(j));
-        load_units(j, unit_of(j));
-    }
+    for (int j = 0; j < D; ++j) load_units(j, unit_of(j));
     for (int step0 = 0; step0 < steps; step0 += D) {
 #pragma unroll
         for (int j = 0; j < D; ++j) {
-            const int step = step0 + j, at = ALONE ? 0 : step & 1, jx = j % DX;
+            const int step = step0 + j, at = ALONE ? 0 : step & 1;
             if (step >= steps || (ALONE && step * KW + kw > last)) break;
             if (ALONE) __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses stay in order)
-            put_x(jx, at, unit_of(step));
+            put_x(at, unit_of(step));
             if (ALONE)
                 __builtin_amdgcn_wave_barrier();
             else
                 lds_barrier();
-            load_x(jx, unit_of(step + DX));
+            load_x(unit_of(step + 1));
             if (ALONE || KW == 1 || step * KW + kw <= last) {  // (else a unit that another wave has)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) pair_units(q[j][n][0], q[j][n][1]);
@@ -632,7 +606,7 @@ __global__ __launch_bounds__(64 * WN * KW, 2) void many_rows_kernel(ProductParam
         }
 }
 
-template <int SHAPE, int WN, int D, int DX, bool AHEAD, bool GATED>
+template <int SHAPE, int WN, int D, bool AHEAD, bool GATED>
 hipError_t run_many(const ProductParams &p, hipStream_t stream) {
     constexpr ProductShape S = GATED ? kGatedShapes[SHAPE] : kProductShapes[SHAPE];
     constexpr int MT = S.rows / 32, NT = GATED ? 2 : S.outs / (32 * WN), PIECE = GATED ? 32 : 32 * NT;
@@ -640,7 +614,7 @@ hipError_t run_many(const ProductParams &p, hipStream_t stream) {
     ProductParams q = p;
     int pieces = ((GATED ? p.g.rows / 2 : p.g.rows) + PIECE - 1) / PIECE;
     void *args[] = {&q, &pieces};
-    return hipLaunchKernel(reinterpret_cast<const void *>(many_rows_kernel<MT, NT, WN, S.waves, D, DX, AHEAD, GATED>),
+    return hipLaunchKernel(reinterpret_cast<const void *>(many_rows_kernel<MT, NT, WN, S.waves, D, AHEAD, GATED>),
                            dim3((unsigned) ((pieces + WN - 1) / WN), (unsigned) ((p.n_rows + S.rows - 1) / S.rows)),
                            dim3(64 * WN * S.waves), args, 0, stream);
 }
@@ -658,23 +632,23 @@ hipError_t launch_product(const ProductParams &p, hipStream_t stream) {
     if (p.activation) {
         switch (product_shape(true, p.n_rows, p.g.rows / 2, p.g.chunks)) {
         case 0: return run_few<0, 1, true>(p, stream);
-        case 1: return run_many<1, 1, 1, 1, false, true>(p, stream);
-        case 2: return run_many<2, 1, 1, 1, false, true>(p, stream);
-        case 3: return run_many<3, 2, 2, 1, false, true>(p, stream);
-        case 4: return run_many<4, 2, 1, 1, true, true>(p, stream);
-        default: return run_many<5, 4, 1, 1, true, true>(p, stream);
+        case 1: return run_many<1, 1, 1, false, true>(p, stream);
+        case 2: return run_many<2, 1, 1, false, true>(p, stream);
+        case 3: return run_many<3, 2, 2, false, true>(p, stream);
+        case 4: return run_many<4, 2, 1, true, true>(p, stream);
+        default: return run_many<5, 4, 1, true, true>(p, stream);
         }
     }
     switch (product_shape(false, p.n_rows, p.g.rows, p.g.chunks)) {
     case 0: return run_few<0, 2, false>(p, stream);
     case 1: return run_few<1, 1, false>(p, stream);
     case 2: return run_few<2, 1, false>(p, stream);
-    case 3: return run_many<3, 1, 2, 1, false, false>(p, stream);
-    case 4: return run_many<4, 1, 2, 1, false, false>(p, stream);
-    case 5: return run_many<5, 1, 1, 1, false, false>(p, stream);
-    case 6: return run_many<6, 2, 2, 1, false, false>(p, stream);
-    case 7: return run_many<7, 2, 1, 1, true, false>(p, stream);
-    default: return run_many<8, 4, 2, 1, false, false>(p, stream);
+    case 3: return run_many<3, 1, 2, false, false>(p, stream);
+    case 4: return run_many<4, 1, 2, false, false>(p, stream);
+    case 5: return run_many<5, 1, 1, false, false>(p, stream);
+    case 6: return run_many<6, 2, 2, false, false>(p, stream);
+    case 7: return run_many<7, 2, 1, true, false>(p, stream);
+    default: return run_many<8, 4, 2, false, false>(p, stream);
     }
 }
 
