@@ -66,4 +66,27 @@ constexpr int product_shape(bool gated, int64_t rows, int64_t outs, int64_t chun
     return best;
 }
 
+// Where a workgroup works.  Workgroups go round the 8 XCDs one by one, x first,
+// and each XCD has an L2 of its own: where the columns of workgroups (x: the
+// outputs) are no multiple of 8 those of a column land on all of them, and each
+// reads its weights.  So an XCD takes whole columns, row after row (y), and what
+// rests of the columns is shared by rows (1984 rows x 12544 outputs x 4096, 49
+// columns: 249 us, 267 as they come).  div_main and div_rest divide by columns / 8
+// and columns % 8.
+struct Place {
+    uint32_t x, y;
+};
+template <class F, class G>
+constexpr Place product_place(uint32_t x, uint32_t y, uint32_t columns, uint32_t rows, F div_main, G div_rest) {
+    const uint32_t main = columns / 8, rest = columns % 8;
+    if (rest == 0 || main == 0 || rows == 1) return {x, y};
+    const uint32_t id = y * columns + x, turn = id / 8;
+    if (turn < main * rows) {
+        const uint32_t row = div_main(turn);
+        return {id % 8 + 8 * (turn - row * main), row};
+    }
+    const uint32_t left = id - 8 * main * rows, row = div_rest(left);
+    return {8 * main + left - row * rest, row};
+}
+
 }  // namespace bmo

@@ -75,6 +75,18 @@ __device__ __forceinline__ float gate(float g, float u, int activation) {
 // A barrier that waits for LDS alone, not for loads under way.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// The two divisions that place a workgroup.
+struct Places {
+    FastDiv main, rest;
+};
+Places make_places(unsigned columns) {
+    return {make_fastdiv(columns / 8 ? columns / 8 : 1), make_fastdiv(columns % 8 ? columns % 8 : 1)};
+}
+__device__ __forceinline__ Place place(const Places &d) {
+    return product_place(blockIdx.x, blockIdx.y, gridDim.x, gridDim.y, [&](uint32_t n) { return d.main.div(n); },
+                         [&](uint32_t n) { return d.rest.div(n); });
+}
+
 // One row: vector units alone, which spend half the instructions on it that the
 // matrix cores' sixteen rows take.  A workgroup takes NT tiles of 16 outputs (of
 // a gated product two of gates and the two that they let through), its KW waves
@@ -215,17 +227,18 @@ constexpr int kRowStride = 144;  // of 128 codes in LDS: 16 rows' octets lie in 
 // against 17.8).  Bound by a load, its use and the joining in turn: 64 x 4096 x
 // 4096 takes 8.1 us, where the bytes alone take 2 and a launch 1.6.
 template <int NT, int KW, int PF, bool GATED>
-__global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p) {
+__global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p, Places places) {
     static_assert(!GATED || NT == 4, "two tiles of gates and the two that they let through");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i16 = lane & 15, g = lane >> 4;
-    const int m0 = blockIdx.y * 16;
+    const Place at = place(places);
+    const int m0 = (int) at.y * 16;
     const int nb = p.g.cols / 32, last = p.g.chunks - 1;
     const int per = (p.g.chunks + KW - 1) / KW, c0 = wave * per, c1 = min(c0 + per, p.g.chunks);
     const uint8_t *w[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        int tile = GATED ? (int) blockIdx.x * 2 + (n & 1) + (n & 2 ? p.g.tiles / 2 : 0) : (int) blockIdx.x * NT + n;
+        int tile = GATED ? (int) at.x * 2 + (n & 1) + (n & 2 ? p.g.tiles / 2 : 0) : (int) at.x * NT + n;
         tile = min(tile, p.g.tiles - 1);
         w[n] = p.w + (int64_t) tile * p.g.chunks * kUnitBytes;
     }
@@ -310,7 +323,7 @@ __global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p) {
     const int64_t row0 = m0 + 4 * g;
     if constexpr (GATED) {
         if (wave != 0) return;
-        const int n_out = p.g.rows / 2, n0 = (int) blockIdx.x * 32 + i16;
+        const int n_out = p.g.rows / 2, n0 = (int) at.x * 32 + i16;
         float h[2][4];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
@@ -331,13 +344,13 @@ __global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p) {
                 if (row < p.n_rows) {
                     p.out_codes[row * n_out + n0] = (int8_t) code1(h[0][r], s.inv);
                     p.out_codes[row * n_out + n0 + 16] = (int8_t) code1(h[1][r], s.inv);
-                    if (i16 == 0) p.out_scales[row * (n_out / 32) + blockIdx.x] = (uint16_t) s.bits;
+                    if (i16 == 0) p.out_scales[row * (n_out / 32) + at.x] = (uint16_t) s.bits;
                 }
             }
         }
     } else {
         static_assert(NT <= KW, "a wave joins one tile at most");
-        const int n = wave, col = ((int) blockIdx.x * NT + n) * 16 + i16;
+        const int n = wave, col = ((int) at.x * NT + n) * 16 + i16;
         if (n >= NT || col >= p.g.rows) return;
         const rw_float4 v = joined(n);
 #pragma unroll
@@ -353,10 +366,11 @@ hipError_t run_few(const ProductParams &p, hipStream_t stream) {
     constexpr int NT = GATED ? 4 : S.outs / 16;
     static_assert(S.rows == 16, "the shape's rows");
     ProductParams q = p;
-    void *args[] = {&q};
-    const int outs = GATED ? p.g.rows / 2 : p.g.rows;
+    const unsigned columns = (unsigned) (((GATED ? p.g.rows / 2 : p.g.rows) + S.outs - 1) / S.outs);
+    Places places = make_places(columns);
+    void *args[] = {&q, &places};
     return hipLaunchKernel(reinterpret_cast<const void *>(few_rows_kernel<NT, S.waves, PF, GATED>),
-                           dim3((unsigned) ((outs + S.outs - 1) / S.outs), (unsigned) ((p.n_rows + S.rows - 1) / S.rows)),
+                           dim3(columns, (unsigned) ((p.n_rows + S.rows - 1) / S.rows)),
                            dim3(64 * S.waves), args, 0, stream);
 }
 
@@ -398,14 +412,15 @@ __device__ __forceinline__ void pair_units(wt_uint4 &a, wt_uint4 &b) {
 }
 
 template <int MT, int NT, int WN, int KW, int D, bool AHEAD, bool GATED>
-__global__ __launch_bounds__(64 * WN * KW, 2) void many_rows_kernel(ProductParams p, int n_pieces) {
+__global__ __launch_bounds__(64 * WN * KW, 2) void many_rows_kernel(ProductParams p, int n_pieces, Places places) {
     static_assert(!GATED || NT == 2, "a tile of gates and the one that they let through");
     constexpr int WAVES = WN * KW, ROWS = 32 * MT, XL = 4 * MT / WN;  // rows of a workgroup; loads of a lane
     constexpr bool ALONE = WN == 1;  // a wave reads only what it puts into LDS itself
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kw = wave % KW, wn = wave / KW;
     const int l32 = lane & 31, h = lane >> 5;
-    const int piece = (int) blockIdx.x * WN + wn;
+    const Place group = place(places);
+    const int piece = (int) group.x * WN + wn;
     const int nb = p.g.cols / 32, last = p.g.chunks - 1;
     // (a tile past the last reads the last and stores nothing)
     const uint32_t tile_bytes = (uint32_t) p.g.chunks * (uint32_t) kUnitBytes;
@@ -417,7 +432,7 @@ __global__ __launch_bounds__(64 * WN * KW, 2) void many_rows_kernel(ProductParam
     }
     const uint32_t scales_at = ((lane >> 4) & 1) * tile_bytes + kUnitScales + (lane & 15) * 8;
     // (the rows' offsets from the workgroup's first fit 32 bits: 63 * 2^24)
-    const int first = (int) blockIdx.y * ROWS;
+    const int first = (int) group.y * ROWS;
     const int8_t *codes = p.codes + (int64_t) first * p.g.cols;
     const uint16_t *scales = p.scales + (int64_t) first * nb;
     const int x_row = wn * (8 * XL) + (lane >> 3), piece16 = lane & 7;
@@ -613,9 +628,11 @@ hipError_t run_many(const ProductParams &p, hipStream_t stream) {
     static_assert(S.outs == PIECE * WN && S.rows == 32 * MT, "the shape's sizes");
     ProductParams q = p;
     int pieces = ((GATED ? p.g.rows / 2 : p.g.rows) + PIECE - 1) / PIECE;
-    void *args[] = {&q, &pieces};
+    const unsigned columns = (unsigned) ((pieces + WN - 1) / WN);
+    Places places = make_places(columns);
+    void *args[] = {&q, &pieces, &places};
     return hipLaunchKernel(reinterpret_cast<const void *>(many_rows_kernel<MT, NT, WN, S.waves, D, AHEAD, GATED>),
-                           dim3((unsigned) ((pieces + WN - 1) / WN), (unsigned) ((p.n_rows + S.rows - 1) / S.rows)),
+                           dim3(columns, (unsigned) ((p.n_rows + S.rows - 1) / S.rows)),
                            dim3(64 * WN * S.waves), args, 0, stream);
 }
 

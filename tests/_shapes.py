@@ -7,10 +7,10 @@ import subprocess
 BUILD = os.path.join(os.path.dirname(os.path.abspath(__file__)), "build")
 
 
-def _ask(program, lines):
+def _ask(program, lines, *args):
     exe = os.path.join(BUILD, program)
     assert os.path.exists(exe), f"tests/build/{program} is not built (run __graft_entry__.build())"
-    res = subprocess.run([exe], input="".join(l + "\n" for l in lines), capture_output=True, text=True,
+    res = subprocess.run([exe, *args], input="".join(l + "\n" for l in lines), capture_output=True, text=True,
                          timeout=60, check=True)
     out = [tuple(map(int, line.split())) for line in res.stdout.splitlines()]
     assert len(out) == len(lines)
@@ -35,3 +35,9 @@ def product_shapes(calls):
     """(rows and outputs of a workgroup, waves of a piece) of each (gated, rows,
     outputs, columns)."""
     return _ask("product_shape_check", ["%d %d %d %d" % (bool(g), m, n, -(-k // 128)) for g, m, n, k in calls])
+
+
+def product_places(grids):
+    """(whether each place is taken once, columns that more than one XCD works
+    on) of each grid's (columns, rows)."""
+    return _ask("product_shape_check", ["%d %d" % g for g in grids], "places")

@@ -1,6 +1,6 @@
 """The rule that gives a product its kernel, on the host."""
 import test_gpu_weights
-from _shapes import product_shapes
+from _shapes import product_places, product_shapes
 
 PRODUCT = {(16, 16, 8), (16, 32, 8), (16, 64, 8), (32, 32, 4), (32, 32, 8), (32, 64, 4), (32, 128, 2),
            (64, 128, 2), (64, 256, 1)}
@@ -25,3 +25,11 @@ def test_launches_stay_within_their_limits():
 def test_few_rows_take_small_pieces_and_many_large_ones():
     assert product_shapes([(False, 2, 4096, 4096), (False, 4096, 12288, 4096)]) == [(16, 16, 8), (64, 256, 1)]
     assert product_shapes([(True, 2, 5632, 4096), (True, 4096, 5632, 4096)]) == [(16, 32, 8), (64, 128, 1)]
+
+
+def test_an_xcd_works_on_whole_columns():
+    """Every place once; columns that XCDs share only where they are no multiple of 8."""
+    grids = [(c, r) for c in (*range(1, 34), 49, 88, 126, 501) for r in (1, 2, 3, 7, 8, 9, 31, 64)]
+    for (c, r), (once, shared) in zip(grids, product_places(grids)):
+        assert once, (c, r)
+        assert shared <= (c if c < 8 else c % 8) or r == 1, (c, r, shared)
