@@ -70,11 +70,15 @@ struct Scale8 {
     float inv;  // 1 / scale, 0 for codes that are 0
 };
 __device__ __forceinline__ Scale8 scale_of(float amax) {
-    const float d = amax / 127.0f;
-    uint32_t h = f32_to_f16_bits(d);
-    if (f16_bits_to_f32(h) * 127.0f < amax) ++h;  // (18 bits, exact: also where the quotient was rounded, or is 0)
-    if (!(d <= 65504.0f)) return {0x7E00u, 0.0f};
-    return {h, h ? 1.0f / f16_bits_to_f32(h) : 0.0f};
+    // (rounded to fp16 that is the scale or the one before it: of a value that has
+    // moved by half a step of fp32 too)
+    uint32_t h = f32_to_f16_bits(amax * (1.0f / 127.0f));
+    if (f16_bits_to_f32(h) * 127.0f < amax) ++h;  // (18 bits, exact: also where the product was rounded, or is 0)
+    if (!(amax <= 127.0f * 65504.0f)) return {0x7E00u, 0.0f};
+    const float d = f16_bits_to_f32(h);
+    float r = __builtin_amdgcn_rcpf(d);
+    r = __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);  // (a scale is normal in fp32)
+    return {h, h ? r : 0.0f};
 }
 // The integer nearest to x * inv (codes of a block whose scale is NaN are 0
 // whatever it holds), and four as bytes.
@@ -104,10 +108,13 @@ __device__ __forceinline__ float row16_max(float v) {
     return __builtin_elementwise_maximum(v, pg_dpp<0x128>(v));      // row_ror:8
 }
 
-// The largest of a half's 32 lanes.
+// The largest of a half's 32 lanes.  (Rows 0 and 2 of one register change places
+// with rows 1 and 3 of the other.  Wait states: the compiler's hazard pass does
+// not see inside.)
 __device__ __forceinline__ float half_max(float v) {
-    v = row16_max(v);
-    return __builtin_elementwise_maximum(v, __shfl_xor(v, 16));
+    float a = row16_max(v), b = a;
+    asm volatile("s_nop 3\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 3" : "+v"(a), "+v"(b));
+    return __builtin_elementwise_maximum(a, b);
 }
 
 }  // namespace bmo

@@ -65,11 +65,16 @@ __device__ __forceinline__ float half_hi(uint32_t u) { return f16_bits_to_f32(u 
 
 __device__ __forceinline__ uint32_t dword(const uint4 &v, int t) { return t == 0 ? v.x : t == 1 ? v.y : t == 2 ? v.z : v.w; }
 
-// The activation of a gate times what it lets through.
+// The activation of a gate times what it lets through.  exp is the hardware's
+// 2^x (its argument off by a rounding: |a| e^-|a| of one in the result), the
+// quotient a product with the hardware's reciprocal, of a sixteenth of the
+// divisor so that it stays normal up to exp's overflow: five instructions for
+// some thirty of expf and a division (1000 x 5632 x 128 @A us, with them @B).
 __device__ __forceinline__ float gate(float g, float u, int activation) {
     // GELU by its tanh form: 0.5 (1 + tanh z) = 1 / (1 + exp(-2 z))
     const float a = activation == kSilu ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
-    return g / (1.0f + expf(-a)) * u;
+    const float e = __builtin_amdgcn_exp2f(a * -1.4426950408889634f);
+    return g * 0.0625f * __builtin_amdgcn_rcpf(__builtin_fmaf(e, 0.0625f, 0.0625f)) * u;
 }
 
 // A barrier that waits for LDS alone, not for loads under way.
@@ -593,32 +598,75 @@ __global__ __launch_bounds__(64 * WN * KW, 2) void many_rows_kernel(ProductParam
             }
     }
     if (piece >= n_pieces) return;
-    // (the waves of a piece store a part each: results r with r % KW == kw)
+    // (the waves of a piece store a part each: results 2 i and 2 i + 1 with i % KW == kw)
+    if constexpr (GATED) {
+        const int n_out = p.g.rows / 2, col = piece * 32 + l32, row0 = first + 4 * h;
+        int8_t *codes_at = p.out_codes + row0 * (int64_t) n_out + col;
+        uint16_t *scales_at8 = p.out_scales + row0 * (int64_t) (n_out / 32) + piece;
+        const bool whole = first + ROWS <= p.n_rows;
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int64_t row = (int64_t) first + m * 32 + 8 * (r >> 2) + 4 * h + (r & 3);
-            if (KW > 1 && r % KW != kw) continue;
-            if constexpr (GATED) {
-                const int n_out = p.g.rows / 2, col = piece * 32 + l32;
+            for (int r = 0; r < 16; ++r) {
+                if (KW > 1 && (r >> 1) % KW != kw) continue;
+                const int dr = m * 32 + 8 * (r >> 2) + (r & 3);
+                const bool real = whole || row0 + dr < p.n_rows;
                 const float v = gate(acc[0][m][r] * kCodeStep, acc[1][m][r] * kCodeStep, p.activation);
-                if (p.out && row < p.n_rows) store1(p.out, row * p.out_stride + col, v, p.type);
+                if (p.out && real) store1(p.out, (row0 + (int64_t) dr) * p.out_stride + col, v, p.type);
                 if (p.out_codes) {
                     const Scale8 s = scale_of(half_max(__builtin_fabsf(v)));
-                    if (row < p.n_rows) {
-                        p.out_codes[row * n_out + col] = (int8_t) code1(v, s.inv);
-                        if (l32 == 0) p.out_scales[row * (n_out / 32) + piece] = (uint16_t) s.bits;
+                    const int code = code1(v, s.inv);
+                    if (real) {
+                        codes_at[(int64_t) dr * n_out] = (int8_t) code;
+                        if (l32 == 0) scales_at8[(int64_t) dr * (n_out / 32)] = (uint16_t) s.bits;
                     }
                 }
-            } else if (row < p.n_rows) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const int col = (NT * piece + n) * 32 + l32;
-                    if (col < p.g.rows) store1(p.out, row * p.out_stride + col, acc[n][m][r] * kCodeStep, p.type);
-                }
             }
+    } else {
+        // Results r and r + 1 are two rows of a column.  Neighbouring lanes change
+        // halves of their 16-bit pairs, so that each stores two columns of one row.
+        auto each = [&](auto store) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) {
+                    if (KW > 1 && (r >> 1) % KW != kw) continue;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        store(m * 32 + 8 * (r >> 2) + (r & 3), n * 32, acc[n][m][r] * kCodeStep, acc[n][m][r + 1] * kCodeStep);
+                }
+        };
+        const int col = NT * piece * 32 + l32, row = first + 4 * h;
+        const bool whole = first + ROWS <= p.n_rows && NT * (piece + 1) * 32 <= p.g.rows;
+        const bool pairs = (p.out_stride & 1) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 3) == 0;
+        if (whole && p.type == kTypeF32) {
+            float *out = static_cast<float *>(p.out) + row * p.out_stride + col;
+            each([&](int dr, int dc, float a, float b) {
+                float *at = out + dr * p.out_stride + dc;
+                at[0] = a;
+                at[p.out_stride] = b;
+            });
+        } else if (whole && pairs) {
+            const bool odd = lane & 1;
+            uint16_t *out = static_cast<uint16_t *>(p.out) + (row + odd) * p.out_stride + (col - odd);
+            const uint32_t take = odd ? 0x07060302u : 0x01000504u;  // bytes of (own, other): their high halves or low ones
+            auto put = [&](int dr, int dc, uint32_t a, uint32_t b) {
+                const uint32_t own = a | b << 16, other = (uint32_t) __builtin_amdgcn_mov_dpp((int) own, 0xB1, 0xF, 0xF, true);
+                *reinterpret_cast<uint32_t *>(out + (dr * p.out_stride + dc)) = __builtin_amdgcn_perm(own, other, take);
+            };
+            if (p.type == kTypeF16)
+                each([&](int dr, int dc, float a, float b) { put(dr, dc, f32_to_f16_bits(a), f32_to_f16_bits(b)); });
+            else
+                each([&](int dr, int dc, float a, float b) { put(dr, dc, bf16_bits(a), bf16_bits(b)); });
+        } else {
+            each([&](int dr, int dc, float a, float b) {
+                if (col + dc >= p.g.rows) return;
+                const int64_t at = (row + (int64_t) dr) * p.out_stride + col + dc;
+                if (row + dr < p.n_rows) store1(p.out, at, a, p.type);
+                if (row + dr + 1 < p.n_rows) store1(p.out, at + p.out_stride, b, p.type);
+            });
         }
+    }
 }
 
 template <int SHAPE, int WN, int D, bool AHEAD, bool GATED>
