@@ -574,73 +574,104 @@ __global__ __launch_bounds__(64 * WN * KW, 2) void many_rows_kernel(ProductParam
             load_units(j, unit_of(step + D));
         }
     }
+    // The waves of a piece add up in the order of their units, each the PART
+    // results from kw * PART on, which it stores.
+    constexpr int PART = 16 / KW;
+    float sum[NT][MT][PART];
     if constexpr (KW > 1) {
-        // the waves of a piece add up in the order of their units
-        __shared__ rw_float4 s_acc[WAVES][4][64];
+        __shared__ float s_acc[WAVES][16 / PART][64][PART];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 __syncthreads();
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    s_acc[wave][j][lane] = rw_float4{acc[n][m][4 * j], acc[n][m][4 * j + 1], acc[n][m][4 * j + 2],
-                                                     acc[n][m][4 * j + 3]};
+                for (int r = 0; r < 16; ++r) s_acc[wave][r / PART][lane][r % PART] = acc[n][m][r];
                 __syncthreads();
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    rw_float4 v = s_acc[wave - kw][j][lane];
+                for (int i = 0; i < PART; ++i) sum[n][m][i] = s_acc[wave - kw][kw][lane][i];
 #pragma unroll
-                    for (int k = 1; k < KW; ++k) v += s_acc[wave - kw + k][j][lane];
+                for (int k = 1; k < KW; ++k)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[n][m][4 * j + r] = v[r];
-                }
+                    for (int i = 0; i < PART; ++i) sum[n][m][i] += s_acc[wave - kw + k][kw][lane][i];
             }
+    } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum[n][m][i] = acc[n][m][i];
     }
     if (piece >= n_pieces) return;
-    // (the waves of a piece store a part each: results 2 i and 2 i + 1 with i % KW == kw)
+    const int row0 = first + 4 * h;
+    // A lane's row of result i, from row0 on.
+    auto below = [&](int m, int i) {
+        const int r = kw * PART + i;
+        return m * 32 + 8 * (r >> 2) + (r & 3);
+    };
     if constexpr (GATED) {
-        const int n_out = p.g.rows / 2, col = piece * 32 + l32, row0 = first + 4 * h;
-        int8_t *codes_at = p.out_codes + row0 * (int64_t) n_out + col;
-        uint16_t *scales_at8 = p.out_scales + row0 * (int64_t) (n_out / 32) + piece;
-        const bool whole = first + ROWS <= p.n_rows;
+        const int n_out = p.g.rows / 2, col = piece * 32 + l32;
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                if (KW > 1 && (r >> 1) % KW != kw) continue;
-                const int dr = m * 32 + 8 * (r >> 2) + (r & 3);
-                const bool real = whole || row0 + dr < p.n_rows;
-                const float v = gate(acc[0][m][r] * kCodeStep, acc[1][m][r] * kCodeStep, p.activation);
-                if (p.out && real) store1(p.out, (row0 + (int64_t) dr) * p.out_stride + col, v, p.type);
-                if (p.out_codes) {
-                    const Scale8 s = scale_of(half_max(__builtin_fabsf(v)));
-                    const int code = code1(v, s.inv);
-                    if (real) {
-                        codes_at[(int64_t) dr * n_out] = (int8_t) code;
-                        if (l32 == 0) scales_at8[(int64_t) dr * (n_out / 32)] = (uint16_t) s.bits;
-                    }
+            for (int i = 0; i < PART; ++i)
+                sum[0][m][i] = gate(sum[0][m][i] * kCodeStep, sum[1][m][i] * kCodeStep, p.activation);
+        if (p.out) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 0; i < PART; ++i)
+                    if (row0 + below(m, i) < p.n_rows)
+                        store1(p.out, (row0 + (int64_t) below(m, i)) * p.out_stride + col, sum[0][m][i], p.type);
+        }
+        if (!p.out_codes) return;
+        // (no branch between the rows, so that their chains of instructions overlap)
+        int8_t *codes_at = p.out_codes + row0 * (int64_t) n_out + col;
+        uint16_t *scales8 = p.out_scales + (row0 * (int64_t) (n_out / 32) + piece);
+        auto quantize = [&](auto real) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                uint32_t bits[PART];
+#pragma unroll
+                for (int i = 0; i < PART; ++i) {
+                    const Scale8 s = scale_of(half_max(__builtin_fabsf(sum[0][m][i])));
+                    const int code = code1(sum[0][m][i], s.inv), dr = below(m, i);
+                    bits[i] = s.bits;
+                    if (real(dr)) codes_at[(int64_t) dr * n_out] = (int8_t) code;
                 }
+                // (lane i of a half stores the scale of its row i)
+                uint32_t mine = bits[0];
+                int dr = below(m, 0);
+#pragma unroll
+                for (int i = 1; i < PART; ++i) {
+                    mine = l32 == i ? bits[i] : mine;
+                    dr = l32 == i ? below(m, i) : dr;
+                }
+                if (l32 < PART && real(dr)) scales8[(int64_t) dr * (n_out / 32)] = (uint16_t) mine;
             }
+        };
+        if (first + ROWS <= p.n_rows)
+            quantize([](int) { return true; });
+        else
+            quantize([&](int dr) { return row0 + dr < p.n_rows; });
     } else {
-        // Results r and r + 1 are two rows of a column.  Neighbouring lanes change
+        // Results i and i + 1 are two rows of a column.  Neighbouring lanes change
         // halves of their 16-bit pairs, so that each stores two columns of one row.
         auto each = [&](auto store) {
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int r = 0; r < 16; r += 2) {
-                    if (KW > 1 && (r >> 1) % KW != kw) continue;
+                for (int i = 0; i < PART; i += 2)
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
-                        store(m * 32 + 8 * (r >> 2) + (r & 3), n * 32, acc[n][m][r] * kCodeStep, acc[n][m][r + 1] * kCodeStep);
-                }
+                        store(below(m, i), n * 32, sum[n][m][i] * kCodeStep, sum[n][m][i + 1] * kCodeStep);
         };
-        const int col = NT * piece * 32 + l32, row = first + 4 * h;
+        const int col = NT * piece * 32 + l32;
         const bool whole = first + ROWS <= p.n_rows && NT * (piece + 1) * 32 <= p.g.rows;
         const bool pairs = (p.out_stride & 1) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 3) == 0;
         if (whole && p.type == kTypeF32) {
-            float *out = static_cast<float *>(p.out) + row * p.out_stride + col;
+            float *out = static_cast<float *>(p.out) + row0 * p.out_stride + col;
             each([&](int dr, int dc, float a, float b) {
                 float *at = out + dr * p.out_stride + dc;
                 at[0] = a;
@@ -648,7 +679,7 @@ __global__ __launch_bounds__(64 * WN * KW, 2) void many_rows_kernel(ProductParam
             });
         } else if (whole && pairs) {
             const bool odd = lane & 1;
-            uint16_t *out = static_cast<uint16_t *>(p.out) + (row + odd) * p.out_stride + (col - odd);
+            uint16_t *out = static_cast<uint16_t *>(p.out) + (row0 + odd) * p.out_stride + (col - odd);
             const uint32_t take = odd ? 0x07060302u : 0x01000504u;  // bytes of (own, other): their high halves or low ones
             auto put = [&](int dr, int dc, uint32_t a, uint32_t b) {
                 const uint32_t own = a | b << 16, other = (uint32_t) __builtin_amdgcn_mov_dpp((int) own, 0xB1, 0xF, 0xF, true);
@@ -661,9 +692,9 @@ __global__ __launch_bounds__(64 * WN * KW, 2) void many_rows_kernel(ProductParam
         } else {
             each([&](int dr, int dc, float a, float b) {
                 if (col + dc >= p.g.rows) return;
-                const int64_t at = (row + (int64_t) dr) * p.out_stride + col + dc;
-                if (row + dr < p.n_rows) store1(p.out, at, a, p.type);
-                if (row + dr + 1 < p.n_rows) store1(p.out, at + p.out_stride, b, p.type);
+                const int64_t at = (row0 + (int64_t) dr) * p.out_stride + col + dc;
+                if (row0 + dr < p.n_rows) store1(p.out, at, a, p.type);
+                if (row0 + dr + 1 < p.n_rows) store1(p.out, at + p.out_stride, b, p.type);
             });
         }
     }
