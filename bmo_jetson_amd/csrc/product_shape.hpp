@@ -8,32 +8,36 @@ namespace bmo {
 
 // A workgroup takes `rows` rows and `outs` outputs (gates, of a gated product);
 // `waves` waves share each piece of it along the columns, a step each a unit of
-// 128.  A CU runs `resident` of them at a time.  Times of a call in us: start +
-// steps * (those of the fullest CU's workgroups, `resident` at a time: alone, or
-// shared for each where that is more).
+// 128.  A CU runs `resident` of them at a time.  Times of a call in us, by the
+// fullest CU's workgroups: start + each for all that is not in a step, and a
+// round of `resident` at a time a step (alone, or shared for each where that is
+// more).
 struct ProductShape {
     int rows, outs, waves, resident;
-    double start, alone, shared;
+    double start, each, alone, shared;
 };
 
 // Few rows (16 x 16 matrix instructions) and many (32 x 32).  The times are
 // fitted to calls with weights from HBM, 2 to 3000 rows by 512 to 32001 outputs
-// of 640 to 11264 columns (gated: 2048 rows by 512 to 11264 outputs of 640 to
+// of 160 to 11264 columns (gated: 2048 rows by 512 to 11264 outputs of 128 to
 // 8192), and moved by up to 15% to where they choose best: against the fastest
-// shape 0.7% in the mean over the 162 calls, 16% at worst (32 rows x 32001 outputs
-// x 1024: 11.2 us, 9.7 with 32 x 64); gated 0.2% over 80, 8% at worst.  What a
-// shape is worth: 16 x 16 at 2 x 512 x 4096 3.5 us, 16 x 32 there 5.7; 16 x 64 at 64 x
-// 4096 x 4096 8.1, 32 x 32 there 9.0; 32 x 32 with eight waves at 48 x 4096 x 5632 9.1,
-// with four 11.1; 64 x 128 with two waves to a piece at 1500 x 12288 x 4096 201, 64 x
-// 256 there 213, at 2048 x 12288 x 4096 267 and 250.
+// shape 0.4% in the mean over the 216 calls, 13% at worst (48 rows x 11264 outputs
+// x 640: 6.6 us, 5.9 with 32 x 32); gated 0.1% over 112, 3% at worst.  What a shape
+// is worth: 16 x 16 at 2 x 512 x 4096 3.5 us, 16 x 32 there 5.8; 32 x 32 with eight waves at 48
+// x 4096 x 5632 8.4, with four 11.1; 32 x 128 with one wave to a piece at 1500 x 1216 x
+// 160 5.8, 32 x 256 at 768 x 11264 x 288 15.3, 64 x 256 there 20.0; 64 x 128 with two
+// waves to a piece at 1500 x 12288 x 4096 200, 64 x 256 there 203, at 2048 rows 260
+// and 244.
 constexpr ProductShape kProductShapes[] = {
-    {16, 16, 8, 1, 2.50, 0.81, 0},     {16, 32, 8, 1, 3.15, 1.00, 0},    {16, 64, 8, 1, 2.90, 1.74, 0},
-    {32, 32, 4, 2, 3.68, 0.75, 0.59},  {32, 32, 8, 1, 3.88, 1.32, 0},    {32, 64, 4, 2, 3.96, 1.25, 1.11},
-    {32, 128, 2, 2, 4.75, 1.30, 1.01}, {64, 128, 2, 2, 6.95, 1.98, 1.29}, {64, 256, 1, 2, 9.38, 1.66, 1.12},
+    {16, 16, 8, 2, 1.47, 0.25, 0.82, 0.58},  {16, 32, 8, 2, 1.58, 0.28, 1.08, 0.84},  {16, 64, 8, 1, 1.63, 0.77, 1.44, 0},
+    {32, 32, 4, 3, 2.30, 0.35, 0.63, 0.51},  {32, 32, 8, 1, 0.80, 1.82, 1.05, 0},     {32, 64, 4, 2, 2.01, 0.73, 1.31, 0.74},
+    {32, 128, 1, 3, 2.14, 0.55, 0.61, 0.38}, {32, 256, 1, 3, 1.85, 0.79, 1.28, 0.70}, {64, 128, 2, 2, 3.33, 1.52, 1.56, 1.23},
+    {64, 256, 1, 2, 2.12, 1.97, 2.24, 1.08},
 };
 constexpr ProductShape kGatedShapes[] = {
-    {16, 32, 8, 1, 3.84, 1.72, 0},    {32, 32, 8, 1, 5.06, 2.10, 0},     {32, 32, 4, 2, 4.59, 1.31, 0.94},
-    {32, 64, 2, 2, 4.71, 1.34, 0.92}, {64, 64, 2, 2, 10.18, 2.07, 1.43}, {64, 128, 1, 2, 13.18, 1.52, 1.38},
+    {16, 32, 8, 1, 2.38, 0.15, 1.48, 0},     {32, 32, 8, 2, 0.66, 2.54, 1.57, 1.80}, {32, 32, 4, 2, 1.85, 0.98, 1.38, 0.80},
+    {32, 64, 2, 2, 2.84, 1.19, 1.49, 0.79},  {32, 128, 1, 3, 4.12, 1.34, 1.37, 0.70}, {64, 64, 2, 2, 4.00, 2.39, 1.70, 1.18},
+    {64, 128, 1, 2, 4.70, 3.38, 1.77, 1.15},
 };
 constexpr int kProductKinds = sizeof(kProductShapes) / sizeof(ProductShape);
 constexpr int kGatedKinds = sizeof(kGatedShapes) / sizeof(ProductShape);
@@ -46,7 +50,7 @@ constexpr double product_cost(const ProductShape &s, int64_t rows, int64_t outs,
     const double full = s.resident * s.shared, part = (double) rest * s.shared;
     const double round = (double) (fullest / s.resident) * (full > s.alone ? full : s.alone);
     const double last = rest == 0 ? 0.0 : part > s.alone ? part : s.alone;
-    return s.start + (double) ((chunks + s.waves - 1) / s.waves) * (round + last);
+    return s.start + (double) fullest * s.each + (double) ((chunks + s.waves - 1) / s.waves) * (round + last);
 }
 
 // The cheapest shape's number.

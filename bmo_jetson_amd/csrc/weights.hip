@@ -69,7 +69,8 @@ __device__ __forceinline__ uint32_t dword(const uint4 &v, int t) { return t == 0
 // 2^x (its argument off by a rounding: |a| e^-|a| of one in the result), the
 // quotient a product with the hardware's reciprocal, of a sixteenth of the
 // divisor so that it stays normal up to exp's overflow: five instructions for
-// some thirty of expf and a division (1000 x 5632 x 128 @A us, with them @B).
+// some thirty of expf and a division (1000 x 5632 x 128 in pieces of 64 x 128 30 us,
+// with them 36).
 __device__ __forceinline__ float gate(float g, float u, int activation) {
     // GELU by its tanh form: 0.5 (1 + tanh z) = 1 / (1 + exp(-2 z))
     const float a = activation == kSilu ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
@@ -393,11 +394,12 @@ hipError_t run_few(const ProductParams &p, hipStream_t stream) {
 // against 144; 64 x 256 plain 250 against 248 at 2048 x 12288 x 4096, narrower ones
 // the same either way).
 //
-// 2048 x 12288 x 4096 takes 249 us, 828 TFLOP/s (64 x 256 outputs a workgroup).
-// In a copy of 128 x 128 (265) that skips work the vector and matrix
-// instructions alone take 205, the accesses to LDS 25 and the loads from memory
-// 40 more: the two waves of a SIMD issue more than half of the time.  Three or
-// four waves a SIMD, in 168 or 128 registers, need narrower pieces: 287 and 292.
+// 2048 x 12288 x 4096 takes 230 to 239 us, 860 to 895 TFLOP/s (64 x 256 outputs a
+// workgroup): of 265 in an earlier form of 128 x 128 the vector and matrix
+// instructions alone took 205, the accesses to LDS 25 and the loads from memory
+// 40 (a copy that skips work); the two waves of a SIMD issue more than half of the
+// time.  Three or four waves a SIMD, in 168 or 128 registers, need narrower pieces:
+// 287 and 292 in that form.
 
 // Two units' codes of 16 outputs each to a 32-column operand: lanes 16 to 31
 // and 48 to 63 of the first change places with lanes 0 to 15 and 32 to 47 of
@@ -731,8 +733,9 @@ hipError_t launch_product(const ProductParams &p, hipStream_t stream) {
         case 1: return run_many<1, 1, 1, false, true>(p, stream);
         case 2: return run_many<2, 1, 1, false, true>(p, stream);
         case 3: return run_many<3, 2, 2, false, true>(p, stream);
-        case 4: return run_many<4, 2, 1, true, true>(p, stream);
-        default: return run_many<5, 4, 1, true, true>(p, stream);
+        case 4: return run_many<4, 4, 1, false, true>(p, stream);
+        case 5: return run_many<5, 2, 1, true, true>(p, stream);
+        default: return run_many<6, 4, 1, true, true>(p, stream);
         }
     }
     switch (product_shape(false, p.n_rows, p.g.rows, p.g.chunks)) {
@@ -742,9 +745,10 @@ hipError_t launch_product(const ProductParams &p, hipStream_t stream) {
     case 3: return run_many<3, 1, 2, false, false>(p, stream);
     case 4: return run_many<4, 1, 2, false, false>(p, stream);
     case 5: return run_many<5, 1, 1, false, false>(p, stream);
-    case 6: return run_many<6, 2, 2, false, false>(p, stream);
-    case 7: return run_many<7, 2, 1, true, false>(p, stream);
-    default: return run_many<8, 4, 2, false, false>(p, stream);
+    case 6: return run_many<6, 4, 2, false, false>(p, stream);
+    case 7: return run_many<7, 4, 1, false, false>(p, stream);
+    case 8: return run_many<8, 2, 1, true, false>(p, stream);
+    default: return run_many<9, 4, 2, false, false>(p, stream);
     }
 }
 

@@ -67,23 +67,45 @@ def test_types_and_larger_sizes(gpu, n, rows, cols, type_):
 
 # rows, outputs, columns and the kernel that takes them (workgroup's rows, outputs; waves of a piece)
 SHAPES = [(2, 97, 416, (16, 16, 8)), (37, 161, 1120, (16, 16, 8)), (69, 1001, 1120, (16, 32, 8)), (33, 2001, 1120, (16, 32, 8)),
-          (37, 4097, 416, (16, 64, 8)), (131, 1001, 736, (16, 64, 8)), (17, 8161, 1248, (32, 32, 4)), (197, 1001, 96, (32, 32, 4)),
-          (325, 1057, 1120, (32, 32, 4)), (131, 1001, 2976, (32, 32, 8)), (49, 4001, 4000, (32, 32, 8)),
-          (131, 6001, 736, (32, 64, 4)), (69, 8193, 1120, (32, 64, 4)),
-          (261, 4097, 96, (32, 128, 2)), (901, 2049, 96, (32, 128, 2)), (131, 8193, 96, (32, 128, 2)),
-          (515, 6001, 1120, (64, 128, 2)), (901, 4097, 1120, (64, 128, 2)), (261, 12001, 1120, (64, 128, 2)),
+          (37, 4097, 416, (16, 32, 8)), (37, 4097, 1120, (16, 64, 8)), (2, 8193, 1120, (16, 64, 8)),
+          (17, 8161, 1248, (32, 32, 4)), (197, 1001, 96, (32, 32, 4)), (325, 1057, 1120, (32, 32, 4)),
+          (131, 1001, 736, (32, 32, 8)), (131, 1001, 2976, (32, 32, 8)), (49, 4001, 4000, (32, 32, 8)),
+          (69, 8193, 416, (32, 64, 4)), (1501, 513, 416, (32, 64, 4)), (131, 4097, 2080, (32, 64, 4)),
+          (131, 6001, 736, (32, 128, 1)), (901, 2049, 96, (32, 128, 1)), (261, 6001, 416, (32, 128, 1)),
+          (261, 4097, 96, (32, 256, 1)), (515, 6001, 1120, (32, 256, 1)), (901, 4097, 1120, (32, 256, 1)),
+          (515, 6001, 4000, (64, 128, 2)), (901, 4097, 4064, (64, 128, 2)),
           (901, 8193, 96, (64, 256, 1)), (515, 12001, 1120, (64, 256, 1)), (3001, 2049, 1120, (64, 256, 1))]
-GATED_SHAPES = [(2, 32, 736, (16, 32, 8)), (261, 32, 2080, (16, 32, 8)), (17, 5632, 4096, (32, 32, 8)), (29, 6016, 4000, (32, 32, 8)), (2, 32, 96, (16, 32, 8)),
-                (69, 160, 416, (16, 32, 8)), (131, 1024, 736, (32, 32, 8)), (69, 2080, 2080, (32, 32, 4)),
-                (131, 1024, 96, (32, 32, 4)), (69, 2080, 160, (32, 32, 4)), (37, 6016, 96, (32, 64, 2)),
-                (901, 4128, 96, (32, 64, 2)), (1101, 3104, 736, (32, 64, 2)), (515, 3104, 2080, (64, 64, 2)),
-                (1501, 1056, 2080, (64, 64, 2)), (515, 6016, 1120, (64, 128, 1)), (1501, 2080, 1120, (64, 128, 1))]
+GATED_SHAPES = [(2, 32, 736, (16, 32, 8)), (261, 32, 2080, (16, 32, 8)), (2, 32, 96, (16, 32, 8)), (69, 160, 416, (16, 32, 8)),
+                (131, 1024, 736, (32, 32, 8)), (69, 2080, 2080, (32, 32, 8)), (29, 6016, 4000, (32, 32, 8)),
+                (131, 1024, 96, (32, 32, 4)), (69, 2080, 160, (32, 32, 4)), (37, 6016, 96, (32, 32, 4)),
+                (901, 736, 736, (32, 64, 2)), (131, 4128, 32, (32, 64, 2)), (901, 4128, 96, (32, 128, 1)),
+                (515, 2080, 736, (32, 128, 1)), (515, 3104, 2080, (64, 64, 2)), (1501, 1056, 2080, (64, 64, 2)),
+                (1101, 3104, 736, (64, 128, 1)), (515, 6016, 1120, (64, 128, 1)), (1501, 2080, 1120, (64, 128, 1))]
 
 
 @pytest.mark.parametrize("n,rows,cols,shape", SHAPES)
 def test_every_kernel(gpu, n, rows, cols, shape):
     assert product_shapes([(False, n, rows, cols)]) == [shape]
     _product(gpu, n, rows, cols, seed=n)
+
+
+@pytest.mark.parametrize("n,rows,cols,shape", SHAPES)
+def test_every_kernel_s_stores(gpu, n, rows, cols, shape):
+    """16-bit results are the 32-bit ones rounded, at every alignment of their
+    rows; what lies between the rows stays."""
+    torch = gpu
+    blocks, _, _ = q4_0(n + 1, rows, cols)
+    w = _weights(torch, blocks)
+    _, _, c, s = _rows8(torch, n, n, cols)
+    want = torch.empty(n, rows, device="cuda")
+    stream = torch.cuda.current_stream()
+    w.product(c, s, want, stream=stream)
+    for type_ in (torch.float16, torch.bfloat16, torch.float32):
+        for stride, shift in ((rows + (rows & 1), 0), (rows + 7, 0), (rows + 6 + (rows & 1), 2), (rows + 6, 1)):
+            big = torch.full((n, stride), 7.0, dtype=type_, device="cuda")
+            w.product(c, s, big[:, shift:shift + rows], stream=stream)
+            assert torch.equal(big[:, shift:shift + rows], want.to(type_)), (type_, stride, shift)
+            assert (big[:, :shift] == 7).all() and (big[:, shift + rows:] == 7).all()
 
 
 def test_gemv_of_each_row(gpu):

@@ -2,9 +2,9 @@
 import test_gpu_weights
 from _shapes import product_places, product_shapes
 
-PRODUCT = {(16, 16, 8), (16, 32, 8), (16, 64, 8), (32, 32, 4), (32, 32, 8), (32, 64, 4), (32, 128, 2),
+PRODUCT = {(16, 16, 8), (16, 32, 8), (16, 64, 8), (32, 32, 4), (32, 32, 8), (32, 64, 4), (32, 128, 1), (32, 256, 1),
            (64, 128, 2), (64, 256, 1)}
-GATED = {(16, 32, 8), (32, 32, 8), (32, 32, 4), (32, 64, 2), (64, 64, 2), (64, 128, 1)}
+GATED = {(16, 32, 8), (32, 32, 8), (32, 32, 4), (32, 64, 2), (32, 128, 1), (64, 64, 2), (64, 128, 1)}
 
 
 def test_the_gpu_tests_meet_every_kernel():
