@@ -3,15 +3,14 @@
 //
 //   y[m][n] = sum over blocks b of d4[n][b] d8[m][b] sum_j (c_j - 8) q_j
 //
-// A block's sum is an exact integer: v_mfma_i32 over its 32 elements, the
-// weights (16 (code - 8), one shift and mask from their nibbles) as the rows
-// and the 8-bit rows as the columns of the result.  It starts from the integer
-// whose bits are the float 1.5 * 2^23, so that the result's bits, read as a
-// float, are that plus the sum, exactly (sums stay below 2^20), and one fma
-// with d8 takes the offset out again: -1.5 * 2^23 * d8 is exact for an fp16
-// d8.  A second one adds d4 times that, so an output is off by the roundings
-// of an fp32 sum of its blocks' parts only.  (Converting the integer takes as
-// long as seven fmas.)
+// A block's sum is an exact integer: v_mfma_i32 over its 32 elements, the 8-bit
+// rows as the rows and the weights (16 (code - 8), one shift and mask from their
+// nibbles) as the columns of the result.  It starts from the integer whose bits
+// are the float 1.5 * 2^23, so that the result's bits, read as a float, are that
+// plus the sum, exactly (sums stay below 2^20), and one fma with d4 takes the
+// offset out again: -1.5 * 2^23 * d4 is exact for an fp16 d4.  A second one adds
+// d8 times that, so an output is off by the roundings of an fp32 sum of its
+// blocks' parts only.  (Converting the integer takes as long as seven fmas.)
 //
 // Few rows are bound by reading the weights once, many by those two fmas: a
 // 32 x 32 tile of a block takes 32 of them a lane and 10 other vector
@@ -387,12 +386,11 @@ hipError_t run_few(const ProductParams &p, hipStream_t stream) {
 // rows, whose scales are read from LDS.  The rows' codes and scales go there a
 // unit ahead: eight lanes read a row's 128 codes, which costs the loads a
 // quarter of what reading them as the matrix cores take them does.  D units'
-// weights are under way at once.  AHEAD: a tile's matrix
-// instruction stands before the fmas of the tile before it, which takes the
-// registers of a second unit (64 x 128, D 1 against D 2 without: 1000 x 4096 x 5632
-// 66 against 71 us, 48 x 4096 x 5632 48.0 against 49.6; gated 1000 x 5632 x 4096 140
-// against 144; 64 x 256 plain 250 against 248 at 2048 x 12288 x 4096, narrower ones
-// the same either way).
+// weights are under way at once.  AHEAD: a tile's matrix instruction stands
+// before the fmas of the tile before it, which takes the registers of a second
+// unit (64 x 128, D 1 against D 2 without: 1000 x 4096 x 5632 66 against 71 us, 48 x
+// 4096 x 5632 48.0 against 49.6; gated 1000 x 5632 x 4096 140 against 144; 64 x 256
+// plain 250 against 248 at 2048 x 12288 x 4096, narrower ones the same either way).
 //
 // 2048 x 12288 x 4096 takes 230 to 239 us, 860 to 895 TFLOP/s (64 x 256 outputs a
 // workgroup): of 265 in an earlier form of 128 x 128 the vector and matrix
