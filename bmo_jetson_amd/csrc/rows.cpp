@@ -13,6 +13,7 @@
 
 #include "../../include/bmo_attn.h"
 #include "rows.hpp"
+#include "spans.hpp"
 
 static_assert(BMO_ATTN_SILU == bmo::kSilu && BMO_ATTN_GELU == bmo::kGelu, "the header's activations");
 
@@ -123,27 +124,15 @@ const char *rows8_fault(const void *codes, const void *scales) {
                                                     : "codes must be aligned to 16 bytes, scales to their elements";
 }
 
-// What a call reads or writes: n rows of `dense` bytes, `stride` bytes apart.
-struct Span {
-    const void *p;
-    int64_t n, dense, stride;
-    bool operator==(const Span &o) const { return p == o.p && dense == o.dense && (n == 1 || stride == o.stride); }
-};
+using bmo::Span;
+using bmo::meet;
+
 Span span(const void *p, int64_t n, int64_t elements, int64_t stride, int size) {
     return {p, n, elements * size, stride * size};
 }
 Span span8(const void *codes, int64_t n, int64_t cols) { return {codes, 1, n * cols, 0}; }
 Span span_scales(const void *scales, int64_t n, int64_t cols) { return {scales, 1, n * (cols / 32) * 2, 0}; }
 
-// Whether two of them share bytes, as far as it can be told at once: rows that
-// lie apart may have others between them, so of those only the starts count.
-bool meet(const Span &a, const Span &b) {
-    if (!a.p || !b.p) return false;
-    if (a.p == b.p) return true;
-    if ((a.n > 1 && a.stride != a.dense) || (b.n > 1 && b.stride != b.dense)) return false;
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
-    return x < y ? y - x < (uintptr_t) (a.n * a.dense) : x - y < (uintptr_t) (b.n * b.dense);
-}
 // Whether anything written meets what else is written or read.
 bool overlap(std::initializer_list<Span> written, std::initializer_list<Span> read) {
     for (const Span *w = written.begin(); w != written.end(); ++w) {
