@@ -713,8 +713,10 @@ BMO_ATTN_API int bmo_weights_load(bmo_weights_t *weights, int row, int n_rows, c
 /* out [n_rows][rows] = 8-bit rows [n_rows][cols] times the matrix:
  *   out[m][n] = sum over blocks of d4 * d8 * sum((code - 8) * q),
  * a block's sum an exact integer, blocks added in fp32; the order, and with it
- * the rounding, depends on the sizes alone.  A scale that is NaN or infinite
- * makes NaN of the outputs that it takes part in.  n_rows at most 2^20. */
+ * the rounding, depends on the sizes alone.  A scale that is NaN, or an infinite
+ * one of the weights, makes NaN of the outputs that it takes part in; an infinite
+ * one of the 8-bit rows makes infinities, or NaN where the block's sum or weight
+ * scale is 0.  n_rows at most 2^20. */
 BMO_ATTN_API int bmo_weights_product(bmo_weights_t *weights, int n_rows, const void *codes,
                                      const void *scales, int type, void *out, int64_t out_stride,
                                      void *stream);
