@@ -7,7 +7,8 @@
 // so), or single pairs, and pieces of the copied elements, as the sizes and
 // alignment allow.  A thread's items are read first; while they are under way
 // the workgroup makes its tokens' cosines and sines, in double, rounded once to
-// fp32.  Each product and sum is rounded as the ring's fused rotation does.
+// fp32 (of angles that are products in double: far positions turn by the rounding
+// of these too).  Each product and sum is rounded as the ring's fused rotation does.
 //
 // Bound by its bytes, and in small calls by one load and one sine in turn: 5600
 // tokens x 40 heads of 128, bf16, in 24.6 us, 4.7 TB/s (a large copy: 5.1); 48 x

@@ -685,9 +685,11 @@ BMO_ATTN_API const char *bmo_rope_last_error(const bmo_rope_t *rope);
 /* Turns rows q [n_tok][n_heads][head_dim] and k [n_tok][n_kv_heads][head_dim]
  * (n_kv_heads 0: none) by positions [n_tok] (device, any int: a plan's
  * tok_pos) into q_out and k_out, which may be q and k with their strides but
- * must not overlap them otherwise.  Cosines and sines are the exact ones
- * rounded to fp32, each product and sum is rounded to fp32, the result to the
- * type.  At most 2^32 elements. */
+ * must not overlap them otherwise.  An angle is a product in fp64, off by at most
+ * |angle| 2^-50 with its rate's roundings (1e-9 radians at a million, 2e-6 at
+ * 2^31); its cosine and sine times the magnitude are rounded once to fp32, each
+ * product and sum is rounded to fp32, the result to the type.  At most 2^32
+ * elements. */
 BMO_ATTN_API int bmo_rope_apply(bmo_rope_t *rope, int n_tok, const int *positions, int type,
                                 int n_heads, const void *q, int64_t q_stride, void *q_out,
                                 int64_t q_out_stride, int n_kv_heads, const void *k,
