@@ -62,8 +62,6 @@ __global__ __launch_bounds__(256) void pack_kernel(PackParams p, FastDiv div_blo
 __device__ __forceinline__ float half_lo(uint32_t u) { return f16_bits_to_f32(u & 0xFFFFu); }
 __device__ __forceinline__ float half_hi(uint32_t u) { return f16_bits_to_f32(u >> 16); }
 
-__device__ __forceinline__ uint32_t dword(const uint4 &v, int t) { return t == 0 ? v.x : t == 1 ? v.y : t == 2 ? v.z : v.w; }
-
 // The activation of a gate times what it lets through.  exp is the hardware's
 // 2^x, whose argument a product would leave |a| 2^-24 off, times 1 + ln 2 of what
 // that product lost: 4 roundings however large |a| is.  (Clamped past exp's range
