@@ -238,6 +238,8 @@ class Rope(_Handle):
         if positions.get_device() != self._device:
             raise _on(positions, self._device, "positions")
         qp, q_stride, type_, heads = self._heads(q, n, "q")
+        if k is None and k_out is not None:
+            raise ValueError("k_out without k")
         parts = [(qp, q_stride) if q_out is None else self._heads(q_out, n, "q_out", q)]
         kp, k_stride, k_type, k_heads = (None, 0, type_, 0) if k is None else self._heads(k, n, "k")
         parts.append((kp, k_stride) if k is None or k_out is None else self._heads(k_out, n, "k_out", k))
