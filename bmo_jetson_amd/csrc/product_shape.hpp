@@ -20,14 +20,14 @@ struct ProductShape {
 // Few rows (16 x 16 matrix instructions) and many (32 x 32).  The times are
 // fitted to calls with weights from HBM, 2 to 3000 rows by 512 to 32001 outputs
 // of 160 to 11264 columns (gated: 2048 rows by 512 to 11264 outputs of 128 to
-// 8192), and moved by up to 15% to where they choose best: against the fastest
-// shape 0.4% in the mean over the 216 calls, 13% at worst (48 rows x 11264 outputs
-// x 640: 6.6 us, 5.9 with 32 x 32); gated 0.1% over 112, 3% at worst.  What a shape
-// is worth: 16 x 16 at 2 x 512 x 4096 3.5 us, 16 x 32 there 5.8; 32 x 32 with eight waves at 48
-// x 4096 x 5632 8.4, with four 11.1; 32 x 128 with one wave to a piece at 1500 x 1216 x
-// 160 5.8, 32 x 256 at 768 x 11264 x 288 15.3, 64 x 256 there 20.0; 64 x 128 with two
-// waves to a piece at 1500 x 12288 x 4096 200, 64 x 256 there 203, at 2048 rows 260
-// and 244.
+// 8192), and moved by up to 15% to where they choose best.  Over these same calls
+// the choice is 0.4% slower than the fastest of the shapes here in the mean of 216,
+// 13% at worst (48 rows x 11264 outputs x 640: 6.6 us, 5.9 with 32 x 32); gated 0.1%
+// over 112, 3% at worst.  What a shape is worth: 16 x 16 at 2 x 512 x 4096 3.5 us, 16
+// x 32 there 5.8; 32 x 32 with eight waves at 48 x 4096 x 5632 8.4, with four 11.1; 32
+// x 128 with one wave to a piece at 1500 x 1216 x 160 5.8, 32 x 256 at 768 x 11264 x
+// 288 15.3, 64 x 256 there 20.0; 64 x 128 with two waves to a piece at 1500 x 12288 x
+// 4096 200, 64 x 256 there 203, at 2048 rows 260 and 244.
 constexpr ProductShape kProductShapes[] = {
     {16, 16, 8, 2, 1.47, 0.25, 0.82, 0.58},  {16, 32, 8, 2, 1.58, 0.28, 1.08, 0.84},  {16, 64, 8, 1, 1.63, 0.77, 1.44, 0},
     {32, 32, 4, 3, 2.30, 0.35, 0.63, 0.51},  {32, 32, 8, 1, 0.80, 1.82, 1.05, 0},     {32, 64, 4, 2, 2.01, 0.73, 1.31, 0.74},

@@ -164,7 +164,10 @@ hipError_t run_norm(const NormParams &p, hipStream_t stream) {
 
 // One step a thread as far as a workgroup goes: 4096 elements in 512 threads 3.3 us
 // for one row and 3.7 for 64 (fp32, residual, both outputs), in 256 x 2 steps 4.6
-// and 5.1, in 64 x 8 12.3 and 13.5; 6000 rows the same but for 64 threads.
+// and 5.1, in 64 x 8 12.3 and 13.5; 6000 rows the same but for 64 threads.  8192
+// elements in 1024 x 1 or 512 x 2: 3.8 and 4.9 us for one row, 5.8 and 6.6 for 200
+// (bf16 into an fp32 residual, 8-bit rows), 21.3 and 19.4 for 1000, 50.3 and 46.5 for
+// 3000, but all in fp16 32.7 and 35.6: the rule stays with few rows.
 template <bool VEC>
 hipError_t pick_norm(const NormParams &p, hipStream_t stream) {
     const int octets = (p.dim + 7) / 8;

@@ -103,7 +103,7 @@ __device__ __forceinline__ Place place(const Places &d) {
 // products that begin with the float's bits, as the matrix instructions do.  The
 // row lies in LDS, its scales in fp32.  Bound by the weights' bytes and the
 // launch: 12288 x 4096 in 6.6 us, 4.3 TB/s (a large copy: 5.1), with the matrix
-// cores 8.1; gated 2 x 5632 x 4096 8.0 against 9.5.
+// cores 8.1; gated 2 x 5632 x 4096 7.8 against 9.5.
 constexpr int kOneRowChunks = 256;  // of a row in LDS, 144 bytes each
 
 // Dword t of lanes 16 g .. to dword g of lanes 16 t ..: from octet g of four
@@ -229,11 +229,13 @@ constexpr int kRowStride = 144;  // of 128 codes in LDS: 16 rows' octets lie in 
 // waves a run of the tiles' units each; their sums are joined in LDS, wave after
 // wave.  The 8-bit rows are the rows of the result here: a lane has one output
 // of four rows, with the output's scales its own and the rows' read from LDS,
-// where the wave puts them.  PF units are under way at once (2 of the narrowest
-// shape: its waves wait for loads; of the others, whose registers they cost
-// waves, 1: 64 x 4096 x 4096 8.1 against 8.4 us, gated 17 x 5632 x 4096 15.6
-// against 17.8).  Bound by a load, its use and the joining in turn: 64 x 4096 x
-// 4096 takes 8.1 us, where the bytes alone take 2 and a launch 1.6.
+// where the wave puts them.  PF units are under way at once: 2 of the narrowest
+// shape, whose waves wait for loads (16 x 4096 x 4096 5.2 against 5.6 us, 64 x 1000 x
+// 11264 10.8 against 11.8), 1 of 16 x 64 and of gated products, whose registers a
+// second costs waves (16 x 32001 x 4096 16.7 against 18.6, gated 16 x 5632 x 4096 9.7
+// against 10.0), and of 16 x 32, whose times in the rule are those of 1 (32 x 4096 x
+// 4096 6.7; with 2 6.1).  Bound by a load, its use and the joining in turn: 16 x 4096
+// x 4096 takes 5.2 us, where the bytes alone take 1.9 and a launch 1.6.
 template <int NT, int KW, int PF, bool GATED>
 __global__ __launch_bounds__(64 * KW) void few_rows_kernel(ProductParams p, Places places) {
     static_assert(!GATED || NT == 4, "two tiles of gates and the two that they let through");
@@ -391,11 +393,12 @@ hipError_t run_few(const ProductParams &p, hipStream_t stream) {
 // quarter of what reading them as the matrix cores take them does.  D units'
 // weights are under way at once.  AHEAD: a tile's matrix instruction stands
 // before the fmas of the tile before it, which takes the registers of a second
-// unit (64 x 128, D 1 against D 2 without: 1000 x 4096 x 5632 66 against 71 us, 48 x
-// 4096 x 5632 48.0 against 49.6; gated 1000 x 5632 x 4096 140 against 144; 64 x 256
-// plain 250 against 248 at 2048 x 12288 x 4096, narrower ones the same either way).
+// unit (64 x 128, D 1 against D 2 without: 1000 x 4096 x 5632 66 against 71 us, 515 x
+// 6001 x 4000 48.6 against 51.8; gated 1000 x 5632 x 4096 133 against 139, 2048 rows
+// 241 against 244; 64 x 256 plain the other way, 243 against 240 at 2048 x 12288 x
+// 4096; narrower ones the same either way).
 //
-// 2048 x 12288 x 4096 takes 230 to 239 us, 860 to 895 TFLOP/s (64 x 256 outputs a
+// 2048 x 12288 x 4096 takes 230 to 243 us, 850 to 895 TFLOP/s (64 x 256 outputs a
 // workgroup): of 265 in an earlier form of 128 x 128 the vector and matrix
 // instructions alone took 205, the accesses to LDS 25 and the loads from memory
 // 40 (a copy that skips work); the two waves of a SIMD issue more than half of the

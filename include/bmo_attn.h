@@ -647,8 +647,9 @@ BMO_ATTN_API const char *bmo_rows_last_error(void);
  *   y = h / sqrt(mean(h^2) + eps) * weight
  * y goes to out, to 8-bit rows (dim a multiple of 32), or to both; what is
  * NULL is not written.  out may be x, and x the residual (h = 2 x), with the
- * same type and stride.  fp32 inside; the squares of a row have to sum below
- * fp32's range.  n_rows below 2^22. */
+ * same type and stride.  fp32 inside: the squares of a row have to sum below
+ * fp32's range, and where their mean and eps are below 2^-100 together they lose
+ * bits (a row of zeros with eps 0 is NaN, as the formula's).  n_rows below 2^22. */
 BMO_ATTN_API int bmo_rms_norm(int n_rows, int dim, int type, const void *x, int64_t x_stride,
                               int residual_type, void *residual, int64_t residual_stride,
                               int weight_type, const void *weight, float eps, int out_type,
