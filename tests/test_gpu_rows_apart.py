@@ -55,13 +55,13 @@ def test_results_over_8_bit_rows(gpu):
     away = torch.zeros(4, 64, dtype=torch.int8, device="cuda"), torch.zeros(4, 2, dtype=torch.float16, device="cuda")
     stream = torch.cuda.current_stream()
     with bmo.Q4Weights(128, 64) as w, bmo.Q4Weights(256, 64) as g:
-        for a in (1024 - 240, 1024, 1024 + 496, 3072 + 496):
+        for a in (1024 - 240, 1024, 1024 + 496, 3 * 1024 + 496):
             _refused(torch, lambda: w.product(at(a, (4, 64), torch.int8), away[1], out, stream=stream), mem)
         for a in (1024 - 14, 1024, 1024 + 510):
             _refused(torch, lambda: w.product(away[0], at(a, (4, 2), torch.float16), out, stream=stream), mem)
         _refused(torch, lambda: g.gated(*away, out=out, out_codes=at(0, (4, 128), torch.int8),
                                         out_scales=at(4096, (4, 4), torch.float16), stream=stream), mem)
-        for a in (512, 1024 - 256, 3072 + 512):  # between the rows
+        for a in (512, 1024 - 256, 3 * 1024 + 512):  # between the rows
             w.product(at(a, (4, 64), torch.int8), away[1], out, stream=stream)
         torch.cuda.synchronize()
         assert not mem.any()
